@@ -362,6 +362,121 @@ PKV_API int pkv_update_tables(int32_t* block_tables, int64_t table_stride, int32
 PKV_API int pkv_copy_blocks(const pkv_pool* pool, const int32_t* src, const int32_t* dst, int32_t n,
                     int32_t* status_dev, pkv_stream_t stream);
 
+/* ------------------------------------------------------------------ speculative decoding step */
+/*
+ * Verifying drafted tokens: each sequence brings a tree of nodes (node 0, its root, is the
+ * last token decided; a node's parent comes before it), all trees packed end to end, tree b's
+ * nodes cu_nodes[b] .. cu_nodes[b + 1] - 1. One step runs pkv_extend_tables (room for the
+ * step's tokens), pkv_build_tree_metadata, then per layer the rotation and
+ * pkv_tree_attention, the LM head on every node, and pkv_accept_tree, which writes the
+ * accepted path to the cache and advances the lengths on the device. No counterpart in the
+ * reference, which decodes one token per sequence and step (engine/engine.py:108-123).
+ * In every call table row seq_rows[b] < 0 marks a padding sequence, which has no cached keys
+ * and writes nothing; two sequences of a call must not name the same row.
+ *
+ * pkv_extend_tables: block tables and slot maps from request lengths, without the host.
+ *   tables->block_tables is written; tables->rows/cols bound it (seq_rows optional)
+ *   lengths[b], new_tokens[b] : cached tokens, tokens of this step (0 allowed)
+ *   held_blocks[b]            : blocks in row b's table; columns from there on are free
+ *   free_blocks, num_free, free_head[1] : block ids to hand out, from index *free_head on
+ *   Sequence b gets max(0, ceil((lengths + new) / block_size) - held) blocks, in batch order.
+ *   cu_seqlens[num_seqs + 1], context_lens[b] = lengths + new, held_out, free_head_out:
+ *             written; each may be the input it continues (in place)
+ *   positions, slot_mapping (NULL = not written) [total_tokens]: of each new token, packed;
+ *             entries past cu_seqlens[num_seqs] get position 0 and slot -1
+ *   All or nothing: a sequence that does not fit its row, a negative or overlong count
+ *   (PKV_ERR_OUT_OF_RANGE in status) or too few free blocks (PKV_ERR_NO_BLOCKS) leave tables,
+ *   held blocks and head as they were; context_lens is lengths and every slot -1.
+ *   num_seqs <= 4096.
+ */
+PKV_API int pkv_extend_tables(const pkv_tables* tables, int32_t num_seqs, const int32_t* lengths,
+                              const int32_t* new_tokens, const int32_t* held_blocks, const int32_t* free_blocks,
+                              int64_t num_free, const int32_t* free_head, int32_t block_size, int32_t* cu_seqlens,
+                              int32_t* context_lens, int64_t* positions, int64_t* slot_mapping, int64_t total_tokens,
+                              int32_t* held_out, int32_t* free_head_out, int32_t* status_dev, pkv_stream_t stream);
+/*
+ * Ancestor masks and positions of drafted trees from their parents:
+ *   parents[n] : index within the tree of node n's parent, before n; -1 for a root
+ *   mask       : [total_nodes, mask_words]: bit j % 64 of word j / 64 = the node itself or an
+ *                ancestor is node j of its tree
+ *   positions[n] = context_lens[b] + depth (a root's depth is 0)
+ * Rows past cu_nodes[num_seqs] get mask 0 and position 0. A parent that does not come before
+ * its node is reported (PKV_ERR_OUT_OF_RANGE) and the node taken as a root; so is a tree of
+ * more than 64 * mask_words nodes, whose further nodes get mask 0. mask_words <= 8.
+ */
+PKV_API int pkv_build_tree_metadata(const int32_t* parents, const int32_t* cu_nodes, int32_t num_seqs,
+                                    const int32_t* context_lens, int64_t total_nodes, int64_t* mask,
+                                    int32_t mask_words, int64_t* positions, int32_t* status_dev,
+                                    pkv_stream_t stream);
+/*
+ * Rotary positions in the layouts pkv_rope_append does not take, fused with the KV append:
+ * element pairs (2i, 2i + 1) (interleaved != 0) or (i, i + rotary_dim / 2), i < rotary_dim / 2,
+ * of every q and k head turned by the angle positions[t] * inv_freq[i] and multiplied by
+ * attention_factor; elements from rotary_dim on are copied. Angles are reduced in float64,
+ * the rotation is float32 and each element is rounded once.
+ *   qkv, q_out, k_out, slot_mapping : as pkv_rope_append; q_out, k_out and v_out may also be
+ *                the columns of qkv themselves (in place)
+ *   v_out (NULL = not written) : the v columns, token t, kv head j at v_out + t*stride_t + j*stride_h
+ *   inv_freq : float64 [rotary_dim / 2] on the device; positions >= 0 (a negative one is
+ *                reported and rotates backwards)
+ * Any head_dim; 16-byte accesses where every row, head and rotary_dim / 2 allow them.
+ */
+PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* qkv, int64_t qkv_stride,
+                              int64_t n_tokens, int32_t num_q_heads, const int64_t* positions,
+                              const double* inv_freq, int32_t rotary_dim, int32_t interleaved,
+                              float attention_factor, void* q_out, int64_t q_out_stride_t, int64_t q_out_stride_h,
+                              void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h, void* v_out,
+                              int64_t v_out_stride_t, int64_t v_out_stride_h, const int64_t* slot_mapping,
+                              int32_t* status_dev, pkv_stream_t stream);
+/*
+ * Attention of the trees' nodes over the paged cache: node n attends to its sequence's
+ * cached keys 0 .. context_lens[b] - 1 (0 allowed), read from the pool through tables, and
+ * to the nodes of its tree whose bit is set in its mask row (any mask, as
+ * pkv_build_tree_metadata makes them or not). A row that sees no key gives zeros.
+ *   q, out           : node n, query head h at q + n*q_stride_n + h*q_stride_h
+ *   k_nodes, v_nodes : node n, kv head j at k_nodes + n*k_stride_n + j*k_stride_h, 16-byte
+ *                aligned rows and heads (strides multiples of 8 elements); not in the pool
+ *   max_nodes        : no tree has more (<= 64 * mask_words, mask_words <= 8)
+ *   workspace        : pkv_tree_attention_workspace_bytes bytes, 256-byte aligned; contents
+ *                do not matter; calls that share one must not overlap on the GPU
+ * Rows past cu_nodes[num_seqs] of out are not written. Slots of the pool past
+ * context_lens may hold anything, NaN included; K/V that any node of a tree may see must be
+ * finite. Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head
+ * <= 16, num_seqs <= 1024, scale > 0; anything else returns PKV_ERR_UNSUPPORTED (a scale
+ * that is not positive PKV_ERR_INVALID_ARGUMENT).
+ */
+PKV_API int64_t pkv_tree_attention_workspace_bytes(int32_t batch, int32_t head_dim);
+PKV_API int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv_tables* tables, int32_t num_seqs,
+                               const int32_t* cu_nodes, const int32_t* context_lens, int32_t max_nodes,
+                               int64_t total_nodes, int32_t num_q_heads, void* out, int64_t out_stride_n,
+                               int64_t out_stride_h, const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                               const void* k_nodes, int64_t k_stride_n, int64_t k_stride_h, const void* v_nodes,
+                               int64_t v_stride_n, int64_t v_stride_h, const int64_t* mask, int32_t mask_words,
+                               float scale, void* workspace, int64_t workspace_bytes, int32_t* status_dev,
+                               pkv_stream_t stream);
+/*
+ * Greedy acceptance of one path per tree, with its K/V written to the cache. From node 0 the
+ * path goes to the lowest node j whose parent is the path's last node c and whose
+ * draft_tokens[j] == target_tokens[c] (the model's greedy choice after c), while there is one
+ * and the path has fewer than path_width nodes.
+ *   counts[b]      : nodes of the path (0 for an empty tree or a padding sequence)
+ *   path, tokens   : [num_seqs, path_width]: the path's node indexes within the tree and their
+ *                target tokens (the step's new tokens), -1 behind them
+ *   lengths_out[b] = context_lens[b] + counts[b]; may be context_lens itself
+ *   k_nodes, v_nodes : layer l, node n, kv head j at k_nodes + l*k_stride_l + n*k_stride_n +
+ *                j*k_stride_h; the path's k-th node goes to position context_lens[b] + k of
+ *                every layer through tables, which must hold blocks for them (a missing one is
+ *                reported, PKV_ERR_OUT_OF_RANGE, and its row skipped)
+ * Trees of up to 512 nodes, path_width <= 64.
+ */
+PKV_API int pkv_accept_tree(const pkv_pool* pool, const pkv_tables* tables, int32_t num_seqs, const int32_t* parents,
+                            const int32_t* cu_nodes, int64_t total_nodes, const int64_t* draft_tokens,
+                            const int64_t* target_tokens, const void* k_nodes, int64_t k_stride_l, int64_t k_stride_n,
+                            int64_t k_stride_h, const void* v_nodes, int64_t v_stride_l, int64_t v_stride_n,
+                            int64_t v_stride_h, const int32_t* context_lens, int32_t* counts, int32_t* path,
+                            int64_t* tokens, int32_t path_width, int32_t* lengths_out, int32_t* status_dev,
+                            pkv_stream_t stream);
+
 /* ------------------------------------------------------------------ block manager (host) */
 /*
  * The reference's allocator and prefix cache (PagedKVCache host bookkeeping,

@@ -93,6 +93,22 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_prefill_attention": (c_int32, [P_POOL, c_int32, P_TABLES, c_int32, c_void_p, c_void_p, c_int32, c_int32,
                                         c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_float, c_void_p,
                                         c_void_p]),
+    "pkv_extend_tables": (c_int32, [P_TABLES, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                    c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                    c_void_p, c_void_p]),
+    "pkv_build_tree_metadata": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int32, c_void_p,
+                                          c_void_p, c_void_p]),
+    "pkv_rotary_append": (c_int32, [P_POOL, c_int32, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32,
+                                    c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                    c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "pkv_tree_attention_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "pkv_tree_attention": (c_int32, [P_POOL, c_int32, P_TABLES, c_int32, c_void_p, c_void_p, c_int32, c_int64, c_int32,
+                                     c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                     c_void_p, c_int64, c_int64, c_void_p, c_int32, c_float, c_void_p, c_int64,
+                                     c_void_p, c_void_p]),
+    "pkv_accept_tree": (c_int32, [P_POOL, P_TABLES, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                  c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
     "pkv_build_decode_metadata": (c_int32, [P_TABLES, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
                                             c_void_p, c_void_p, c_void_p]),
     "pkv_build_prefill_metadata": (c_int32, [P_TABLES, c_int32, c_void_p, c_void_p, c_int32, c_int64, c_void_p,

@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pkv.h"
 
 namespace pkv {
@@ -16,6 +18,23 @@ namespace pkv {
 // ---------------------------------------------------------------- host-side error plumbing
 void set_last_cuda_error(cudaError_t e);
 int cuda_status(cudaError_t e);  // PKV_OK or PKV_ERR_CUDA (and records the message)
+
+// A kernel's dynamic shared memory limit, raised once per device.
+class SmemAttribute {
+  std::atomic<uint64_t> done_{0};  // bit per device
+
+ public:
+  cudaError_t set(const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done_.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done_.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+  }
+};
 
 inline int launch_status() { return cuda_status(cudaGetLastError()); }
 
@@ -312,6 +331,12 @@ bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int h
 // for the 128-byte swizzle). Rows past `rows` read as zeros.
 int make_matrix_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows,
                            uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_rows);
+// 4-D tensor map over rows [rows, heads, d] of 16-bit elements (strides in elements, multiples
+// of 8; d a multiple of 64), viewed as {64, d/64, heads, rows} with a box of {64, 1, 1,
+// box_rows}: one 64-wide chunk of one head of consecutive rows per copy, 128-byte swizzle.
+// Rows past `rows` read as zeros.
+int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
+                         int64_t head_stride, int64_t row_stride, int box_rows);
 // Streaming multiprocessors of the current device (queried once).
 int num_sms();
 

@@ -1,0 +1,526 @@
+// The steps around tree attention that a speculative decoding step runs on the GPU: block
+// tables and slot maps from request lengths, the drafted trees' ancestor masks and
+// positions, and the acceptance of a path with its K/V written to the cache. None has a
+// counterpart in the reference, which decodes one token per sequence and plans every step
+// on the host (engine/kv_cache.py:542-573, 597-609). With these three a step's lengths
+// never visit the host: accept_tree advances them where the next extend_tables reads them.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace pkv {
+namespace {
+
+namespace cg = cooperative_groups;
+
+// ---------------------------------------------------------------- block tables from lengths
+// For request b (len_b cached tokens, new_b new ones, held_b blocks in its table row):
+//   need_b  = max(held_b, ceil((len_b + new_b) / bs)),  fresh_b = need_b - held_b
+//   its fresh blocks are free[head + F_b ..], F_b = sum of fresh over earlier requests
+//   cu[b]   = sum of new over earlier requests; token t of b sits at position
+//             len_b + (t - cu[b]) and slot block(position / bs) * bs + position % bs
+// All or nothing: when a request does not fit its row, or the free list is too short, no
+// table, held count or head changes and every slot is -1.
+//
+// Every CTA of one cluster scans all requests for itself (a few thousand integers, read
+// from L2) and then takes its share of the tokens and table entries, so one launch does
+// what a scan kernel and a scatter kernel would; the cluster barrier between the reads
+// and the writes lets the outputs be the inputs' own buffers.
+constexpr int kPlanSeqs = 4096;   // requests per call
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanCtas = 8;      // the portable cluster size
+
+struct PlanParams {
+  int32_t* tables;
+  const int32_t* seq_rows;
+  const int32_t* lengths;
+  const int32_t* new_tokens;
+  const int32_t* held;
+  const int32_t* free_blocks;
+  const int32_t* free_head;
+  int32_t* cu;
+  int32_t* ctx;
+  int64_t* positions;
+  int64_t* slots;
+  int32_t* held_out;
+  int32_t* head_out;
+  int32_t* status;
+  int64_t table_stride, num_free, total_tokens;
+  int32_t rows, cols, batch, bs;
+};
+
+// Exclusive prefix sums of two values per thread over the CTA; totals in *ta, *tb.
+__device__ inline void block_scan2(int64_t& a, int64_t& b, int64_t* ta, int64_t* tb) {
+  __shared__ int64_t wa[32], wb[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int64_t ia = a, ib = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t ua = __shfl_up_sync(0xffffffffu, ia, o), ub = __shfl_up_sync(0xffffffffu, ib, o);
+    if (lane >= o) ia += ua, ib += ub;
+  }
+  if (lane == 31) wa[warp] = ia, wb[warp] = ib;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t xa = lane < nw ? wa[lane] : 0, xb = lane < nw ? wb[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t ua = __shfl_up_sync(0xffffffffu, xa, o), ub = __shfl_up_sync(0xffffffffu, xb, o);
+      if (lane >= o) xa += ua, xb += ub;
+    }
+    if (lane < nw) wa[lane] = xa, wb[lane] = xb;
+  }
+  __syncthreads();
+  *ta = wa[nw - 1];
+  *tb = wb[nw - 1];
+  a = ia - a + (warp ? wa[warp - 1] : 0);
+  b = ib - b + (warp ? wb[warp - 1] : 0);
+}
+
+// The last i in [0, n) with first[i] <= x, for non-decreasing first with first[0] <= x.
+__device__ inline int last_at_most(const int32_t* first, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads, 1) extend_tables_kernel(const PlanParams p) {
+  extern __shared__ int32_t plan_smem[];
+  const int B = p.batch;
+  int32_t* s_len = plan_smem;    // [B] cached tokens
+  int32_t* s_held = s_len + B;   // [B] blocks held
+  int32_t* s_row = s_held + B;   // [B] table row, -1 = padding
+  int32_t* s_cu = s_row + B;     // [B + 1] tokens before request b
+  int32_t* s_fp = s_cu + B + 1;  // [B + 1] fresh blocks before request b
+  const int tid = threadIdx.x;
+  const int per = (B + blockDim.x - 1) / blockDim.x;
+  const int b0 = min(B, tid * per), b1 = min(B, b0 + per);
+  const int64_t head = *p.free_head;
+  int64_t sum_new = 0, sum_fresh = 0;
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) {
+    int row = p.seq_rows ? p.seq_rows[b] : b;
+    int64_t len = p.lengths[b], n = p.new_tokens[b], held = p.held[b];
+    if (row >= p.rows || n < 0 || (row >= 0 && (len < 0 || held < 0 || held > p.cols))) bad = true;
+    n = max(n, (int64_t)0);
+    int64_t fresh = 0;
+    if (row >= 0) {
+      const int64_t need = (len + n + p.bs - 1) / p.bs;
+      if (need > p.cols) bad = true;
+      fresh = max(need - held, (int64_t)0);
+    }
+    s_len[b] = (int32_t)max(len, (int64_t)0);
+    s_held[b] = (int32_t)held;
+    s_row[b] = row;
+    sum_new += n;
+    sum_fresh += fresh;
+  }
+  int64_t pre_new = sum_new, pre_fresh = sum_fresh, total_new, total_fresh;
+  block_scan2(pre_new, pre_fresh, &total_new, &total_fresh);
+  for (int b = b0; b < b1; ++b) {  // the sums once more, now with what came before
+    const int64_t n = max((int64_t)p.new_tokens[b], (int64_t)0);
+    s_cu[b] = (int32_t)min(pre_new, p.total_tokens);
+    s_fp[b] = (int32_t)min(pre_fresh, (int64_t)0x7fffffff);
+    pre_new += n;
+    if (s_row[b] >= 0) pre_fresh += max(((int64_t)s_len[b] + n + p.bs - 1) / p.bs - s_held[b], (int64_t)0);
+  }
+  if (tid == 0) {
+    s_cu[B] = (int32_t)min(total_new, p.total_tokens);
+    s_fp[B] = (int32_t)min(total_fresh, (int64_t)0x7fffffff);
+  }
+  bad = __syncthreads_or(bad || total_new > p.total_tokens || head < 0);
+  const bool short_of = !bad && total_fresh > max(p.num_free - head, (int64_t)0);
+  const bool ok = !bad && !short_of;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  cluster.sync();  // every CTA has read the lengths, held counts and the head
+
+  if (rank == 0) {
+    if (tid == 0) {
+      if (bad) report(p.status, PKV_ERR_OUT_OF_RANGE);
+      if (short_of) report(p.status, PKV_ERR_NO_BLOCKS);
+      *p.head_out = (int32_t)(head + (ok ? total_fresh : 0));
+    }
+    for (int b = tid; b < B; b += blockDim.x) {
+      p.cu[b] = s_cu[b];
+      p.ctx[b] = s_row[b] >= 0 ? s_len[b] + (ok ? s_cu[b + 1] - s_cu[b] : 0) : 0;
+      p.held_out[b] = s_held[b] + (ok ? s_fp[b + 1] - s_fp[b] : 0);
+    }
+    if (tid == 0) p.cu[B] = s_cu[B];
+  }
+  const int32_t* fresh_blocks = p.free_blocks + head;
+  if (ok) {
+    for (int64_t k = (int64_t)rank * blockDim.x + tid; k < total_fresh; k += (int64_t)ctas * blockDim.x) {
+      const int b = last_at_most(s_fp, B, (int)k);
+      const int32_t blk = fresh_blocks[k];
+      if (blk < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+      p.tables[s_row[b] * p.table_stride + s_held[b] + (k - s_fp[b])] = blk;
+    }
+  }
+  if (!p.positions && !p.slots) return;
+  const int used = s_cu[B];
+  for (int64_t t = (int64_t)rank * blockDim.x + tid; t < p.total_tokens; t += (int64_t)ctas * blockDim.x) {
+    int64_t pos = 0, slot = -1;
+    if (ok && t < used) {
+      const int b = last_at_most(s_cu, B, (int)t);
+      if (s_row[b] >= 0) {
+        pos = (int64_t)s_len[b] + (t - s_cu[b]);
+        const int col = (int)(pos / p.bs);
+        const int32_t blk = col < s_held[b] ? p.tables[s_row[b] * p.table_stride + col]
+                                            : fresh_blocks[s_fp[b] + (col - s_held[b])];
+        if (blk < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+        else slot = (int64_t)blk * p.bs + pos % p.bs;
+      }
+    }
+    if (p.positions) p.positions[t] = pos;
+    if (p.slots) p.slots[t] = slot;
+  }
+}
+
+// ---------------------------------------------------------------- tree metadata
+// mask[n] = bits of node n's ancestors and itself, 64 nodes to a word; position =
+// context_lens[b] + depth, depth = popcount(mask) - 1. A node's ancestors are gathered by
+// pointer doubling in shared memory: after round k a node's mask covers its 2^k nearest
+// ancestors and jump points 2^k up, so a chain of 512 nodes takes 9 rounds instead of 512
+// dependent loads. One CTA per tree, one thread per node.
+constexpr int kTreeWords = 8;                  // mask words
+constexpr int kTreeNodes = 64 * kTreeWords;    // nodes of a tree
+
+__global__ void tree_metadata_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ cu,
+                                     int32_t batch, const int32_t* __restrict__ ctx, int64_t total,
+                                     uint64_t* __restrict__ mask, int32_t words, int64_t* __restrict__ positions,
+                                     int32_t* status) {
+  extern __shared__ uint64_t tree_smem[];
+  const int b = blockIdx.x, tid = threadIdx.x, cap = 64 * words;
+  if (b == batch) {  // rows behind the last tree: padding of a captured step
+    for (int64_t n = max(cu[batch], 0) + tid; n < total; n += blockDim.x) {
+      for (int w = 0; w < words; ++w) mask[n * words + w] = 0;
+      positions[n] = 0;
+    }
+    return;
+  }
+  const int lo = cu[b], hi = cu[b + 1];
+  if (lo < 0 || hi < lo || hi > total) {
+    if (tid == 0) report(status, PKV_ERR_OUT_OF_RANGE);
+    return;
+  }
+  const int all = hi - lo, n = min(all, cap);
+  if (all > cap && tid == 0) report(status, PKV_ERR_OUT_OF_RANGE);
+  uint64_t* bits = tree_smem;                               // [words][n]
+  int32_t* jump = reinterpret_cast<int32_t*>(bits + (size_t)words * cap);  // [n]
+  for (int i = tid; i < n; i += blockDim.x) {
+    int up = parents[lo + i];
+    if (up < -1 || up >= i) {
+      report(status, PKV_ERR_OUT_OF_RANGE);
+      up = -1;
+    }
+    jump[i] = up;
+    for (int w = 0; w < words; ++w) bits[w * cap + i] = w == i / 64 ? 1ull << (i % 64) : 0;
+  }
+  // Each thread owns the nodes tid, tid + blockDim, ...: reads of the round before the
+  // barrier, writes after it.
+  constexpr int kOwn = kTreeNodes / 128;
+  int next[kOwn];
+  uint64_t got[kOwn][kTreeWords];
+  for (bool more = true; more;) {
+    __syncthreads();
+    more = false;
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+      const int i = tid + o * 128;
+      next[o] = -2;
+      if (i < n && jump[i] >= 0) {
+        const int j = jump[i];
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w) got[o][w] = w < words ? bits[w * cap + j] : 0;
+        next[o] = jump[j];
+        more |= next[o] >= 0;
+      }
+    }
+    more = __syncthreads_or(more);
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+      const int i = tid + o * 128;
+      if (next[o] != -2) {
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w)
+          if (w < words) bits[w * cap + i] |= got[o][w];
+        jump[i] = next[o];
+      }
+    }
+  }
+  const int64_t at = ctx[b];
+  for (int i = tid; i < all; i += blockDim.x) {
+    int depth = -1;
+    for (int w = 0; w < words; ++w) {
+      const uint64_t m = i < n ? bits[w * cap + i] : 0;
+      mask[(int64_t)(lo + i) * words + w] = m;
+      depth += __popcll(m);
+    }
+    positions[lo + i] = at + max(depth, 0);
+  }
+}
+
+// ---------------------------------------------------------------- acceptance
+// The path of tree b starts at its node 0 (the last token decided); from node c it goes to
+// the lowest j with parent[j] = c and draft[j] = target[c], while there is one. Its nodes'
+// targets are the step's new tokens, and its K/V rows of every layer move from the nodes'
+// buffers to positions len_b, len_b + 1, ... of the sequence.
+//
+// One cluster per tree: every CTA walks the tree for itself (one warp, 32 candidates a
+// step by ballot; a path has a handful of nodes), then copies its share of the layers. The
+// copies are all the bytes there are; the walk is a chain of shared-memory reads.
+constexpr int kAcceptThreads = 256;
+constexpr int kAcceptWidth = 64;  // longest path
+
+struct AcceptParams {
+  const int32_t* tables;
+  const int32_t* seq_rows;
+  const int32_t* parents;
+  const int32_t* cu;
+  const int64_t* draft;
+  const int64_t* target;
+  const void* k_nodes;
+  const void* v_nodes;
+  void* k_pool;
+  void* v_pool;
+  const int32_t* lengths;
+  int32_t* counts;
+  int32_t* path;
+  int64_t* tokens;
+  int32_t* lengths_out;
+  int32_t* status;
+  int64_t table_stride, k_sl, k_sn, k_sh, v_sl, v_sn, v_sh, total;
+  int32_t rows, cols, batch, width, layers, hkv, d, bs, nbt;
+};
+
+template <int EW> struct Bytes;
+template <> struct Bytes<8> { using type = uint4; };
+template <> struct Bytes<1> { using type = uint16_t; };
+
+template <int EW>
+__global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const AcceptParams p) {
+  __shared__ int32_t s_parent[kTreeNodes];
+  __shared__ int64_t s_draft[kTreeNodes], s_target[kTreeNodes];
+  __shared__ int32_t s_path[kAcceptWidth], s_block[kAcceptWidth], s_count;
+  using V = typename Bytes<EW>::type;
+  const int tid = threadIdx.x, lane = tid & 31;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int b = blockIdx.x / ctas;
+  int row = p.seq_rows ? p.seq_rows[b] : b;
+  const int lo = p.cu[b], hi = p.cu[b + 1], len = p.lengths[b];
+  bool bad = row >= p.rows || lo < 0 || hi < lo || hi > p.total || (row >= 0 && len < 0);
+  int n = bad || row < 0 ? 0 : hi - lo;
+  if (n > kTreeNodes) bad = true, n = kTreeNodes;
+  if (bad && tid == 0 && rank == 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+  for (int i = tid; i < n; i += kAcceptThreads) {
+    s_parent[i] = p.parents[lo + i];
+    s_draft[i] = p.draft[lo + i];
+    s_target[i] = p.target[lo + i];
+  }
+  __syncthreads();
+  if (tid < 32) {
+    int count = n > 0 ? 1 : 0, cur = 0;
+    if (lane == 0) s_path[0] = 0;
+    while (count > 0 && count < p.width) {
+      const int64_t want = s_target[cur];
+      int found = -1;
+      for (int j0 = cur + 1; j0 < n && found < 0; j0 += 32) {
+        const int j = j0 + lane;
+        const unsigned hit = __ballot_sync(0xffffffffu, j < n && s_parent[j] == cur && s_draft[j] == want);
+        if (hit) found = j0 + __ffs(hit) - 1;
+      }
+      if (found < 0) break;
+      cur = found;
+      if (lane == 0) s_path[count] = cur;
+      ++count;
+    }
+    for (int k = lane; k < count; k += 32) {
+      const int64_t col = ((int64_t)len + k) / p.bs;
+      int blk = col < p.cols ? p.tables[row * p.table_stride + col] : -1;
+      if (blk < 0 || blk >= p.nbt) {
+        report(p.status, PKV_ERR_OUT_OF_RANGE);
+        blk = -1;
+      }
+      s_block[k] = blk;
+    }
+    if (lane == 0) s_count = count;
+  }
+  __syncthreads();
+  const int count = s_count;
+  cluster.sync();  // every CTA has read the length: lengths_out may be the same buffer
+  if (rank == 0) {
+    for (int k = tid; k < p.width; k += kAcceptThreads) {
+      p.path[(int64_t)b * p.width + k] = k < count ? s_path[k] : -1;
+      p.tokens[(int64_t)b * p.width + k] = k < count ? s_target[s_path[k]] : -1;
+    }
+    if (tid == 0) {
+      p.counts[b] = count;
+      p.lengths_out[b] = len + count;
+    }
+  }
+  // (layer, K or V, path node, head, vector): a vector of EW elements per thread and turn.
+  const int vecs = p.d / EW, per_row = p.hkv * vecs, per_layer = 2 * count * per_row;
+  for (int l = rank; l < p.layers; l += ctas) {
+    for (int i = tid; i < per_layer; i += kAcceptThreads) {
+      const int which = i / (count * per_row), r = i - which * count * per_row;
+      const int k = r / per_row, hv = r - k * per_row, h = hv / vecs, c = (hv - h * vecs) * EW;
+      if (s_block[k] < 0) continue;
+      const int64_t node = lo + s_path[k];
+      const uint16_t* src = which ? static_cast<const uint16_t*>(p.v_nodes) + l * p.v_sl + node * p.v_sn + h * p.v_sh
+                                  : static_cast<const uint16_t*>(p.k_nodes) + l * p.k_sl + node * p.k_sn + h * p.k_sh;
+      uint16_t* dst = static_cast<uint16_t*>(which ? p.v_pool : p.k_pool) +
+                      (((int64_t)l * p.nbt + s_block[k]) * p.hkv + h) * p.bs * p.d + (int64_t)((len + k) % p.bs) * p.d;
+      *reinterpret_cast<V*>(dst + c) = *reinterpret_cast<const V*>(src + c);
+    }
+  }
+}
+
+// A launch of `ctas` CTAs in clusters of `cluster` CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), int ctas, int cluster, int threads, size_t smem, cudaStream_t st,
+                           Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int pkv_extend_tables(const pkv_tables* tables, int32_t num_seqs, const int32_t* lengths,
+                                 const int32_t* new_tokens, const int32_t* held_blocks, const int32_t* free_blocks,
+                                 int64_t num_free, const int32_t* free_head, int32_t block_size, int32_t* cu_seqlens,
+                                 int32_t* context_lens, int64_t* positions, int64_t* slot_mapping, int64_t total_tokens,
+                                 int32_t* held_out, int32_t* free_head_out, int32_t* status_dev, pkv_stream_t stream) {
+  if (!tables || !free_head || !free_head_out || !cu_seqlens || (!free_blocks && num_free > 0)) return PKV_ERR_INVALID_ARGUMENT;
+  if (num_seqs > 0 && (!tables->block_tables || !lengths || !new_tokens || !held_blocks || !context_lens || !held_out))
+    return PKV_ERR_INVALID_ARGUMENT;
+  if (num_seqs < 0 || block_size <= 0 || num_free < 0 || total_tokens < 0 || total_tokens > 0x7fffffff ||
+      num_free > 0x7fffffff || tables->rows < 0 || tables->cols < 0 || tables->stride < 0 ||
+      (!tables->seq_rows && tables->rows < num_seqs))
+    return PKV_ERR_INVALID_ARGUMENT;
+  if (num_seqs > kPlanSeqs) return PKV_ERR_UNSUPPORTED;
+  PlanParams p;
+  p.tables = const_cast<int32_t*>(tables->block_tables);
+  p.seq_rows = tables->seq_rows;
+  p.lengths = lengths;
+  p.new_tokens = new_tokens;
+  p.held = held_blocks;
+  p.free_blocks = free_blocks;
+  p.free_head = free_head;
+  p.cu = cu_seqlens;
+  p.ctx = context_lens;
+  p.positions = positions;
+  p.slots = slot_mapping;
+  p.held_out = held_out;
+  p.head_out = free_head_out;
+  p.status = status_dev;
+  p.table_stride = tables->stride;
+  p.num_free = num_free;
+  p.total_tokens = total_tokens;
+  p.rows = tables->rows;
+  p.cols = tables->cols;
+  p.batch = num_seqs;
+  p.bs = block_size;
+  const size_t smem = (5 * (size_t)num_seqs + 2) * 4;
+  if (smem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(extend_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e);
+  }
+  return cuda_status(launch_cluster(extend_tables_kernel, kPlanCtas, kPlanCtas, kPlanThreads, smem,
+                                    reinterpret_cast<cudaStream_t>(stream), p));
+}
+
+extern "C" int pkv_build_tree_metadata(const int32_t* parents, const int32_t* cu_nodes, int32_t num_seqs,
+                                       const int32_t* context_lens, int64_t total_nodes, int64_t* mask,
+                                       int32_t mask_words, int64_t* positions, int32_t* status_dev,
+                                       pkv_stream_t stream) {
+  if (num_seqs < 0 || total_nodes < 0 || total_nodes > 0x7fffffff || mask_words <= 0) return PKV_ERR_INVALID_ARGUMENT;
+  if (mask_words > kTreeWords) return PKV_ERR_UNSUPPORTED;
+  if (total_nodes == 0) return PKV_OK;
+  if (!parents || !cu_nodes || !mask || !positions || (num_seqs > 0 && !context_lens)) return PKV_ERR_INVALID_ARGUMENT;
+  const size_t smem = (size_t)64 * mask_words * (8 * mask_words + 4);
+  tree_metadata_kernel<<<num_seqs + 1, 128, smem, reinterpret_cast<cudaStream_t>(stream)>>>(
+      parents, cu_nodes, num_seqs, context_lens, total_nodes, reinterpret_cast<uint64_t*>(mask), mask_words, positions,
+      status_dev);
+  return launch_status();
+}
+
+extern "C" int pkv_accept_tree(const pkv_pool* pool, const pkv_tables* tables, int32_t num_seqs, const int32_t* parents,
+                               const int32_t* cu_nodes, int64_t total_nodes, const int64_t* draft_tokens,
+                               const int64_t* target_tokens, const void* k_nodes, int64_t k_stride_l, int64_t k_stride_n,
+                               int64_t k_stride_h, const void* v_nodes, int64_t v_stride_l, int64_t v_stride_n,
+                               int64_t v_stride_h, const int32_t* context_lens, int32_t* counts, int32_t* path,
+                               int64_t* tokens, int32_t path_width, int32_t* lengths_out, int32_t* status_dev,
+                               pkv_stream_t stream) {
+  if (!pool || !pool->k || !pool->v || !tables) return PKV_ERR_INVALID_ARGUMENT;
+  if (num_seqs < 0 || total_nodes < 0 || total_nodes > 0x7fffffff || path_width <= 0 || pool->num_layers <= 0 ||
+      pool->num_kv_heads <= 0 || pool->head_dim <= 0 || pool->block_size <= 0 || pool->num_blocks_total <= 0 ||
+      tables->stride < 0 || (!tables->seq_rows && tables->rows < num_seqs))
+    return PKV_ERR_INVALID_ARGUMENT;
+  if (pool->dtype != PKV_F16 && pool->dtype != PKV_BF16) return PKV_ERR_UNSUPPORTED;
+  if (path_width > kAcceptWidth) return PKV_ERR_UNSUPPORTED;
+  if (num_seqs == 0) return PKV_OK;
+  if (!tables->block_tables || !cu_nodes || !context_lens || !counts || !path || !tokens || !lengths_out)
+    return PKV_ERR_INVALID_ARGUMENT;
+  if (total_nodes > 0 && (!parents || !draft_tokens || !target_tokens || !k_nodes || !v_nodes))
+    return PKV_ERR_INVALID_ARGUMENT;
+  AcceptParams p;
+  p.tables = tables->block_tables;
+  p.seq_rows = tables->seq_rows;
+  p.parents = parents;
+  p.cu = cu_nodes;
+  p.draft = draft_tokens;
+  p.target = target_tokens;
+  p.k_nodes = k_nodes;
+  p.v_nodes = v_nodes;
+  p.k_pool = pool->k;
+  p.v_pool = pool->v;
+  p.lengths = context_lens;
+  p.counts = counts;
+  p.path = path;
+  p.tokens = tokens;
+  p.lengths_out = lengths_out;
+  p.status = status_dev;
+  p.table_stride = tables->stride;
+  p.k_sl = k_stride_l, p.k_sn = k_stride_n, p.k_sh = k_stride_h;
+  p.v_sl = v_stride_l, p.v_sn = v_stride_n, p.v_sh = v_stride_h;
+  p.total = total_nodes;
+  p.rows = tables->rows;
+  p.cols = tables->cols;
+  p.batch = num_seqs;
+  p.width = path_width;
+  p.layers = pool->num_layers;
+  p.hkv = pool->num_kv_heads;
+  p.d = pool->head_dim;
+  p.bs = pool->block_size;
+  p.nbt = pool->num_blocks_total;
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(k_nodes) | reinterpret_cast<uintptr_t>(v_nodes) |
+                         reinterpret_cast<uintptr_t>(pool->k) | reinterpret_cast<uintptr_t>(pool->v);
+  if (addr & 1) return PKV_ERR_INVALID_ARGUMENT;
+  const int64_t strides = k_stride_l | k_stride_n | k_stride_h | v_stride_l | v_stride_n | v_stride_h | p.d;
+  const bool vec16 = (addr & 15) == 0 && (strides & 7) == 0;
+  const int cluster = std::min(8, p.layers >= 8 ? 8 : p.layers >= 4 ? 4 : p.layers >= 2 ? 2 : 1);
+  auto kernel = vec16 ? accept_tree_kernel<8> : accept_tree_kernel<1>;
+  return cuda_status(launch_cluster(kernel, num_seqs * cluster, cluster, kAcceptThreads, 0,
+                                    reinterpret_cast<cudaStream_t>(stream), p));
+}

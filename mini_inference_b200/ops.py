@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from dataclasses import dataclass
 
 import torch
 
@@ -413,6 +414,270 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
     return out
 
 
+# ---------------------------------------------------------------- speculative decoding step
+
+def _call(device: torch.device, fn, what: str, *args) -> None:
+    """Call ``fn(*args, stream)`` on ``device``'s current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    check(status, what)
+
+
+def _ints(device: torch.device, dtype: torch.dtype, what: str, *ts: torch.Tensor | None) -> None:
+    for t in ts:
+        if t is not None and (t.dtype != dtype or t.device != device or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous {dtype} tensors on {device}")
+
+
+def extend_tables(tables: PkvTables, lengths: torch.Tensor, new_tokens: torch.Tensor, held: torch.Tensor,
+                  free_blocks: torch.Tensor, free_head: torch.Tensor, block_size: int, cu_seqlens: torch.Tensor,
+                  context_lens: torch.Tensor, positions: torch.Tensor | None = None,
+                  slot_mapping: torch.Tensor | None = None, held_out: torch.Tensor | None = None,
+                  free_head_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Grow the block tables to hold each request's new tokens and map them to slots, on the GPU.
+
+    Request ``b`` has ``lengths[b]`` cached tokens in ``held[b]`` blocks and brings
+    ``new_tokens[b]`` more (int32 ``[B]`` each). It takes the blocks it lacks from
+    ``free_blocks`` (int32), from index ``free_head[0]`` on, in batch order; its table row is
+    extended in place. Written: ``cu_seqlens`` (int32 ``[B + 1]``), ``context_lens`` (int32
+    ``[B]``, lengths + new), ``positions`` and ``slot_mapping`` (int64, one entry per new
+    token; further entries get 0 and -1), ``held_out`` and ``free_head_out`` (``held`` and
+    ``free_head`` themselves unless given). All or nothing: when a request does not fit its
+    row or the free list runs out, nothing is extended, every slot is -1 and the status
+    word says so (see pkv_extend_tables in include/pkv.h).
+    """
+    _require_cuda(lengths)
+    dev = lengths.device
+    held_out = held if held_out is None else held_out
+    free_head_out = free_head if free_head_out is None else free_head_out
+    _ints(dev, torch.int32, "extend_tables: lengths, counts and block ids", lengths, new_tokens, held, free_blocks,
+          free_head, cu_seqlens, context_lens, held_out, free_head_out, status)
+    _ints(dev, torch.int64, "extend_tables: positions and slot_mapping", positions, slot_mapping)
+    batch = lengths.numel()
+    if (new_tokens.numel() != batch or held.numel() != batch or context_lens.numel() < batch or
+            held_out.numel() < batch or cu_seqlens.numel() < batch + 1 or free_head.numel() < 1 or
+            free_head_out.numel() < 1):
+        raise ValueError("extend_tables: one entry per request (cu_seqlens one more, free_head one)")
+    total = positions.numel() if positions is not None else slot_mapping.numel() if slot_mapping is not None else 2**31 - 1
+    if positions is not None and slot_mapping is not None and slot_mapping.numel() != total:
+        raise ValueError("extend_tables: positions and slot_mapping must have one size")
+    _call(dev, lib.pkv_extend_tables, "extend_tables", ctypes.byref(tables), batch, lengths.data_ptr(),
+          new_tokens.data_ptr(), held.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), free_head.data_ptr(),
+          block_size, cu_seqlens.data_ptr(), context_lens.data_ptr(), _ptr(positions), _ptr(slot_mapping), total,
+          held_out.data_ptr(), free_head_out.data_ptr(), _ptr(status))
+
+
+def build_tree_metadata(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch.Tensor,
+                        mask: torch.Tensor, positions: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """Ancestor masks and positions of drafted trees.
+
+    ``parents`` (int32 ``[N]``) holds each node's parent as an index within its tree (-1 for a
+    root; a parent comes before its nodes), tree ``b`` being nodes ``cu_nodes[b] ..
+    cu_nodes[b + 1] - 1``. ``mask`` (int64 ``[N, W]``, trees of up to 64 W nodes) receives one
+    bit per ancestor and the node's own, ``positions`` (int64 ``[N]``) ``context_lens[b]`` +
+    depth; rows behind the last tree get 0.
+    """
+    _require_cuda(parents)
+    dev = parents.device
+    _ints(dev, torch.int32, "build_tree_metadata: parents, cu_nodes and context_lens", parents, cu_nodes, context_lens,
+          status)
+    _ints(dev, torch.int64, "build_tree_metadata: mask and positions", mask, positions)
+    n, batch = parents.numel(), cu_nodes.numel() - 1
+    if mask.dim() != 2 or mask.shape[0] != n or positions.numel() != n or context_lens.numel() < batch or batch < 0:
+        raise ValueError("build_tree_metadata: mask [N, W], positions [N], context_lens [B], cu_nodes [B + 1]")
+    _call(dev, lib.pkv_build_tree_metadata, "build_tree_metadata", parents.data_ptr(), cu_nodes.data_ptr(), batch,
+          context_lens.data_ptr(), n, mask.data_ptr(), mask.shape[1], positions.data_ptr(), _ptr(status))
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How rotary frequencies are stretched for contexts past the trained length.
+
+    ``linear`` divides every frequency by ``factor``; ``ntk`` raises the base to
+    ``theta * factor^(r / (r - 2))``, which leaves the fastest pair alone and divides the
+    slowest by ``factor``; ``yarn`` divides the pairs that turn less than ``beta_slow`` times
+    over ``original_max_positions``, keeps those that turn more than ``beta_fast`` times,
+    blends linearly between, and multiplies q and k by ``0.1 ln(factor) + 1``.
+    """
+
+    kind: str
+    factor: float
+    original_max_positions: int = 32768
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+
+    def __post_init__(self) -> None:
+        if self.kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"rope scaling must be 'linear', 'ntk' or 'yarn', got {self.kind!r}")
+        if not self.factor >= 1.0 or self.original_max_positions < 1 or not self.beta_fast > self.beta_slow > 0:
+            raise ValueError("rope scaling needs factor >= 1, original_max_positions >= 1, beta_fast > beta_slow > 0")
+
+
+def rotary_frequencies(rotary_dim: int, theta: float, scaling: RopeScaling | None = None,
+                       device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """``(inv_freq, attention_factor)`` of :func:`rotary_append`: float64 ``[rotary_dim / 2]`` on ``device``, a float."""
+    if rotary_dim <= 0 or rotary_dim % 2 or not theta > 0:
+        raise ValueError("rotary_dim must be positive and even, theta positive")
+    pair = torch.arange(rotary_dim // 2, dtype=torch.float64) * 2
+    freq, factor = theta ** (-pair / rotary_dim), 1.0
+    if scaling is not None and scaling.kind == "linear":
+        freq = freq / scaling.factor
+    elif scaling is not None and scaling.kind == "ntk":
+        base = theta * scaling.factor ** (rotary_dim / (rotary_dim - 2)) if rotary_dim > 2 else theta
+        freq = base ** (-pair / rotary_dim)
+    elif scaling is not None:
+        def pair_turning(turns: float) -> float:  # the (fractional) pair that makes `turns` turns over the trained length
+            return rotary_dim * math.log(scaling.original_max_positions / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low = max(math.floor(pair_turning(scaling.beta_fast)), 0)
+        high = min(math.ceil(pair_turning(scaling.beta_slow)), rotary_dim - 1)
+        ramp = ((pair / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq / scaling.factor * ramp + freq * (1 - ramp)
+        factor = 0.1 * math.log(scaling.factor) + 1.0
+    if scaling is not None and scaling.attention_factor is not None:
+        factor = scaling.attention_factor
+    return freq.to(device), factor
+
+
+def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                  num_q_heads: int, interleaved: bool = False, attention_factor: float = 1.0,
+                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | bool = False,
+                  v_out: torch.Tensor | bool = False, slot_mapping: torch.Tensor | None = None,
+                  status: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Rotate the first ``2 * len(inv_freq)`` elements of each q and k head of ``qkv`` rows by ``positions``.
+
+    :func:`rope_append` for the layouts it does not take: pairs side by side
+    (``interleaved``) or half a rotation apart, part of the head, any frequencies
+    (:func:`rotary_frequencies`); angles in float64, one rounding per element. Returns
+    ``(q_out [N, Hq, d], k_out or None, v_out or None)``; ``k_out`` / ``v_out`` are allocated
+    when True, written when tensors. With ``slot_mapping`` (int64 [N], negative = skip) the
+    rotated keys and the values are also written to the pool at ``layer``.
+    """
+    _require_cuda(qkv, positions, inv_freq)
+    dev, dt = qkv.device, qkv.dtype
+    hkv, d = pool.num_kv_heads, pool.head_dim
+    if qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * hkv) * d or qkv.stride(1) != 1:
+        raise ValueError("qkv must be [N, (Hq + 2 Hkv) * head_dim] with a contiguous last dimension")
+    if pkv_dtype(dt) != pool.dtype:
+        raise ValueError("qkv and the pool must share one dtype")
+    n = qkv.shape[0]
+    _ints(dev, torch.int64, "rotary_append: positions and slot_mapping", positions, slot_mapping)
+    _ints(dev, torch.int32, "rotary_append: status", status)
+    _ints(dev, torch.float64, "rotary_append: inv_freq", inv_freq)
+    if positions.numel() != n or (slot_mapping is not None and slot_mapping.numel() != n):
+        raise ValueError("rotary_append: positions and slot_mapping must have one entry per row")
+    if q_out is None:
+        q_out = torch.empty(n, num_q_heads, d, dtype=dt, device=dev)
+    k_out = torch.empty(n, hkv, d, dtype=dt, device=dev) if k_out is True else None if k_out is False else k_out
+    v_out = torch.empty(n, hkv, d, dtype=dt, device=dev) if v_out is True else None if v_out is False else v_out
+    for t, heads in ((q_out, num_q_heads), (k_out, hkv), (v_out, hkv)):
+        if t is not None and (t.shape != (n, heads, d) or t.dtype != dt or t.device != dev or t.stride(2) != 1):
+            raise ValueError("rotary_append: outputs must be [N, heads, head_dim] like qkv, last dimension contiguous")
+    ks, vs = ((t.stride(0), t.stride(1)) if t is not None else (0, 0) for t in (k_out, v_out))
+    _call(dev, lib.pkv_rotary_append, "rotary_append", ctypes.byref(pool), layer, qkv.data_ptr(), qkv.stride(0), n,
+          num_q_heads, positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved),
+          attention_factor, q_out.data_ptr(), q_out.stride(0), q_out.stride(1), _ptr(k_out), *ks, _ptr(v_out), *vs,
+          _ptr(slot_mapping), _ptr(status))
+    return q_out, k_out, v_out
+
+
+def tree_attention_workspace(pool: PkvPool, max_seqs: int, device: torch.device | str) -> torch.Tensor:
+    """A workspace for :func:`tree_attention` of up to ``max_seqs`` sequences (its contents do not matter)."""
+    nbytes = int(lib.pkv_tree_attention_workspace_bytes(max_seqs, pool.head_dim))
+    if nbytes == 0:
+        raise ValueError("tree_attention takes 1 to 1024 sequences and head_dim 64 or 128")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [N, H, d] as rows and heads that start on 16 bytes (a copy only where they do not)."""
+    ok = t.stride(2) == 1 and (t.stride(0) | t.stride(1)) % 8 == 0 and t.data_ptr() % 16 == 0
+    return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor, k_nodes: torch.Tensor,
+                   v_nodes: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch.Tensor, mask: torch.Tensor,
+                   max_nodes: int, workspace: torch.Tensor, out: torch.Tensor | None = None,
+                   scale: float | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted trees' nodes on one layer: q ``[N, Hq, d]`` -> ``[N, Hq, d]``.
+
+    Node ``n`` of sequence ``b`` (nodes ``cu_nodes[b] .. cu_nodes[b + 1] - 1``, at most
+    ``max_nodes`` each) attends to the sequence's ``context_lens[b]`` cached keys in the pool
+    and to the nodes of its tree whose bits are set in ``mask[n]`` (int64 ``[N, W]``,
+    :func:`build_tree_metadata`). The nodes' own keys and values ``[N, Hkv, d]`` (any
+    strides) are not in the pool; :func:`accept_tree` writes the accepted ones there.
+    """
+    _require_cuda(q, k_nodes, v_nodes)
+    dev = q.device
+    n, hq, d = q.shape
+    if d != pool.head_dim or pkv_dtype(q.dtype) != pool.dtype or k_nodes.dtype != q.dtype or v_nodes.dtype != q.dtype:
+        raise ValueError("q, the nodes' keys and values and the pool must share head_dim and dtype")
+    if k_nodes.shape != (n, pool.num_kv_heads, d) or v_nodes.shape != k_nodes.shape:
+        raise ValueError("k_nodes and v_nodes must be [N, kv_heads, head_dim]")
+    if k_nodes.device != dev or v_nodes.device != dev or workspace.device != dev:
+        raise ValueError(f"tree_attention: every tensor must be on {dev}")
+    _ints(dev, torch.int32, "tree_attention: cu_nodes and context_lens", cu_nodes, context_lens, status)
+    _ints(dev, torch.int64, "tree_attention: mask", mask)
+    batch = cu_nodes.numel() - 1
+    if mask.dim() != 2 or mask.shape[0] != n or batch < 0 or context_lens.numel() < batch:
+        raise ValueError("tree_attention: mask [N, W], context_lens [B], cu_nodes [B + 1]")
+    q = _rows_last_contiguous(q)
+    k_nodes, v_nodes = _rows16(k_nodes), _rows16(v_nodes)
+    if out is None:
+        out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+        raise ValueError("out must match q, last dimension contiguous")
+    _call(dev, lib.pkv_tree_attention, "tree_attention", ctypes.byref(pool), layer, ctypes.byref(tables), batch,
+          cu_nodes.data_ptr(), context_lens.data_ptr(), max_nodes, n, hq, out.data_ptr(), out.stride(0), out.stride(1),
+          q.data_ptr(), q.stride(0), q.stride(1), k_nodes.data_ptr(), k_nodes.stride(0), k_nodes.stride(1),
+          v_nodes.data_ptr(), v_nodes.stride(0), v_nodes.stride(1), mask.data_ptr(), mask.shape[1],
+          d ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+          _ptr(status))
+    return out
+
+
+def accept_tree(pool: PkvPool, tables: PkvTables, parents: torch.Tensor, cu_nodes: torch.Tensor,
+                draft_tokens: torch.Tensor, target_tokens: torch.Tensor, k_nodes: torch.Tensor, v_nodes: torch.Tensor,
+                context_lens: torch.Tensor, counts: torch.Tensor, path: torch.Tensor, tokens: torch.Tensor,
+                lengths_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Accept each tree's greedy path and write its K/V of every layer to the cache.
+
+    From node 0 (the last token decided) the path follows the drafted tokens that equal the
+    model's choice: node ``c`` to its lowest child ``j`` with ``draft_tokens[j] ==
+    target_tokens[c]`` (int64 ``[N]``). Written: ``counts`` (int32 ``[B]``, nodes on the path),
+    ``path`` (int32 ``[B, W]``, their indexes), ``tokens`` (int64 ``[B, W]``, their target
+    tokens: the step's new tokens), both -1 behind the path and ``W`` its greatest length;
+    ``lengths_out`` (``context_lens`` itself unless given) = ``context_lens + counts``; and the
+    path's rows of ``k_nodes`` / ``v_nodes`` ``[layers, N, Hkv, d]`` at positions
+    ``context_lens[b] ...`` of the sequence's blocks.
+    """
+    _require_cuda(parents)
+    dev = parents.device
+    n, batch = parents.numel(), cu_nodes.numel() - 1
+    lengths_out = context_lens if lengths_out is None else lengths_out
+    _ints(dev, torch.int32, "accept_tree: parents, cu_nodes, lengths, counts and path", parents, cu_nodes, context_lens,
+          counts, path, lengths_out, status)
+    _ints(dev, torch.int64, "accept_tree: tokens", draft_tokens, target_tokens, tokens)
+    if (draft_tokens.numel() != n or target_tokens.numel() != n or batch < 0 or context_lens.numel() < batch or
+            counts.numel() < batch or lengths_out.numel() < batch or path.dim() != 2 or path.shape != tokens.shape or
+            path.shape[0] < batch):
+        raise ValueError("accept_tree: one token per node, counts and lengths per tree, path and tokens [B, W]")
+    shape = (pool.num_layers, n, pool.num_kv_heads, pool.head_dim)
+    for t in (k_nodes, v_nodes):
+        if t.shape != shape or pkv_dtype(t.dtype) != pool.dtype or t.device != dev or t.stride(3) != 1:
+            raise ValueError("accept_tree: k_nodes and v_nodes must be [layers, N, kv_heads, head_dim] of the pool's dtype")
+    _call(dev, lib.pkv_accept_tree, "accept_tree", ctypes.byref(pool), ctypes.byref(tables), batch, parents.data_ptr(),
+          cu_nodes.data_ptr(), n, draft_tokens.data_ptr(), target_tokens.data_ptr(), k_nodes.data_ptr(),
+          k_nodes.stride(0), k_nodes.stride(1), k_nodes.stride(2), v_nodes.data_ptr(), v_nodes.stride(0),
+          v_nodes.stride(1), v_nodes.stride(2), context_lens.data_ptr(), counts.data_ptr(), path.data_ptr(),
+          tokens.data_ptr(), path.shape[1], lengths_out.data_ptr(), _ptr(status))
+
+
 def build_decode_metadata(tables: PkvTables, lengths: torch.Tensor, block_size: int, scratch_block: int,
                           positions: torch.Tensor, slot_mapping: torch.Tensor, context_lens: torch.Tensor,
                           status: torch.Tensor | None = None) -> None:
@@ -451,6 +716,7 @@ def copy_blocks(pool: PkvPool, src: torch.Tensor, dst: torch.Tensor, status: tor
 
 
 _STATUS_ERRORS = {
+    5: (RuntimeError, "not enough free KV cache blocks"),
     2: (IndexError, "a block id, slot or position on the device was outside the pool or its table"),
     9: (RuntimeError, "a device-side wait timed out"),
 }
