@@ -12,21 +12,25 @@
 // stream (2 * 2 * D bytes per key and KV head) up to a full tile, and the exponentials
 // (one per row and key) for wider trees.
 //
-// Work split. Unit = (sequence, run of context stages of 64 keys, KV head, tile of 128
-// rows); the first run also takes the tree's own keys. Every CTA derives the same split
-// from the lengths on the device: its ten warps try run lengths of 2 .. 128 stages (and
-// whole contexts) and the one with the least cost, waves x (run + overhead), wins; nothing
-// of the plan needs the host to know a length. A sequence left whole writes its output; one
-// cut into several runs leaves per-run states (running maximum, sum, unnormalised output,
-// all float32) that a second small kernel joins. Tiles of one run come next to each other,
-// so that a wide tree's tiles read the same keys from L2 at the same time.
+// Work split. Item = (sequence, KV head, tile of 128 rows), W = ceil(T / 64) + ceil(len / 64)
+// stages of 64 keys (the tree's own first) plus a charge of kItemCost for its start and end.
+// All items are laid end to end and cut into equal ranges, one per CTA, whatever the mix of
+// lengths; every CTA derives the same ranges from the lengths on the device, so nothing of
+// the plan needs the host to know one. An item inside one range writes its output; one cut
+// between ranges leaves its pieces' states (running maximum, sum, unnormalised output, all
+// float32; a range has at most two cut pieces, its first and its last), which a second small
+// kernel joins. Where every tree has the same number of tiles, the tiles of an item go to as
+// many CTAs side by side over the same range of keys, so that they share its reads in L2.
 //
-// Inside a CTA: one warp issues the TMA copies (K and V rings of their own), one thread the
-// tcgen05 MMAs, the others the softmax. S = Q K^T (128 x 64, float32 in TMEM, Q resident in
-// TMEM), P = 2^(S - m) rounded to the storage type over S in its own buffer (two buffers in
-// turn), O += P V in TMEM against a maximum m that moves only when a row's maximum grew by
-// more than 8 (in log2). Rounding P costs each weight half a step of its type, as much as
-// the output's own rounding; the row sum is taken before it, in float32.
+// Inside a CTA: one warp issues the TMA copies (K and V rings of their own). The stages go
+// in turn to kStreams streams, each a warp that issues tcgen05 MMAs and four softmax warps
+// (a row per thread) with a score buffer and an accumulator of its own in TMEM: S = Q K^T
+// (128 x 64, float32, Q resident in TMEM), P = 2^(S - m) rounded to the storage type over S,
+// O += P V against a maximum m that moves only when a row's maximum grew by more than 8 (in
+// log2). While one stream waits for its MMAs another computes exponentials, and no stage
+// waits for another stream's; the streams' states are joined at the end of a piece.
+// Rounding P costs each weight half a step of its type, as much as the output's own
+// rounding; the row sum is taken before it, in float32.
 #include <algorithm>
 
 #include "common.cuh"
@@ -37,34 +41,36 @@ namespace {
 
 constexpr int kBS = 16;
 constexpr int kNK = 64;          // keys per stage
-constexpr int kKS = 4;           // K ring stages
-constexpr int kVS = 4;           // V ring stages
-constexpr int kBars = 2 * (kKS + kVS) + 4;
+constexpr int kStreams = 2;
+constexpr int kRing = 6;         // stages of the K ring and of the V ring
+constexpr int kBars = 4 * kRing + 2 * kStreams + 1;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
-constexpr int kWaves = 2;        // cut units per resident CTA that the workspace has room for
+constexpr int kItemCost = 4;     // an item's start and end, in stages
+constexpr int kMinRange = 6;     // no CTA gets less than this
 constexpr float kLog2e = 1.4426950408889634f;
-// Run lengths (stages) the plan tries; the last leaves every context whole.
-constexpr int kRuns = 20;
-__host__ __device__ constexpr int run_candidate(int i) {
-  constexpr int runs[kRuns] = {2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 40, 48, 64, 96, 128, 1 << 24};
-  return runs[i];
-}
-constexpr int kUnitCost = 4;     // a unit's start and end, in stages
-constexpr int kJoinCost = 4;     // the join and its traffic, in stages
+// Every slot of a ring belongs to one stream, so that a wait sees each of its phases.
+static_assert(kRing % kStreams == 0, "ring slots per stream");
 
 template <int D> struct TreeShape {
   static constexpr int DC = D / 64;             // 64-wide head_dim chunks
   static constexpr int KSB = DC * kNK * 128;    // one stage of K (or V): [DC][64 keys][64], 128B-swizzled
-  // TMEM columns: two S / P buffers, O, Q (packed 16-bit pairs).
-  static constexpr int OCOL = 2 * kNK;
-  static constexpr int QCOL = OCOL + D;
-  static constexpr int NCOLS = QCOL + D / 2 <= 256 ? 256 : 512;
-  static constexpr int MIN_BLOCKS = NCOLS <= 256 ? 2 : 1;
-  static constexpr int SW = MIN_BLOCKS == 2 ? 4 : 8;  // softmax warps: a row, or half a row, per thread
-  static constexpr int HALVES = SW / 4;
-  static constexpr int THREADS = (SW + 2) * 32;
-  static constexpr int SMEM = 1024 + (kKS + kVS) * KSB + (kBars + 2) * 8 + 3 * 2 * 128 * 4 + (3 * kMaxSeqs + 2) * 4;
+  // TMEM columns: a score buffer and an accumulator per stream, Q (packed 16-bit pairs).
+  static constexpr int OCOL = kStreams * kNK;
+  static constexpr int QCOL = OCOL + kStreams * D;
+  static constexpr int NCOLS = 512;
+  static_assert(QCOL + D / 2 <= NCOLS, "TMEM columns");
+  static constexpr int SW = 4 * kStreams;       // softmax warps
+  static constexpr int THREADS = (SW + 1 + kStreams) * 32;
+  static constexpr int SMEM = 1024 + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
+                              (kMaxSeqs + 1) * 8 + 3 * kMaxSeqs * 4;
+};
+
+// What every CTA derives from the lengths, for the join.
+struct TreePlan {
+  int64_t total;   // stages and charges of all items
+  int32_t ranges;  // CTAs (or groups of them) that share them
+  int32_t gang;    // tiles side by side: a group's CTAs; 1 = a tile is an item of its own
 };
 
 struct TreeParams {
@@ -76,19 +82,17 @@ struct TreeParams {
   const int32_t* tables;
   const int32_t* seq_rows;
   int32_t* status;
-  int32_t* plan;       // [0] run length, [1 + b] first unit of sequence b
-  float* part_ml;      // [units][2][128] running maximum and sum
-  float* part_o;       // [units][D][128]
+  TreePlan* plan;
+  int64_t* offsets;    // [batch] where each sequence's items begin
+  float* part_ml;      // [2 per CTA][2][128] running maximum and sum
+  float* part_o;       // [2 per CTA][D][128]
   int64_t out_st, out_sh, q_st, q_sh, table_stride, total_nodes;
-  int32_t table_rows, table_cols, batch, hkv, group, tile_nodes, words, layer, nbt, max_units;
+  int32_t table_rows, table_cols, batch, hkv, group, tile_nodes, words, layer, nbt;
   int32_t q_vec16, out_vec16, max_nodes;
   float scale_log2;
 };
 
 __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// Tiles, context stages and runs of a sequence with n nodes and c cached keys.
-__device__ inline int runs_of(int stages, int run) { return max(1, ceil_div(stages, run)); }
 
 // 4-D bulk tensor copy global -> shared (no multicast), completion on an mbarrier.
 __device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
@@ -100,45 +104,64 @@ __device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c
       : "memory");
 }
 
+// The lengths of sequence b, clamped to what the call's own sizes allow.
+struct SeqLens {
+  int first, nodes, ctx;
+};
+__device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) {
+  SeqLens s;
+  const int lo = p.cu[b], hi = p.cu[b + 1];
+  const int n = p.ctx[b], row = p.seq_rows ? p.seq_rows[b] : b;
+  bool bad = lo < 0 || hi < lo || hi > p.total_nodes || hi - lo > p.max_nodes || n < 0 ||
+             n > (int64_t)p.table_cols * kBS || row >= p.table_rows;
+  s.first = (int)min((int64_t)max(lo, 0), p.total_nodes);
+  s.nodes = min(max((int)min((int64_t)hi, p.total_nodes) - s.first, 0), p.max_nodes);
+  // A padding row has no cached keys.
+  s.ctx = row < 0 || row >= p.table_rows ? 0 : (int)min((int64_t)max(n, 0), (int64_t)p.table_cols * kBS);
+  if (bad) report(status, PKV_ERR_OUT_OF_RANGE);
+  return s;
+}
+__device__ inline int item_cost(int nodes, int ctx) { return kItemCost + ceil_div(nodes, kNK) + ceil_div(ctx, kNK); }
+__device__ inline int64_t range_start(const TreePlan& pl, int64_t g) { return pl.total * g / pl.ranges; }
+// The range that holds position x.
+__device__ inline int range_of(const TreePlan& pl, int64_t x) { return (int)(((x + 1) * pl.ranges - 1) / pl.total); }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(TreeShape<D>::THREADS, TreeShape<D>::MIN_BLOCKS)
+__global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                 const __grid_constant__ CUtensorMap nmap_k, const __grid_constant__ CUtensorMap nmap_v,
                 const TreeParams p) {
   using S = TreeShape<D>;
-  constexpr int DC = S::DC, SW = S::SW, HALVES = S::HALVES;
+  constexpr int DC = S::DC, SW = S::SW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sK = smem;                     // [kKS][KSB]
-  uint8_t* sV = sK + kKS * S::KSB;        // [kVS][KSB]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kVS * S::KSB);
-  uint64_t* k_full = bars;                // [kKS] K landed
-  uint64_t* v_full = k_full + kKS;        // [kVS] V landed
-  uint64_t* s_done = v_full + kVS;        // [kKS] S(j) = Q K(j)^T done: S ready, K stage free
-  uint64_t* o_done = s_done + kKS;        // [kVS] O += P(j) V(j) done: V stage free
-  uint64_t* p_full = o_done + kVS;        // [2] P(j) stored, j even / odd
-  uint64_t* q_ready = p_full + 2;         // Q stored
-  uint64_t* mma_done = q_ready + 1;       // every MMA of the CTA completed
+  uint8_t* sK = smem;                     // [kRing][KSB]
+  uint8_t* sV = sK + kRing * S::KSB;      // [kRing][KSB]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kRing * S::KSB);
+  uint64_t* k_full = bars;                // [kRing] K landed
+  uint64_t* v_full = k_full + kRing;      // [kRing] V landed
+  uint64_t* s_done = v_full + kRing;      // [kRing] S(j) = Q K(j)^T done: S ready, K slot free
+  uint64_t* o_done = s_done + kRing;      // [kRing] O += P(j) V(j) done: V slot and score buffer free
+  uint64_t* p_full = o_done + kRing;      // [kStreams] P stored
+  uint64_t* q_ready = p_full + kStreams;  // [kStreams] Q stored, for a stream with stages in the piece
+  uint64_t* mma_done = q_ready + kStreams;  // every MMA of the CTA completed
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kBars);
-  float* s_mx = reinterpret_cast<float*>(bars + kBars + 2);  // [2 parities][2 halves][128] partial maxima
-  float* s_l = s_mx + 2 * 2 * 128;                           // [2 halves][128] partial sums
-  int32_t* s_cu = reinterpret_cast<int32_t*>(s_l + 2 * 128);  // [batch + 1]
-  int32_t* s_ctx = s_cu + kMaxSeqs + 1;                       // [batch] cached keys
-  int32_t* s_unit = s_ctx + kMaxSeqs;                         // [batch + 1] units before sequence b
-  __shared__ uint64_t s_cost[kRuns];
-  __shared__ int s_warp[16], s_stages;
+  float* s_ml = reinterpret_cast<float*>(bars + kBars + 2);  // [2 parities][kStreams][2][128] maxima and sums
+  int64_t* s_off = reinterpret_cast<int64_t*>(s_ml + 2 * kStreams * 2 * 128);  // [batch + 1] items' begin
+  int32_t* s_first = reinterpret_cast<int32_t*>(s_off + kMaxSeqs + 1);         // [batch] first node
+  int32_t* s_nodes = s_first + kMaxSeqs;                                       // [batch] nodes
+  int32_t* s_ctx = s_nodes + kMaxSeqs;                                         // [batch] cached keys
+  __shared__ int64_t s_warp[32];
+  __shared__ int s_least[32], s_most[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.batch, G = p.group;
 
   grid_dep_launch_dependents();  // the join's CTAs may wait in place
   if (tid == 0) {
-    for (int i = 0; i < kKS; ++i) mbar_init(&k_full[i], 1), mbar_init(&s_done[i], 1);
-    for (int i = 0; i < kVS; ++i) mbar_init(&v_full[i], 1), mbar_init(&o_done[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], SW);
-    mbar_init(q_ready, SW);
-    mbar_init(mma_done, 1);
+    for (int i = 0; i < 4 * kRing; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < kStreams; ++i) mbar_init(&p_full[i], 4), mbar_init(&q_ready[i], SW);
+    mbar_init(mma_done, kStreams);
     fence_mbar_init();
-    s_stages = 0;
   }
   if (warp == 0) {
     tmem_alloc(tslot, S::NCOLS);
@@ -151,124 +174,100 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, TreeShape<D>::MIN_BLOCK
     prefetch_tensormap(&nmap_v);
   }
   // ------------------------------------------------------------------ plan
-  // Lengths, clamped to what the call's own sizes allow (a bad one is reported and its
-  // sequence shortened, so every index below stays in range).
-  for (int b = tid; b <= B; b += S::THREADS) {
-    int c = p.cu[b];
-    if (c < 0 || c > p.total_nodes) {
-      report(p.status, PKV_ERR_OUT_OF_RANGE);
-      c = (int)min((int64_t)max(c, 0), p.total_nodes);
-    }
-    s_cu[b] = c;
-    if (b < B) {
-      int n = p.ctx[b];
-      if (n < 0 || n > (int64_t)p.table_cols * kBS) {
-        report(p.status, PKV_ERR_OUT_OF_RANGE);
-        n = (int)min((int64_t)max(n, 0), (int64_t)p.table_cols * kBS);
+  const int per = ceil_div(B, S::THREADS), b0 = min(B, tid * per), b1 = min(B, b0 + per);
+  TreePlan plan;
+  {
+    int least = 1 << 30, most = 0;
+    for (int b = b0; b < b1; ++b) {
+      const SeqLens s = seq_lens(p, b, blockIdx.x == 0 ? p.status : nullptr);
+      s_first[b] = s.first;
+      s_nodes[b] = s.nodes;
+      s_ctx[b] = s.ctx;
+      if (s.nodes > 0) {
+        const int tiles = ceil_div(s.nodes, p.tile_nodes);
+        least = min(least, tiles);
+        most = max(most, tiles);
       }
-      const int row = p.seq_rows ? p.seq_rows[b] : b;
-      if (row >= p.table_rows) report(p.status, PKV_ERR_OUT_OF_RANGE);
-      if (row < 0 || row >= p.table_rows) n = 0;  // a padding row has no cached keys
-      s_ctx[b] = n;
     }
-  }
-  __syncthreads();
-  auto nodes_of = [&](int b) {
-    const int n = s_cu[b + 1] - s_cu[b];
-    return n < 0 ? 0 : min(n, p.max_nodes);
-  };
-  {
-    int most = 0;
-    for (int b = tid; b < B; b += S::THREADS) {
-      const int n = s_cu[b + 1] - s_cu[b];
-      if (n < 0 || n > p.max_nodes) report(p.status, PKV_ERR_OUT_OF_RANGE);
-      most = max(most, ceil_div(s_ctx[b], kNK));
-    }
+    least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) atomicMax(&s_stages, most);
-  }
-  __syncthreads();
-  const int max_stages = s_stages;
-  for (int c = warp; c < kRuns; c += SW + 2) {
-    const int run = run_candidate(c);
-    int64_t units = 0;
-    for (int b = lane; b < B; b += 32)
-      units += (int64_t)ceil_div(nodes_of(b), p.tile_nodes) * p.hkv * runs_of(ceil_div(s_ctx[b], kNK), run);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-    if (lane == 0) {
-      const bool cut = run < max_stages;
-      const int64_t waves = (units + gridDim.x - 1) / gridDim.x;
-      s_cost[c] = cut && units > p.max_units ? ~0ull  // more states than the workspace holds
-                                             : waves * (min(run, max_stages) + kUnitCost) + (cut ? kJoinCost : 0);
-    }
-  }
-  __syncthreads();
-  int best = 0;
-#pragma unroll
-  for (int c = 1; c < kRuns; ++c)
-    if (s_cost[c] < s_cost[best]) best = c;
-  const int run = run_candidate(best);
-  // Units before each sequence: a scan over the CTA, a few sequences per thread.
-  {
-    const int per = ceil_div(B, S::THREADS), b0 = min(B, tid * per), b1 = min(B, b0 + per);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b)
-      mine += ceil_div(nodes_of(b), p.tile_nodes) * p.hkv * runs_of(ceil_div(s_ctx[b], kNK), run);
-    int inc = mine;
+    if (lane == 0) s_least[warp] = least, s_most[warp] = most;
+    __syncthreads();
+    for (int w = 0; w < S::THREADS / 32; ++w) least = min(least, s_least[w]), most = max(most, s_most[w]);
+    plan.gang = least == most && most <= (int)gridDim.x ? most : 1;
+    auto cost_of = [&](int b) -> int64_t {
+      const int n = s_nodes[b];
+      if (n == 0) return 0;
+      return (int64_t)p.hkv * (plan.gang > 1 ? 1 : ceil_div(n, p.tile_nodes)) * item_cost(n, s_ctx[b]);
+    };
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += cost_of(b);
+    int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    int before = inc - mine;
-    for (int w = 0; w < warp; ++w) before += s_warp[w];
-    for (int b = b0; b < b1; ++b) {
-      s_unit[b] = before;
-      if (blockIdx.x == 0) p.plan[1 + b] = before;
-      before += ceil_div(nodes_of(b), p.tile_nodes) * p.hkv * runs_of(ceil_div(s_ctx[b], kNK), run);
+    int64_t before = inc - mine;
+    plan.total = 0;
+    for (int w = 0; w < S::THREADS / 32; ++w) {
+      if (w < warp) before += s_warp[w];
+      plan.total += s_warp[w];
     }
-    if (b1 == B && b0 < B) s_unit[B] = before;
-    if (blockIdx.x == 0 && tid == 0) p.plan[0] = run;
+    for (int b = b0; b < b1; ++b) {
+      s_off[b] = before;
+      if (blockIdx.x == 0) p.offsets[b] = before;
+      before += cost_of(b);
+    }
+    plan.ranges = (int)max((int64_t)1, min((int64_t)(gridDim.x / max(plan.gang, 1)), plan.total / kMinRange));
+    if (blockIdx.x == 0 && tid == 0) *p.plan = plan;
   }
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tslot;
   const uint64_t deadline = global_ns() + kWaitBudgetNs;
-  auto s_col = [](int b) { return (uint32_t)(b * kNK); };
-  const int n_units = s_unit[B];
+  const int gang = max(plan.gang, 1), range = blockIdx.x / gang, member = blockIdx.x % gang;
+  const int64_t pos0 = range < plan.ranges ? range_start(plan, range) : 0;
+  const int64_t pos_end = range < plan.ranges ? range_start(plan, range + 1) : 0;
 
-  // Every role walks the same units and numbers stages across them, so ring slots and
-  // barrier parities continue from one unit to the next.
-  struct Unit {
-    int b, head, tile, rows, n, ctx, first, nst, nns;  // nns: leading stages of the tree's own keys
-    bool cut;
+  // Every role walks the same pieces and numbers stages across them, so ring slots and
+  // barrier parities continue from one piece to the next.
+  struct Piece {
+    int b, head, tile, rows, nodes, ctx, nns;  // nns: the item's stages of the tree's own keys, its first
+    int s0, nst;                               // first stage, stages
+    bool begins, ends;
   };
-  auto unit_at = [&](int w) {
-    Unit u;
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_unit[mid] <= w) lo = mid; else hi = mid - 1;
+  auto next_piece = [&](int64_t& pos, Piece& u) -> bool {
+    while (pos < pos_end) {
+      int lo = 0, hi = B - 1;  // the last sequence that begins at or before pos (empty ones take no room)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_off[mid] <= pos) lo = mid; else hi = mid - 1;
+      }
+      u.b = lo;
+      u.nodes = s_nodes[lo];
+      u.ctx = s_ctx[lo];
+      const int cost = item_cost(u.nodes, u.ctx), tiles = ceil_div(u.nodes, p.tile_nodes);
+      const int64_t rel = pos - s_off[lo];
+      const int item = (int)(rel / cost), x0 = (int)(rel - (int64_t)item * cost);
+      const int x1 = (int)min((int64_t)cost, x0 + (pos_end - pos));
+      pos += x1 - x0;
+      u.s0 = max(0, x0 - kItemCost);
+      u.nst = max(0, x1 - kItemCost) - u.s0;
+      if (u.nst <= 0) continue;
+      u.head = plan.gang > 1 ? item : item / tiles;
+      u.tile = plan.gang > 1 ? member : item % tiles;
+      u.rows = min(p.tile_nodes, u.nodes - u.tile * p.tile_nodes) * G;
+      u.nns = ceil_div(u.nodes, kNK);
+      u.begins = u.s0 == 0;
+      u.ends = x1 == cost;
+      return true;
     }
-    u.b = lo;
-    u.n = nodes_of(lo);
-    u.ctx = s_ctx[lo];
-    const int tiles = ceil_div(u.n, p.tile_nodes), cst = ceil_div(u.ctx, kNK), ch = runs_of(cst, run);
-    int r = w - s_unit[lo];
-    u.tile = r % tiles;
-    r /= tiles;
-    u.head = r % p.hkv;
-    const int k = r / p.hkv;
-    u.rows = min(p.tile_nodes, u.n - u.tile * p.tile_nodes) * G;
-    u.first = (int)((int64_t)k * cst / ch);
-    u.nns = k == 0 ? ceil_div(u.n, kNK) : 0;
-    u.nst = u.nns + (int)((int64_t)(k + 1) * cst / ch) - u.first;
-    u.cut = ch > 1;
-    return u;
+    return false;
   };
+  auto first_of = [](int stream, int gs) { return (stream + kStreams - gs % kStreams) % kStreams; };  // its first stage
 
   if (warp == SW) {
     // ---------------------------------------------------------------- TMA copies
@@ -276,11 +275,13 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, TreeShape<D>::MIN_BLOCK
     const int bl = lane / DC, c = lane % DC;
     bool ok = true;
     int gs = 0;
-    for (int w = blockIdx.x; w < n_units && ok; w += gridDim.x) {
-      const Unit u = unit_at(w);
-      int row = p.seq_rows ? p.seq_rows[u.b] : u.b;
+    Piece u;
+    for (int64_t pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
+      const int row = p.seq_rows ? p.seq_rows[u.b] : u.b;
       const int32_t* table = row >= 0 && row < p.table_rows ? p.tables + (int64_t)row * p.table_stride : nullptr;
-      const int nkb = ceil_div(u.ctx, kBS), kb0 = u.first * (kNK / kBS);
+      const int nkb = ceil_div(u.ctx, kBS);
+      const int own = max(0, u.nns - u.s0);                          // leading stages of the tree's own keys
+      const int kb0 = max(0, u.s0 - u.nns) * (kNK / kBS);
       auto lookup = [&](int kb) -> int {  // blocks past the sequence: masked, any block will do
         int blk = kb < nkb && table ? table[kb] : p.nbt - 1;
         if (blk < 0 || blk >= p.nbt) {
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, TreeShape<D>::MIN_BLOCK
       constexpr int kPerWindow = 32 / (kNK / kBS);  // stages per window of 32 block ids
       int win = lookup(kb0 + lane), win_next = lookup(kb0 + 32 + lane);
       for (int i = 0; i < u.nst && ok; ++i) {
-        const int ci = i - u.nns;  // context stage of the unit
+        const int ci = i - own;  // context stage of the piece
         int blk = 0;
         if (ci >= 0) {
           if (ci > 0 && ci % kPerWindow == 0) {
@@ -301,263 +302,283 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, TreeShape<D>::MIN_BLOCK
           }
           blk = __shfl_sync(0xffffffffu, win, (ci * (kNK / kBS) + bl) % 32);
         }
-        const int c4 = p.layer * p.nbt + blk, j = gs + i, sk = j % kKS, sv = j % kVS;
-        const int node = s_cu[u.b] + i * kNK;
-        if (lane == 0) {
-          if (j >= kKS && !mbar_wait_until(&s_done[sk], ((j / kKS) - 1) & 1, deadline)) {
-            report(p.status, PKV_ERR_TIMEOUT);
-            ok = false;
+        const int c4 = p.layer * p.nbt + blk, j = gs + i, st = j % kRing;
+        const int node = s_first[u.b] + (u.s0 + i) * kNK;
+        auto wait_free = [&](uint64_t* bar, uint64_t* full) {
+          if (lane == 0 && ok) {
+            if (j >= kRing && !mbar_wait_until(&bar[st], ((j / kRing) - 1) & 1, deadline)) {
+              report(p.status, PKV_ERR_TIMEOUT);
+              ok = false;
+            }
+            if (ok) mbar_arrive_expect_tx(&full[st], S::KSB);
           }
-          if (ok) mbar_arrive_expect_tx(&k_full[sk], S::KSB);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+        };
+        wait_free(s_done, k_full);
         if (ok && ci >= 0 && lane < kCopies)
-          tma_load_5d(sK + sk * S::KSB + c * kNK * 128 + bl * kBS * 128, &tmap_k, 0, 0, c, u.head, c4, &k_full[sk]);
-        if (ok && ci < 0 && lane < DC) tma_load_4d(sK + sk * S::KSB + lane * kNK * 128, &nmap_k, 0, lane, u.head, node, &k_full[sk]);
-        if (lane == 0 && ok) {
-          if (j >= kVS && !mbar_wait_until(&o_done[sv], ((j / kVS) - 1) & 1, deadline)) {
-            report(p.status, PKV_ERR_TIMEOUT);
-            ok = false;
-          }
-          if (ok) mbar_arrive_expect_tx(&v_full[sv], S::KSB);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+          tma_load_5d(sK + st * S::KSB + c * kNK * 128 + bl * kBS * 128, &tmap_k, 0, 0, c, u.head, c4, &k_full[st]);
+        if (ok && ci < 0 && lane < DC)
+          tma_load_4d(sK + st * S::KSB + lane * kNK * 128, &nmap_k, 0, lane, u.head, node, &k_full[st]);
+        wait_free(o_done, v_full);
         if (ok && ci >= 0 && lane < kCopies)
-          tma_load_5d(sV + sv * S::KSB + c * kNK * 128 + bl * kBS * 128, &tmap_v, 0, 0, c, u.head, c4, &v_full[sv]);
-        if (ok && ci < 0 && lane < DC) tma_load_4d(sV + sv * S::KSB + lane * kNK * 128, &nmap_v, 0, lane, u.head, node, &v_full[sv]);
+          tma_load_5d(sV + st * S::KSB + c * kNK * 128 + bl * kBS * 128, &tmap_v, 0, 0, c, u.head, c4, &v_full[st]);
+        if (ok && ci < 0 && lane < DC)
+          tma_load_4d(sV + st * S::KSB + lane * kNK * 128, &nmap_v, 0, lane, u.head, node, &v_full[st]);
       }
-      gs += u.nst;
     }
-  } else if (warp == SW + 1) {
-    // ---------------------------------------------------------------- MMA issue
+  } else if (warp > SW) {
+    // ---------------------------------------------------------------- MMA issue, one warp per stream
     if (lane == 0) {
+      const int stream = warp - SW - 1;
       constexpr bool kBf16 = Dt<T>::code == PKV_BF16;
       constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, false, 128, kNK);
       constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, true, 128, D);
+      const uint32_t ts = tmem + stream * kNK, to = tmem + S::OCOL + stream * D;
+      // Descriptors are computed before the waits, so that the MMAs issue back to back.
       auto pin = [](uint64_t& x) { asm volatile("" : "+l"(x)); };
-      auto issue_s = [&](int j, bool after_o) -> bool {  // S(j) into buffer j % 2, over P(j - 2)
-        const int st = j % kKS, b = j % 2;
+      auto issue_s = [&](int j) -> bool {
+        const int st = j % kRing;
         uint64_t bk[D / 16];
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           bk[kk] = umma_desc_sw128(smem_u32(sK + st * S::KSB + (kk / 4) * kNK * 128 + (kk % 4) * 32), 16, 1024);
           pin(bk[kk]);
         }
-        if (!mbar_wait_until(&k_full[st], (j / kKS) & 1, deadline)) return false;
-        if (after_o && !mbar_wait_until(&o_done[(j - 2) % kVS], ((j - 2) / kVS) & 1, deadline)) return false;
+        if (!mbar_wait_until(&k_full[st], (j / kRing) & 1, deadline)) return false;
+        // The score buffer still holds P(j - kStreams) of this piece until its O has read it.
         tc_fence_after_sync();
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16_ts(tmem + s_col(b), tmem + S::QCOL + kk * 8, bk[kk], idesc_s, kk > 0);
+        for (int kk = 0; kk < D / 16; ++kk) umma_f16_ts(ts, tmem + S::QCOL + kk * 8, bk[kk], idesc_s, kk > 0);
         umma_commit(&s_done[st]);
         return true;
       };
       auto issue_o = [&](int j, bool first) -> bool {
-        const int st = j % kVS, b = j % 2;
+        const int st = j % kRing;
         uint64_t bv[kNK / 16];
 #pragma unroll
         for (int kb = 0; kb < kNK / 16; ++kb) {
           bv[kb] = umma_desc_sw128(smem_u32(sV + st * S::KSB + kb * 16 * 128), kNK * 128, 1024);
           pin(bv[kb]);
         }
-        if (!mbar_wait_until(&p_full[b], (j / 2) & 1, deadline)) return false;
-        if (!mbar_wait_until(&v_full[st], (j / kVS) & 1, deadline)) return false;
+        if (!mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) return false;
+        if (!mbar_wait_until(&p_full[stream], (j / kStreams) & 1, deadline)) return false;
         tc_fence_after_sync();
 #pragma unroll
-        for (int kb = 0; kb < kNK / 16; ++kb)
-          umma_f16_ts(tmem + S::OCOL, tmem + s_col(b) + kb * 8, bv[kb], idesc_o, !first || kb > 0);
+        for (int kb = 0; kb < kNK / 16; ++kb) umma_f16_ts(to, ts + kb * 8, bv[kb], idesc_o, !first || kb > 0);
         umma_commit(&o_done[st]);
         return true;
       };
       bool ok = true;
       int gs = 0, k = 0;
-      for (int w = blockIdx.x; w < n_units && ok; w += gridDim.x, ++k) {
-        const int nst = unit_at(w).nst;
-        ok = mbar_wait_until(q_ready, k & 1, deadline) && issue_s(gs, false) && (nst < 2 || issue_s(gs + 1, false));
-        for (int i = 0; i < nst && ok; ++i) ok = issue_o(gs + i, i == 0) && (i + 2 >= nst || issue_s(gs + i + 2, true));
-        gs += nst;
+      Piece u;
+      for (int64_t pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
+        const int i0 = first_of(stream, gs);
+        if (i0 >= u.nst) continue;
+        ok = mbar_wait_until(&q_ready[stream], k++ & 1, deadline) && issue_s(gs + i0);
+        for (int i = i0; i < u.nst && ok; i += kStreams) {
+          const int j = gs + i;
+          ok = issue_o(j, i == i0) &&
+               (i + kStreams >= u.nst ||
+                (mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline) && issue_s(j + kStreams)));
+        }
       }
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       if (k > 0) umma_commit(mma_done); else mbar_arrive(mma_done);
     }
   } else {
     // ---------------------------------------------------------------- softmax warps
-    constexpr int KH = kNK / HALVES, DH = D / HALVES;
-    const int hf = warp / 4;
+    const int stream = warp / 4;
     const int r = (warp % 4) * 32 + lane;  // TMEM lane = tile row
     const int t = r / G, gq = r - t * G;   // node of the tile, query head of the group
     const uint32_t tl = tmem + ((uint32_t)((warp % 4) * 32) << 16);
-    const int pair_bar = 1 + warp % 4;     // the two warps of a row
+    const uint32_t ts = tl + stream * kNK, to = tl + S::OCOL + stream * D;
     constexpr float kSlack = 8.f;
     bool ok = true;
-    auto confirm = [&](int j) {
-      if (ok && !mbar_wait_until(&o_done[j % kVS], (j / kVS) & 1, deadline)) ok = false;
+    auto confirm = [&](int j) {  // O += P(j) V(j) has completed
+      if (ok && !mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline)) ok = false;
     };
-    int gs = 0;
-    for (int w = blockIdx.x; w < n_units; w += gridDim.x) {
-      const Unit u = unit_at(w);
-      const int nst = u.nst;
+    int gs = 0, k = 0;
+    Piece u;
+    for (int64_t pos = pos0; next_piece(pos, u); gs += u.nst, ++k) {
       const bool valid = r < u.rows;
       const bool live = (warp % 4) * 32 < u.rows;  // some row of the warp has a query
-      const int64_t node = (int64_t)s_cu[u.b] + u.tile * p.tile_nodes + t;
-      {
-        const T* qrow = reinterpret_cast<const T*>(p.q) + node * p.q_st + (int64_t)(u.head * G + gq) * p.q_sh + hf * DH;
-#pragma unroll
-        for (int c = 0; c < DH / 32; ++c) {
+      const int64_t node = (int64_t)s_first[u.b] + u.tile * p.tile_nodes + t;
+      {  // Q: each stream's warps store their share of the columns
+        const T* qrow = reinterpret_cast<const T*>(p.q) + node * p.q_st + (int64_t)(u.head * G + gq) * p.q_sh;
+        for (int c = stream; c < D / 32; c += kStreams) {
           uint32_t qv[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int x = 0; x < 4; ++x) {
             uint4 v = make_uint4(0, 0, 0, 0);
             if (valid) {
               if (p.q_vec16) {
-                v = *reinterpret_cast<const uint4*>(qrow + c * 32 + 8 * k);
+                v = *reinterpret_cast<const uint4*>(qrow + c * 32 + 8 * x);
               } else {
-                const uint32_t* q32 = reinterpret_cast<const uint32_t*>(qrow + c * 32 + 8 * k);
+                const uint32_t* q32 = reinterpret_cast<const uint32_t*>(qrow + c * 32 + 8 * x);
                 v = make_uint4(q32[0], q32[1], q32[2], q32[3]);
               }
             }
-            qv[4 * k] = v.x, qv[4 * k + 1] = v.y, qv[4 * k + 2] = v.z, qv[4 * k + 3] = v.w;
+            qv[4 * x] = v.x, qv[4 * x + 1] = v.y, qv[4 * x + 2] = v.z, qv[4 * x + 3] = v.w;
           }
-          tmem_st16(tl + S::QCOL + hf * (DH / 2) + c * 16, qv);
+          tmem_st16(tl + S::QCOL + c * 16, qv);
         }
       }
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
+      if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < kStreams; ++s)
+          if (first_of(s, gs) < u.nst) mbar_arrive(&q_ready[s]);
+      }
 
       float m = -INFINITY, l = 0.f;
-      for (int i = 0; i < nst; ++i) {
-        const int j = gs + i, b = j % 2;
-        const bool own = i < u.nns;  // the tree's own keys
-        const int keys = own ? u.n - i * kNK : u.ctx - (u.first + i - u.nns) * kNK;  // keys of the stage, if < kNK
+      const int i0 = first_of(stream, gs);
+      for (int i = i0; i < u.nst; i += kStreams) {
+        const int j = gs + i, sg = u.s0 + i, st = j % kRing;
+        const bool own = sg < u.nns;  // the tree's own keys
+        const int keys = own ? u.nodes - sg * kNK : u.ctx - (sg - u.nns) * kNK;  // of the stage, if < kNK
         uint64_t see = ~0ull;
-        if (own) see = valid ? p.mask[node * p.words + i] : 0;
+        if (own) see = valid ? p.mask[node * p.words + sg] : 0;
         if (keys < kNK) see &= (1ull << keys) - 1;
-        if (ok && !mbar_wait_until(&s_done[j % kKS], (j / kKS) & 1, deadline)) ok = false;
+        if (ok && !mbar_wait_until(&s_done[st], (j / kRing) & 1, deadline)) ok = false;
         tc_fence_after_sync();
         // Rows of V past the sequence or the tree hold whatever was there, infinities and NaN
         // included: 0 x NaN would reach the output, so they are cleared in place.
         if (keys < kNK) {
-          const int st = j % kVS;
-          if (ok && !mbar_wait_until(&v_full[st], (j / kVS) & 1, deadline)) ok = false;
-          for (int x = tid; x < (kNK - keys) * DC * 8; x += SW * 32) {
-            const int c = x / ((kNK - keys) * 8), y = x - c * (kNK - keys) * 8;
+          if (ok && !mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) ok = false;
+          const int gap = (kNK - keys) * 8;
+          for (int x = r; x < gap * DC; x += 128) {
+            const int c = x / gap, y = x - c * gap;
             *reinterpret_cast<uint4*>(sV + st * S::KSB + c * kNK * 128 + keys * 128 + y * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
         if (live) {
-          uint32_t sa[KH];
+          uint32_t sa[kNK];
 #pragma unroll
-          for (int c = 0; c < KH / 32; ++c)
-            tmem_ld32(tl + s_col(b) + hf * KH + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sa + c * 32));
+          for (int c = 0; c < kNK / 32; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sa + c * 32));
           tmem_wait_ld();
           if (own || keys < kNK) {
-            const uint32_t lo32 = (uint32_t)(see >> (hf * KH)), hi32 = KH > 32 ? (uint32_t)(see >> 32) : 0;
+            const uint32_t lo32 = (uint32_t)see, hi32 = (uint32_t)(see >> 32);
 #pragma unroll
-            for (int e = 0; e < KH; ++e)
-              if (!((e < 32 ? lo32 >> (e & 31) : hi32 >> (e & 31)) & 1)) sa[e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < kNK; ++e)
+              if (!(((e < 32 ? lo32 : hi32) >> (e & 31)) & 1)) sa[e] = __float_as_uint(-INFINITY);
           }
-          float mt[KH / 2];
+          float mt[4];
 #pragma unroll
-          for (int e = 0; e < KH / 2; ++e) mt[e] = fmaxf(__uint_as_float(sa[e]), __uint_as_float(sa[e + KH / 2]));
+          for (int e = 0; e < 4; ++e) mt[e] = fmaxf(__uint_as_float(sa[e]), __uint_as_float(sa[e + 4]));
 #pragma unroll
-          for (int x = KH / 4; x > 0; x >>= 1) {
+          for (int e = 8; e < kNK; e += 8) {
 #pragma unroll
-            for (int e = 0; e < x; ++e) mt[e] = fmaxf(mt[e], mt[e + x]);
+            for (int x = 0; x < 4; ++x)
+              mt[x] = fmaxf(fmaxf(mt[x], __uint_as_float(sa[e + x])), __uint_as_float(sa[e + 4 + x]));
           }
-          float mx = mt[0] * p.scale_log2;
-          if (HALVES == 2) {
-            float* mxb = s_mx + (j % 2) * 256;
-            mxb[hf * 128 + r] = mx;
-            named_barrier_sync(pair_bar, 64);
-            mx = fmaxf(mx, mxb[(1 - hf) * 128 + r]);
-          }
+          const float mx = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])) * p.scale_log2;
           const float m_cand = fmaxf(m, mx);
           float alpha = 1.f;
-          if (m_cand - m > kSlack) {
+          if (m_cand - m > kSlack) {  // false while both are -inf
             alpha = ex2(m - m_cand);
             m = m_cand;
             l *= alpha;
           }
-          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            confirm(j - 1);
+          if (i > i0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            confirm(j - kStreams);
             tc_fence_after_sync();
 #pragma unroll
-            for (int c = 0; c < DH / 32; ++c) {
+            for (int c = 0; c < D / 32; ++c) {
               uint32_t ob[32];
-              tmem_ld32(tl + S::OCOL + hf * DH + c * 32, ob);
+              tmem_ld32(to + c * 32, ob);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * alpha);
-              tmem_st32(tl + S::OCOL + hf * DH + c * 32, ob);
+              tmem_st32(to + c * 32, ob);
             }
           }
           const float mref = m == -INFINITY ? 0.f : m;
           float2 lsum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), negm2 = make_float2(-mref, -mref);
-          uint32_t pk[KH / 2];
-#pragma unroll
-          for (int e = 0; e < KH; e += 2) {
-            const float2 x = ffma2(make_float2(__uint_as_float(sa[e]), __uint_as_float(sa[e + 1])), scale2, negm2);
-            const float p0 = ex2(x.x), p1 = ex2(x.y);
-            pk[e / 2] = Dt<T>::pack(p0, p1);
-            lsum[(e / 2) % 2] = fadd2(lsum[(e / 2) % 2], make_float2(p0, p1));
-          }
           tc_fence_after_sync();
 #pragma unroll
-          for (int c = 0; c < KH / 32; ++c)
-            tmem_st16(tl + s_col(b) + hf * (KH / 2) + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(pk + c * 16));
+          for (int c = 0; c < kNK / 32; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 x = ffma2(make_float2(__uint_as_float(sa[c * 32 + e]), __uint_as_float(sa[c * 32 + e + 1])), scale2,
+                                     negm2);
+              const float p0 = ex2(x.x), p1 = ex2(x.y);
+              pk[e / 2] = Dt<T>::pack(p0, p1);
+              lsum[(e / 2) % 2] = fadd2(lsum[(e / 2) % 2], make_float2(p0, p1));
+            }
+            tmem_st16(ts + c * 16, pk);
+          }
           tmem_wait_st();
           l += (lsum[0].x + lsum[1].x) + (lsum[0].y + lsum[1].y);
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) mbar_arrive(&p_full[stream]);
       }
-      confirm(gs + nst - 1);
+      // The piece's streams joined: maxima and sums through shared memory, then each stream's
+      // warps take their share of the output columns from every accumulator.
+      if (i0 < u.nst) confirm(gs + (u.nst - 1 - i0) / kStreams * kStreams + i0);
+      float* ml = s_ml + (k & 1) * kStreams * 256;
+      ml[stream * 256 + r] = m;
+      ml[stream * 256 + 128 + r] = l;
+      tc_fence_before_sync();
+      named_barrier_sync(1, SW * 32);
       tc_fence_after_sync();
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       if (live) {
-        if (HALVES == 2) {
-          s_l[hf * 128 + r] = l;
-          named_barrier_sync(pair_bar, 64);
-          l += s_l[(1 - hf) * 128 + r];
-        }
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // no visible key: zeros
-        T* orow = reinterpret_cast<T*>(p.out) + node * p.out_st + (int64_t)(u.head * G + gq) * p.out_sh + hf * DH;
-        if (u.cut && hf == 0 && ok) {
-          p.part_ml[(int64_t)w * 256 + r] = m;
-          p.part_ml[(int64_t)w * 256 + 128 + r] = l;
-        }
+        float top = -INFINITY, sum = 0.f, wgt[kStreams];
 #pragma unroll
-        for (int c = 0; c < DH / 32; ++c) {
-          uint32_t ob[32];
-          tmem_ld32(tl + S::OCOL + hf * DH + c * 32, ob);
-          tmem_wait_ld();
-          if (u.cut) {
-            if (valid && ok) {
-              float* po = p.part_o + ((int64_t)w * D + hf * DH + c * 32) * 128 + r;
+        for (int s = 0; s < kStreams; ++s) top = fmaxf(top, ml[s * 256 + r]);
+        const float mref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) po[e * 128] = __uint_as_float(ob[e]);
-            }
-          } else if (valid && ok) {
-            auto pack = [&](int e) {
-              return Dt<T>::pack(__uint_as_float(ob[e]) * inv, __uint_as_float(ob[e + 1]) * inv);
-            };
+        for (int s = 0; s < kStreams; ++s) {
+          wgt[s] = ex2(ml[s * 256 + r] - mref);
+          sum += wgt[s] * ml[s * 256 + 128 + r];
+        }
+        const bool cut = !(u.begins && u.ends);
+        const int64_t slot = 2 * (int64_t)blockIdx.x + u.begins;
+        if (cut && stream == 0) {
+          p.part_ml[slot * 256 + r] = top;
+          p.part_ml[slot * 256 + 128 + r] = sum;
+        }
+        const float inv = cut ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // no visible key: zeros
+        T* orow = reinterpret_cast<T*>(p.out) + node * p.out_st + (int64_t)(u.head * G + gq) * p.out_sh;
+        for (int c = stream; c < D / 16; c += kStreams) {
+          float acc[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+          for (int s = 0; s < kStreams; ++s) {
+            if (first_of(s, gs) >= u.nst) continue;  // its accumulator holds nothing of this piece
+            uint32_t ob[16];
+            tmem_ld16(tl + S::OCOL + s * D + c * 16, ob);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] += wgt[s] * __uint_as_float(ob[e]);
+          }
+          if (!valid || !ok) continue;
+          if (cut) {
+            float* po = p.part_o + (slot * D + c * 16) * 128 + r;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) po[e * 128] = acc[e];
+          } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = Dt<T>::pack(acc[2 * e] * inv, acc[2 * e + 1] * inv);
             if (p.out_vec16) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                *reinterpret_cast<uint4*>(orow + c * 32 + e) = make_uint4(pack(e), pack(e + 2), pack(e + 4), pack(e + 6));
+              *reinterpret_cast<uint4*>(orow + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(orow + c * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) *reinterpret_cast<uint32_t*>(orow + c * 32 + e) = pack(e);
+              for (int e = 0; e < 8; ++e) reinterpret_cast<uint32_t*>(orow + c * 16)[e] = w[e];
             }
           }
         }
       }
-      gs += nst;
     }
   }
   __syncthreads();
@@ -568,40 +589,35 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, TreeShape<D>::MIN_BLOCK
   }
 }
 
-// Joins the runs of a cut sequence: with M the largest of their maxima,
+// Joins the pieces of a cut item: with M the largest of their maxima,
 //   out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// One CTA per (8 output columns x 8, tile, KV head, sequence); a thread takes one row and
+// One CTA per (64 output columns, tile, KV head, sequence); a thread takes one row and
 // eight columns, so the states are read a row to a lane, and its output is one 16-byte write.
-constexpr int kJoinCols = 64;  // columns of a CTA: 8 threads' eight
+constexpr int kJoinCols = 64;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const TreeParams p) {
-  grid_dep_wait();
-  const int run = p.plan[0];
   const int b = blockIdx.z, head = blockIdx.y;
   const int tile = blockIdx.x / (D / kJoinCols), part = blockIdx.x % (D / kJoinCols);
-  int ctx = p.ctx[b];
-  ctx = min(max(ctx, 0), p.table_cols * kBS);
-  const int row = p.seq_rows ? p.seq_rows[b] : b;
-  if (row < 0 || row >= p.table_rows) ctx = 0;
-  const int ch = runs_of(ceil_div(ctx, kNK), run);
-  if (ch == 1) return;
-  const int64_t total = p.total_nodes;
-  const int lo = (int)min(max((int64_t)p.cu[b], (int64_t)0), total);
-  const int hi = (int)min(max((int64_t)p.cu[b + 1], (int64_t)0), total);
-  const int n = hi < lo ? 0 : min(hi - lo, p.max_nodes);
-  const int tiles = ceil_div(n, p.tile_nodes);
+  const SeqLens s = seq_lens(p, b, nullptr);
+  const int tiles = ceil_div(s.nodes, p.tile_nodes);
   const int r = threadIdx.x % 128, c0 = part * kJoinCols + (threadIdx.x / 128) * 8;
-  if (tile >= tiles || r >= min(p.tile_nodes, n - tile * p.tile_nodes) * p.group) return;
-  const int64_t step = (int64_t)p.hkv * tiles;
-  const int64_t u0 = p.plan[1 + b] + (int64_t)head * tiles + tile;
+  grid_dep_wait();
+  if (tile >= tiles) return;
+  const TreePlan plan = *p.plan;
+  const int cost = item_cost(s.nodes, s.ctx);
+  const int64_t begin = p.offsets[b] + (int64_t)(plan.gang > 1 ? head : head * tiles + tile) * cost + kItemCost;
+  const int g0 = range_of(plan, begin), pieces = range_of(plan, begin + cost - kItemCost - 1) - g0 + 1;
+  if (pieces == 1 || r >= min(p.tile_nodes, s.nodes - tile * p.tile_nodes) * p.group) return;
+  const int gang = plan.gang, member = gang > 1 ? tile : 0;
+  auto slot = [&](int k) { return 2 * ((int64_t)(g0 + k) * gang + member) + (k == 0); };
   float top = -INFINITY;
-  for (int k = 0; k < ch; ++k) top = fmaxf(top, p.part_ml[(u0 + k * step) * 256 + r]);
+  for (int k = 0; k < pieces; ++k) top = fmaxf(top, p.part_ml[slot(k) * 256 + r]);
   const float mref = top == -INFINITY ? 0.f : top;
   float sum = 0.f, acc[8] = {};
 #pragma unroll 2
-  for (int k = 0; k < ch; ++k) {
-    const int64_t u = u0 + k * step;
+  for (int k = 0; k < pieces; ++k) {
+    const int64_t u = slot(k);
     const float wgt = ex2(p.part_ml[u * 256 + r] - mref);
     sum += wgt * p.part_ml[u * 256 + 128 + r];
     const float* o = p.part_o + (u * D + c0) * 128 + r;
@@ -610,7 +626,7 @@ __global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const 
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   const int t = r / p.group, gq = r - t * p.group;
-  T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)lo + tile * p.tile_nodes + t) * p.out_st +
+  T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)s.first + tile * p.tile_nodes + t) * p.out_st +
             (int64_t)(head * p.group + gq) * p.out_sh + c0;
   uint32_t w[4];
 #pragma unroll
@@ -623,8 +639,8 @@ __global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const 
   }
 }
 
-int64_t plan_bytes(int batch) { return ((int64_t)(batch + 1) * 4 + 255) / 256 * 256; }
-int resident(int d) { return num_sms() * (d == 64 ? TreeShape<64>::MIN_BLOCKS : TreeShape<128>::MIN_BLOCKS); }
+// The plan, then every sequence's offset.
+int64_t plan_bytes(int batch) { return (256 + (int64_t)batch * 8 + 255) / 256 * 256; }
 
 template <typename T, int D>
 int launch(const CUtensorMap (&maps)[4], const TreeParams& p, cudaStream_t st) {
@@ -632,7 +648,7 @@ int launch(const CUtensorMap (&maps)[4], const TreeParams& p, cudaStream_t st) {
   static SmemAttribute attribute;
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(tree_kernel<T, D>), S::SMEM);
   if (e != cudaSuccess) return cuda_status(e);
-  tree_kernel<T, D><<<resident(D), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], p);
+  tree_kernel<T, D><<<num_sms(), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], p);
   const int rc = launch_status();
   if (rc != PKV_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -654,7 +670,7 @@ using namespace pkv;
 
 extern "C" int64_t pkv_tree_attention_workspace_bytes(int32_t batch, int32_t head_dim) {
   if (batch <= 0 || batch > kMaxSeqs || (head_dim != 64 && head_dim != 128)) return 0;
-  return plan_bytes(batch) + (int64_t)kWaves * resident(head_dim) * 128 * (head_dim + 2) * 4;
+  return plan_bytes(batch) + 2 * (int64_t)num_sms() * 128 * (head_dim + 2) * 4;
 }
 
 extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv_tables* tables, int32_t num_seqs,
@@ -703,10 +719,10 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   p.tables = tables->block_tables;
   p.seq_rows = tables->seq_rows;
   p.status = status_dev;
-  p.max_units = kWaves * resident(d);
-  p.plan = static_cast<int32_t*>(workspace);
+  p.plan = static_cast<TreePlan*>(workspace);
+  p.offsets = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(workspace) + 256);
   p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan_bytes(num_seqs));
-  p.part_o = p.part_ml + (int64_t)p.max_units * 256;
+  p.part_o = p.part_ml + 2 * (int64_t)num_sms() * 256;
   p.out_st = out_stride_n, p.out_sh = out_stride_h;
   p.q_st = q_stride_n, p.q_sh = q_stride_h;
   p.table_stride = tables->stride;
