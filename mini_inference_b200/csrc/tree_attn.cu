@@ -22,7 +22,7 @@
 // kernel joins. Where every tree has the same number of tiles, the tiles of an item go to as
 // many CTAs side by side over the same range of keys, so that they share its reads in L2.
 //
-// Inside a CTA: one warp issues the TMA copies (K and V rings of their own). The stages go
+// Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go
 // in turn to kStreams streams, each a warp that issues tcgen05 MMAs and four softmax warps
 // (a row per thread) with a score buffer and an accumulator of its own in TMEM: S = Q K^T
 // (128 x 64, float32, Q resident in TMEM), P = 2^(S - m) rounded to the storage type over S,
@@ -61,7 +61,7 @@ template <int D> struct TreeShape {
   static constexpr int NCOLS = 512;
   static_assert(QCOL + D / 2 <= NCOLS, "TMEM columns");
   static constexpr int SW = 4 * kStreams;       // softmax warps
-  static constexpr int THREADS = (SW + 1 + kStreams) * 32;
+  static constexpr int THREADS = (SW + 2 + kStreams) * 32;
   static constexpr int SMEM = 1024 + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
                               (kMaxSeqs + 1) * 8 + 3 * kMaxSeqs * 4;
 };
@@ -269,8 +269,17 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   };
   auto first_of = [](int stream, int gs) { return (stream + kStreams - gs % kStreams) % kStreams; };  // its first stage
 
-  if (warp == SW) {
-    // ---------------------------------------------------------------- TMA copies
+  if (warp < SW + 2 && warp >= SW) {
+    // ---------------------------------------------------------------- TMA copies: a warp for K, one for V
+    // A copy costs the issuing warp about 85 cycles whichever lane issues it (measured): with
+    // one warp for both, 16 copies and two waits made 2000 cycles a stage at head_dim 128 and
+    // set the pace of the whole CTA.
+    const bool is_v = warp != SW;
+    uint8_t* const ring = is_v ? sV : sK;
+    uint64_t* const full = is_v ? v_full : k_full;
+    uint64_t* const done = is_v ? o_done : s_done;  // the slot's last reader
+    const CUtensorMap* const cmap = is_v ? &tmap_v : &tmap_k;
+    const CUtensorMap* const nmap = is_v ? &nmap_v : &nmap_k;
     constexpr int kCopies = (kNK / kBS) * DC;  // a context stage: one copy per lane
     const int bl = lane / DC, c = lane % DC;
     bool ok = true;
@@ -280,7 +289,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       const int row = p.seq_rows ? p.seq_rows[u.b] : u.b;
       const int32_t* table = row >= 0 && row < p.table_rows ? p.tables + (int64_t)row * p.table_stride : nullptr;
       const int nkb = ceil_div(u.ctx, kBS);
-      const int own = max(0, u.nns - u.s0);                          // leading stages of the tree's own keys
+      const int own = max(0, u.nns - u.s0);  // leading stages of the tree's own keys
       const int kb0 = max(0, u.s0 - u.nns) * (kNK / kBS);
       auto lookup = [&](int kb) -> int {  // blocks past the sequence: masked, any block will do
         int blk = kb < nkb && table ? table[kb] : p.nbt - 1;
@@ -292,7 +301,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       };
       constexpr int kPerWindow = 32 / (kNK / kBS);  // stages per window of 32 block ids
       int win = lookup(kb0 + lane), win_next = lookup(kb0 + 32 + lane);
-      for (int i = 0; i < u.nst && ok; ++i) {
+      for (int i = 0; i < u.nst; ++i) {
         const int ci = i - own;  // context stage of the piece
         int blk = 0;
         if (ci >= 0) {
@@ -302,34 +311,28 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           }
           blk = __shfl_sync(0xffffffffu, win, (ci * (kNK / kBS) + bl) % 32);
         }
-        const int c4 = p.layer * p.nbt + blk, j = gs + i, st = j % kRing;
-        const int node = s_first[u.b] + (u.s0 + i) * kNK;
-        auto wait_free = [&](uint64_t* bar, uint64_t* full) {
-          if (lane == 0 && ok) {
-            if (j >= kRing && !mbar_wait_until(&bar[st], ((j / kRing) - 1) & 1, deadline)) {
-              report(p.status, PKV_ERR_TIMEOUT);
-              ok = false;
-            }
-            if (ok) mbar_arrive_expect_tx(&full[st], S::KSB);
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-        };
-        wait_free(s_done, k_full);
-        if (ok && ci >= 0 && lane < kCopies)
-          tma_load_5d(sK + st * S::KSB + c * kNK * 128 + bl * kBS * 128, &tmap_k, 0, 0, c, u.head, c4, &k_full[st]);
-        if (ok && ci < 0 && lane < DC)
-          tma_load_4d(sK + st * S::KSB + lane * kNK * 128, &nmap_k, 0, lane, u.head, node, &k_full[st]);
-        wait_free(o_done, v_full);
-        if (ok && ci >= 0 && lane < kCopies)
-          tma_load_5d(sV + st * S::KSB + c * kNK * 128 + bl * kBS * 128, &tmap_v, 0, 0, c, u.head, c4, &v_full[st]);
-        if (ok && ci < 0 && lane < DC)
-          tma_load_4d(sV + st * S::KSB + lane * kNK * 128, &nmap_v, 0, lane, u.head, node, &v_full[st]);
+        const int j = gs + i, st = j % kRing;
+        if (j >= kRing) ok = mbar_wait_until(&done[st], ((j / kRing) - 1) & 1, deadline);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], S::KSB);
+        __syncwarp();
+        uint8_t* const slot = ring + st * S::KSB;
+        if (ci >= 0) {
+          if (lane < kCopies)
+            tma_load_5d(slot + c * kNK * 128 + bl * kBS * 128, cmap, 0, 0, c, u.head, p.layer * p.nbt + blk, &full[st]);
+        } else if (lane < DC) {
+          tma_load_4d(slot + lane * kNK * 128, nmap, 0, lane, u.head, s_first[u.b] + (u.s0 + i) * kNK, &full[st]);
+        }
       }
     }
-  } else if (warp > SW) {
+    if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
+  } else if (warp >= SW + 2) {
     // ---------------------------------------------------------------- MMA issue, one warp per stream
     if (lane == 0) {
-      const int stream = warp - SW - 1;
+      const int stream = warp - SW - 2;
       constexpr bool kBf16 = Dt<T>::code == PKV_BF16;
       constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, false, 128, kNK);
       constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, true, 128, D);
