@@ -22,8 +22,7 @@
 // kernel joins. Where every tree has the same number of tiles, the tiles of an item go to as
 // many CTAs side by side over the same range of keys, so that they share its reads in L2.
 //
-// Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go
-// in turn to kStreams streams, each a warp that issues tcgen05 MMAs and four softmax warps
+// Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to kStreams streams, each a warp that issues tcgen05 MMAs and four softmax warps
 // (a row per thread) with a score buffer and an accumulator of its own in TMEM: S = Q K^T
 // (128 x 64, float32, Q resident in TMEM), P = 2^(S - m) rounded to the storage type over S,
 // O += P V against a maximum m that moves only when a row's maximum grew by more than 8 (in
@@ -63,14 +62,19 @@ template <int D> struct TreeShape {
   static constexpr int SW = 4 * kStreams;       // softmax warps
   static constexpr int THREADS = (SW + 2 + kStreams) * 32;
   static constexpr int SMEM = 1024 + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
-                              (kMaxSeqs + 1) * 8 + 3 * kMaxSeqs * 4;
+                              5 * kMaxSeqs * 4;
 };
 
-// What every CTA derives from the lengths, for the join.
+// The CTAs' equal shares of all stages, as every CTA derives them from the lengths.
 struct TreePlan {
-  int64_t total;   // stages and charges of all items
-  int32_t ranges;  // CTAs (or groups of them) that share them
-  int32_t gang;    // tiles side by side: a group's CTAs; 1 = a tile is an item of its own
+  int ranges;     // CTAs (or gangs of them) that share the stages
+  int gang;       // tiles side by side: a gang's CTAs; 1 = a tile is an item of its own
+  int quota, rem; // range g: quota stages, one more if g < rem
+  __device__ int start(int g) const { return g * quota + min(g, rem); }
+  __device__ int range_of(int x) const {  // the range that holds position x
+    const int big = rem * (quota + 1);
+    return x < big ? x / (quota + 1) : rem + (x - big) / quota;
+  }
 };
 
 struct TreeParams {
@@ -82,8 +86,8 @@ struct TreeParams {
   const int32_t* tables;
   const int32_t* seq_rows;
   int32_t* status;
-  TreePlan* plan;
-  int64_t* offsets;    // [batch] where each sequence's items begin
+  int4* cut;           // [CTAs] the item that begins in a CTA's range and ends in another: its first node,
+                       // KV head | gang << 16, rows, pieces (0: none)
   float* part_ml;      // [2 per CTA][2][128] running maximum and sum
   float* part_o;       // [2 per CTA][D][128]
   int64_t out_st, out_sh, q_st, q_sh, table_stride, total_nodes;
@@ -106,25 +110,23 @@ __device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c
 
 // The lengths of sequence b, clamped to what the call's own sizes allow.
 struct SeqLens {
-  int first, nodes, ctx;
+  int first, nodes, ctx, row;
 };
 __device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) {
   SeqLens s;
   const int lo = p.cu[b], hi = p.cu[b + 1];
   const int n = p.ctx[b], row = p.seq_rows ? p.seq_rows[b] : b;
-  bool bad = lo < 0 || hi < lo || hi > p.total_nodes || hi - lo > p.max_nodes || n < 0 ||
+  const bool bad = lo < 0 || hi < lo || hi > p.total_nodes || hi - lo > p.max_nodes || n < 0 ||
              n > (int64_t)p.table_cols * kBS || row >= p.table_rows;
   s.first = (int)min((int64_t)max(lo, 0), p.total_nodes);
   s.nodes = min(max((int)min((int64_t)hi, p.total_nodes) - s.first, 0), p.max_nodes);
+  s.row = row;
   // A padding row has no cached keys.
   s.ctx = row < 0 || row >= p.table_rows ? 0 : (int)min((int64_t)max(n, 0), (int64_t)p.table_cols * kBS);
   if (bad) report(status, PKV_ERR_OUT_OF_RANGE);
   return s;
 }
 __device__ inline int item_cost(int nodes, int ctx) { return kItemCost + ceil_div(nodes, kNK) + ceil_div(ctx, kNK); }
-__device__ inline int64_t range_start(const TreePlan& pl, int64_t g) { return pl.total * g / pl.ranges; }
-// The range that holds position x.
-__device__ inline int range_of(const TreePlan& pl, int64_t x) { return (int)(((x + 1) * pl.ranges - 1) / pl.total); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
@@ -147,12 +149,12 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   uint64_t* mma_done = q_ready + kStreams;  // every MMA of the CTA completed
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kBars);
   float* s_ml = reinterpret_cast<float*>(bars + kBars + 2);  // [2 parities][kStreams][2][128] maxima and sums
-  int64_t* s_off = reinterpret_cast<int64_t*>(s_ml + 2 * kStreams * 2 * 128);  // [batch + 1] items' begin
-  int32_t* s_first = reinterpret_cast<int32_t*>(s_off + kMaxSeqs + 1);         // [batch] first node
+  int32_t* s_off = reinterpret_cast<int32_t*>(s_ml + 2 * kStreams * 2 * 128);  // [batch] where its items begin
+  int32_t* s_first = s_off + kMaxSeqs;                                         // [batch] first node
   int32_t* s_nodes = s_first + kMaxSeqs;                                       // [batch] nodes
   int32_t* s_ctx = s_nodes + kMaxSeqs;                                         // [batch] cached keys
-  __shared__ int64_t s_warp[32];
-  __shared__ int s_least[32], s_most[32];
+  int32_t* s_row = s_ctx + kMaxSeqs;                                           // [batch] table row
+  __shared__ int4 s_warp[32];  // per warp: least and most tiles, stages with a tile an item and with tiles in gangs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.batch, G = p.group;
 
@@ -177,69 +179,68 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   const int per = ceil_div(B, S::THREADS), b0 = min(B, tid * per), b1 = min(B, b0 + per);
   TreePlan plan;
   {
-    int least = 1 << 30, most = 0;
+    int least = 1 << 30, most = 0, alone = 0, ganged = 0;  // stages if a tile is an item; if its item's tiles go together
     for (int b = b0; b < b1; ++b) {
       const SeqLens s = seq_lens(p, b, blockIdx.x == 0 ? p.status : nullptr);
       s_first[b] = s.first;
       s_nodes[b] = s.nodes;
       s_ctx[b] = s.ctx;
+      s_row[b] = s.row;
       if (s.nodes > 0) {
-        const int tiles = ceil_div(s.nodes, p.tile_nodes);
+        const int tiles = ceil_div(s.nodes, p.tile_nodes), cost = p.hkv * item_cost(s.nodes, s.ctx);
         least = min(least, tiles);
         most = max(most, tiles);
+        alone += tiles * cost;
+        ganged += cost;
       }
     }
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) s_least[warp] = least, s_most[warp] = most;
-    __syncthreads();
-    for (int w = 0; w < S::THREADS / 32; ++w) least = min(least, s_least[w]), most = max(most, s_most[w]);
-    plan.gang = least == most && most <= (int)gridDim.x ? most : 1;
-    auto cost_of = [&](int b) -> int64_t {
-      const int n = s_nodes[b];
-      if (n == 0) return 0;
-      return (int64_t)p.hkv * (plan.gang > 1 ? 1 : ceil_div(n, p.tile_nodes)) * item_cost(n, s_ctx[b]);
-    };
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += cost_of(b);
-    int64_t inc = mine;
+    int ia = alone, ig = ganged;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
+      const int ua = __shfl_up_sync(0xffffffffu, ia, o), ug = __shfl_up_sync(0xffffffffu, ig, o);
+      if (lane >= o) ia += ua, ig += ug;
     }
-    if (lane == 31) s_warp[warp] = inc;
+    if (lane == 31) s_warp[warp] = make_int4(least, most, ia, ig);
     __syncthreads();
-    int64_t before = inc - mine;
-    plan.total = 0;
+    int total_a = 0, total_g = 0;
+    ia -= alone, ig -= ganged;  // before this thread's first sequence
     for (int w = 0; w < S::THREADS / 32; ++w) {
-      if (w < warp) before += s_warp[w];
-      plan.total += s_warp[w];
+      const int4 x = s_warp[w];
+      least = min(least, x.x), most = max(most, x.y);
+      if (w < warp) ia += x.z, ig += x.w;
+      total_a += x.z, total_g += x.w;
     }
+    plan.gang = least == most && most > 1 && most <= (int)gridDim.x ? most : 1;
+    const int total = plan.gang > 1 ? total_g : total_a;
+    int before = plan.gang > 1 ? ig : ia;
     for (int b = b0; b < b1; ++b) {
       s_off[b] = before;
-      if (blockIdx.x == 0) p.offsets[b] = before;
-      before += cost_of(b);
+      const int n = s_nodes[b];
+      if (n > 0) before += p.hkv * (plan.gang > 1 ? 1 : ceil_div(n, p.tile_nodes)) * item_cost(n, s_ctx[b]);
     }
-    plan.ranges = (int)max((int64_t)1, min((int64_t)(gridDim.x / max(plan.gang, 1)), plan.total / kMinRange));
-    if (blockIdx.x == 0 && tid == 0) *p.plan = plan;
+    plan.ranges = max(1, min((int)gridDim.x / plan.gang, total / kMinRange));
+    plan.quota = total / plan.ranges;
+    plan.rem = total - plan.quota * plan.ranges;
+    if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tslot;
   const uint64_t deadline = global_ns() + kWaitBudgetNs;
-  const int gang = max(plan.gang, 1), range = blockIdx.x / gang, member = blockIdx.x % gang;
-  const int64_t pos0 = range < plan.ranges ? range_start(plan, range) : 0;
-  const int64_t pos_end = range < plan.ranges ? range_start(plan, range + 1) : 0;
+  const int range = blockIdx.x / plan.gang, member = blockIdx.x - range * plan.gang;
+  const int pos0 = range < plan.ranges ? plan.start(range) : 0;
+  const int pos_end = range < plan.ranges ? plan.start(range + 1) : 0;
 
   // Every role walks the same pieces and numbers stages across them, so ring slots and
   // barrier parities continue from one piece to the next.
   struct Piece {
     int b, head, tile, rows, nodes, ctx, nns;  // nns: the item's stages of the tree's own keys, its first
-    int s0, nst;                               // first stage, stages
+    int s0, nst, item_end;                     // first stage, stages; position behind the item
     bool begins, ends;
   };
-  auto next_piece = [&](int64_t& pos, Piece& u) -> bool {
+  auto next_piece = [&](int& pos, Piece& u) -> bool {
     while (pos < pos_end) {
       int lo = 0, hi = B - 1;  // the last sequence that begins at or before pos (empty ones take no room)
       while (lo < hi) {
@@ -250,9 +251,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       u.nodes = s_nodes[lo];
       u.ctx = s_ctx[lo];
       const int cost = item_cost(u.nodes, u.ctx), tiles = ceil_div(u.nodes, p.tile_nodes);
-      const int64_t rel = pos - s_off[lo];
-      const int item = (int)(rel / cost), x0 = (int)(rel - (int64_t)item * cost);
-      const int x1 = (int)min((int64_t)cost, x0 + (pos_end - pos));
+      const int rel = pos - s_off[lo], item = rel / cost, x0 = rel - item * cost;
+      const int x1 = min(cost, x0 + (pos_end - pos)), item_end = pos + cost - x0;
       pos += x1 - x0;
       u.s0 = max(0, x0 - kItemCost);
       u.nst = max(0, x1 - kItemCost) - u.s0;
@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       u.nns = ceil_div(u.nodes, kNK);
       u.begins = u.s0 == 0;
       u.ends = x1 == cost;
+      u.item_end = item_end;
       return true;
     }
     return false;
@@ -285,14 +286,13 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     bool ok = true;
     int gs = 0;
     Piece u;
-    for (int64_t pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
-      const int row = p.seq_rows ? p.seq_rows[u.b] : u.b;
-      const int32_t* table = row >= 0 && row < p.table_rows ? p.tables + (int64_t)row * p.table_stride : nullptr;
+    for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
+      const int32_t* table = u.ctx > 0 ? p.tables + (int64_t)s_row[u.b] * p.table_stride : nullptr;
       const int nkb = ceil_div(u.ctx, kBS);
       const int own = max(0, u.nns - u.s0);  // leading stages of the tree's own keys
       const int kb0 = max(0, u.s0 - u.nns) * (kNK / kBS);
       auto lookup = [&](int kb) -> int {  // blocks past the sequence: masked, any block will do
-        int blk = kb < nkb && table ? table[kb] : p.nbt - 1;
+        int blk = kb < nkb ? table[kb] : p.nbt - 1;
         if (blk < 0 || blk >= p.nbt) {
           report(p.status, PKV_ERR_OUT_OF_RANGE);
           blk = p.nbt - 1;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       bool ok = true;
       int gs = 0, k = 0;
       Piece u;
-      for (int64_t pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
+      for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
         const int i0 = first_of(stream, gs);
         if (i0 >= u.nst) continue;
         ok = mbar_wait_until(&q_ready[stream], k++ & 1, deadline) && issue_s(gs + i0);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     };
     int gs = 0, k = 0;
     Piece u;
-    for (int64_t pos = pos0; next_piece(pos, u); gs += u.nst, ++k) {
+    for (int pos = pos0; next_piece(pos, u); gs += u.nst, ++k) {
       const bool valid = r < u.rows;
       const bool live = (warp % 4) * 32 < u.rows;  // some row of the warp has a query
       const int64_t node = (int64_t)s_first[u.b] + u.tile * p.tile_nodes + t;
@@ -544,6 +544,9 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         }
         const bool cut = !(u.begins && u.ends);
         const int64_t slot = 2 * (int64_t)blockIdx.x + u.begins;
+        if (u.begins && !u.ends && tid == 0)
+          p.cut[blockIdx.x] = make_int4(s_first[u.b] + u.tile * p.tile_nodes, u.head | plan.gang << 16, u.rows,
+                                        plan.range_of(u.item_end - 1) - range + 1);
         if (cut && stream == 0) {
           p.part_ml[slot * 256 + r] = top;
           p.part_ml[slot * 256 + 128 + r] = sum;
@@ -594,31 +597,25 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
 
 // Joins the pieces of a cut item: with M the largest of their maxima,
 //   out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// One CTA per (64 output columns, tile, KV head, sequence); a thread takes one row and
-// eight columns, so the states are read a row to a lane, and its output is one 16-byte write.
-constexpr int kJoinCols = 64;
+// One CTA per (CTA of the first kernel whose range cuts an item it begins, 32 output columns);
+// a thread takes one row and eight columns, so the states are read a row to a lane, and its
+// output is one 16-byte write.
+constexpr int kJoinCols = 32;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const TreeParams p) {
-  const int b = blockIdx.z, head = blockIdx.y;
-  const int tile = blockIdx.x / (D / kJoinCols), part = blockIdx.x % (D / kJoinCols);
-  const SeqLens s = seq_lens(p, b, nullptr);
-  const int tiles = ceil_div(s.nodes, p.tile_nodes);
-  const int r = threadIdx.x % 128, c0 = part * kJoinCols + (threadIdx.x / 128) * 8;
   grid_dep_wait();
-  if (tile >= tiles) return;
-  const TreePlan plan = *p.plan;
-  const int cost = item_cost(s.nodes, s.ctx);
-  const int64_t begin = p.offsets[b] + (int64_t)(plan.gang > 1 ? head : head * tiles + tile) * cost + kItemCost;
-  const int g0 = range_of(plan, begin), pieces = range_of(plan, begin + cost - kItemCost - 1) - g0 + 1;
-  if (pieces == 1 || r >= min(p.tile_nodes, s.nodes - tile * p.tile_nodes) * p.group) return;
-  const int gang = plan.gang, member = gang > 1 ? tile : 0;
-  auto slot = [&](int k) { return 2 * ((int64_t)(g0 + k) * gang + member) + (k == 0); };
+  const int4 cut = p.cut[blockIdx.x];
+  const int head = cut.y & 0xffff, gang = cut.y >> 16, pieces = cut.w;
+  const int r = threadIdx.x % 128, c0 = blockIdx.y * kJoinCols + (threadIdx.x / 128) * 8;
+  if (r >= cut.z || pieces == 0) return;
+  auto slot = [&](int k) { return 2 * ((int64_t)blockIdx.x + k * gang) + (k == 0); };
   float top = -INFINITY;
+#pragma unroll 4
   for (int k = 0; k < pieces; ++k) top = fmaxf(top, p.part_ml[slot(k) * 256 + r]);
   const float mref = top == -INFINITY ? 0.f : top;
   float sum = 0.f, acc[8] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int k = 0; k < pieces; ++k) {
     const int64_t u = slot(k);
     const float wgt = ex2(p.part_ml[u * 256 + r] - mref);
@@ -629,8 +626,7 @@ __global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const 
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   const int t = r / p.group, gq = r - t * p.group;
-  T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)s.first + tile * p.tile_nodes + t) * p.out_st +
-            (int64_t)(head * p.group + gq) * p.out_sh + c0;
+  T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)cut.x + t) * p.out_st + (int64_t)(head * p.group + gq) * p.out_sh + c0;
   uint32_t w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = Dt<T>::pack(acc[2 * e] * inv, acc[2 * e + 1] * inv);
@@ -642,8 +638,8 @@ __global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const 
   }
 }
 
-// The plan, then every sequence's offset.
-int64_t plan_bytes(int batch) { return (256 + (int64_t)batch * 8 + 255) / 256 * 256; }
+int tree_ctas() { return num_sms(); }
+int64_t cut_bytes() { return ((int64_t)tree_ctas() * 16 + 255) / 256 * 256; }
 
 template <typename T, int D>
 int launch(const CUtensorMap (&maps)[4], const TreeParams& p, cudaStream_t st) {
@@ -651,11 +647,11 @@ int launch(const CUtensorMap (&maps)[4], const TreeParams& p, cudaStream_t st) {
   static SmemAttribute attribute;
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(tree_kernel<T, D>), S::SMEM);
   if (e != cudaSuccess) return cuda_status(e);
-  tree_kernel<T, D><<<num_sms(), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], p);
+  tree_kernel<T, D><<<tree_ctas(), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], p);
   const int rc = launch_status();
   if (rc != PKV_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.max_nodes + p.tile_nodes - 1) / p.tile_nodes * (D / kJoinCols), p.hkv, p.batch);
+  cfg.gridDim = dim3(tree_ctas(), D / kJoinCols);
   cfg.blockDim = dim3(128 * (kJoinCols / 8));
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -673,7 +669,7 @@ using namespace pkv;
 
 extern "C" int64_t pkv_tree_attention_workspace_bytes(int32_t batch, int32_t head_dim) {
   if (batch <= 0 || batch > kMaxSeqs || (head_dim != 64 && head_dim != 128)) return 0;
-  return plan_bytes(batch) + 2 * (int64_t)num_sms() * 128 * (head_dim + 2) * 4;
+  return cut_bytes() + 2 * (int64_t)tree_ctas() * 128 * (head_dim + 2) * 4;
 }
 
 extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv_tables* tables, int32_t num_seqs,
@@ -695,6 +691,10 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
       mask_words > kMaxWords || (pool->dtype != PKV_F16 && pool->dtype != PKV_BF16))
     return PKV_ERR_UNSUPPORTED;
   if (max_nodes > 64 * mask_words) return PKV_ERR_INVALID_ARGUMENT;
+  // Stages are counted in 32 bits: every tile of every head against a full table row.
+  const int64_t tiles = std::min((int64_t)num_seqs * ((max_nodes + 128 / group - 1) / (128 / group)),
+                                 total_nodes / (128 / group) + num_seqs);
+  if (tiles * hkv * (kItemCost + 2 + max_nodes / kNK + tables->cols / (kNK / kBS)) > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
   if (num_seqs == 0 || max_nodes == 0 || total_nodes == 0) return PKV_OK;
   if (!tables->block_tables || !cu_nodes || !context_lens || !out || !q || !k_nodes || !v_nodes || !mask)
     return PKV_ERR_INVALID_ARGUMENT;
@@ -722,10 +722,9 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   p.tables = tables->block_tables;
   p.seq_rows = tables->seq_rows;
   p.status = status_dev;
-  p.plan = static_cast<TreePlan*>(workspace);
-  p.offsets = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(workspace) + 256);
-  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan_bytes(num_seqs));
-  p.part_o = p.part_ml + 2 * (int64_t)num_sms() * 256;
+  p.cut = static_cast<int4*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + cut_bytes());
+  p.part_o = p.part_ml + 2 * (int64_t)tree_ctas() * 256;
   p.out_st = out_stride_n, p.out_sh = out_stride_h;
   p.q_st = q_stride_n, p.q_sh = q_stride_h;
   p.table_stride = tables->stride;
