@@ -22,12 +22,13 @@
 // kernel joins. Where every tree has the same number of tiles, the tiles of an item go to as
 // many CTAs side by side over the same range of keys, so that they share its reads in L2.
 //
-// Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to kStreams streams, each a warp that issues tcgen05 MMAs and four softmax warps
-// (a row per thread) with a score buffer and an accumulator of its own in TMEM: S = Q K^T
-// (128 x 64, float32, Q resident in TMEM), P = 2^(S - m) rounded to the storage type over S,
-// O += P V against a maximum m that moves only when a row's maximum grew by more than 8 (in
-// log2). While one stream waits for its MMAs another computes exponentials, and no stage
-// waits for another stream's; the streams' states are joined at the end of a piece.
+// Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to
+// two streams, each a warp that issues tcgen05 MMAs and four softmax warps (a row per
+// thread) with two score buffers and an accumulator of its own in TMEM: S = Q K^T (128 x 64,
+// float32), P = 2^(S - m) rounded to the storage type over S, O += P V against a maximum m
+// that moves only when a row's maximum grew by more than 8 (in log2). The scores of a
+// stream's next stage are made while its warps work on the present one's, and one stream
+// computes exponentials while the other waits; their states are joined at the end of a piece.
 // Rounding P costs each weight half a step of its type, as much as the output's own
 // rounding; the row sum is taken before it, in float32.
 #include <algorithm>
@@ -41,27 +42,27 @@ namespace {
 constexpr int kBS = 16;
 constexpr int kNK = 64;          // keys per stage
 constexpr int kStreams = 2;
-constexpr int kRing = 6;         // stages of the K ring and of the V ring
-constexpr int kBars = 4 * kRing + 2 * kStreams + 1;
+constexpr int kRing = 4;         // stages of the K ring and of the V ring
+constexpr int kBars = 4 * kRing + 3 * kStreams + 1;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
 constexpr int kItemCost = 4;     // an item's start and end, in stages
 constexpr int kMinRange = 6;     // no CTA gets less than this
 constexpr float kLog2e = 1.4426950408889634f;
 // Every slot of a ring belongs to one stream, so that a wait sees each of its phases.
-static_assert(kRing % kStreams == 0, "ring slots per stream");
+static_assert(kRing % (2 * kStreams) == 0, "ring slots per stream and score buffer");
 
 template <int D> struct TreeShape {
   static constexpr int DC = D / 64;             // 64-wide head_dim chunks
   static constexpr int KSB = DC * kNK * 128;    // one stage of K (or V): [DC][64 keys][64], 128B-swizzled
-  // TMEM columns: a score buffer and an accumulator per stream, Q (packed 16-bit pairs).
-  static constexpr int OCOL = kStreams * kNK;
-  static constexpr int QCOL = OCOL + kStreams * D;
+  static constexpr int QB = DC * 128 * 128;     // the Q tile: [DC][128 rows][64], 128B-swizzled
+  // TMEM columns: two score buffers and an accumulator per stream.
+  static constexpr int OCOL = kStreams * 2 * kNK;
   static constexpr int NCOLS = 512;
-  static_assert(QCOL + D / 2 <= NCOLS, "TMEM columns");
+  static_assert(OCOL + kStreams * D <= NCOLS, "TMEM columns");
   static constexpr int SW = 4 * kStreams;       // softmax warps
   static constexpr int THREADS = (SW + 2 + kStreams) * 32;
-  static constexpr int SMEM = 1024 + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
+  static constexpr int SMEM = 1024 + QB + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
                               5 * kMaxSeqs * 4;
 };
 
@@ -137,15 +138,16 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   constexpr int DC = S::DC, SW = S::SW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sK = smem;                     // [kRing][KSB]
+  uint8_t* sQ = smem;                     // [QB]
+  uint8_t* sK = sQ + S::QB;               // [kRing][KSB]
   uint8_t* sV = sK + kRing * S::KSB;      // [kRing][KSB]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kRing * S::KSB);
   uint64_t* k_full = bars;                // [kRing] K landed
   uint64_t* v_full = k_full + kRing;      // [kRing] V landed
   uint64_t* s_done = v_full + kRing;      // [kRing] S(j) = Q K(j)^T done: S ready, K slot free
   uint64_t* o_done = s_done + kRing;      // [kRing] O += P(j) V(j) done: V slot and score buffer free
-  uint64_t* p_full = o_done + kRing;      // [kStreams] P stored
-  uint64_t* q_ready = p_full + kStreams;  // [kStreams] Q stored, for a stream with stages in the piece
+  uint64_t* p_full = o_done + kRing;      // [kStreams][2] P stored, by score buffer
+  uint64_t* q_ready = p_full + 2 * kStreams;  // [kStreams] Q stored, for a stream with stages in the piece
   uint64_t* mma_done = q_ready + kStreams;  // every MMA of the CTA completed
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kBars);
   float* s_ml = reinterpret_cast<float*>(bars + kBars + 2);  // [2 parities][kStreams][2][128] maxima and sums
@@ -161,7 +163,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   grid_dep_launch_dependents();  // the join's CTAs may wait in place
   if (tid == 0) {
     for (int i = 0; i < 4 * kRing; ++i) mbar_init(&bars[i], 1);
-    for (int i = 0; i < kStreams; ++i) mbar_init(&p_full[i], 4), mbar_init(&q_ready[i], SW);
+    for (int i = 0; i < 2 * kStreams; ++i) mbar_init(&p_full[i], 4);
+    for (int i = 0; i < kStreams; ++i) mbar_init(&q_ready[i], SW);
     mbar_init(mma_done, kStreams);
     fence_mbar_init();
   }
@@ -336,22 +339,24 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       constexpr bool kBf16 = Dt<T>::code == PKV_BF16;
       constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, false, 128, kNK);
       constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, true, 128, D);
-      const uint32_t ts = tmem + stream * kNK, to = tmem + S::OCOL + stream * D;
+      const uint32_t to = tmem + S::OCOL + stream * D;
+      auto ts_of = [&](int j) { return tmem + (stream * 2 + j / kStreams % 2) * kNK; };  // S(j), then P(j)
       // Descriptors are computed before the waits, so that the MMAs issue back to back.
       auto pin = [](uint64_t& x) { asm volatile("" : "+l"(x)); };
       auto issue_s = [&](int j) -> bool {
         const int st = j % kRing;
-        uint64_t bk[D / 16];
+        uint64_t aq[D / 16], bk[D / 16];
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
+          aq[kk] = umma_desc_sw128(smem_u32(sQ + (kk / 4) * 128 * 128 + (kk % 4) * 32), 16, 1024);
           bk[kk] = umma_desc_sw128(smem_u32(sK + st * S::KSB + (kk / 4) * kNK * 128 + (kk % 4) * 32), 16, 1024);
+          pin(aq[kk]);
           pin(bk[kk]);
         }
         if (!mbar_wait_until(&k_full[st], (j / kRing) & 1, deadline)) return false;
-        // The score buffer still holds P(j - kStreams) of this piece until its O has read it.
         tc_fence_after_sync();
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) umma_f16_ts(ts, tmem + S::QCOL + kk * 8, bk[kk], idesc_s, kk > 0);
+        for (int kk = 0; kk < D / 16; ++kk) umma_f16_ss(ts_of(j), aq[kk], bk[kk], idesc_s, kk > 0);
         umma_commit(&s_done[st]);
         return true;
       };
@@ -364,10 +369,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           pin(bv[kb]);
         }
         if (!mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) return false;
-        if (!mbar_wait_until(&p_full[stream], (j / kStreams) & 1, deadline)) return false;
+        if (!mbar_wait_until(&p_full[stream * 2 + j / kStreams % 2], (j / (2 * kStreams)) & 1, deadline)) return false;
         tc_fence_after_sync();
 #pragma unroll
-        for (int kb = 0; kb < kNK / 16; ++kb) umma_f16_ts(to, ts + kb * 8, bv[kb], idesc_o, !first || kb > 0);
+        for (int kb = 0; kb < kNK / 16; ++kb) umma_f16_ts(to, ts_of(j) + kb * 8, bv[kb], idesc_o, !first || kb > 0);
         umma_commit(&o_done[st]);
         return true;
       };
@@ -377,12 +382,13 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
         const int i0 = first_of(stream, gs);
         if (i0 >= u.nst) continue;
-        ok = mbar_wait_until(&q_ready[stream], k++ & 1, deadline) && issue_s(gs + i0);
+        ok = mbar_wait_until(&q_ready[stream], k++ & 1, deadline) && issue_s(gs + i0) &&
+             (i0 + kStreams >= u.nst || issue_s(gs + i0 + kStreams));
         for (int i = i0; i < u.nst && ok; i += kStreams) {
-          const int j = gs + i;
+          const int j = gs + i;  // S two stages on goes over P(j), once O has read it
           ok = issue_o(j, i == i0) &&
-               (i + kStreams >= u.nst ||
-                (mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline) && issue_s(j + kStreams)));
+               (i + 2 * kStreams >= u.nst ||
+                (mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline) && issue_s(j + 2 * kStreams)));
         }
       }
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
@@ -394,7 +400,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     const int r = (warp % 4) * 32 + lane;  // TMEM lane = tile row
     const int t = r / G, gq = r - t * G;   // node of the tile, query head of the group
     const uint32_t tl = tmem + ((uint32_t)((warp % 4) * 32) << 16);
-    const uint32_t ts = tl + stream * kNK, to = tl + S::OCOL + stream * D;
+    const uint32_t to = tl + S::OCOL + stream * D;
     constexpr float kSlack = 8.f;
     bool ok = true;
     auto confirm = [&](int j) {  // O += P(j) V(j) has completed
@@ -409,7 +415,6 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       {  // Q: each stream's warps store their share of the columns
         const T* qrow = reinterpret_cast<const T*>(p.q) + node * p.q_st + (int64_t)(u.head * G + gq) * p.q_sh;
         for (int c = stream; c < D / 32; c += kStreams) {
-          uint32_t qv[16];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             uint4 v = make_uint4(0, 0, 0, 0);
@@ -421,12 +426,12 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
                 v = make_uint4(q32[0], q32[1], q32[2], q32[3]);
               }
             }
-            qv[4 * x] = v.x, qv[4 * x + 1] = v.y, qv[4 * x + 2] = v.z, qv[4 * x + 3] = v.w;
+            const int g = (c % 2) * 4 + x;  // 16-byte granule of the row's 128
+            *reinterpret_cast<uint4*>(sQ + (c / 2) * 128 * 128 + r * 128 + ((g ^ (r & 7)) * 16)) = v;
           }
-          tmem_st16(tl + S::QCOL + c * 16, qv);
         }
       }
-      tmem_wait_st();
+      fence_proxy_async_smem();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -441,6 +446,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         const int j = gs + i, sg = u.s0 + i, st = j % kRing;
         const bool own = sg < u.nns;  // the tree's own keys
         const int keys = own ? u.nodes - sg * kNK : u.ctx - (sg - u.nns) * kNK;  // of the stage, if < kNK
+        const int buf = j / kStreams % 2;
+        const uint32_t ts = tl + (stream * 2 + buf) * kNK;
         uint64_t see = ~0ull;
         if (own) see = valid ? p.mask[node * p.words + sg] : 0;
         if (keys < kNK) see &= (1ull << keys) - 1;
@@ -520,7 +527,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[stream]);
+        if (lane == 0) mbar_arrive(&p_full[stream * 2 + buf]);
       }
       // The piece's streams joined: maxima and sums through shared memory, then each stream's
       // warps take their share of the output columns from every accumulator.
