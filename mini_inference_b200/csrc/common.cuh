@@ -332,11 +332,11 @@ bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int h
 int make_matrix_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows,
                            uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_rows);
 // 4-D tensor map over rows [rows, heads, d] of 16-bit elements (strides in elements, multiples
-// of 8; d a multiple of 64), viewed as {64, d/64, heads, rows} with a box of {64, 1, 1,
-// box_rows}: one 64-wide chunk of one head of consecutive rows per copy, 128-byte swizzle.
+// of 8; d a multiple of 64), viewed as {64, d/64, heads, rows} with a box of {64, 1,
+// box_heads, box_rows}: one 64-wide chunk of consecutive rows' heads per copy, 128-byte swizzle.
 // Rows past `rows` read as zeros.
 int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
-                         int64_t head_stride, int64_t row_stride, int box_rows);
+                         int64_t head_stride, int64_t row_stride, int box_heads, int box_rows);
 // Streaming multiprocessors of the current device (queried once).
 int num_sms();
 

@@ -108,7 +108,7 @@ int make_matrix_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64
 }
 
 int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
-                         int64_t head_stride, int64_t row_stride, int box_rows) {
+                         int64_t head_stride, int64_t row_stride, int box_heads, int box_rows) {
   auto fn = encode_fn();
   if (!fn) {
     g_last_cuda_error = "cuTensorMapEncodeTiled is not available from the driver";
@@ -117,7 +117,7 @@ int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, i
   cuuint64_t dims[4] = {64, (cuuint64_t)(d / 64), (cuuint64_t)heads, (cuuint64_t)rows};
   // A dimension of one entry is never stepped over: any valid stride will do.
   cuuint64_t strides[3] = {128, heads > 1 ? (cuuint64_t)head_stride * 2 : 128, rows > 1 ? (cuuint64_t)row_stride * 2 : 128};
-  cuuint32_t box[4] = {64, 1, 1, (cuuint32_t)box_rows};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType dt = dtype == PKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUresult r = fn(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

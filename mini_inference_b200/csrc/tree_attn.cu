@@ -43,7 +43,7 @@ constexpr int kBS = 16;
 constexpr int kNK = 64;          // keys per stage
 constexpr int kStreams = 2;
 constexpr int kRing = 4;         // stages of the K ring and of the V ring
-constexpr int kBars = 4 * kRing + 3 * kStreams + 1;
+constexpr int kBars = 4 * kRing + 3 * kStreams + 5;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
 constexpr int kItemCost = 4;     // an item's start and end, in stages
@@ -62,7 +62,7 @@ template <int D> struct TreeShape {
   static_assert(OCOL + kStreams * D <= NCOLS, "TMEM columns");
   static constexpr int SW = 4 * kStreams;       // softmax warps
   static constexpr int THREADS = (SW + 2 + kStreams) * 32;
-  static constexpr int SMEM = 1024 + QB + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
+  static constexpr int SMEM = 1024 + 2 * QB + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
                               5 * kMaxSeqs * 4;
 };
 
@@ -80,7 +80,6 @@ struct TreePlan {
 
 struct TreeParams {
   void* out;
-  const void* q;
   const int32_t* cu;
   const int32_t* ctx;
   const uint64_t* mask;
@@ -91,9 +90,9 @@ struct TreeParams {
                        // KV head | gang << 16, rows, pieces (0: none)
   float* part_ml;      // [2 per CTA][2][128] running maximum and sum
   float* part_o;       // [2 per CTA][D][128]
-  int64_t out_st, out_sh, q_st, q_sh, table_stride, total_nodes;
+  int64_t out_st, out_sh, table_stride, total_nodes;
   int32_t table_rows, table_cols, batch, hkv, group, tile_nodes, words, layer, nbt;
-  int32_t q_vec16, out_vec16, max_nodes;
+  int32_t out_vec16, max_nodes;
   float scale_log2;
 };
 
@@ -133,13 +132,13 @@ template <typename T, int D>
 __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                 const __grid_constant__ CUtensorMap nmap_k, const __grid_constant__ CUtensorMap nmap_v,
-                const TreeParams p) {
+                const __grid_constant__ CUtensorMap qmap, const TreeParams p) {
   using S = TreeShape<D>;
   constexpr int DC = S::DC, SW = S::SW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                     // [QB]
-  uint8_t* sK = sQ + S::QB;               // [kRing][KSB]
+  uint8_t* sQ = smem;                     // [2][QB]
+  uint8_t* sK = sQ + 2 * S::QB;           // [kRing][KSB]
   uint8_t* sV = sK + kRing * S::KSB;      // [kRing][KSB]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kRing * S::KSB);
   uint64_t* k_full = bars;                // [kRing] K landed
@@ -147,8 +146,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   uint64_t* s_done = v_full + kRing;      // [kRing] S(j) = Q K(j)^T done: S ready, K slot free
   uint64_t* o_done = s_done + kRing;      // [kRing] O += P(j) V(j) done: V slot and score buffer free
   uint64_t* p_full = o_done + kRing;      // [kStreams][2] P stored, by score buffer
-  uint64_t* q_ready = p_full + 2 * kStreams;  // [kStreams] Q stored, for a stream with stages in the piece
-  uint64_t* mma_done = q_ready + kStreams;  // every MMA of the CTA completed
+  uint64_t* o_free = p_full + 2 * kStreams;  // [kStreams] accumulators read, for a stream with stages in the piece
+  uint64_t* q_full = o_free + kStreams;   // [2] Q landed, pieces in turn
+  uint64_t* q_free = q_full + 2;          // [2] the piece's every MMA done
+  uint64_t* mma_done = q_free + 2;        // every MMA of the CTA completed
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kBars);
   float* s_ml = reinterpret_cast<float*>(bars + kBars + 2);  // [2 parities][kStreams][2][128] maxima and sums
   int32_t* s_off = reinterpret_cast<int32_t*>(s_ml + 2 * kStreams * 2 * 128);  // [batch] where its items begin
@@ -161,22 +162,25 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   const int B = p.batch, G = p.group;
 
   grid_dep_launch_dependents();  // the join's CTAs may wait in place
-  if (tid == 0) {
+  // Set-up by warps that have no lengths to read in a small batch.
+  if (warp == SW && lane == 0) {
     for (int i = 0; i < 4 * kRing; ++i) mbar_init(&bars[i], 1);
     for (int i = 0; i < 2 * kStreams; ++i) mbar_init(&p_full[i], 4);
-    for (int i = 0; i < kStreams; ++i) mbar_init(&q_ready[i], SW);
+    for (int i = 0; i < kStreams; ++i) mbar_init(&o_free[i], SW);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_free[i], 1);
     mbar_init(mma_done, kStreams);
     fence_mbar_init();
   }
-  if (warp == 0) {
+  if (warp == SW - 1) {
     tmem_alloc(tslot, S::NCOLS);
     tc_fence_before_sync();
   }
-  if (warp == SW && lane == 0) {
+  if (warp == SW + 1 && lane == 0) {
     prefetch_tensormap(&tmap_k);
     prefetch_tensormap(&tmap_v);
     prefetch_tensormap(&nmap_k);
     prefetch_tensormap(&nmap_v);
+    prefetch_tensormap(&qmap);
   }
   // ------------------------------------------------------------------ plan
   const int per = ceil_div(B, S::THREADS), b0 = min(B, tid * per), b1 = min(B, b0 + per);
@@ -287,9 +291,21 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     constexpr int kCopies = (kNK / kBS) * DC;  // a context stage: one copy per lane
     const int bl = lane / DC, c = lane % DC;
     bool ok = true;
-    int gs = 0;
+    int gs = 0, k = 0;
     Piece u;
-    for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
+    for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst, ++k) {
+      if (!is_v) {  // the piece's Q: rows (node, head of the group), those past the tree unused
+        if (k >= 2) ok = mbar_wait_until(&q_free[k & 1], ((k >> 1) - 1) & 1, deadline);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&q_full[k & 1], DC * 128 * G * p.tile_nodes);
+        __syncwarp();
+        if (lane < DC)
+          tma_load_4d(sQ + (k & 1) * S::QB + lane * 128 * 128, &qmap, 0, lane, u.head * G,
+                      s_first[u.b] + u.tile * p.tile_nodes, &q_full[k & 1]);
+      }
       const int32_t* table = u.ctx > 0 ? p.tables + (int64_t)s_row[u.b] * p.table_stride : nullptr;
       const int nkb = ceil_div(u.ctx, kBS);
       const int own = max(0, u.nns - u.s0);  // leading stages of the tree's own keys
@@ -343,17 +359,19 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       auto ts_of = [&](int j) { return tmem + (stream * 2 + j / kStreams % 2) * kNK; };  // S(j), then P(j)
       // Descriptors are computed before the waits, so that the MMAs issue back to back.
       auto pin = [](uint64_t& x) { asm volatile("" : "+l"(x)); };
-      auto issue_s = [&](int j) -> bool {
+      auto issue_s = [&](int j, int k) -> bool {  // of piece k
         const int st = j % kRing;
         uint64_t aq[D / 16], bk[D / 16];
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          aq[kk] = umma_desc_sw128(smem_u32(sQ + (kk / 4) * 128 * 128 + (kk % 4) * 32), 16, 1024);
+          aq[kk] = umma_desc_sw128(smem_u32(sQ + (k & 1) * S::QB + (kk / 4) * 128 * 128 + (kk % 4) * 32), 16, 1024);
           bk[kk] = umma_desc_sw128(smem_u32(sK + st * S::KSB + (kk / 4) * kNK * 128 + (kk % 4) * 32), 16, 1024);
           pin(aq[kk]);
           pin(bk[kk]);
         }
         if (!mbar_wait_until(&k_full[st], (j / kRing) & 1, deadline)) return false;
+        const int jb = j - 2 * kStreams;  // whose P the score buffer holds, until its O has read it
+        if (jb >= 0 && !mbar_wait_until(&o_done[jb % kRing], (jb / kRing) & 1, deadline)) return false;
         tc_fence_after_sync();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) umma_f16_ss(ts_of(j), aq[kk], bk[kk], idesc_s, kk > 0);
@@ -376,21 +394,22 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         umma_commit(&o_done[st]);
         return true;
       };
+      // A piece's first scores are made while the softmax warps still finish the one before;
+      // only its first O waits until they have read the accumulators.
       bool ok = true;
-      int gs = 0, k = 0;
+      int gs = 0, k = 0, mine = 0;
       Piece u;
-      for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst) {
+      for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst, ++k) {
         const int i0 = first_of(stream, gs);
         if (i0 >= u.nst) continue;
-        ok = mbar_wait_until(&q_ready[stream], k++ & 1, deadline) && issue_s(gs + i0) &&
-             (i0 + kStreams >= u.nst || issue_s(gs + i0 + kStreams));
-        for (int i = i0; i < u.nst && ok; i += kStreams) {
-          const int j = gs + i;  // S two stages on goes over P(j), once O has read it
-          ok = issue_o(j, i == i0) &&
-               (i + 2 * kStreams >= u.nst ||
-                (mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline) && issue_s(j + 2 * kStreams)));
-        }
+        ok = mbar_wait_until(&q_full[k & 1], (k >> 1) & 1, deadline) && issue_s(gs + i0, k) &&
+             (i0 + kStreams >= u.nst || issue_s(gs + i0 + kStreams, k)) &&
+             (mine == 0 || mbar_wait_until(&o_free[stream], (mine - 1) & 1, deadline));
+        for (int i = i0; i < u.nst && ok; i += kStreams)
+          ok = issue_o(gs + i, i == i0) && (i + 2 * kStreams >= u.nst || issue_s(gs + i + 2 * kStreams, k));
+        ++mine;
       }
+      k = mine;
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       if (k > 0) umma_commit(mma_done); else mbar_arrive(mma_done);
     }
@@ -406,39 +425,19 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     auto confirm = [&](int j) {  // O += P(j) V(j) has completed
       if (ok && !mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline)) ok = false;
     };
-    int gs = 0, k = 0;
-    Piece u;
-    for (int pos = pos0; next_piece(pos, u); gs += u.nst, ++k) {
+    int gs = 0, k = 0, pos = pos0;
+    Piece u, ahead;
+    // The mask word of a piece's stage, for this row: the tree's own keys that it may see.
+    auto mask_of = [&](const Piece& x, int stage) -> uint64_t {
+      return stage < x.nns && r < x.rows
+                 ? p.mask[((int64_t)s_first[x.b] + x.tile * p.tile_nodes + t) * p.words + stage] : 0;
+    };
+    bool more = next_piece(pos, u);
+    uint64_t see_next = more ? mask_of(u, u.s0 + first_of(stream, 0)) : 0;
+    for (; more; gs += u.nst, ++k, u = ahead) {
       const bool valid = r < u.rows;
       const bool live = (warp % 4) * 32 < u.rows;  // some row of the warp has a query
       const int64_t node = (int64_t)s_first[u.b] + u.tile * p.tile_nodes + t;
-      {  // Q: each stream's warps store their share of the columns
-        const T* qrow = reinterpret_cast<const T*>(p.q) + node * p.q_st + (int64_t)(u.head * G + gq) * p.q_sh;
-        for (int c = stream; c < D / 32; c += kStreams) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (valid) {
-              if (p.q_vec16) {
-                v = *reinterpret_cast<const uint4*>(qrow + c * 32 + 8 * x);
-              } else {
-                const uint32_t* q32 = reinterpret_cast<const uint32_t*>(qrow + c * 32 + 8 * x);
-                v = make_uint4(q32[0], q32[1], q32[2], q32[3]);
-              }
-            }
-            const int g = (c % 2) * 4 + x;  // 16-byte granule of the row's 128
-            *reinterpret_cast<uint4*>(sQ + (c / 2) * 128 * 128 + r * 128 + ((g ^ (r & 7)) * 16)) = v;
-          }
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-#pragma unroll
-        for (int s = 0; s < kStreams; ++s)
-          if (first_of(s, gs) < u.nst) mbar_arrive(&q_ready[s]);
-      }
 
       float m = -INFINITY, l = 0.f;
       const int i0 = first_of(stream, gs);
@@ -448,8 +447,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         const int keys = own ? u.nodes - sg * kNK : u.ctx - (sg - u.nns) * kNK;  // of the stage, if < kNK
         const int buf = j / kStreams % 2;
         const uint32_t ts = tl + (stream * 2 + buf) * kNK;
-        uint64_t see = ~0ull;
-        if (own) see = valid ? p.mask[node * p.words + sg] : 0;
+        uint64_t see = own ? see_next : ~0ull;
+        if (i + kStreams < u.nst) see_next = mask_of(u, sg + kStreams);
         if (keys < kNK) see &= (1ull << keys) - 1;
         if (ok && !mbar_wait_until(&s_done[st], (j / kRing) & 1, deadline)) ok = false;
         tc_fence_after_sync();
@@ -457,10 +456,11 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         // included: 0 x NaN would reach the output, so they are cleared in place.
         if (keys < kNK) {
           if (ok && !mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) ok = false;
-          const int gap = (kNK - keys) * 8;
-          for (int x = r; x < gap * DC; x += 128) {
-            const int c = x / gap, y = x - c * gap;
-            *reinterpret_cast<uint4*>(sV + st * S::KSB + c * kNK * 128 + keys * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+          uint8_t* const gap = sV + st * S::KSB + keys * 128 + r * 16;
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            for (int x = 0; x < (kNK - keys) * 8 - r; x += 128)
+              *reinterpret_cast<uint4*>(gap + c * kNK * 128 + x * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
@@ -529,6 +529,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[stream * 2 + buf]);
       }
+      more = next_piece(pos, ahead);
+      see_next = more ? mask_of(ahead, ahead.s0 + first_of(stream, gs + u.nst)) : 0;
       // The piece's streams joined: maxima and sums through shared memory, then each stream's
       // warps take their share of the output columns from every accumulator.
       if (i0 < u.nst) confirm(gs + (u.nst - 1 - i0) / kStreams * kStreams + i0);
@@ -537,6 +539,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       ml[stream * 256 + 128 + r] = l;
       tc_fence_before_sync();
       named_barrier_sync(1, SW * 32);
+      if (tid == 0) mbar_arrive(&q_free[k & 1]);  // every stream's last O is done, so every S is
       tc_fence_after_sync();
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       if (live) {
@@ -591,6 +594,13 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
             }
           }
         }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int x = 0; x < kStreams; ++x)
+          if (first_of(x, gs) < u.nst) mbar_arrive(&o_free[x]);
       }
     }
   }
@@ -649,12 +659,12 @@ int tree_ctas() { return num_sms(); }
 int64_t cut_bytes() { return ((int64_t)tree_ctas() * 16 + 255) / 256 * 256; }
 
 template <typename T, int D>
-int launch(const CUtensorMap (&maps)[4], const TreeParams& p, cudaStream_t st) {
+int launch(const CUtensorMap (&maps)[5], const TreeParams& p, cudaStream_t st) {
   using S = TreeShape<D>;
   static SmemAttribute attribute;
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(tree_kernel<T, D>), S::SMEM);
   if (e != cudaSuccess) return cuda_status(e);
-  tree_kernel<T, D><<<tree_ctas(), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], p);
+  tree_kernel<T, D><<<tree_ctas(), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
   const int rc = launch_status();
   if (rc != PKV_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -706,23 +716,25 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   if (!tables->block_tables || !cu_nodes || !context_lens || !out || !q || !k_nodes || !v_nodes || !mask)
     return PKV_ERR_INVALID_ARGUMENT;
   auto addr = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
-  if (((addr(q) | addr(out)) & 3) || ((q_stride_n | q_stride_h | out_stride_n | out_stride_h) & 1))
-    return PKV_ERR_INVALID_ARGUMENT;
-  // The nodes' K/V are read by TMA: rows and heads on 16 bytes.
-  if (((addr(k_nodes) | addr(v_nodes)) & 15) || ((k_stride_n | k_stride_h | v_stride_n | v_stride_h) & 7) ||
-      k_stride_n < 0 || v_stride_n < 0 || k_stride_h < 0 || v_stride_h < 0)
-    return PKV_ERR_INVALID_ARGUMENT;
+  if ((addr(out) & 3) || ((out_stride_n | out_stride_h) & 1)) return PKV_ERR_INVALID_ARGUMENT;
+  // Q and the nodes' K/V are read by TMA: rows and heads on 16 bytes.
+  const int64_t strides[6] = {q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h};
+  if ((addr(q) | addr(k_nodes) | addr(v_nodes)) & 15) return PKV_ERR_INVALID_ARGUMENT;
+  for (int64_t x : strides)
+    if (x < 0 || x % 8 || x >= (int64_t)1 << 38) return PKV_ERR_INVALID_ARGUMENT;
   if (!workspace || (addr(workspace) & 255)) return PKV_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < pkv_tree_attention_workspace_bytes(num_seqs, d)) return PKV_ERR_WORKSPACE;
-  CUtensorMap maps[4];
+  CUtensorMap maps[5];
   if (!get_pool_maps(*pool, &maps[0], &maps[1], 1, 1)) return PKV_ERR_CUDA;
-  int rc = make_rows_tensor_map(&maps[2], k_nodes, pool->dtype, d, hkv, total_nodes, k_stride_h, k_stride_n, kNK);
+  int rc = make_rows_tensor_map(&maps[2], k_nodes, pool->dtype, d, hkv, total_nodes, k_stride_h, k_stride_n, 1, kNK);
   if (rc == PKV_OK)
-    rc = make_rows_tensor_map(&maps[3], v_nodes, pool->dtype, d, hkv, total_nodes, v_stride_h, v_stride_n, kNK);
+    rc = make_rows_tensor_map(&maps[3], v_nodes, pool->dtype, d, hkv, total_nodes, v_stride_h, v_stride_n, 1, kNK);
+  if (rc == PKV_OK)
+    rc = make_rows_tensor_map(&maps[4], q, pool->dtype, d, num_q_heads, total_nodes, q_stride_h, q_stride_n, group,
+                              128 / group);
   if (rc != PKV_OK) return rc;
   TreeParams p;
   p.out = out;
-  p.q = q;
   p.cu = cu_nodes;
   p.ctx = context_lens;
   p.mask = reinterpret_cast<const uint64_t*>(mask);
@@ -733,7 +745,6 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + cut_bytes());
   p.part_o = p.part_ml + 2 * (int64_t)tree_ctas() * 256;
   p.out_st = out_stride_n, p.out_sh = out_stride_h;
-  p.q_st = q_stride_n, p.q_sh = q_stride_h;
   p.table_stride = tables->stride;
   p.total_nodes = total_nodes;
   p.table_rows = tables->rows;
@@ -747,7 +758,6 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   p.nbt = pool->num_blocks_total;
   p.max_nodes = max_nodes;
   p.scale_log2 = scale * kLog2e;
-  p.q_vec16 = (addr(q) & 15) == 0 && ((q_stride_n | q_stride_h) & 7) == 0;
   p.out_vec16 = (addr(out) & 15) == 0 && ((out_stride_n | out_stride_h) & 7) == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (pool->dtype == PKV_F16)

@@ -626,8 +626,7 @@ def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor
     batch = cu_nodes.numel() - 1
     if mask.dim() != 2 or mask.shape[0] != n or batch < 0 or context_lens.numel() < batch:
         raise ValueError("tree_attention: mask [N, W], context_lens [B], cu_nodes [B + 1]")
-    q = _rows_last_contiguous(q)
-    k_nodes, v_nodes = _rows16(k_nodes), _rows16(v_nodes)
+    q, k_nodes, v_nodes = _rows16(q), _rows16(k_nodes), _rows16(v_nodes)
     if out is None:
         out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
