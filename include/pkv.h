@@ -438,8 +438,10 @@ PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* q
  *                pool. q, k_nodes and v_nodes have 16-byte aligned rows and heads (strides
  *                multiples of 8 elements, >= 0)
  *   max_nodes        : no tree has more (<= 64 * mask_words, mask_words <= 8)
- *   workspace        : pkv_tree_attention_workspace_bytes bytes, 256-byte aligned; contents
- *                do not matter; calls that share one must not overlap on the GPU
+ *   workspace        : pkv_tree_attention_workspace_bytes bytes, 256-byte aligned, zeroed once
+ *                before first use; every call leaves it ready for the next, whatever its sizes.
+ *                Calls that share a workspace must not overlap on the GPU. After a call that
+ *                reported a timed-out wait, pkv_decode_reset_workspace clears its counters.
  * Rows past cu_nodes[num_seqs] of out are not written. Slots of the pool past
  * context_lens may hold anything, NaN included; K/V that any node of a tree may see must be
  * finite. Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head

@@ -46,8 +46,9 @@ constexpr int kRing = 4;         // stages of the K ring and of the V ring
 constexpr int kBars = 4 * kRing + 3 * kStreams + 5;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
-constexpr int kItemCost = 4;     // an item's start and end, in stages
-constexpr int kMinRange = 6;     // no CTA gets less than this
+constexpr int kItemCost = 6;     // an item's start and end, in stages
+constexpr int kMinRange = 8;     // no CTA gets less than this
+constexpr int kMaxPieces = 160;  // CTAs at most: an item's pieces
 constexpr float kLog2e = 1.4426950408889634f;
 // Every slot of a ring belongs to one stream, so that a wait sees each of its phases.
 static_assert(kRing % (2 * kStreams) == 0, "ring slots per stream and score buffer");
@@ -60,6 +61,7 @@ template <int D> struct TreeShape {
   static constexpr int OCOL = kStreams * 2 * kNK;
   static constexpr int NCOLS = 512;
   static_assert(OCOL + kStreams * D <= NCOLS, "TMEM columns");
+  static_assert(kMaxPieces * 128 * 4 <= 2 * QB + 2 * kRing * KSB, "the join's maxima");
   static constexpr int SW = 4 * kStreams;       // softmax warps
   static constexpr int THREADS = (SW + 2 + kStreams) * 32;
   static constexpr int SMEM = 1024 + 2 * QB + 2 * kRing * KSB + (kBars + 2) * 8 + 2 * kStreams * 2 * 128 * 4 +
@@ -78,6 +80,13 @@ struct TreePlan {
   }
 };
 
+// A CTA's piece of an item that several ranges share, for the join.
+struct CutPiece {
+  int node, head, rows;    // the tile's first node, KV head, rows
+  int pieces, index;       // of the item (0: no such piece); which of them this is
+  int first;               // CTA of the first piece
+};
+
 struct TreeParams {
   void* out;
   const int32_t* cu;
@@ -86,10 +95,9 @@ struct TreeParams {
   const int32_t* tables;
   const int32_t* seq_rows;
   int32_t* status;
-  int4* cut;           // [CTAs] the item that begins in a CTA's range and ends in another: its first node,
-                       // KV head | gang << 16, rows, pieces (0: none)
+  int32_t* counts;     // [CTAs][2] of the cut item that begins in a CTA's range: pieces stored, shares joined
   float* part_ml;      // [2 per CTA][2][128] running maximum and sum
-  float* part_o;       // [2 per CTA][D][128]
+  float4* part_o;      // [2 per CTA][D / 4][128 rows]: four columns of a row, so a warp moves 512 bytes at a time
   int64_t out_st, out_sh, table_stride, total_nodes;
   int32_t table_rows, table_cols, batch, hkv, group, tile_nodes, words, layer, nbt;
   int32_t out_vec16, max_nodes;
@@ -97,6 +105,18 @@ struct TreeParams {
 };
 
 __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// A load past L1 (kept in program order, but not waited for).
+__device__ inline float ld_cg(const float* ptr) {
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(ptr));
+  return v;
+}
+__device__ inline float4 ld_cg(const float4* ptr) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(ptr));
+  return v;
+}
 
 // 4-D bulk tensor copy global -> shared (no multicast), completion on an mbarrier.
 __device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
@@ -157,13 +177,14 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   int32_t* s_nodes = s_first + kMaxSeqs;                                       // [batch] nodes
   int32_t* s_ctx = s_nodes + kMaxSeqs;                                         // [batch] cached keys
   int32_t* s_row = s_ctx + kMaxSeqs;                                           // [batch] table row
+  __shared__ CutPiece s_cut[2];  // this range's cut pieces: one that began before it, one that ends behind it
   __shared__ int4 s_warp[32];  // per warp: least and most tiles, stages with a tile an item and with tiles in gangs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.batch, G = p.group;
 
-  grid_dep_launch_dependents();  // the join's CTAs may wait in place
   // Set-up by warps that have no lengths to read in a small batch.
   if (warp == SW && lane == 0) {
+    s_cut[0].pieces = s_cut[1].pieces = 0;
     for (int i = 0; i < 4 * kRing; ++i) mbar_init(&bars[i], 1);
     for (int i = 0; i < 2 * kStreams; ++i) mbar_init(&p_full[i], 4);
     for (int i = 0; i < kStreams; ++i) mbar_init(&o_free[i], SW);
@@ -230,7 +251,6 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     plan.ranges = max(1, min((int)gridDim.x / plan.gang, total / kMinRange));
     plan.quota = total / plan.ranges;
     plan.rem = total - plan.quota * plan.ranges;
-    if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   __syncthreads();
   tc_fence_after_sync();
@@ -277,7 +297,12 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   };
   auto first_of = [](int stream, int gs) { return (stream + kStreams - gs % kStreams) % kStreams; };  // its first stage
 
-  if (warp < SW + 2 && warp >= SW) {
+  // Registers: the copy and MMA warps (one warpgroup) hand most of theirs to the softmax
+  // warps. 256 x 224 + 128 x 56 = 384 x 168, what the launch got.
+  static_assert(S::THREADS == 384 && SW == 8, "register split");
+  if (warp >= SW) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp < SW + 2) {
     // ---------------------------------------------------------------- TMA copies: a warp for K, one for V
     // A copy costs the issuing warp about 85 cycles whichever lane issues it (measured): with
     // one warp for both, 16 copies and two waits made 2000 cycles a stage at head_dim 128 and
@@ -348,7 +373,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       }
     }
     if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
-  } else if (warp >= SW + 2) {
+  } else {
     // ---------------------------------------------------------------- MMA issue, one warp per stream
     if (lane == 0) {
       const int stream = warp - SW - 2;
@@ -413,8 +438,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       if (k > 0) umma_commit(mma_done); else mbar_arrive(mma_done);
     }
+  }
   } else {
     // ---------------------------------------------------------------- softmax warps
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int stream = warp / 4;
     const int r = (warp % 4) * 32 + lane;  // TMEM lane = tile row
     const int t = r / G, gq = r - t * G;   // node of the tile, query head of the group
@@ -531,6 +558,31 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       }
       more = next_piece(pos, ahead);
       see_next = more ? mask_of(ahead, ahead.s0 + first_of(stream, gs + u.nst)) : 0;
+      // An item of two pieces is finished by the CTA of the first, at the end of its range: the
+      // other piece was its CTA's first, stored long ago. One of more pieces is finished by all
+      // of its CTAs, below.
+      int first = 0, pieces = 1;  // of the item: CTA of the first piece, pieces
+      if (!(u.begins && u.ends)) {
+        const int g0 = plan.range_of(u.item_end - (ceil_div(u.ctx, kNK) + u.nns));  // the first stage's range
+        first = g0 * plan.gang + member;
+        pieces = plan.range_of(u.item_end - 1) - g0 + 1;
+      }
+      const bool takes = pieces == 2 && u.begins, gives = pieces > 1 && !takes;
+      constexpr int kChunks = D / 16 / kStreams;  // a stream's share of the output, in 16 columns
+      float4 taken[kChunks * 4];
+      float m2 = -INFINITY, l2 = 0.f;
+      if (takes) {
+        const int64_t rest = 2 * ((int64_t)blockIdx.x + plan.gang);
+        if (lane == 0) {
+          while (ok && ld_acquire_gpu(&p.counts[2 * first]) < 1) ok = global_ns() <= deadline;
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        m2 = ld_cg(&p.part_ml[rest * 256 + r]);
+        l2 = ld_cg(&p.part_ml[rest * 256 + 128 + r]);
+#pragma unroll
+        for (int x = 0; x < kChunks * 4; ++x)
+          taken[x] = ld_cg(p.part_o + (rest * (D / 4) + (stream + x / 4 * kStreams) * 4 + x % 4) * 128 + r);
+      }
       // The piece's streams joined: maxima and sums through shared memory, then each stream's
       // warps take their share of the output columns from every accumulator.
       if (i0 < u.nst) confirm(gs + (u.nst - 1 - i0) / kStreams * kStreams + i0);
@@ -539,7 +591,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       ml[stream * 256 + 128 + r] = l;
       tc_fence_before_sync();
       named_barrier_sync(1, SW * 32);
-      if (tid == 0) mbar_arrive(&q_free[k & 1]);  // every stream's last O is done, so every S is
+      if (tid == 0) {
+        mbar_arrive(&q_free[k & 1]);  // every stream's last O is done, so every S is
+        if (takes) st_relaxed_gpu(&p.counts[2 * first], 0);  // as the next call needs it
+      }
       tc_fence_after_sync();
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       if (live) {
@@ -552,21 +607,34 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           wgt[s] = ex2(ml[s * 256 + r] - mref);
           sum += wgt[s] * ml[s * 256 + 128 + r];
         }
-        const bool cut = !(u.begins && u.ends);
         const int64_t slot = 2 * (int64_t)blockIdx.x + u.begins;
-        if (u.begins && !u.ends && tid == 0)
-          p.cut[blockIdx.x] = make_int4(s_first[u.b] + u.tile * p.tile_nodes, u.head | plan.gang << 16, u.rows,
-                                        plan.range_of(u.item_end - 1) - range + 1);
-        if (cut && stream == 0) {
+        float w_rest = 0.f;
+        if (takes) {
+          const float all = fmaxf(top, m2), aref = all == -INFINITY ? 0.f : all, w_own = ex2(top - aref);
+          w_rest = ex2(m2 - aref);
+          sum = w_own * sum + w_rest * l2;
+#pragma unroll
+          for (int s = 0; s < kStreams; ++s) wgt[s] *= w_own;
+        }
+        if (gives && stream == 0) {
           p.part_ml[slot * 256 + r] = top;
           p.part_ml[slot * 256 + 128 + r] = sum;
         }
-        const float inv = cut ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // no visible key: zeros
+        const float inv = gives ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // no visible key: zeros
         T* orow = reinterpret_cast<T*>(p.out) + node * p.out_st + (int64_t)(u.head * G + gq) * p.out_sh;
-        for (int c = stream; c < D / 16; c += kStreams) {
+#pragma unroll
+        for (int share = 0; share < kChunks; ++share) {
+          const int c = stream + share * kStreams;
           float acc[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+          if (takes) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 v = taken[share * 4 + e / 4];
+              acc[e] = w_rest * v.x, acc[e + 1] = w_rest * v.y, acc[e + 2] = w_rest * v.z, acc[e + 3] = w_rest * v.w;
+            }
+          }
 #pragma unroll
           for (int s = 0; s < kStreams; ++s) {
             if (first_of(s, gs) >= u.nst) continue;  // its accumulator holds nothing of this piece
@@ -577,10 +645,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
             for (int e = 0; e < 16; ++e) acc[e] += wgt[s] * __uint_as_float(ob[e]);
           }
           if (!valid || !ok) continue;
-          if (cut) {
-            float* po = p.part_o + (slot * D + c * 16) * 128 + r;
+          if (gives) {
+            float4* po = p.part_o + (slot * (D / 4) + c * 4) * 128 + r;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) po[e * 128] = acc[e];
+            for (int e = 0; e < 16; e += 4) po[e / 4 * 128] = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
           } else {
             uint32_t w[8];
 #pragma unroll
@@ -602,6 +670,118 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         for (int x = 0; x < kStreams; ++x)
           if (first_of(x, gs) < u.nst) mbar_arrive(&o_free[x]);
       }
+      if (gives) {  // the piece's state is stored: count it
+        named_barrier_sync(1, SW * 32);
+        if (tid == 0) {
+          if (pieces > 2)
+            s_cut[u.begins] = CutPiece{(int)node, u.head, u.rows, pieces, range - first / plan.gang, first};
+          atom_add_acq_rel_gpu(&p.counts[2 * first], 1);
+        }
+      }
+    }
+    // ---------------------------------------------------------------- join of items of three pieces and more
+    // With M the largest of an item's pieces' maxima,
+    //   out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
+    // The item's CTAs each wait for all of its pieces (a CTA has stored its own two before it
+    // waits for anyone's, and all CTAs are resident) and take a share of the columns, so an
+    // item cut into many pieces has as many CTAs to read them. The pieces' maxima go to
+    // shared memory, over the drained rings; a thread takes one row.
+    auto slot_of = [&](const CutPiece& cut, int x) { return 2 * ((int64_t)cut.first + x * plan.gang) + (x == 0); };
+    float* const maxima = reinterpret_cast<float*>(smem) + r;  // [pieces] of this row
+    named_barrier_sync(1, SW * 32);
+    for (int side = 0; side < 2; ++side) {
+      const CutPiece cut = s_cut[side];
+      if (cut.pieces == 0) continue;
+      int32_t* const counts = p.counts + 2 * cut.first;
+      if (tid == 0) {
+        while (ok && ld_acquire_gpu(counts) < cut.pieces) ok = global_ns() <= deadline;
+        if (!ok) report(p.status, PKV_ERR_TIMEOUT);
+        s_warp[0].x = ok;
+      }
+      named_barrier_sync(1, SW * 32);
+      // Loads go out in batches (past L1, which other CTAs' stores do not reach); an index past
+      // the end repeats the last with weight 0. Each stream's warps read every other piece's
+      // maximum and sum.
+      const bool joins = s_warp[0].x && r < cut.rows;
+      const int last = cut.pieces - 1;
+      float* const ml = s_ml + r;
+      float top = -INFINITY, sum = 0.f;
+      if (joins) {
+        for (int x0 = stream; x0 <= last; x0 += 8 * kStreams) {
+          float v[8], w[8], most = top, part = 0.f;
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const int64_t at = slot_of(cut, min(x0 + y * kStreams, last)) * 256 + r;
+            v[y] = ld_cg(&p.part_ml[at]);
+            w[y] = ld_cg(&p.part_ml[at + 128]);
+          }
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            if (x0 + y * kStreams > last) continue;
+            maxima[(x0 + y * kStreams) * 128] = v[y];
+            most = fmaxf(most, v[y]);
+          }
+          const float mref = most == -INFINITY ? 0.f : most;
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            if (x0 + y * kStreams <= last) part += ex2(v[y] - mref) * w[y];
+          sum = sum * ex2(top - mref) + part;
+          top = most;
+        }
+      }
+      ml[stream * 256] = top;
+      ml[stream * 256 + 128] = sum;
+      named_barrier_sync(1, SW * 32);
+      if (joins) {
+        const float t2 = ml[(1 - stream) * 256], all = fmaxf(top, t2), mref = all == -INFINITY ? 0.f : all;
+        sum = sum * ex2(top - mref) + ml[(1 - stream) * 256 + 128] * ex2(t2 - mref);
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        auto weight = [&](int x) { return x <= last ? ex2(maxima[x * 128] - mref) : 0.f; };
+        // Quads of columns: this CTA's share, the streams' warps taking every other one. Few
+        // pieces: a batch is four quads of four pieces; many: a quad of sixteen pieces.
+        const int q_end = (cut.index + 1) * (D / 4) / cut.pieces;
+        T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)cut.node + t) * p.out_st + (int64_t)(cut.head * G + gq) * p.out_sh;
+        auto add = [](float4& a, float w, const float4& v) { a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w; };
+        auto put = [&](int qd, const float4& a) {
+          uint32_t* o = reinterpret_cast<uint32_t*>(orow + 4 * qd);
+          o[0] = Dt<T>::pack(a.x * inv, a.y * inv);
+          o[1] = Dt<T>::pack(a.z * inv, a.w * inv);
+        };
+        auto state = [&](int x, int qd) { return ld_cg(p.part_o + (slot_of(cut, x) * (D / 4) + qd) * 128 + r); };
+        const int step = cut.pieces < 8 ? 4 : 1;
+        for (int qd = cut.index * (D / 4) / cut.pieces + stream; qd < q_end; qd += kStreams * step) {
+          float4 acc[4] = {};
+          if (step > 1) {
+            for (int x0 = 0; x0 <= last; x0 += 4) {
+              float4 v[16];
+#pragma unroll
+              for (int y = 0; y < 16; ++y) v[y] = state(min(x0 + y / 4, last), min(qd + y % 4 * kStreams, q_end - 1));
+#pragma unroll
+              for (int y = 0; y < 16; ++y)
+                if (x0 + y / 4 <= last) add(acc[y % 4], weight(x0 + y / 4), v[y]);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (qd + y * kStreams < q_end) put(qd + y * kStreams, acc[y]);
+          } else {
+            for (int x0 = 0; x0 <= last; x0 += 16) {
+              float4 v[16];
+#pragma unroll
+              for (int y = 0; y < 16; ++y) v[y] = state(min(x0 + y, last), qd);
+#pragma unroll
+              for (int y = 0; y < 16; ++y)
+                if (x0 + y <= last) add(acc[0], weight(x0 + y), v[y]);
+            }
+            put(qd, acc[0]);
+          }
+        }
+      }
+      named_barrier_sync(1, SW * 32);
+      // The last share to be joined leaves the counters as the next call needs them.
+      if (tid == 0 && ok && atom_add_acq_rel_gpu(counts + 1, 1) == cut.pieces - 1) {
+        st_relaxed_gpu(counts, 0);
+        st_relaxed_gpu(counts + 1, 0);
+      }
     }
   }
   __syncthreads();
@@ -612,51 +792,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   }
 }
 
-// Joins the pieces of a cut item: with M the largest of their maxima,
-//   out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// One CTA per (CTA of the first kernel whose range cuts an item it begins, 32 output columns);
-// a thread takes one row and eight columns, so the states are read a row to a lane, and its
-// output is one 16-byte write.
-constexpr int kJoinCols = 32;
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128 * (kJoinCols / 8)) tree_join_kernel(const TreeParams p) {
-  grid_dep_wait();
-  const int4 cut = p.cut[blockIdx.x];
-  const int head = cut.y & 0xffff, gang = cut.y >> 16, pieces = cut.w;
-  const int r = threadIdx.x % 128, c0 = blockIdx.y * kJoinCols + (threadIdx.x / 128) * 8;
-  if (r >= cut.z || pieces == 0) return;
-  auto slot = [&](int k) { return 2 * ((int64_t)blockIdx.x + k * gang) + (k == 0); };
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int k = 0; k < pieces; ++k) top = fmaxf(top, p.part_ml[slot(k) * 256 + r]);
-  const float mref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, acc[8] = {};
-#pragma unroll 4
-  for (int k = 0; k < pieces; ++k) {
-    const int64_t u = slot(k);
-    const float wgt = ex2(p.part_ml[u * 256 + r] - mref);
-    sum += wgt * p.part_ml[u * 256 + 128 + r];
-    const float* o = p.part_o + (u * D + c0) * 128 + r;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += wgt * o[e * 128];
-  }
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  const int t = r / p.group, gq = r - t * p.group;
-  T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)cut.x + t) * p.out_st + (int64_t)(head * p.group + gq) * p.out_sh + c0;
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = Dt<T>::pack(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  if (p.out_vec16) {
-    *reinterpret_cast<uint4*>(orow) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(orow)[e] = w[e];
-  }
-}
-
-int tree_ctas() { return num_sms(); }
-int64_t cut_bytes() { return ((int64_t)tree_ctas() * 16 + 255) / 256 * 256; }
+int tree_ctas() { return std::min(num_sms(), kMaxPieces); }
+constexpr int kCountBytes = 4096;  // the items' counters, at the front of the workspace
 
 template <typename T, int D>
 int launch(const CUtensorMap (&maps)[5], const TreeParams& p, cudaStream_t st) {
@@ -664,19 +801,18 @@ int launch(const CUtensorMap (&maps)[5], const TreeParams& p, cudaStream_t st) {
   static SmemAttribute attribute;
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(tree_kernel<T, D>), S::SMEM);
   if (e != cudaSuccess) return cuda_status(e);
-  tree_kernel<T, D><<<tree_ctas(), S::THREADS, S::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
-  const int rc = launch_status();
-  if (rc != PKV_OK) return rc;
+  // Cooperative: the CTAs wait for one another's pieces, so they must all be resident.
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tree_ctas(), D / kJoinCols);
-  cfg.blockDim = dim3(128 * (kJoinCols / 8));
+  cfg.gridDim = dim3(tree_ctas());
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, p));
+  return cuda_status(cudaLaunchKernelEx(&cfg, tree_kernel<T, D>, maps[0], maps[1], maps[2], maps[3], maps[4], p));
 }
 
 }  // namespace
@@ -686,7 +822,7 @@ using namespace pkv;
 
 extern "C" int64_t pkv_tree_attention_workspace_bytes(int32_t batch, int32_t head_dim) {
   if (batch <= 0 || batch > kMaxSeqs || (head_dim != 64 && head_dim != 128)) return 0;
-  return cut_bytes() + 2 * (int64_t)tree_ctas() * 128 * (head_dim + 2) * 4;
+  return kCountBytes + 2 * (int64_t)tree_ctas() * 128 * (head_dim + 2) * 4;
 }
 
 extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv_tables* tables, int32_t num_seqs,
@@ -741,9 +877,9 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   p.tables = tables->block_tables;
   p.seq_rows = tables->seq_rows;
   p.status = status_dev;
-  p.cut = static_cast<int4*>(workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + cut_bytes());
-  p.part_o = p.part_ml + 2 * (int64_t)tree_ctas() * 256;
+  p.counts = static_cast<int32_t*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCountBytes);
+  p.part_o = reinterpret_cast<float4*>(p.part_ml + 2 * (int64_t)tree_ctas() * 256);
   p.out_st = out_stride_n, p.out_sh = out_stride_h;
   p.table_stride = tables->stride;
   p.total_nodes = total_nodes;

@@ -587,11 +587,15 @@ def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch
 
 
 def tree_attention_workspace(pool: PkvPool, max_seqs: int, device: torch.device | str) -> torch.Tensor:
-    """A workspace for :func:`tree_attention` of up to ``max_seqs`` sequences (its contents do not matter)."""
+    """A zeroed workspace for :func:`tree_attention` of up to ``max_seqs`` sequences (each call leaves it ready).
+
+    Calls that share one must not overlap on the GPU. After a call whose status reports a
+    timed-out wait, :func:`decode_reset_workspace` clears its counters.
+    """
     nbytes = int(lib.pkv_tree_attention_workspace_bytes(max_seqs, pool.head_dim))
     if nbytes == 0:
         raise ValueError("tree_attention takes 1 to 1024 sequences and head_dim 64 or 128")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
