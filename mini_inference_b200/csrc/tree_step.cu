@@ -24,13 +24,17 @@ namespace cg = cooperative_groups;
 // All or nothing: when a request does not fit its row, or the free list is too short, no
 // table, held count or head changes and every slot is -1.
 //
-// Every CTA of one cluster scans all requests for itself (a few thousand integers, read
-// from L2) and then takes its share of the tokens and table entries, so one launch does
-// what a scan kernel and a scatter kernel would; the cluster barrier between the reads
-// and the writes lets the outputs be the inputs' own buffers.
+// Every CTA scans all requests for itself (a few thousand integers, read from L2) and then
+// takes its share of the tokens and table entries, so one launch does what a scan kernel and
+// a scatter kernel would. What the call costs is latency: a launch, one round of loads, the
+// scan's two barriers, a table lookup and the stores. Up to 16 K tokens run as one cluster,
+// whose barrier between the reads and the writes lets the outputs be the inputs' own
+// buffers; more tokens take as many CTAs as they fill (2048 tokens each), and outputs that
+// continue an input in place are then written by a second launch of one CTA.
 constexpr int kPlanSeqs = 4096;   // requests per call
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;      // the portable cluster size
+constexpr int kPlanTokens = 2 * kPlanThreads;  // tokens of a CTA: two per thread
 
 struct PlanParams {
   int32_t* tables;
@@ -48,7 +52,10 @@ struct PlanParams {
   int32_t* head_out;
   int32_t* status;
   int64_t table_stride, num_free, total_tokens;
-  int32_t rows, cols, batch, bs;
+  int32_t rows, cols, batch, bs, shift;  // shift: log2(bs), or -1
+  int32_t clustered, writes_map, writes_state;
+  // n / bs for 0 <= n < 2^31
+  __device__ uint32_t blocks_before(uint32_t n) const { return shift >= 0 ? n >> shift : n / (uint32_t)bs; }
 };
 
 // Exclusive prefix sums of two values per thread over the CTA; totals in *ta, *tb.
@@ -136,49 +143,61 @@ __global__ void __launch_bounds__(kPlanThreads, 1) extend_tables_kernel(const Pl
   bad = __syncthreads_or(bad || total_new > p.total_tokens || head < 0);
   const bool short_of = !bad && total_fresh > max(p.num_free - head, (int64_t)0);
   const bool ok = !bad && !short_of;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  cluster.sync();  // every CTA has read the lengths, held counts and the head
+  if (p.clustered) cg::this_cluster().sync();  // every CTA has read the lengths, held counts and the head
+  const int rank = blockIdx.x, ctas = gridDim.x;
 
-  if (rank == 0) {
+  if (rank == 0 && p.writes_state) {
     if (tid == 0) {
       if (bad) report(p.status, PKV_ERR_OUT_OF_RANGE);
       if (short_of) report(p.status, PKV_ERR_NO_BLOCKS);
       *p.head_out = (int32_t)(head + (ok ? total_fresh : 0));
+      p.cu[B] = s_cu[B];
     }
     for (int b = tid; b < B; b += blockDim.x) {
       p.cu[b] = s_cu[b];
       p.ctx[b] = s_row[b] >= 0 ? s_len[b] + (ok ? s_cu[b + 1] - s_cu[b] : 0) : 0;
       p.held_out[b] = s_held[b] + (ok ? s_fp[b + 1] - s_fp[b] : 0);
     }
-    if (tid == 0) p.cu[B] = s_cu[B];
   }
+  if (!p.writes_map) return;
   const int32_t* fresh_blocks = p.free_blocks + head;
   if (ok) {
-    for (int64_t k = (int64_t)rank * blockDim.x + tid; k < total_fresh; k += (int64_t)ctas * blockDim.x) {
-      const int b = last_at_most(s_fp, B, (int)k);
+    for (int k = rank * blockDim.x + tid; k < (int)total_fresh; k += ctas * blockDim.x) {
+      const int b = last_at_most(s_fp, B, k);
       const int32_t blk = fresh_blocks[k];
       if (blk < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
       p.tables[s_row[b] * p.table_stride + s_held[b] + (k - s_fp[b])] = blk;
     }
   }
   if (!p.positions && !p.slots) return;
-  const int used = s_cu[B];
-  for (int64_t t = (int64_t)rank * blockDim.x + tid; t < p.total_tokens; t += (int64_t)ctas * blockDim.x) {
-    int64_t pos = 0, slot = -1;
-    if (ok && t < used) {
-      const int b = last_at_most(s_cu, B, (int)t);
-      if (s_row[b] >= 0) {
-        pos = (int64_t)s_len[b] + (t - s_cu[b]);
-        const int col = (int)(pos / p.bs);
-        const int32_t blk = col < s_held[b] ? p.tables[s_row[b] * p.table_stride + col]
-                                            : fresh_blocks[s_fp[b] + (col - s_held[b])];
-        if (blk < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
-        else slot = (int64_t)blk * p.bs + pos % p.bs;
+  // Two tokens per thread and turn, written as one 16-byte store where the arrays allow it.
+  const int used = ok ? s_cu[B] : 0, total = (int)p.total_tokens;
+  const bool wide = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.slots)) & 15) == 0;
+  for (int64_t t0 = 2 * ((int64_t)rank * blockDim.x + tid); t0 < total; t0 += 2 * (int64_t)ctas * blockDim.x) {
+    int64_t pos[2] = {0, 0}, slot[2] = {-1, -1};
+    int b = t0 < used ? last_at_most(s_cu, B, (int)t0) : 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int t = (int)t0 + e;
+      if (t0 + e >= used) break;
+      while (s_cu[b + 1] <= t) ++b;  // t is before the batch's end
+      if (s_row[b] < 0) continue;
+      const uint32_t at = (uint32_t)(s_len[b] + (t - s_cu[b])), col = p.blocks_before(at);
+      const int32_t blk = (int)col < s_held[b] ? p.tables[s_row[b] * p.table_stride + col]
+                                               : fresh_blocks[s_fp[b] + ((int)col - s_held[b])];
+      pos[e] = at;
+      if (blk < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+      else slot[e] = (int64_t)blk * p.bs + (at - col * (uint32_t)p.bs);
+    }
+    if (wide && t0 + 1 < total) {
+      if (p.positions) *reinterpret_cast<longlong2*>(p.positions + t0) = make_longlong2(pos[0], pos[1]);
+      if (p.slots) *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
+    } else {
+      for (int e = 0; e < 2 && t0 + e < total; ++e) {
+        if (p.positions) p.positions[t0 + e] = pos[e];
+        if (p.slots) p.slots[t0 + e] = slot[e];
       }
     }
-    if (p.positions) p.positions[t] = pos;
-    if (p.slots) p.slots[t] = slot;
   }
 }
 
@@ -186,83 +205,69 @@ __global__ void __launch_bounds__(kPlanThreads, 1) extend_tables_kernel(const Pl
 // mask[n] = bits of node n's ancestors and itself, 64 nodes to a word; position =
 // context_lens[b] + depth, depth = popcount(mask) - 1. A node's ancestors are gathered by
 // pointer doubling in shared memory: after round k a node's mask covers its 2^k nearest
-// ancestors and jump points 2^k up, so a chain of 512 nodes takes 9 rounds instead of 512
-// dependent loads. One CTA per tree, one thread per node.
+// ancestors and its jump points 2^k up, so a chain of 512 nodes takes 9 rounds instead of 512
+// dependent loads. One CTA per tree, one thread per node that the mask has room for.
 constexpr int kTreeWords = 8;                  // mask words
 constexpr int kTreeNodes = 64 * kTreeWords;    // nodes of a tree
 
-__global__ void tree_metadata_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ cu,
-                                     int32_t batch, const int32_t* __restrict__ ctx, int64_t total,
-                                     uint64_t* __restrict__ mask, int32_t words, int64_t* __restrict__ positions,
-                                     int32_t* status) {
-  extern __shared__ uint64_t tree_smem[];
-  const int b = blockIdx.x, tid = threadIdx.x, cap = 64 * words;
+template <int WORDS>
+__global__ void __launch_bounds__(64 * WORDS)
+    tree_metadata_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ cu, int32_t batch,
+                         const int32_t* __restrict__ ctx, int64_t total, uint64_t* __restrict__ mask, int32_t words,
+                         int64_t* __restrict__ positions, int32_t* status) {
+  constexpr int kCap = 64 * WORDS;
+  __shared__ uint64_t bits[WORDS][kCap];
+  __shared__ int32_t jump[kCap];
+  const int b = blockIdx.x, i = threadIdx.x;
   if (b == batch) {  // rows behind the last tree: padding of a captured step
-    for (int64_t n = max(cu[batch], 0) + tid; n < total; n += blockDim.x) {
+    for (int64_t n = max(cu[batch], 0) + i; n < total; n += kCap) {
       for (int w = 0; w < words; ++w) mask[n * words + w] = 0;
       positions[n] = 0;
     }
     return;
   }
   const int lo = cu[b], hi = cu[b + 1];
+  const int64_t at = ctx[b];
   if (lo < 0 || hi < lo || hi > total) {
-    if (tid == 0) report(status, PKV_ERR_OUT_OF_RANGE);
+    if (i == 0) report(status, PKV_ERR_OUT_OF_RANGE);
     return;
   }
-  const int all = hi - lo, n = min(all, cap);
-  if (all > cap && tid == 0) report(status, PKV_ERR_OUT_OF_RANGE);
-  uint64_t* bits = tree_smem;                               // [words][n]
-  int32_t* jump = reinterpret_cast<int32_t*>(bits + (size_t)words * cap);  // [n]
-  for (int i = tid; i < n; i += blockDim.x) {
-    int up = parents[lo + i];
+  const int all = hi - lo, n = min(all, 64 * words);
+  if (all > n && i == 0) report(status, PKV_ERR_OUT_OF_RANGE);
+  uint64_t own[WORDS];
+  int up = -1;
+  if (i < n) {
+    up = parents[lo + i];
     if (up < -1 || up >= i) {
       report(status, PKV_ERR_OUT_OF_RANGE);
       up = -1;
     }
+  }
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) own[w] = w == i / 64 ? 1ull << (i % 64) : 0;
+  while (__syncthreads_or(up >= 0)) {  // (the round before has read what this one overwrites)
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) bits[w][i] = own[w];
     jump[i] = up;
-    for (int w = 0; w < words; ++w) bits[w * cap + i] = w == i / 64 ? 1ull << (i % 64) : 0;
-  }
-  // Each thread owns the nodes tid, tid + blockDim, ...: reads of the round before the
-  // barrier, writes after it.
-  constexpr int kOwn = kTreeNodes / 128;
-  int next[kOwn];
-  uint64_t got[kOwn][kTreeWords];
-  for (bool more = true; more;) {
     __syncthreads();
-    more = false;
+    if (up >= 0) {
 #pragma unroll
-    for (int o = 0; o < kOwn; ++o) {
-      const int i = tid + o * 128;
-      next[o] = -2;
-      if (i < n && jump[i] >= 0) {
-        const int j = jump[i];
-#pragma unroll
-        for (int w = 0; w < kTreeWords; ++w) got[o][w] = w < words ? bits[w * cap + j] : 0;
-        next[o] = jump[j];
-        more |= next[o] >= 0;
-      }
-    }
-    more = __syncthreads_or(more);
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) {
-      const int i = tid + o * 128;
-      if (next[o] != -2) {
-#pragma unroll
-        for (int w = 0; w < kTreeWords; ++w)
-          if (w < words) bits[w * cap + i] |= got[o][w];
-        jump[i] = next[o];
-      }
+      for (int w = 0; w < WORDS; ++w) own[w] |= bits[w][up];
+      up = jump[up];
     }
   }
-  const int64_t at = ctx[b];
-  for (int i = tid; i < all; i += blockDim.x) {
+  if (i < n) {
     int depth = -1;
-    for (int w = 0; w < words; ++w) {
-      const uint64_t m = i < n ? bits[w * cap + i] : 0;
-      mask[(int64_t)(lo + i) * words + w] = m;
-      depth += __popcll(m);
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      if (w < words) mask[(int64_t)(lo + i) * words + w] = own[w];
+      depth += __popcll(own[w]);
     }
-    positions[lo + i] = at + max(depth, 0);
+    positions[lo + i] = at + depth;
+  }
+  for (int x = n + i; x < all; x += kCap) {  // nodes the mask has no room for
+    for (int w = 0; w < words; ++w) mask[(int64_t)(lo + x) * words + w] = 0;
+    positions[lo + x] = at;
   }
 }
 
@@ -307,7 +312,7 @@ template <int EW>
 __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const AcceptParams p) {
   __shared__ int32_t s_parent[kTreeNodes];
   __shared__ int64_t s_draft[kTreeNodes], s_target[kTreeNodes];
-  __shared__ int32_t s_path[kAcceptWidth], s_block[kAcceptWidth], s_count;
+  __shared__ int32_t s_path[kAcceptWidth], s_block[kAcceptWidth], s_offset[kAcceptWidth], s_count;
   using V = typename Bytes<EW>::type;
   const int tid = threadIdx.x, lane = tid & 31;
   cg::cluster_group cluster = cg::this_cluster();
@@ -349,12 +354,40 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const Accep
         blk = -1;
       }
       s_block[k] = blk;
+      s_offset[k] = (int)(((int64_t)len + k) % p.bs);
     }
     if (lane == 0) s_count = count;
   }
   __syncthreads();
   const int count = s_count;
-  cluster.sync();  // every CTA has read the length: lengths_out may be the same buffer
+  cluster.barrier_arrive();  // this CTA has read the length: lengths_out may be the same buffer
+  // Rows to copy (K or V, path node, head): where each starts in layer 0 of its source and of
+  // the pool. A thread keeps one vector of a row and takes it through four layers at a time.
+  const int per_kind = count * p.hkv, rows = 2 * per_kind, vecs = p.d / EW;
+  const int64_t pool_layer = (int64_t)p.nbt * p.hkv * p.bs * p.d;
+  const int team = max(1, kAcceptThreads / vecs), in_row = tid % vecs, my_row = tid / vecs;
+  for (int x = my_row; x < rows && my_row < team; x += team) {
+    const int which = x >= per_kind, r = x - which * per_kind, k = r / p.hkv, h = r - k * p.hkv;
+    if (s_block[k] < 0) continue;
+    const int64_t node = lo + s_path[k];
+    const uint16_t* src = which ? static_cast<const uint16_t*>(p.v_nodes) + node * p.v_sn + h * p.v_sh
+                                : static_cast<const uint16_t*>(p.k_nodes) + node * p.k_sn + h * p.k_sh;
+    uint16_t* dst = static_cast<uint16_t*>(which ? p.v_pool : p.k_pool) +
+                    ((int64_t)s_block[k] * p.hkv + h) * p.bs * p.d + (int64_t)s_offset[k] * p.d;
+    const int64_t src_layer = which ? p.v_sl : p.k_sl;
+    for (int c = in_row; c < vecs; c += kAcceptThreads) {
+      for (int l0 = rank; l0 < p.layers; l0 += 4 * ctas) {
+        V v[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (l0 + y * ctas < p.layers) v[y] = *reinterpret_cast<const V*>(src + (l0 + y * ctas) * src_layer + c * EW);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (l0 + y * ctas < p.layers) *reinterpret_cast<V*>(dst + (l0 + y * ctas) * pool_layer + c * EW) = v[y];
+      }
+    }
+  }
+  cluster.barrier_wait();
   if (rank == 0) {
     for (int k = tid; k < p.width; k += kAcceptThreads) {
       p.path[(int64_t)b * p.width + k] = k < count ? s_path[k] : -1;
@@ -363,21 +396,6 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const Accep
     if (tid == 0) {
       p.counts[b] = count;
       p.lengths_out[b] = len + count;
-    }
-  }
-  // (layer, K or V, path node, head, vector): a vector of EW elements per thread and turn.
-  const int vecs = p.d / EW, per_row = p.hkv * vecs, per_layer = 2 * count * per_row;
-  for (int l = rank; l < p.layers; l += ctas) {
-    for (int i = tid; i < per_layer; i += kAcceptThreads) {
-      const int which = i / (count * per_row), r = i - which * count * per_row;
-      const int k = r / per_row, hv = r - k * per_row, h = hv / vecs, c = (hv - h * vecs) * EW;
-      if (s_block[k] < 0) continue;
-      const int64_t node = lo + s_path[k];
-      const uint16_t* src = which ? static_cast<const uint16_t*>(p.v_nodes) + l * p.v_sl + node * p.v_sn + h * p.v_sh
-                                  : static_cast<const uint16_t*>(p.k_nodes) + l * p.k_sl + node * p.k_sn + h * p.k_sh;
-      uint16_t* dst = static_cast<uint16_t*>(which ? p.v_pool : p.k_pool) +
-                      (((int64_t)l * p.nbt + s_block[k]) * p.hkv + h) * p.bs * p.d + (int64_t)((len + k) % p.bs) * p.d;
-      *reinterpret_cast<V*>(dst + c) = *reinterpret_cast<const V*>(src + c);
     }
   }
 }
@@ -440,14 +458,44 @@ extern "C" int pkv_extend_tables(const pkv_tables* tables, int32_t num_seqs, con
   p.cols = tables->cols;
   p.batch = num_seqs;
   p.bs = block_size;
+  p.shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+  p.writes_map = p.writes_state = 1;
   const size_t smem = (5 * (size_t)num_seqs + 2) * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(extend_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
+  static SmemAttribute attribute;
+  const cudaError_t e = attribute.set(reinterpret_cast<const void*>(extend_tables_kernel), (5 * kPlanSeqs + 2) * 4);
+  if (e != cudaSuccess) return cuda_status(e);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t tokens = positions || slot_mapping ? total_tokens : 0;
+  const int ctas = (int)std::max<int64_t>(1, (tokens + kPlanTokens - 1) / kPlanTokens);
+  if (ctas <= kPlanCtas) {
+    int cluster = 1;
+    while (cluster < ctas) cluster *= 2;
+    // One CTA of few tokens: no more threads than they and the requests need.
+    const int threads = cluster > 1 ? kPlanThreads
+                                    : std::min<int>(kPlanThreads, (int)(std::max<int64_t>(num_seqs, (tokens + 1) / 2) + 127) / 128 * 128);
+    p.clustered = cluster > 1;
+    return cuda_status(launch_cluster(extend_tables_kernel, cluster, cluster, std::max(threads, 128), smem, st, p));
   }
-  return cuda_status(launch_cluster(extend_tables_kernel, kPlanCtas, kPlanCtas, kPlanThreads, smem,
-                                    reinterpret_cast<cudaStream_t>(stream), p));
+  p.clustered = 0;
+  auto overlaps = [](const void* x, const void* y, int64_t n) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    return a < b + 4 * n && b < a + 4 * n;
+  };
+  // Whether anything the first CTA writes of the new state is still read by another.
+  const int32_t* in[4] = {lengths, new_tokens, held_blocks, free_head};
+  const int64_t in_n[4] = {num_seqs, num_seqs, num_seqs, 1};
+  int32_t* out[4] = {cu_seqlens, context_lens, held_out, free_head_out};
+  const int64_t out_n[4] = {(int64_t)num_seqs + 1, num_seqs, num_seqs, 1};
+  bool in_place = false;
+  for (int i = 0; i < 4; ++i)
+    for (int o = 0; o < 4; ++o) in_place = in_place || overlaps(in[i], out[o], std::max(in_n[i], out_n[o]));
+  p.writes_state = !in_place;
+  extend_tables_kernel<<<std::min(ctas, num_sms()), kPlanThreads, smem, st>>>(p);
+  if (!in_place) return launch_status();
+  p.writes_map = 0;
+  p.writes_state = 1;
+  extend_tables_kernel<<<1, kPlanThreads, smem, st>>>(p);
+  return launch_status();
 }
 
 extern "C" int pkv_build_tree_metadata(const int32_t* parents, const int32_t* cu_nodes, int32_t num_seqs,
@@ -458,8 +506,12 @@ extern "C" int pkv_build_tree_metadata(const int32_t* parents, const int32_t* cu
   if (mask_words > kTreeWords) return PKV_ERR_UNSUPPORTED;
   if (total_nodes == 0) return PKV_OK;
   if (!parents || !cu_nodes || !mask || !positions || (num_seqs > 0 && !context_lens)) return PKV_ERR_INVALID_ARGUMENT;
-  const size_t smem = (size_t)64 * mask_words * (8 * mask_words + 4);
-  tree_metadata_kernel<<<num_seqs + 1, 128, smem, reinterpret_cast<cudaStream_t>(stream)>>>(
+  auto kernel = mask_words == 1   ? tree_metadata_kernel<1>
+                : mask_words == 2 ? tree_metadata_kernel<2>
+                : mask_words <= 4 ? tree_metadata_kernel<4>
+                                  : tree_metadata_kernel<8>;
+  const int threads = 64 * (mask_words <= 2 ? mask_words : mask_words <= 4 ? 4 : 8);
+  kernel<<<num_seqs + 1, threads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       parents, cu_nodes, num_seqs, context_lens, total_nodes, reinterpret_cast<uint64_t*>(mask), mask_words, positions,
       status_dev);
   return launch_status();

@@ -415,21 +415,34 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
 
 
 # ---------------------------------------------------------------- speculative decoding step
+#
+# These wrappers are called once or more per layer of a step that takes the GPU a few
+# microseconds a call, so they read each tensor attribute once and ask for the raw stream of
+# the tensors' own device (torch.cuda.current_stream() builds an object, 3 us).
 
-def _call(device: torch.device, fn, what: str, *args) -> None:
-    """Call ``fn(*args, stream)`` on ``device``'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+def _call(index: int, fn, what: str, *args) -> None:
+    """Call ``fn(*args, stream)`` on CUDA device ``index``'s current stream, whichever device is current."""
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream().cuda_stream)
-    check(status, what)
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status, what)
 
 
-def _ints(device: torch.device, dtype: torch.dtype, what: str, *ts: torch.Tensor | None) -> None:
+def _device_of(t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0:
+        _require_cuda(t)
+    return index
+
+
+def _flat(index: int, dtype: torch.dtype, what: str, *ts: torch.Tensor | None) -> None:
+    """Require contiguous tensors of ``dtype`` on CUDA device ``index`` (None is skipped)."""
     for t in ts:
-        if t is not None and (t.dtype != dtype or t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous {dtype} tensors on {device}")
+        if t is not None and (t.dtype is not dtype or t.get_device() != index or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous {dtype} tensors on cuda:{index}")
 
 
 def extend_tables(tables: PkvTables, lengths: torch.Tensor, new_tokens: torch.Tensor, held: torch.Tensor,
@@ -449,13 +462,12 @@ def extend_tables(tables: PkvTables, lengths: torch.Tensor, new_tokens: torch.Te
     row or the free list runs out, nothing is extended, every slot is -1 and the status
     word says so (see pkv_extend_tables in include/pkv.h).
     """
-    _require_cuda(lengths)
-    dev = lengths.device
+    dev = _device_of(lengths)
     held_out = held if held_out is None else held_out
     free_head_out = free_head if free_head_out is None else free_head_out
-    _ints(dev, torch.int32, "extend_tables: lengths, counts and block ids", lengths, new_tokens, held, free_blocks,
+    _flat(dev, torch.int32, "extend_tables: lengths, counts and block ids", lengths, new_tokens, held, free_blocks,
           free_head, cu_seqlens, context_lens, held_out, free_head_out, status)
-    _ints(dev, torch.int64, "extend_tables: positions and slot_mapping", positions, slot_mapping)
+    _flat(dev, torch.int64, "extend_tables: positions and slot_mapping", positions, slot_mapping)
     batch = lengths.numel()
     if (new_tokens.numel() != batch or held.numel() != batch or context_lens.numel() < batch or
             held_out.numel() < batch or cu_seqlens.numel() < batch + 1 or free_head.numel() < 1 or
@@ -480,16 +492,15 @@ def build_tree_metadata(parents: torch.Tensor, cu_nodes: torch.Tensor, context_l
     bit per ancestor and the node's own, ``positions`` (int64 ``[N]``) ``context_lens[b]`` +
     depth; rows behind the last tree get 0.
     """
-    _require_cuda(parents)
-    dev = parents.device
-    _ints(dev, torch.int32, "build_tree_metadata: parents, cu_nodes and context_lens", parents, cu_nodes, context_lens,
+    dev = _device_of(parents)
+    _flat(dev, torch.int32, "build_tree_metadata: parents, cu_nodes and context_lens", parents, cu_nodes, context_lens,
           status)
-    _ints(dev, torch.int64, "build_tree_metadata: mask and positions", mask, positions)
+    _flat(dev, torch.int64, "build_tree_metadata: mask and positions", mask, positions)
     n, batch = parents.numel(), cu_nodes.numel() - 1
-    if mask.dim() != 2 or mask.shape[0] != n or positions.numel() != n or context_lens.numel() < batch or batch < 0:
+    if mask.dim() != 2 or mask.size(0) != n or positions.numel() != n or context_lens.numel() < batch or batch < 0:
         raise ValueError("build_tree_metadata: mask [N, W], positions [N], context_lens [B], cu_nodes [B + 1]")
     _call(dev, lib.pkv_build_tree_metadata, "build_tree_metadata", parents.data_ptr(), cu_nodes.data_ptr(), batch,
-          context_lens.data_ptr(), n, mask.data_ptr(), mask.shape[1], positions.data_ptr(), _ptr(status))
+          context_lens.data_ptr(), n, mask.data_ptr(), mask.size(1), positions.data_ptr(), _ptr(status))
 
 
 @dataclass(frozen=True)
@@ -558,31 +569,35 @@ def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch
     when True, written when tensors. With ``slot_mapping`` (int64 [N], negative = skip) the
     rotated keys and the values are also written to the pool at ``layer``.
     """
-    _require_cuda(qkv, positions, inv_freq)
-    dev, dt = qkv.device, qkv.dtype
+    dev, dt = _device_of(qkv), qkv.dtype
     hkv, d = pool.num_kv_heads, pool.head_dim
-    if qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * hkv) * d or qkv.stride(1) != 1:
+    if qkv.dim() != 2 or qkv.size(1) != (num_q_heads + 2 * hkv) * d or qkv.stride(1) != 1:
         raise ValueError("qkv must be [N, (Hq + 2 Hkv) * head_dim] with a contiguous last dimension")
     if pkv_dtype(dt) != pool.dtype:
         raise ValueError("qkv and the pool must share one dtype")
-    n = qkv.shape[0]
-    _ints(dev, torch.int64, "rotary_append: positions and slot_mapping", positions, slot_mapping)
-    _ints(dev, torch.int32, "rotary_append: status", status)
-    _ints(dev, torch.float64, "rotary_append: inv_freq", inv_freq)
+    n, half = qkv.size(0), inv_freq.numel()
+    _flat(dev, torch.int64, "rotary_append: positions and slot_mapping", positions, slot_mapping)
+    _flat(dev, torch.int32, "rotary_append: status", status)
+    _flat(dev, torch.float64, "rotary_append: inv_freq", inv_freq)
     if positions.numel() != n or (slot_mapping is not None and slot_mapping.numel() != n):
         raise ValueError("rotary_append: positions and slot_mapping must have one entry per row")
-    if q_out is None:
-        q_out = torch.empty(n, num_q_heads, d, dtype=dt, device=dev)
-    k_out = torch.empty(n, hkv, d, dtype=dt, device=dev) if k_out is True else None if k_out is False else k_out
-    v_out = torch.empty(n, hkv, d, dtype=dt, device=dev) if v_out is True else None if v_out is False else v_out
-    for t, heads in ((q_out, num_q_heads), (k_out, hkv), (v_out, hkv)):
-        if t is not None and (t.shape != (n, heads, d) or t.dtype != dt or t.device != dev or t.stride(2) != 1):
+
+    def output(t: torch.Tensor | bool | None, heads: int) -> tuple[torch.Tensor | None, int | None, int, int]:
+        if t is None or t is False:
+            return None, None, 0, 0
+        if t is True:
+            t = qkv.new_empty((n, heads, d))
+            return t, t.data_ptr(), heads * d, d
+        if t.shape != (n, heads, d) or t.dtype is not dt or t.get_device() != dev or t.stride(2) != 1:
             raise ValueError("rotary_append: outputs must be [N, heads, head_dim] like qkv, last dimension contiguous")
-    ks, vs = ((t.stride(0), t.stride(1)) if t is not None else (0, 0) for t in (k_out, v_out))
+        return t, t.data_ptr(), t.stride(0), t.stride(1)
+
+    q_out, *q_at = output(True if q_out is None else q_out, num_q_heads)
+    k_out, *k_at = output(k_out, hkv)
+    v_out, *v_at = output(v_out, hkv)
     _call(dev, lib.pkv_rotary_append, "rotary_append", ctypes.byref(pool), layer, qkv.data_ptr(), qkv.stride(0), n,
-          num_q_heads, positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved),
-          attention_factor, q_out.data_ptr(), q_out.stride(0), q_out.stride(1), _ptr(k_out), *ks, _ptr(v_out), *vs,
-          _ptr(slot_mapping), _ptr(status))
+          num_q_heads, positions.data_ptr(), inv_freq.data_ptr(), 2 * half, int(interleaved), attention_factor, *q_at,
+          *k_at, *v_at, _ptr(slot_mapping), _ptr(status))
     return q_out, k_out, v_out
 
 
@@ -598,10 +613,16 @@ def tree_attention_workspace(pool: PkvPool, max_seqs: int, device: torch.device 
     return torch.zeros(nbytes, dtype=torch.uint8, device=device)
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [N, H, d] as rows and heads that start on 16 bytes (a copy only where they do not)."""
-    ok = t.stride(2) == 1 and (t.stride(0) | t.stride(1)) % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
+def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """``t`` [N, H, d] with rows and heads that start on 16 bytes (a copy only where they do not), its
+    address and its two strides."""
+    row, head, last = t.stride()
+    at = t.data_ptr()
+    if last != 1 or (row | head) & 7 or at & 15 or row < 0 or head < 0:
+        t = t.clone(memory_format=torch.contiguous_format)
+        row, head, _ = t.stride()
+        at = t.data_ptr()
+    return t, at, row, head
 
 
 def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor, k_nodes: torch.Tensor,
@@ -616,30 +637,31 @@ def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor
     :func:`build_tree_metadata`). The nodes' own keys and values ``[N, Hkv, d]`` (any
     strides) are not in the pool; :func:`accept_tree` writes the accepted ones there.
     """
-    _require_cuda(q, k_nodes, v_nodes)
-    dev = q.device
-    n, hq, d = q.shape
-    if d != pool.head_dim or pkv_dtype(q.dtype) != pool.dtype or k_nodes.dtype != q.dtype or v_nodes.dtype != q.dtype:
+    dev, dt = _device_of(q), q.dtype
+    shape = n, hq, d = q.shape
+    hkv = pool.num_kv_heads
+    if d != pool.head_dim or pkv_dtype(dt) != pool.dtype or k_nodes.dtype is not dt or v_nodes.dtype is not dt:
         raise ValueError("q, the nodes' keys and values and the pool must share head_dim and dtype")
-    if k_nodes.shape != (n, pool.num_kv_heads, d) or v_nodes.shape != k_nodes.shape:
+    if k_nodes.shape != (n, hkv, d) or v_nodes.shape != (n, hkv, d):
         raise ValueError("k_nodes and v_nodes must be [N, kv_heads, head_dim]")
-    if k_nodes.device != dev or v_nodes.device != dev or workspace.device != dev:
-        raise ValueError(f"tree_attention: every tensor must be on {dev}")
-    _ints(dev, torch.int32, "tree_attention: cu_nodes and context_lens", cu_nodes, context_lens, status)
-    _ints(dev, torch.int64, "tree_attention: mask", mask)
+    if k_nodes.get_device() != dev or v_nodes.get_device() != dev or workspace.get_device() != dev:
+        raise ValueError(f"tree_attention: every tensor must be on cuda:{dev}")
+    _flat(dev, torch.int32, "tree_attention: cu_nodes and context_lens", cu_nodes, context_lens, status)
+    _flat(dev, torch.int64, "tree_attention: mask", mask)
     batch = cu_nodes.numel() - 1
-    if mask.dim() != 2 or mask.shape[0] != n or batch < 0 or context_lens.numel() < batch:
+    if mask.dim() != 2 or mask.size(0) != n or batch < 0 or context_lens.numel() < batch:
         raise ValueError("tree_attention: mask [N, W], context_lens [B], cu_nodes [B + 1]")
-    q, k_nodes, v_nodes = _rows16(q), _rows16(k_nodes), _rows16(v_nodes)
+    q, *q_at = _rows16(q)
+    k_nodes, *k_at = _rows16(k_nodes)
+    v_nodes, *v_at = _rows16(v_nodes)
     if out is None:
-        out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not dt or out.get_device() != dev or out.stride(2) != 1:
         raise ValueError("out must match q, last dimension contiguous")
+    row, head, _ = out.stride()
     _call(dev, lib.pkv_tree_attention, "tree_attention", ctypes.byref(pool), layer, ctypes.byref(tables), batch,
-          cu_nodes.data_ptr(), context_lens.data_ptr(), max_nodes, n, hq, out.data_ptr(), out.stride(0), out.stride(1),
-          q.data_ptr(), q.stride(0), q.stride(1), k_nodes.data_ptr(), k_nodes.stride(0), k_nodes.stride(1),
-          v_nodes.data_ptr(), v_nodes.stride(0), v_nodes.stride(1), mask.data_ptr(), mask.shape[1],
-          d ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+          cu_nodes.data_ptr(), context_lens.data_ptr(), max_nodes, n, hq, out.data_ptr(), row, head, *q_at, *k_at, *v_at,
+          mask.data_ptr(), mask.size(1), d ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.nbytes,
           _ptr(status))
     return out
 
@@ -659,26 +681,25 @@ def accept_tree(pool: PkvPool, tables: PkvTables, parents: torch.Tensor, cu_node
     path's rows of ``k_nodes`` / ``v_nodes`` ``[layers, N, Hkv, d]`` at positions
     ``context_lens[b] ...`` of the sequence's blocks.
     """
-    _require_cuda(parents)
-    dev = parents.device
+    dev = _device_of(parents)
     n, batch = parents.numel(), cu_nodes.numel() - 1
     lengths_out = context_lens if lengths_out is None else lengths_out
-    _ints(dev, torch.int32, "accept_tree: parents, cu_nodes, lengths, counts and path", parents, cu_nodes, context_lens,
+    _flat(dev, torch.int32, "accept_tree: parents, cu_nodes, lengths, counts and path", parents, cu_nodes, context_lens,
           counts, path, lengths_out, status)
-    _ints(dev, torch.int64, "accept_tree: tokens", draft_tokens, target_tokens, tokens)
+    _flat(dev, torch.int64, "accept_tree: tokens", draft_tokens, target_tokens, tokens)
     if (draft_tokens.numel() != n or target_tokens.numel() != n or batch < 0 or context_lens.numel() < batch or
             counts.numel() < batch or lengths_out.numel() < batch or path.dim() != 2 or path.shape != tokens.shape or
-            path.shape[0] < batch):
+            path.size(0) < batch):
         raise ValueError("accept_tree: one token per node, counts and lengths per tree, path and tokens [B, W]")
-    shape = (pool.num_layers, n, pool.num_kv_heads, pool.head_dim)
-    for t in (k_nodes, v_nodes):
-        if t.shape != shape or pkv_dtype(t.dtype) != pool.dtype or t.device != dev or t.stride(3) != 1:
+    shape, code = (pool.num_layers, n, pool.num_kv_heads, pool.head_dim), pool.dtype
+    k_strides, v_strides = k_nodes.stride(), v_nodes.stride()
+    for t, strides in ((k_nodes, k_strides), (v_nodes, v_strides)):
+        if t.shape != shape or pkv_dtype(t.dtype) != code or t.get_device() != dev or strides[3] != 1:
             raise ValueError("accept_tree: k_nodes and v_nodes must be [layers, N, kv_heads, head_dim] of the pool's dtype")
     _call(dev, lib.pkv_accept_tree, "accept_tree", ctypes.byref(pool), ctypes.byref(tables), batch, parents.data_ptr(),
-          cu_nodes.data_ptr(), n, draft_tokens.data_ptr(), target_tokens.data_ptr(), k_nodes.data_ptr(),
-          k_nodes.stride(0), k_nodes.stride(1), k_nodes.stride(2), v_nodes.data_ptr(), v_nodes.stride(0),
-          v_nodes.stride(1), v_nodes.stride(2), context_lens.data_ptr(), counts.data_ptr(), path.data_ptr(),
-          tokens.data_ptr(), path.shape[1], lengths_out.data_ptr(), _ptr(status))
+          cu_nodes.data_ptr(), n, draft_tokens.data_ptr(), target_tokens.data_ptr(), k_nodes.data_ptr(), *k_strides[:3],
+          v_nodes.data_ptr(), *v_strides[:3], context_lens.data_ptr(), counts.data_ptr(), path.data_ptr(),
+          tokens.data_ptr(), path.size(1), lengths_out.data_ptr(), _ptr(status))
 
 
 def build_decode_metadata(tables: PkvTables, lengths: torch.Tensor, block_size: int, scratch_block: int,
