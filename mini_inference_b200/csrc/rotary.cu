@@ -43,8 +43,7 @@ template <typename T, int EW> struct alignas(EW * sizeof(T)) Vec {
 
 // One CTA per token: the pairs' cos and sin once into shared memory, then every head's
 // units from there. A unit is EW pairs: two vectors of EW elements, half a rotation apart
-// or side by side; the elements past the rotated part and the V rows are units of one
-// vector that is copied. A thread's first unit is on its way while the angles are made.
+// or side by side; the elements past the rotated part and the V rows are copied.
 template <typename T, int EW, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
   __shared__ float2 cs[kMaxHalf];
@@ -52,36 +51,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
   const int64_t t = blockIdx.x;
   const int64_t pos = p.positions[t];
   int64_t slot = p.slots ? p.slots[t] : -1;
-  const T* row = static_cast<const T*>(p.qkv) + t * p.qkv_stride;
-  const int heads = p.hq + p.hkv, per_head = p.half / EW;
-  const int rest = (p.d - 2 * p.half) / EW, per_v = p.d / EW;
-  const int rot_units = heads * per_head, rest_units = rot_units + heads * rest;
-  const int units = rest_units + (p.v_out || p.slots ? p.hkv * per_v : 0);
-  // Unit u's head and its one or two vectors' first elements.
-  struct Unit {
-    int head, ca, cb;
-    V a, b;
-  };
-  auto load = [&](int u) {
-    Unit x;
-    if (u < rot_units) {
-      x.head = u / per_head;
-      const int i0 = (u - x.head * per_head) * EW;
-      x.ca = INTER ? 2 * i0 : i0;
-      x.cb = INTER ? 2 * i0 + EW : i0 + p.half;
-      x.b = *reinterpret_cast<const V*>(row + x.head * p.d + x.cb);
-    } else {
-      const int per = u < rest_units ? rest : per_v, w = u - (u < rest_units ? rot_units : rest_units);
-      x.head = w / per;
-      x.ca = (w - x.head * per) * EW + (u < rest_units ? 2 * p.half : 0);
-      x.cb = 0;
-      if (u >= rest_units) x.head += heads;
-    }
-    x.a = *reinterpret_cast<const V*>(row + x.head * p.d + x.ca);
-    return x;
-  };
-  Unit x;
-  if (threadIdx.x < units) x = load(threadIdx.x);
+  if (slot >= (int64_t)p.nbt * p.bs) {
+    if (threadIdx.x == 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+    slot = -1;
+  }
+  if (pos < 0 && threadIdx.x == 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
   for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
     const double turns = (double)pos * p.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
     const float r = (float)(turns - rint(turns));                             // [-1/2, 1/2]
@@ -89,55 +63,62 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     sincospif(2.f * r, &s, &c);
     cs[i] = make_float2(c * p.factor, s * p.factor);
   }
-  if (slot >= (int64_t)p.nbt * p.bs) {
-    if (threadIdx.x == 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
-    slot = -1;
-  }
-  if (pos < 0 && threadIdx.x == 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+  __syncthreads();
+  const T* row = static_cast<const T*>(p.qkv) + t * p.qkv_stride;
+  const int heads = p.hq + p.hkv, per_head = p.half / EW;
+  const int rest = (p.d - 2 * p.half) / EW, per_v = p.d / EW;
+  const int rot_units = heads * per_head, rest_units = heads * rest;
+  const bool want_v = p.v_out || slot >= 0;
+  const int units = rot_units + rest_units + (want_v ? p.hkv * per_v : 0);
   const int64_t in_block = slot >= 0 ? ((p.layer_base + slot / p.bs) * p.hkv * p.bs + slot % p.bs) * p.d : 0;
   const int64_t head_step = (int64_t)p.bs * p.d;
-  auto put = [&](int head, int c, const V& v) {  // element c of a head of the row
+  auto put = [&](int head, int c, const V& x) {  // element c of a q or k head
     if (head < p.hq) {
-      *reinterpret_cast<V*>(static_cast<T*>(p.q_out) + t * p.q_st + head * p.q_sh + c) = v;
-    } else if (head < heads) {
-      const int kh = head - p.hq;
-      if (p.k_out) *reinterpret_cast<V*>(static_cast<T*>(p.k_out) + t * p.k_st + kh * p.k_sh + c) = v;
-      if (slot >= 0) *reinterpret_cast<V*>(static_cast<T*>(p.k_pool) + in_block + kh * head_step + c) = v;
+      *reinterpret_cast<V*>(static_cast<T*>(p.q_out) + t * p.q_st + head * p.q_sh + c) = x;
     } else {
-      const int kh = head - heads;
-      if (p.v_out) *reinterpret_cast<V*>(static_cast<T*>(p.v_out) + t * p.v_st + kh * p.v_sh + c) = v;
-      if (slot >= 0) *reinterpret_cast<V*>(static_cast<T*>(p.v_pool) + in_block + kh * head_step + c) = v;
+      const int kh = head - p.hq;
+      if (p.k_out) *reinterpret_cast<V*>(static_cast<T*>(p.k_out) + t * p.k_st + kh * p.k_sh + c) = x;
+      if (slot >= 0) *reinterpret_cast<V*>(static_cast<T*>(p.k_pool) + in_block + kh * head_step + c) = x;
     }
   };
-  __syncthreads();
   for (int u = threadIdx.x; u < units; u += blockDim.x) {
-    Unit next;
-    if (u + blockDim.x < units) next = load(u + blockDim.x);
     if (u < rot_units) {
-      const int i0 = INTER ? x.ca / 2 : x.ca;  // first pair
+      const int head = u / per_head, i0 = (u - head * per_head) * EW;  // first pair
+      const int ca = INTER ? 2 * i0 : i0, cb = INTER ? 2 * i0 + EW : i0 + p.half;
+      V a = *reinterpret_cast<const V*>(row + head * p.d + ca);
+      V b = *reinterpret_cast<const V*>(row + head * p.d + cb);
 #pragma unroll
       for (int e = 0; e < EW; ++e) {
         // INTER: the two vectors hold pairs (a0 a1) (a2 a3) .. (b0 b1) ..; pair e of the unit.
-        T& vx = INTER ? (2 * e < EW ? x.a.v[(2 * e) % EW] : x.b.v[(2 * e) % EW]) : x.a.v[e];
-        T& vy = INTER ? (2 * e + 1 < EW ? x.a.v[(2 * e + 1) % EW] : x.b.v[(2 * e + 1) % EW]) : x.b.v[e];
+        T& x = INTER ? (2 * e < EW ? a.v[(2 * e) % EW] : b.v[(2 * e) % EW]) : a.v[e];
+        T& y = INTER ? (2 * e + 1 < EW ? a.v[(2 * e + 1) % EW] : b.v[(2 * e + 1) % EW]) : b.v[e];
         const float2 w = cs[i0 + e];
-        const float fx = Dt<T>::to_f(vx), fy = Dt<T>::to_f(vy);
-        vx = Dt<T>::from_f(fx * w.x - fy * w.y);
-        vy = Dt<T>::from_f(fy * w.x + fx * w.y);
+        const float fx = Dt<T>::to_f(x), fy = Dt<T>::to_f(y);
+        x = Dt<T>::from_f(fx * w.x - fy * w.y);
+        y = Dt<T>::from_f(fy * w.x + fx * w.y);
       }
-      put(x.head, x.cb, x.b);
+      put(head, ca, a);
+      put(head, cb, b);
+    } else if (u < rot_units + rest_units) {
+      const int w = u - rot_units, head = w / rest, c = 2 * p.half + (w - head * rest) * EW;
+      put(head, c, *reinterpret_cast<const V*>(row + head * p.d + c));
+    } else {
+      const int w = u - rot_units - rest_units, kh = w / per_v, c = (w - kh * per_v) * EW;
+      const V x = *reinterpret_cast<const V*>(row + (heads + kh) * p.d + c);
+      if (p.v_out) *reinterpret_cast<V*>(static_cast<T*>(p.v_out) + t * p.v_st + kh * p.v_sh + c) = x;
+      if (slot >= 0) *reinterpret_cast<V*>(static_cast<T*>(p.v_pool) + in_block + kh * head_step + c) = x;
     }
-    put(x.head, x.ca, x.a);
-    x = next;
   }
 }
 
 template <typename T>
 int launch(const RotaryParams& p, int64_t n, bool vec16, bool inter, cudaStream_t st) {
-  // Two units per thread, a whole number of warps.
+  // Few tokens: a unit per thread, for latency. More than the SMs hold at once: four units
+  // per thread, so that more tokens are under way (a CTA's chain is position, angles, rows).
   const int ew = vec16 ? 8 : 1;
   const int units = (p.hq + p.hkv) * (p.d - p.half) / ew + (p.v_out || p.slots ? p.hkv * p.d / ew : 0);
-  const int threads = std::min(kThreads, std::max(64, (units / 2 + 31) / 32 * 32));
+  const int per = n > 4 * num_sms() ? 4 : 1;
+  const int threads = std::min(kThreads, std::max(64, (units + per * 32 - 1) / (per * 32) * 32));
   auto kernel = vec16 ? inter ? rotary_kernel<T, 8, true> : rotary_kernel<T, 8, false>
                       : inter ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>;
   kernel<<<(unsigned)n, threads, 0, st>>>(p);
