@@ -571,7 +571,10 @@ extern "C" int pkv_accept_tree(const pkv_pool* pool, const pkv_tables* tables, i
   if (addr & 1) return PKV_ERR_INVALID_ARGUMENT;
   const int64_t strides = k_stride_l | k_stride_n | k_stride_h | v_stride_l | v_stride_n | v_stride_h | p.d;
   const bool vec16 = (addr & 15) == 0 && (strides & 7) == 0;
-  const int cluster = std::min(8, p.layers >= 8 ? 8 : p.layers >= 4 ? 4 : p.layers >= 2 ? 2 : 1);
+  // As many CTAs per tree as have a layer to copy and fit one wave (four of them on an SM):
+  // every CTA walks its tree first, about as long as a few layers' copies take.
+  int cluster = 1;
+  while (cluster < 8 && 2 * cluster <= p.layers && 2 * cluster * (int64_t)num_seqs <= 4 * num_sms()) cluster *= 2;
   auto kernel = vec16 ? accept_tree_kernel<8> : accept_tree_kernel<1>;
   return cuda_status(launch_cluster(kernel, num_seqs * cluster, cluster, kAcceptThreads, 0,
                                     reinterpret_cast<cudaStream_t>(stream), p));
