@@ -10,9 +10,9 @@ metadata builder and block copy-on-write. Importing the package loads
 """
 
 from ._lib import PkvError
-from .cache import NativeBlockManager, PackedPrefillContext, PagedDecodeContext, PagedKVCache
+from .cache import NativeBlockManager, PackedPrefillContext, PagedDecodeContext, PagedKVCache, TreeContext
 from .cuda_graphs import GraphedDecoder
 
 __all__ = ["PagedKVCache", "PagedDecodeContext", "PackedPrefillContext", "NativeBlockManager", "GraphedDecoder",
-           "PkvError"]
+           "PkvError", "TreeContext"]
 __version__ = "0.1.0"

@@ -319,7 +319,7 @@ class PagedKVCache:
             self._edits_dev = torch.empty((cap, 3), dtype=torch.int32, device=self.device)
             self._edits_sent = torch.cuda.Event()
             self._bm.set_journal(True)
-            self._workspaces: dict[tuple[int, int], torch.Tensor] = {}
+            self._workspaces: dict[tuple[int, int] | str, torch.Tensor] = {}
 
     @classmethod
     def for_model(cls, cfg, num_blocks: int, block_size: int, max_seqs: int, max_len: int, dtype: torch.dtype,
@@ -471,6 +471,17 @@ class PagedKVCache:
     def decode_context(self, slots: Sequence[int]) -> "PagedDecodeContext":
         return PagedDecodeContext(self, slots)
 
+    def tree_context(self, slots: Sequence[int], parents: Sequence[Sequence[int]]) -> "TreeContext":
+        """A step that verifies a tree of drafted tokens per slot (no counterpart in the reference)."""
+        return TreeContext(self, slots, parents)
+
+    def tree_workspace(self) -> torch.Tensor:
+        """Workspace of :class:`TreeContext`'s attention (zeroed once, reused)."""
+        ws = self._workspaces.get("tree")
+        if ws is None:
+            ws = self._workspaces["tree"] = ops.tree_attention_workspace(self.pool, self.max_seqs, self.device)
+        return ws
+
 
 class PagedDecodeContext:
     """A batched decode step on the paged cache (engine/kv_cache.py:582-624).
@@ -546,6 +557,15 @@ class PagedDecodeContext:
         self._attends += 1
         return out.transpose(1, 2)
 
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
+        """:meth:`attend_qkv` for the rotary layouts of ``ops.rotary_append``: the rotation, then the append and attention."""
+        batch = qkv.shape[0]
+        rows = qkv.reshape(batch, -1)
+        q, k, v = ops.rotary_append(self.cache.pool, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
+                                    interleaved=rotary.interleaved, attention_factor=rotary.attention_factor, k_out=True,
+                                    v_out=True, status=self.cache.status)
+        return self.attend(layer_idx, q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
+
     def commit(self) -> None:
         self.cache._bm.commit_decode(self._slots_np)
 
@@ -616,6 +636,123 @@ class PackedPrefillContext:
                               self.max_new, out=out, status=self.cache.status)
         return out.unsqueeze(0).transpose(1, 2)
 
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
+        """:meth:`attend_qkv` for the rotary layouts of ``ops.rotary_append`` (appended as it is rotated)."""
+        rows = qkv.reshape(-1, qkv.shape[-1])
+        q_rot, _, _ = ops.rotary_append(self.cache.pool, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
+                                        interleaved=rotary.interleaved, attention_factor=rotary.attention_factor,
+                                        slot_mapping=self.slot_mapping, status=self.cache.status)
+        out = torch.empty(rows.shape[0], num_q_heads, self.cache.head_dim, dtype=qkv.dtype, device=qkv.device)
+        ops.prefill_attention(self.cache.pool, layer_idx, self.tables, q_rot, self.cu_seqlens, self.starts_dev,
+                              self.max_new, out=out, status=self.cache.status)
+        return out.unsqueeze(0).transpose(1, 2)
+
     def commit(self) -> None:
         for slot, start, n in zip(self.slots, self.starts, self.lengths):
             self.cache.lengths[slot] = start + n
+
+
+class TreeContext:
+    """A step that verifies drafted tokens: one tree per sequence, all nodes in one forward pass.
+
+    No counterpart in the reference, which decodes one token per sequence and step. Node 0
+    of a tree is the sequence's last token (not cached yet, as in a decode step); every other
+    node hangs below an earlier one (``parents``, -1 for node 0) and holds a drafted token.
+    The model runs over all nodes packed end to end, node ``n`` at position ``length +
+    depth``; each attends to its sequence's cached keys and to its ancestors. The nodes' keys
+    and values stay outside the cache until :meth:`accept` writes the accepted path's.
+    """
+
+    def __init__(self, cache: PagedKVCache, slots: Sequence[int], parents: Sequence[Sequence[int]]) -> None:
+        cache._require_gpu()
+        self.cache = cache
+        self.slots = list(slots)
+        if len(parents) != len(self.slots) or len(set(self.slots)) != len(self.slots):
+            raise ValueError("one tree per slot, each slot once")
+        sizes = [len(p) for p in parents]
+        depth: list[int] = []  # of each tree's longest path, in nodes
+        for tree in parents:
+            at: list[int] = []
+            for i, up in enumerate(tree):
+                if not (up == -1 if i == 0 else 0 <= up < i):
+                    raise ValueError("a tree's node 0 is its root (-1) and every other node's parent comes before it")
+                at.append(1 if i == 0 else at[up] + 1)
+            if not at:
+                raise ValueError("a tree has at least its root")
+            depth.append(max(at))
+        if max(sizes, default=1) > 512 or max(depth, default=1) > 64:
+            raise ValueError("trees of up to 512 nodes and 64 levels")
+        self.starts = [cache.lengths[s] for s in self.slots]
+        for s, start, n in zip(self.slots, self.starts, depth):
+            if not cache.ensure_capacity(s, start + n):
+                raise ValueError(f"no room in the KV cache for {start + n} tokens")
+        cache.copy_on_write(list(zip(self.slots, self.starts, depth)))
+        cache.sync_tables()
+        dev, b = cache.device, len(self.slots)
+        cu = np.zeros(b + 1, np.int32)
+        np.cumsum(sizes, out=cu[1:])
+        self.total, self.max_nodes, self.max_path = int(cu[-1]), max(sizes, default=0), max(depth, default=1)
+        flat = np.fromiter((up for tree in parents for up in tree), np.int32, self.total)
+        host = np.concatenate([np.asarray(self.slots, np.int32), np.asarray(self.starts, np.int32), cu, flat])
+        staged = torch.from_numpy(host).pin_memory().to(dev, non_blocking=True)
+        self.seq_rows, self.context_lens, self.cu_nodes, self.parents = staged.split([b, b, b + 1, self.total])
+        self.tables = ops.make_tables(cache.tables_dev, self.seq_rows)
+        self.mask = torch.empty(self.total, max(1, -(-self.max_nodes // 64)), dtype=torch.int64, device=dev)
+        self.positions = torch.empty(self.total, dtype=torch.int64, device=dev)
+        ops.build_tree_metadata(self.parents, self.cu_nodes, self.context_lens, self.mask, self.positions, cache.status)
+        # The nodes' keys and values of every layer, as a pool of one-token blocks: node n is slot n.
+        shape = (cache.num_layers, self.total, cache.num_kv_heads, 1, cache.head_dim)
+        self.k_nodes = torch.empty(shape, dtype=cache.k.dtype, device=dev)
+        self.v_nodes = torch.empty(shape, dtype=cache.k.dtype, device=dev)
+        self.nodes = ops.make_pool(self.k_nodes, self.v_nodes)
+        self.node_slots = torch.arange(self.total, dtype=torch.int64, device=dev)
+
+    def _attention(self, layer_idx: int, q: torch.Tensor) -> torch.Tensor:
+        cache = self.cache
+        out = ops.tree_attention(cache.pool, layer_idx, self.tables, q, self.k_nodes[layer_idx, :, :, 0],
+                                 self.v_nodes[layer_idx, :, :, 0], self.cu_nodes, self.context_lens, self.mask, self.max_nodes,
+                                 cache.tree_workspace(), status=cache.status)
+        return out.unsqueeze(0).transpose(1, 2)
+
+    def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """q ``[1, Hq, N, d]``, k / v ``[1, Hkv, N, d]`` -> ``[1, Hq, N, d]``."""
+        if q.dtype != self.cache.k.dtype:
+            raise TypeError(f"q is {q.dtype} but the cache holds {self.cache.k.dtype}")
+        ops.kv_append(self.nodes, layer_idx, k[0].transpose(0, 1), v[0].transpose(0, 1), self.node_slots, self.cache.status)
+        return self._attention(layer_idx, q[0].transpose(0, 1))
+
+    def attend_qkv(self, layer_idx: int, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                   num_q_heads: int) -> torch.Tensor:
+        """The ``qkv_proj`` output ``[1, N, (Hq + 2 Hkv) d]`` -> ``[1, Hq, N, d]``, RoPE as a decode step's."""
+        rows = qkv.reshape(-1, qkv.shape[-1])
+        q, _ = ops.rope_append(self.nodes, layer_idx, rows, self.positions, cos, sin, num_q_heads,
+                               slot_mapping=self.node_slots, status=self.cache.status)
+        return self._attention(layer_idx, q)
+
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
+        """:meth:`attend_qkv` for the rotary layouts of ``ops.rotary_append``."""
+        rows = qkv.reshape(-1, qkv.shape[-1])
+        q, _, _ = ops.rotary_append(self.nodes, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
+                                    interleaved=rotary.interleaved, attention_factor=rotary.attention_factor,
+                                    slot_mapping=self.node_slots, status=self.cache.status)
+        return self._attention(layer_idx, q)
+
+    def accept(self, draft_tokens: torch.Tensor, target_tokens: torch.Tensor) -> list[list[int]]:
+        """Accept each tree's greedy path; the new tokens of each sequence (at least one).
+
+        ``draft_tokens`` (int64 ``[N]``) are the tokens the nodes hold, ``target_tokens`` the
+        model's greedy choice after each. The path's keys and values go to the cache and the
+        sequence's length grows by its nodes; the last new token is not cached yet, as after
+        a decode step. Every layer must have attended. Reads the tokens back (synchronises).
+        """
+        cache, b = self.cache, len(self.slots)
+        i32, i64 = dict(dtype=torch.int32, device=cache.device), dict(dtype=torch.int64, device=cache.device)
+        counts, path = torch.empty(b, **i32), torch.empty(b, self.max_path, **i32)
+        tokens, lengths = torch.empty(b, self.max_path, **i64), torch.empty(b, **i32)
+        ops.accept_tree(cache.pool, self.tables, self.parents, self.cu_nodes, draft_tokens, target_tokens,
+                        self.k_nodes[:, :, :, 0], self.v_nodes[:, :, :, 0], self.context_lens, counts, path, tokens,
+                        lengths_out=lengths, status=cache.status)
+        new = [row[:n] for n, row in zip(counts.tolist(), tokens.tolist())]
+        for slot, start, row in zip(self.slots, self.starts, new):
+            cache.lengths[slot] = start + len(row)
+        return new

@@ -78,6 +78,14 @@ class _GraphDecodeContext:
         self._attends += 1
         return out.transpose(1, 2)
 
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
+        """As ``PagedDecodeContext.attend_rotary``."""
+        rows = qkv.reshape(qkv.shape[0], -1)
+        q, k, v = ops.rotary_append(self.cache.pool, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
+                                    interleaved=rotary.interleaved, attention_factor=rotary.attention_factor, k_out=True,
+                                    v_out=True, status=self.cache.status)
+        return self.attend(layer_idx, q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
+
 
 class GraphedDecoder:
     """Captures the decode step as CUDA graphs (one per batch bucket) and replays them."""

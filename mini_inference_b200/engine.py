@@ -113,6 +113,10 @@ class EngineConfig:
     # Prefill long prompts across steps under the token budget (opt-in; the reference has
     # none, README.md:470-473). With it a prompt may be longer than the budget.
     chunked_prefill: bool = False
+    # Speculative decoding (opt-in; the reference has none): each decode step also verifies up
+    # to this many tokens drafted by draft_by_lookup, and may emit that many more. The tokens
+    # are the model's own greedy choices either way.
+    speculative_tokens: int = 0
 
     def __post_init__(self) -> None:
         if self.max_num_seqs < 1:
@@ -127,6 +131,8 @@ class EngineConfig:
             raise ValueError("kv_cache_tokens must be >= max_model_len")
         if self.max_num_batched_tokens < self.max_model_len and not self.chunked_prefill:
             raise ValueError("max_num_batched_tokens must be >= max_model_len")
+        if not 0 <= self.speculative_tokens <= 63:
+            raise ValueError("speculative_tokens must be between 0 and 63")
         if self.max_num_batched_tokens < 1:
             raise ValueError("max_num_batched_tokens must be at least 1")
         if self.cuda_graph_max_batch is None:
@@ -145,6 +151,22 @@ def pack_by_budget(lengths: SequenceOf[int], budget: int) -> list[list[int]]:
             groups.append([i])
             total = n
     return groups
+
+
+def draft_by_lookup(token_ids: SequenceOf[int], count: int, longest: int = 3) -> list[int]:
+    """Up to ``count`` tokens that followed the latest earlier occurrence of the sequence's last tokens.
+
+    Matches the last ``longest`` tokens first, then fewer; empty when even the last token
+    has not occurred before. Text that repeats itself (quotations, code, structured output)
+    is continued as it went before.
+    """
+    ids, n = list(token_ids), len(token_ids)
+    for size in range(min(longest, n - 1), 0, -1):
+        tail = ids[n - size:]
+        for at in range(n - size - 1, -1, -1):
+            if ids[at:at + size] == tail:
+                return ids[at + size:at + size + count]
+    return []
 
 
 class ModelRunner:
@@ -208,6 +230,25 @@ class ModelRunner:
         if while_running is not None:
             while_running()
         return self._tokens(hidden[:, -1])
+
+
+    @torch.inference_mode()
+    def verify_tokens(self, slots: SequenceOf[int], trees: SequenceOf[tuple[SequenceOf[int], SequenceOf[int]]]
+                      ) -> list[list[int]]:
+        """One speculative step: each sequence's new tokens (one and more), the model's greedy choices.
+
+        ``trees[i] = (tokens, parents)``: node 0 is the sequence's last token (parent -1),
+        the others drafted tokens, each below an earlier node. The accepted path's keys and
+        values are in the cache afterwards, so the next step goes on from the last new token.
+        """
+        if any(len(t) != len(p) for t, p in trees):
+            raise ValueError("a tree has one parent per token")
+        ctx = self.cache.tree_context(slots, [p for _, p in trees])
+        ids = self._ids_to_device([t for tokens, _ in trees for t in tokens])
+        hidden = self.model(ids.unsqueeze(0), ctx.positions.unsqueeze(0), ctx)[0]
+        step = self.head.max_batch
+        targets = torch.cat([self.head(hidden[a:a + step]).clone() for a in range(0, ctx.total, step)])
+        return ctx.accept(ids, targets)
 
 
 @dataclass
@@ -299,17 +340,45 @@ class LLMEngine:
             # The token at each sequence's last position (its last output, or with chunked
             # prefill the last prompt token when the final chunk left exactly that one), as
             # the native scheduler reports it.
-            tokens = self.runner.decode_tokens(self.scheduler.decode_slots(), self.scheduler.decode_last_tokens(),
-                                               while_running=count_context)
+            if self.config.speculative_tokens:
+                count_context()
+                n_finished += self._verify(batch.decodes, new_tokens)
+            else:
+                tokens = self.runner.decode_tokens(self.scheduler.decode_slots(), self.scheduler.decode_last_tokens(),
+                                                   while_running=count_context)
+                n_finished += self.scheduler.append_tokens(batch.decodes, tokens, time.perf_counter())
+                new_tokens.extend(zip((s.seq_id for s in batch.decodes), tokens))
             ctx_tokens = context[0]
-            n_finished += self.scheduler.append_tokens(batch.decodes, tokens, time.perf_counter())
-            new_tokens.extend(zip((s.seq_id for s in batch.decodes), tokens))
         self.step_stats.append(StepStats(
             step=len(self.step_stats), time=time.perf_counter(), num_prefills=len(batch.prefills),
             num_prefill_tokens=n_prefill_tokens, num_decodes=len(batch.decodes), decode_context_tokens=ctx_tokens,
             num_finished=n_finished,
             num_running=self.scheduler.num_running, num_waiting=self.scheduler.num_waiting))
         return new_tokens
+
+    def _verify(self, seqs: list[Sequence], new_tokens: list[tuple[int, int]]) -> int:
+        """A decode step that verifies drafted tokens with each sequence's last; how many finished.
+
+        A draft takes no more than the request's remaining tokens, the model length and the
+        free blocks allow; without one the step is a plain decode.
+        """
+        lasts = self.scheduler.decode_last_tokens()
+        trees = []
+        for s, last in zip(seqs, lasts):
+            ids = s.token_ids[:self.cache.lengths[s.slot]] + [int(last)]  # a chunked prefill may leave one prompt token
+            room = min(self.config.speculative_tokens, s.sampling.max_tokens - len(s.output_token_ids) - 1,
+                       self.config.max_model_len - len(ids) - 1)
+            draft = draft_by_lookup(ids, room) if room > 0 else []
+            if draft and not self.cache.ensure_capacity(s.slot, len(ids) + len(draft)):
+                draft = []
+            trees.append(([int(last), *draft], list(range(-1, len(draft)))))
+        rows = self.runner.verify_tokens([s.slot for s in seqs], trees)
+        now, finished = time.perf_counter(), 0
+        for k in range(max(map(len, rows), default=0)):  # the scheduler takes a token per sequence at a time
+            live = [(s, row[k]) for s, row in zip(seqs, rows) if k < len(row) and not s.is_finished]
+            finished += self.scheduler.append_tokens([s for s, _ in live], [t for _, t in live], now)
+            new_tokens.extend((s.seq_id, t) for s, t in live)
+        return finished
 
     def abort_request(self, request_id: int) -> None:
         self.scheduler.abort(self.sequences[request_id], time.perf_counter())

@@ -46,6 +46,11 @@ class Qwen2Config:
     max_position_embeddings: int = 32768
     tie_word_embeddings: bool = True
     attention_bias: bool = True
+    # Rotary layouts the reference does not have: frequencies stretched for contexts past the
+    # trained length, pairs side by side, part of each head (None: all of it).
+    rope_scaling: ops.RopeScaling | None = None
+    rope_interleaved: bool = False
+    rotary_dim: int | None = None
 
     @property
     def q_size(self) -> int:
@@ -183,8 +188,14 @@ class Qwen2Model:
                                 weights[p + "mlp.down_proj.weight"]))
         self.norm = weights["norm.weight"]
         # The reference's RoPE tables (float32, cast to the model dtype per lookup), built once.
-        self.cos, self.sin = ops.rope_tables(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta, self.dtype,
-                                             self.device)
+        # Other layouts take no tables: ops.rotary_append makes the angles.
+        self.cos = self.sin = self.rotary = None
+        if cfg.rope_interleaved or cfg.rotary_dim not in (None, cfg.head_dim):
+            self.rotary = ops.Rotary.build(cfg.rotary_dim or cfg.head_dim, cfg.rope_theta, cfg.rope_interleaved,
+                                           cfg.rope_scaling, self.device)
+        else:
+            self.cos, self.sin = ops.rope_tables(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta, self.dtype,
+                                                 self.device, cfg.rope_scaling)
 
     def weight_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self.w.values())
@@ -193,7 +204,9 @@ class Qwen2Model:
         cfg = self.cfg
         b, t, _ = x.shape
         qkv = F.linear(x, wqkv, bqkv)
-        if hasattr(ctx, "attend_qkv"):
+        if self.rotary is not None:  # this package's contexts only
+            out = ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads)
+        elif hasattr(ctx, "attend_qkv"):
             out = ctx.attend_qkv(layer, qkv, self.cos, self.sin, cfg.num_heads)  # [B, Hq, T, d]
         else:  # engine/model.py:241-250 for a context that only has attend()
             q, k, v = qkv.split([cfg.q_size, cfg.kv_size, cfg.kv_size], dim=-1)

@@ -86,8 +86,8 @@ def kv_append(pool: PkvPool, layer: int, k_rows: torch.Tensor, v_rows: torch.Ten
                             k_rows.stride(1), slot_mapping.data_ptr(), _ptr(status), _stream()), "kv_append")
 
 
-def rope_tables(head_dim: int, max_positions: int, theta: float, dtype: torch.dtype,
-                device: torch.device | str) -> tuple[torch.Tensor, torch.Tensor]:
+def rope_tables(head_dim: int, max_positions: int, theta: float, dtype: torch.dtype, device: torch.device | str,
+                scaling: "RopeScaling | None" = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The reference's cos / sin tables ``[max_positions, head_dim]``, cast to ``dtype``.
 
     The same torch calls as ``RotaryEmbedding._build`` (engine/model.py:190-199): one
@@ -95,7 +95,15 @@ def rope_tables(head_dim: int, max_positions: int, theta: float, dtype: torch.dt
     times frequencies on ``device``, the half-table repeated twice, cos and sin in float32,
     then the cast the reference applies per lookup (engine/model.py:208-210). Built on the
     same device, the tables are bit-identical to the reference's.
+
+    With ``scaling`` (the reference has none) the frequencies and the factor on cos and sin
+    are :func:`rotary_frequencies`', the angles float64.
     """
+    if scaling is not None:
+        freq, factor = rotary_frequencies(head_dim, theta, scaling, device)
+        freqs = torch.outer(torch.arange(max_positions, device=device, dtype=torch.float64), freq)
+        angles = torch.cat([freqs, freqs], dim=-1)
+        return (angles.cos() * factor).to(dtype).contiguous(), (angles.sin() * factor).to(dtype).contiguous()
     exponents = torch.arange(0, head_dim, 2, dtype=torch.int64).float() / head_dim
     inv_freq = (1.0 / (theta**exponents)).to(device)
     positions = torch.arange(max_positions, device=device, dtype=torch.float32)
@@ -552,6 +560,21 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: RopeScaling | Non
     if scaling is not None and scaling.attention_factor is not None:
         factor = scaling.attention_factor
     return freq.to(device), factor
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """What :func:`rotary_append` rotates by: the frequencies, the pairs' layout and the factor on q and k."""
+
+    inv_freq: torch.Tensor
+    interleaved: bool = False
+    attention_factor: float = 1.0
+
+    @classmethod
+    def build(cls, rotary_dim: int, theta: float, interleaved: bool = False, scaling: RopeScaling | None = None,
+              device: torch.device | str = "cuda") -> "Rotary":
+        freq, factor = rotary_frequencies(rotary_dim, theta, scaling, device)
+        return cls(freq, interleaved, factor)
 
 
 def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
