@@ -8,6 +8,7 @@ and every op of the package is unusable.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_void_p
 from pathlib import Path
 
@@ -165,6 +166,22 @@ def _load() -> ctypes.CDLL:
 
 
 lib = _load()
+
+
+def _load_binding():
+    """The compiled binding of the speculative step's calls (``_speculative.so``), as loud when it is missing."""
+    path = LIB_PATH.with_name("_speculative.so")
+    if not path.exists():
+        raise ImportError(f"{path.name} is not built; run `python mini_inference_b200/build.py`")
+    import torch  # noqa: F401  (the binding's own libraries)
+
+    spec = importlib.util.spec_from_file_location("_speculative", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+speculative = _load_binding()
 
 
 class PkvError(RuntimeError):

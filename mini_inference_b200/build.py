@@ -6,16 +6,20 @@ Every ``csrc/*.cu`` and ``csrc/*.cpp`` is compiled for
 ``-gencode arch=compute_100a,code=sm_100a`` into ``_build/`` (in parallel; a file
 is rebuilt only when it or a header changed) and linked with the static CUDA
 runtime into ``mini_inference_b200/libpkv.so``. nvcc cross-compiles, so no GPU
-is needed to build.
+is needed to build. ``csrc/bindings/speculative.cpp`` (tensors to the C ABI for the calls
+of a speculative decoding step) becomes ``mini_inference_b200/_speculative.so``, compiled
+by g++ against the installed torch's headers and linked to ``libpkv.so``.
 """
 
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -24,6 +28,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB = PKG / "libpkv.so"
+BINDING = PKG / "_speculative.so"
+BINDING_SRC = CSRC / "bindings" / "speculative.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-I", str(INCLUDE)]
@@ -62,6 +68,29 @@ def _compile(src: Path, verbose_ptxas: bool) -> Path:
     return obj
 
 
+def _bind() -> Path:
+    """The compiled binding: rebuilt when its source, the C ABI or the installed torch changed."""
+    spec = importlib.util.find_spec("torch")  # found, not imported: that takes seconds
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("torch not found: its headers are needed to build the binding")
+    torch_dir = Path(spec.submodule_search_locations[0])
+    include = torch_dir / "include"
+    if not _stale(BINDING, [BINDING_SRC, INCLUDE / "pkv.h", torch_dir / "version.py"]):
+        return BINDING
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"]]
+    for path in (include, include / "torch" / "csrc" / "api" / "include", cuda):
+        cmd += ["-isystem", str(path)]
+    cmd += [str(BINDING_SRC), "-o", str(tmp), "-L", str(PKG), "-l:libpkv.so", "-Wl,-rpath,$ORIGIN", "-L",
+            str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(verbose_ptxas: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cpp"))
@@ -74,6 +103,7 @@ def build(verbose_ptxas: bool = False) -> Path:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    _bind()
     return LIB
 
 

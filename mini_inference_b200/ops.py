@@ -16,6 +16,7 @@ import torch
 
 from ._lib import (PKV_BF16, PKV_DECODE_INPUTS_READY, PKV_DECODE_STATIC_SCRATCH_BYTES, PKV_ERR_WORKSPACE, PKV_F16,
                    PKV_LM_WEIGHT_READY, PkvError, PkvPool, PkvTables, check, lib)
+from ._lib import speculative as _speculative
 
 _DTYPES = {torch.float16: PKV_F16, torch.bfloat16: PKV_BF16}
 
@@ -424,33 +425,14 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
 
 # ---------------------------------------------------------------- speculative decoding step
 #
-# These wrappers are called once or more per layer of a step that takes the GPU a few
-# microseconds a call, so they read each tensor attribute once and ask for the raw stream of
-# the tensors' own device (torch.cuda.current_stream() builds an object, 3 us).
+# These go through a compiled binding (csrc/bindings/speculative.cpp), which checks the
+# tensors, allocates outputs and calls the C ABI on the tensors' own device and its current
+# stream: called once or more per layer, they take 2-9 us on the GPU, and the same work from
+# Python and ctypes took 7-17 us of host time a call.
 
-def _call(index: int, fn, what: str, *args) -> None:
-    """Call ``fn(*args, stream)`` on CUDA device ``index``'s current stream, whichever device is current."""
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
+def _done(status, what: str) -> None:
+    if status is not None:
         check(status, what)
-
-
-def _device_of(t: torch.Tensor) -> int:
-    index = t.get_device()
-    if index < 0:
-        _require_cuda(t)
-    return index
-
-
-def _flat(index: int, dtype: torch.dtype, what: str, *ts: torch.Tensor | None) -> None:
-    """Require contiguous tensors of ``dtype`` on CUDA device ``index`` (None is skipped)."""
-    for t in ts:
-        if t is not None and (t.dtype is not dtype or t.get_device() != index or not t.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous {dtype} tensors on cuda:{index}")
 
 
 def extend_tables(tables: PkvTables, lengths: torch.Tensor, new_tokens: torch.Tensor, held: torch.Tensor,
@@ -470,24 +452,9 @@ def extend_tables(tables: PkvTables, lengths: torch.Tensor, new_tokens: torch.Te
     row or the free list runs out, nothing is extended, every slot is -1 and the status
     word says so (see pkv_extend_tables in include/pkv.h).
     """
-    dev = _device_of(lengths)
-    held_out = held if held_out is None else held_out
-    free_head_out = free_head if free_head_out is None else free_head_out
-    _flat(dev, torch.int32, "extend_tables: lengths, counts and block ids", lengths, new_tokens, held, free_blocks,
-          free_head, cu_seqlens, context_lens, held_out, free_head_out, status)
-    _flat(dev, torch.int64, "extend_tables: positions and slot_mapping", positions, slot_mapping)
-    batch = lengths.numel()
-    if (new_tokens.numel() != batch or held.numel() != batch or context_lens.numel() < batch or
-            held_out.numel() < batch or cu_seqlens.numel() < batch + 1 or free_head.numel() < 1 or
-            free_head_out.numel() < 1):
-        raise ValueError("extend_tables: one entry per request (cu_seqlens one more, free_head one)")
-    total = positions.numel() if positions is not None else slot_mapping.numel() if slot_mapping is not None else 2**31 - 1
-    if positions is not None and slot_mapping is not None and slot_mapping.numel() != total:
-        raise ValueError("extend_tables: positions and slot_mapping must have one size")
-    _call(dev, lib.pkv_extend_tables, "extend_tables", ctypes.byref(tables), batch, lengths.data_ptr(),
-          new_tokens.data_ptr(), held.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), free_head.data_ptr(),
-          block_size, cu_seqlens.data_ptr(), context_lens.data_ptr(), _ptr(positions), _ptr(slot_mapping), total,
-          held_out.data_ptr(), free_head_out.data_ptr(), _ptr(status))
+    _done(_speculative.extend_tables(ctypes.addressof(tables), lengths, new_tokens, held, free_blocks, free_head, block_size,
+                                     cu_seqlens, context_lens, positions, slot_mapping, held_out, free_head_out, status),
+          "extend_tables")
 
 
 def build_tree_metadata(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch.Tensor,
@@ -500,15 +467,7 @@ def build_tree_metadata(parents: torch.Tensor, cu_nodes: torch.Tensor, context_l
     bit per ancestor and the node's own, ``positions`` (int64 ``[N]``) ``context_lens[b]`` +
     depth; rows behind the last tree get 0.
     """
-    dev = _device_of(parents)
-    _flat(dev, torch.int32, "build_tree_metadata: parents, cu_nodes and context_lens", parents, cu_nodes, context_lens,
-          status)
-    _flat(dev, torch.int64, "build_tree_metadata: mask and positions", mask, positions)
-    n, batch = parents.numel(), cu_nodes.numel() - 1
-    if mask.dim() != 2 or mask.size(0) != n or positions.numel() != n or context_lens.numel() < batch or batch < 0:
-        raise ValueError("build_tree_metadata: mask [N, W], positions [N], context_lens [B], cu_nodes [B + 1]")
-    _call(dev, lib.pkv_build_tree_metadata, "build_tree_metadata", parents.data_ptr(), cu_nodes.data_ptr(), batch,
-          context_lens.data_ptr(), n, mask.data_ptr(), mask.size(1), positions.data_ptr(), _ptr(status))
+    _done(_speculative.build_tree_metadata(parents, cu_nodes, context_lens, mask, positions, status), "build_tree_metadata")
 
 
 @dataclass(frozen=True)
@@ -592,36 +551,11 @@ def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch
     when True, written when tensors. With ``slot_mapping`` (int64 [N], negative = skip) the
     rotated keys and the values are also written to the pool at ``layer``.
     """
-    dev, dt = _device_of(qkv), qkv.dtype
-    hkv, d = pool.num_kv_heads, pool.head_dim
-    if qkv.dim() != 2 or qkv.size(1) != (num_q_heads + 2 * hkv) * d or qkv.stride(1) != 1:
-        raise ValueError("qkv must be [N, (Hq + 2 Hkv) * head_dim] with a contiguous last dimension")
-    if pkv_dtype(dt) != pool.dtype:
-        raise ValueError("qkv and the pool must share one dtype")
-    n, half = qkv.size(0), inv_freq.numel()
-    _flat(dev, torch.int64, "rotary_append: positions and slot_mapping", positions, slot_mapping)
-    _flat(dev, torch.int32, "rotary_append: status", status)
-    _flat(dev, torch.float64, "rotary_append: inv_freq", inv_freq)
-    if positions.numel() != n or (slot_mapping is not None and slot_mapping.numel() != n):
-        raise ValueError("rotary_append: positions and slot_mapping must have one entry per row")
-
-    def output(t: torch.Tensor | bool | None, heads: int) -> tuple[torch.Tensor | None, int | None, int, int]:
-        if t is None or t is False:
-            return None, None, 0, 0
-        if t is True:
-            t = qkv.new_empty((n, heads, d))
-            return t, t.data_ptr(), heads * d, d
-        if t.shape != (n, heads, d) or t.dtype is not dt or t.get_device() != dev or t.stride(2) != 1:
-            raise ValueError("rotary_append: outputs must be [N, heads, head_dim] like qkv, last dimension contiguous")
-        return t, t.data_ptr(), t.stride(0), t.stride(1)
-
-    q_out, *q_at = output(True if q_out is None else q_out, num_q_heads)
-    k_out, *k_at = output(k_out, hkv)
-    v_out, *v_at = output(v_out, hkv)
-    _call(dev, lib.pkv_rotary_append, "rotary_append", ctypes.byref(pool), layer, qkv.data_ptr(), qkv.stride(0), n,
-          num_q_heads, positions.data_ptr(), inv_freq.data_ptr(), 2 * half, int(interleaved), attention_factor, *q_at,
-          *k_at, *v_at, _ptr(slot_mapping), _ptr(status))
-    return q_out, k_out, v_out
+    out = _speculative.rotary_append(ctypes.addressof(pool), layer, qkv, positions, inv_freq, num_q_heads, interleaved,
+                                     attention_factor, q_out, k_out, v_out, slot_mapping, status)
+    if type(out) is int:
+        check(out, "rotary_append")
+    return out
 
 
 def tree_attention_workspace(pool: PkvPool, max_seqs: int, device: torch.device | str) -> torch.Tensor:
@@ -636,18 +570,6 @@ def tree_attention_workspace(pool: PkvPool, max_seqs: int, device: torch.device 
     return torch.zeros(nbytes, dtype=torch.uint8, device=device)
 
 
-def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
-    """``t`` [N, H, d] with rows and heads that start on 16 bytes (a copy only where they do not), its
-    address and its two strides."""
-    row, head, last = t.stride()
-    at = t.data_ptr()
-    if last != 1 or (row | head) & 7 or at & 15 or row < 0 or head < 0:
-        t = t.clone(memory_format=torch.contiguous_format)
-        row, head, _ = t.stride()
-        at = t.data_ptr()
-    return t, at, row, head
-
-
 def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor, k_nodes: torch.Tensor,
                    v_nodes: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch.Tensor, mask: torch.Tensor,
                    max_nodes: int, workspace: torch.Tensor, out: torch.Tensor | None = None,
@@ -660,33 +582,12 @@ def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor
     :func:`build_tree_metadata`). The nodes' own keys and values ``[N, Hkv, d]`` (any
     strides) are not in the pool; :func:`accept_tree` writes the accepted ones there.
     """
-    dev, dt = _device_of(q), q.dtype
-    shape = n, hq, d = q.shape
-    hkv = pool.num_kv_heads
-    if d != pool.head_dim or pkv_dtype(dt) != pool.dtype or k_nodes.dtype is not dt or v_nodes.dtype is not dt:
-        raise ValueError("q, the nodes' keys and values and the pool must share head_dim and dtype")
-    if k_nodes.shape != (n, hkv, d) or v_nodes.shape != (n, hkv, d):
-        raise ValueError("k_nodes and v_nodes must be [N, kv_heads, head_dim]")
-    if k_nodes.get_device() != dev or v_nodes.get_device() != dev or workspace.get_device() != dev:
-        raise ValueError(f"tree_attention: every tensor must be on cuda:{dev}")
-    _flat(dev, torch.int32, "tree_attention: cu_nodes and context_lens", cu_nodes, context_lens, status)
-    _flat(dev, torch.int64, "tree_attention: mask", mask)
-    batch = cu_nodes.numel() - 1
-    if mask.dim() != 2 or mask.size(0) != n or batch < 0 or context_lens.numel() < batch:
-        raise ValueError("tree_attention: mask [N, W], context_lens [B], cu_nodes [B + 1]")
-    q, *q_at = _rows16(q)
-    k_nodes, *k_at = _rows16(k_nodes)
-    v_nodes, *v_at = _rows16(v_nodes)
-    if out is None:
-        out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype is not dt or out.get_device() != dev or out.stride(2) != 1:
-        raise ValueError("out must match q, last dimension contiguous")
-    row, head, _ = out.stride()
-    _call(dev, lib.pkv_tree_attention, "tree_attention", ctypes.byref(pool), layer, ctypes.byref(tables), batch,
-          cu_nodes.data_ptr(), context_lens.data_ptr(), max_nodes, n, hq, out.data_ptr(), row, head, *q_at, *k_at, *v_at,
-          mask.data_ptr(), mask.size(1), d ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.nbytes,
-          _ptr(status))
-    return out
+    result = _speculative.tree_attention(ctypes.addressof(pool), layer, ctypes.addressof(tables), q, k_nodes, v_nodes,
+                                         cu_nodes, context_lens, mask, max_nodes, workspace, out,
+                                         pool.head_dim ** -0.5 if scale is None else scale, status)
+    if type(result) is int:
+        check(result, "tree_attention")
+    return result
 
 
 def accept_tree(pool: PkvPool, tables: PkvTables, parents: torch.Tensor, cu_nodes: torch.Tensor,
@@ -704,25 +605,9 @@ def accept_tree(pool: PkvPool, tables: PkvTables, parents: torch.Tensor, cu_node
     path's rows of ``k_nodes`` / ``v_nodes`` ``[layers, N, Hkv, d]`` at positions
     ``context_lens[b] ...`` of the sequence's blocks.
     """
-    dev = _device_of(parents)
-    n, batch = parents.numel(), cu_nodes.numel() - 1
-    lengths_out = context_lens if lengths_out is None else lengths_out
-    _flat(dev, torch.int32, "accept_tree: parents, cu_nodes, lengths, counts and path", parents, cu_nodes, context_lens,
-          counts, path, lengths_out, status)
-    _flat(dev, torch.int64, "accept_tree: tokens", draft_tokens, target_tokens, tokens)
-    if (draft_tokens.numel() != n or target_tokens.numel() != n or batch < 0 or context_lens.numel() < batch or
-            counts.numel() < batch or lengths_out.numel() < batch or path.dim() != 2 or path.shape != tokens.shape or
-            path.size(0) < batch):
-        raise ValueError("accept_tree: one token per node, counts and lengths per tree, path and tokens [B, W]")
-    shape, code = (pool.num_layers, n, pool.num_kv_heads, pool.head_dim), pool.dtype
-    k_strides, v_strides = k_nodes.stride(), v_nodes.stride()
-    for t, strides in ((k_nodes, k_strides), (v_nodes, v_strides)):
-        if t.shape != shape or pkv_dtype(t.dtype) != code or t.get_device() != dev or strides[3] != 1:
-            raise ValueError("accept_tree: k_nodes and v_nodes must be [layers, N, kv_heads, head_dim] of the pool's dtype")
-    _call(dev, lib.pkv_accept_tree, "accept_tree", ctypes.byref(pool), ctypes.byref(tables), batch, parents.data_ptr(),
-          cu_nodes.data_ptr(), n, draft_tokens.data_ptr(), target_tokens.data_ptr(), k_nodes.data_ptr(), *k_strides[:3],
-          v_nodes.data_ptr(), *v_strides[:3], context_lens.data_ptr(), counts.data_ptr(), path.data_ptr(),
-          tokens.data_ptr(), path.size(1), lengths_out.data_ptr(), _ptr(status))
+    _done(_speculative.accept_tree(ctypes.addressof(pool), ctypes.addressof(tables), parents, cu_nodes, draft_tokens,
+                                   target_tokens, k_nodes, v_nodes, context_lens, counts, path, tokens, lengths_out, status),
+          "accept_tree")
 
 
 def build_decode_metadata(tables: PkvTables, lengths: torch.Tensor, block_size: int, scratch_block: int,
