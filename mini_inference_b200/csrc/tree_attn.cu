@@ -46,7 +46,7 @@ constexpr int kRing = 4;         // stages of the K ring and of the V ring
 constexpr int kBars = 4 * kRing + 3 * kStreams + 5;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
-constexpr int kItemCost = 6;     // an item's start and end, in stages
+constexpr int kItemCost = 8;     // an item's start and end, in stages
 constexpr int kMinRange = 8;     // no CTA gets less than this
 constexpr int kMaxPieces = 160;  // CTAs at most: an item's pieces
 constexpr float kLog2e = 1.4426950408889634f;
@@ -74,10 +74,7 @@ struct TreePlan {
   int gang;       // tiles side by side: a gang's CTAs; 1 = a tile is an item of its own
   int quota, rem; // range g: quota stages, one more if g < rem
   __device__ int start(int g) const { return g * quota + min(g, rem); }
-  __device__ int range_of(int x) const {  // the range that holds position x
-    const int big = rem * (quota + 1);
-    return x < big ? x / (quota + 1) : rem + (x - big) / quota;
-  }
+  __device__ int range_of(int x) const;  // the range that holds position x
 };
 
 // A CTA's piece of an item that several ranges share, for the join.
@@ -106,6 +103,14 @@ struct TreeParams {
 
 __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// a / b for 0 <= a, 0 < b: by the reciprocal with one correction where float32 holds a
+// exactly (the quotient is off by one at most), a third of an integer division's latency.
+__device__ inline int quotient(int a, int b) {
+  if (a >= 1 << 22) return a / b;
+  const int q = (int)__fdividef((float)a, (float)b), r = a - q * b;
+  return q + (r >= b) - (r < 0);
+}
+
 // A load past L1 (kept in program order, but not waited for).
 __device__ inline float ld_cg(const float* ptr) {
   float v;
@@ -128,6 +133,11 @@ __device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c
       : "memory");
 }
 
+__device__ inline int TreePlan::range_of(int x) const {
+  const int big = rem * (quota + 1);
+  return x < big ? quotient(x, quota + 1) : rem + quotient(x - big, quota);
+}
+
 // The lengths of sequence b, clamped to what the call's own sizes allow.
 struct SeqLens {
   int first, nodes, ctx, row;
@@ -145,6 +155,9 @@ __device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) 
   s.ctx = row < 0 || row >= p.table_rows ? 0 : (int)min((int64_t)max(n, 0), (int64_t)p.table_cols * kBS);
   if (bad) report(status, PKV_ERR_OUT_OF_RANGE);
   return s;
+}
+__device__ inline int tiles_of(const TreeParams& p, int nodes) {
+  return nodes <= p.tile_nodes ? nodes > 0 : quotient(nodes + p.tile_nodes - 1, p.tile_nodes);
 }
 __device__ inline int item_cost(int nodes, int ctx) { return kItemCost + ceil_div(nodes, kNK) + ceil_div(ctx, kNK); }
 
@@ -178,7 +191,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   int32_t* s_ctx = s_nodes + kMaxSeqs;                                         // [batch] cached keys
   int32_t* s_row = s_ctx + kMaxSeqs;                                           // [batch] table row
   __shared__ CutPiece s_cut[2];  // this range's cut pieces: one that began before it, one that ends behind it
-  __shared__ int4 s_warp[32];  // per warp: least and most tiles, stages with a tile an item and with tiles in gangs
+  __shared__ int s_joins[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.batch, G = p.group;
 
@@ -204,59 +217,54 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     prefetch_tensormap(&qmap);
   }
   // ------------------------------------------------------------------ plan
-  const int per = ceil_div(B, S::THREADS), b0 = min(B, tid * per), b1 = min(B, b0 + per);
-  TreePlan plan;
-  {
-    int least = 1 << 30, most = 0, alone = 0, ganged = 0;  // stages if a tile is an item; if its item's tiles go together
-    for (int b = b0; b < b1; ++b) {
-      const SeqLens s = seq_lens(p, b, blockIdx.x == 0 ? p.status : nullptr);
-      s_first[b] = s.first;
-      s_nodes[b] = s.nodes;
-      s_ctx[b] = s.ctx;
-      s_row[b] = s.row;
-      if (s.nodes > 0) {
-        const int tiles = ceil_div(s.nodes, p.tile_nodes), cost = p.hkv * item_cost(s.nodes, s.ctx);
-        least = min(least, tiles);
-        most = max(most, tiles);
-        alone += tiles * cost;
-        ganged += cost;
-      }
-    }
-    least = __reduce_min_sync(0xffffffffu, least);
-    most = __reduce_max_sync(0xffffffffu, most);
-    int ia = alone, ig = ganged;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int ua = __shfl_up_sync(0xffffffffu, ia, o), ug = __shfl_up_sync(0xffffffffu, ig, o);
-      if (lane >= o) ia += ua, ig += ug;
-    }
-    if (lane == 31) s_warp[warp] = make_int4(least, most, ia, ig);
-    __syncthreads();
-    int total_a = 0, total_g = 0;
-    ia -= alone, ig -= ganged;  // before this thread's first sequence
-    for (int w = 0; w < S::THREADS / 32; ++w) {
-      const int4 x = s_warp[w];
-      least = min(least, x.x), most = max(most, x.y);
-      if (w < warp) ia += x.z, ig += x.w;
-      total_a += x.z, total_g += x.w;
-    }
-    plan.gang = least == most && most > 1 && most <= (int)gridDim.x ? most : 1;
-    const int total = plan.gang > 1 ? total_g : total_a;
-    int before = plan.gang > 1 ? ig : ia;
-    for (int b = b0; b < b1; ++b) {
-      s_off[b] = before;
-      const int n = s_nodes[b];
-      if (n > 0) before += p.hkv * (plan.gang > 1 ? 1 : ceil_div(n, p.tile_nodes)) * item_cost(n, s_ctx[b]);
-    }
-    plan.ranges = max(1, min((int)gridDim.x / plan.gang, total / kMinRange));
-    plan.quota = total / plan.ranges;
-    plan.rem = total - plan.quota * plan.ranges;
+  for (int b = tid; b < B; b += S::THREADS) {
+    const SeqLens s = seq_lens(p, b, blockIdx.x == 0 ? p.status : nullptr);
+    s_first[b] = s.first;
+    s_nodes[b] = s.nodes;
+    s_ctx[b] = s.ctx;
+    s_row[b] = s.row;
   }
   __syncthreads();
   tc_fence_after_sync();
+  // The rest by every warp for itself: no further barrier, and all write the same offsets.
+  TreePlan plan;
+  {
+    const int per = ceil_div(B, 32), b0 = min(B, lane * per), b1 = min(B, b0 + per);
+    int least = 1 << 30, most = 0, alone = 0, ganged = 0;  // stages if a tile is an item; if its item's tiles go together
+    for (int b = b0; b < b1; ++b) {
+      const int n = s_nodes[b];
+      if (n == 0) continue;
+      const int tiles = tiles_of(p, n), cost = p.hkv * item_cost(n, s_ctx[b]);
+      least = min(least, tiles);
+      most = max(most, tiles);
+      alone += tiles * cost;
+      ganged += cost;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    plan.gang = least == most && most > 1 && most <= (int)gridDim.x ? most : 1;
+    const int mine = plan.gang > 1 ? ganged : alone;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += u;
+    }
+    const int total = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    for (int b = b0; b < b1; ++b) {
+      s_off[b] = before;
+      const int n = s_nodes[b];
+      if (n > 0) before += p.hkv * (plan.gang > 1 ? 1 : tiles_of(p, n)) * item_cost(n, s_ctx[b]);
+    }
+    plan.ranges = max(1, min(quotient(gridDim.x, plan.gang), total / kMinRange));
+    plan.quota = quotient(total, plan.ranges);
+    plan.rem = total - plan.quota * plan.ranges;
+    __syncwarp();
+  }
   const uint32_t tmem = *tslot;
   const uint64_t deadline = global_ns() + kWaitBudgetNs;
-  const int range = blockIdx.x / plan.gang, member = blockIdx.x - range * plan.gang;
+  const int range = quotient(blockIdx.x, plan.gang), member = blockIdx.x - range * plan.gang;
   const int pos0 = range < plan.ranges ? plan.start(range) : 0;
   const int pos_end = range < plan.ranges ? plan.start(range + 1) : 0;
 
@@ -277,15 +285,15 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       u.b = lo;
       u.nodes = s_nodes[lo];
       u.ctx = s_ctx[lo];
-      const int cost = item_cost(u.nodes, u.ctx), tiles = ceil_div(u.nodes, p.tile_nodes);
-      const int rel = pos - s_off[lo], item = rel / cost, x0 = rel - item * cost;
+      const int cost = item_cost(u.nodes, u.ctx), tiles = plan.gang > 1 ? 1 : tiles_of(p, u.nodes);
+      const int rel = pos - s_off[lo], item = quotient(rel, cost), x0 = rel - item * cost;
       const int x1 = min(cost, x0 + (pos_end - pos)), item_end = pos + cost - x0;
       pos += x1 - x0;
       u.s0 = max(0, x0 - kItemCost);
       u.nst = max(0, x1 - kItemCost) - u.s0;
       if (u.nst <= 0) continue;
-      u.head = plan.gang > 1 ? item : item / tiles;
-      u.tile = plan.gang > 1 ? member : item % tiles;
+      u.head = tiles == 1 ? item : quotient(item, tiles);
+      u.tile = plan.gang > 1 ? member : item - u.head * tiles;
       u.rows = min(p.tile_nodes, u.nodes - u.tile * p.tile_nodes) * G;
       u.nns = ceil_div(u.nodes, kNK);
       u.begins = u.s0 == 0;
@@ -319,18 +327,6 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     int gs = 0, k = 0;
     Piece u;
     for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst, ++k) {
-      if (!is_v) {  // the piece's Q: rows (node, head of the group), those past the tree unused
-        if (k >= 2) ok = mbar_wait_until(&q_free[k & 1], ((k >> 1) - 1) & 1, deadline);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&q_full[k & 1], DC * 128 * G * p.tile_nodes);
-        __syncwarp();
-        if (lane < DC)
-          tma_load_4d(sQ + (k & 1) * S::QB + lane * 128 * 128, &qmap, 0, lane, u.head * G,
-                      s_first[u.b] + u.tile * p.tile_nodes, &q_full[k & 1]);
-      }
       const int32_t* table = u.ctx > 0 ? p.tables + (int64_t)s_row[u.b] * p.table_stride : nullptr;
       const int nkb = ceil_div(u.ctx, kBS);
       const int own = max(0, u.nns - u.s0);  // leading stages of the tree's own keys
@@ -345,6 +341,18 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       };
       constexpr int kPerWindow = 32 / (kNK / kBS);  // stages per window of 32 block ids
       int win = lookup(kb0 + lane), win_next = lookup(kb0 + 32 + lane);
+      if (!is_v) {  // the piece's Q: rows (node, head of the group), those past the tree unused
+        if (k >= 2) ok = mbar_wait_until(&q_free[k & 1], ((k >> 1) - 1) & 1, deadline);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&q_full[k & 1], DC * 128 * G * p.tile_nodes);
+        __syncwarp();
+        if (lane < DC)
+          tma_load_4d(sQ + (k & 1) * S::QB + lane * 128 * 128, &qmap, 0, lane, u.head * G,
+                      s_first[u.b] + u.tile * p.tile_nodes, &q_full[k & 1]);
+      }
       for (int i = 0; i < u.nst; ++i) {
         const int ci = i - own;  // context stage of the piece
         int blk = 0;
@@ -674,7 +682,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         named_barrier_sync(1, SW * 32);
         if (tid == 0) {
           if (pieces > 2)
-            s_cut[u.begins] = CutPiece{(int)node, u.head, u.rows, pieces, range - first / plan.gang, first};
+            s_cut[u.begins] = CutPiece{(int)node, u.head, u.rows, pieces, range - quotient(first, plan.gang), first};
           atom_add_acq_rel_gpu(&p.counts[2 * first], 1);
         }
       }
@@ -686,45 +694,69 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     // waits for anyone's, and all CTAs are resident) and take a share of the columns, so an
     // item cut into many pieces has as many CTAs to read them. The pieces' maxima go to
     // shared memory, over the drained rings; a thread takes one row.
-    auto slot_of = [&](const CutPiece& cut, int x) { return 2 * ((int64_t)cut.first + x * plan.gang) + (x == 0); };
-    float* const maxima = reinterpret_cast<float*>(smem) + r;  // [pieces] of this row
+    named_barrier_sync(1, SW * 32);
+    if (tid == 0 || tid == 32) {  // a range has at most two such pieces: one thread waits for each
+      const int side = tid / 32;
+      const CutPiece cut = s_cut[side];
+      if (cut.pieces > 0) {
+        int32_t* const counts = p.counts + 2 * cut.first;
+        bool all = true;
+        while (all && ld_acquire_gpu(counts) < cut.pieces) all = global_ns() <= deadline;
+        if (!all) report(p.status, PKV_ERR_TIMEOUT);
+        // Whoever is last to see the count complete leaves the counters as the next call needs them.
+        if (all && atomicAdd(counts + 1, 1) == cut.pieces - 1) {
+          st_relaxed_gpu(counts, 0);
+          st_relaxed_gpu(counts + 1, 0);
+        }
+        s_joins[side] = all;
+      }
+    }
     named_barrier_sync(1, SW * 32);
     for (int side = 0; side < 2; ++side) {
       const CutPiece cut = s_cut[side];
-      if (cut.pieces == 0) continue;
-      int32_t* const counts = p.counts + 2 * cut.first;
-      if (tid == 0) {
-        while (ok && ld_acquire_gpu(counts) < cut.pieces) ok = global_ns() <= deadline;
-        if (!ok) report(p.status, PKV_ERR_TIMEOUT);
-        s_warp[0].x = ok;
-      }
-      named_barrier_sync(1, SW * 32);
-      // Loads go out in batches (past L1, which other CTAs' stores do not reach); an index past
-      // the end repeats the last with weight 0. Each stream's warps read every other piece's
-      // maximum and sum.
-      const bool joins = s_warp[0].x && r < cut.rows;
-      const int last = cut.pieces - 1;
-      float* const ml = s_ml + r;
+      if (cut.pieces == 0 || !s_joins[side]) continue;
+      // Quads of columns: this CTA's share, the streams' warps taking every other one; about
+      // D / 8 quads of states per thread however many pieces there are. Loads (past L1, which
+      // other CTAs' stores do not reach) go out sixteen at a time, quad by quad and piece by
+      // piece, the first of them before the weights are known.
+      const bool joins = r < cut.rows;
+      const int last = cut.pieces - 1, q0 = cut.index * (D / 4) / cut.pieces + stream;
+      const int q_end = (cut.index + 1) * (D / 4) / cut.pieces;
+      auto slot_of = [&](int x) { return 2 * ((int64_t)cut.first + x * plan.gang) + (x == 0); };
+      float4 v[16];
+      int fx = 0, fq = q0;  // piece and quad of the next load
+      auto fetch = [&]() {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+          v[y] = ld_cg(p.part_o + (slot_of(fx) * (D / 4) + min(fq, D / 4 - 1)) * 128 + r);
+          if (fx == last) fx = 0, fq += kStreams;
+          else ++fx;
+        }
+      };
+      if (joins && q0 < q_end) fetch();
+      // Each stream's warps read every other piece's maximum and sum.
+      float* const maxima = reinterpret_cast<float*>(smem) + side * s_cut[0].pieces * 128 + r;  // [pieces] of this row
+      float* const ml = s_ml + side * kStreams * 256 + r;
       float top = -INFINITY, sum = 0.f;
       if (joins) {
         for (int x0 = stream; x0 <= last; x0 += 8 * kStreams) {
-          float v[8], w[8], most = top, part = 0.f;
+          float m8[8], l8[8], most = top, part = 0.f;
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
-            const int64_t at = slot_of(cut, min(x0 + y * kStreams, last)) * 256 + r;
-            v[y] = ld_cg(&p.part_ml[at]);
-            w[y] = ld_cg(&p.part_ml[at + 128]);
+            const int64_t at = slot_of(min(x0 + y * kStreams, last)) * 256 + r;
+            m8[y] = ld_cg(&p.part_ml[at]);
+            l8[y] = ld_cg(&p.part_ml[at + 128]);
           }
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             if (x0 + y * kStreams > last) continue;
-            maxima[(x0 + y * kStreams) * 128] = v[y];
-            most = fmaxf(most, v[y]);
+            maxima[(x0 + y * kStreams) * 128] = m8[y];
+            most = fmaxf(most, m8[y]);
           }
           const float mref = most == -INFINITY ? 0.f : most;
 #pragma unroll
           for (int y = 0; y < 8; ++y)
-            if (x0 + y * kStreams <= last) part += ex2(v[y] - mref) * w[y];
+            if (x0 + y * kStreams <= last) part += ex2(m8[y] - mref) * l8[y];
           sum = sum * ex2(top - mref) + part;
           top = most;
         }
@@ -736,51 +768,25 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         const float t2 = ml[(1 - stream) * 256], all = fmaxf(top, t2), mref = all == -INFINITY ? 0.f : all;
         sum = sum * ex2(top - mref) + ml[(1 - stream) * 256 + 128] * ex2(t2 - mref);
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        auto weight = [&](int x) { return x <= last ? ex2(maxima[x * 128] - mref) : 0.f; };
-        // Quads of columns: this CTA's share, the streams' warps taking every other one. Few
-        // pieces: a batch is four quads of four pieces; many: a quad of sixteen pieces.
-        const int q_end = (cut.index + 1) * (D / 4) / cut.pieces;
         T* orow = reinterpret_cast<T*>(p.out) + ((int64_t)cut.node + t) * p.out_st + (int64_t)(cut.head * G + gq) * p.out_sh;
-        auto add = [](float4& a, float w, const float4& v) { a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w; };
-        auto put = [&](int qd, const float4& a) {
-          uint32_t* o = reinterpret_cast<uint32_t*>(orow + 4 * qd);
-          o[0] = Dt<T>::pack(a.x * inv, a.y * inv);
-          o[1] = Dt<T>::pack(a.z * inv, a.w * inv);
-        };
-        auto state = [&](int x, int qd) { return ld_cg(p.part_o + (slot_of(cut, x) * (D / 4) + qd) * 128 + r); };
-        const int step = cut.pieces < 8 ? 4 : 1;
-        for (int qd = cut.index * (D / 4) / cut.pieces + stream; qd < q_end; qd += kStreams * step) {
-          float4 acc[4] = {};
-          if (step > 1) {
-            for (int x0 = 0; x0 <= last; x0 += 4) {
-              float4 v[16];
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        int x = 0, q = q0;
+        while (q < q_end) {
 #pragma unroll
-              for (int y = 0; y < 16; ++y) v[y] = state(min(x0 + y / 4, last), min(qd + y % 4 * kStreams, q_end - 1));
-#pragma unroll
-              for (int y = 0; y < 16; ++y)
-                if (x0 + y / 4 <= last) add(acc[y % 4], weight(x0 + y / 4), v[y]);
-            }
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (qd + y * kStreams < q_end) put(qd + y * kStreams, acc[y]);
-          } else {
-            for (int x0 = 0; x0 <= last; x0 += 16) {
-              float4 v[16];
-#pragma unroll
-              for (int y = 0; y < 16; ++y) v[y] = state(min(x0 + y, last), qd);
-#pragma unroll
-              for (int y = 0; y < 16; ++y)
-                if (x0 + y <= last) add(acc[0], weight(x0 + y), v[y]);
-            }
-            put(qd, acc[0]);
+          for (int y = 0; y < 16; ++y) {
+            if (q >= q_end) continue;
+            const float w = ex2(maxima[x * 128] - mref);
+            acc.x += w * v[y].x, acc.y += w * v[y].y, acc.z += w * v[y].z, acc.w += w * v[y].w;
+            if (x++ < last) continue;
+            uint32_t* o = reinterpret_cast<uint32_t*>(orow + 4 * q);
+            o[0] = Dt<T>::pack(acc.x * inv, acc.y * inv);
+            o[1] = Dt<T>::pack(acc.z * inv, acc.w * inv);
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            x = 0;
+            q += kStreams;
           }
+          if (q < q_end) fetch();
         }
-      }
-      named_barrier_sync(1, SW * 32);
-      // The last share to be joined leaves the counters as the next call needs them.
-      if (tid == 0 && ok && atom_add_acq_rel_gpu(counts + 1, 1) == cut.pieces - 1) {
-        st_relaxed_gpu(counts, 0);
-        st_relaxed_gpu(counts + 1, 0);
       }
     }
   }
