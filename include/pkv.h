@@ -436,7 +436,7 @@ PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* q
  *   q, out           : node n, query head h at q + n*q_stride_n + h*q_stride_h
  *   k_nodes, v_nodes : node n, kv head j at k_nodes + n*k_stride_n + j*k_stride_h; not in the
  *                pool. q, k_nodes and v_nodes have 16-byte aligned rows and heads (strides
- *                multiples of 8 elements, >= 0)
+ *                positive multiples of 8 elements). out overlaps none of the inputs
  *   max_nodes        : no tree has more (<= 64 * mask_words, mask_words <= 8)
  *   workspace        : pkv_tree_attention_workspace_bytes bytes, 256-byte aligned, zeroed once
  *                before first use; every call leaves it ready for the next, whatever its sizes.

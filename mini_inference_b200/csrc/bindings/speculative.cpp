@@ -216,7 +216,7 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t) {
 // Rows and heads that start on 16 bytes: the tensor itself, or a contiguous copy of it.
 Tensor rows16(const Tensor& t) {
   const int64_t row = t.stride(0), head = t.stride(1);
-  const bool ok = t.stride(2) == 1 && row >= 0 && head >= 0 && ((row | head) & 7) == 0 &&
+  const bool ok = t.stride(2) == 1 && row >= (t.size(0) > 1) && head >= (t.size(1) > 1) && ((row | head) & 7) == 0 &&
                   (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }

@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     __syncwarp();
   }
   const uint32_t tmem = *tslot;
-  const uint64_t deadline = global_ns() + kWaitBudgetNs;
+  uint64_t deadline = global_ns() + kWaitBudgetNs;  // per piece: a long call is no hang
   const int range = quotient(blockIdx.x, plan.gang), member = blockIdx.x - range * plan.gang;
   const int pos0 = range < plan.ranges ? plan.start(range) : 0;
   const int pos_end = range < plan.ranges ? plan.start(range + 1) : 0;
@@ -299,6 +299,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       u.begins = u.s0 == 0;
       u.ends = x1 == cost;
       u.item_end = item_end;
+      deadline = global_ns() + kWaitBudgetNs;
       return true;
     }
     return false;
@@ -695,6 +696,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     // item cut into many pieces has as many CTAs to read them. The pieces' maxima go to
     // shared memory, over the drained rings; a thread takes one row.
     named_barrier_sync(1, SW * 32);
+    deadline = global_ns() + kWaitBudgetNs;
     if (tid == 0 || tid == 32) {  // a range has at most two such pieces: one thread waits for each
       const int side = tid / 32;
       const CutPiece cut = s_cut[side];
@@ -854,16 +856,17 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   const int64_t tiles = std::min((int64_t)num_seqs * ((max_nodes + 128 / group - 1) / (128 / group)),
                                  total_nodes / (128 / group) + num_seqs);
   if (tiles * hkv * (kItemCost + 2 + max_nodes / kNK + tables->cols / (kNK / kBS)) > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-  if (num_seqs == 0 || max_nodes == 0 || total_nodes == 0) return PKV_OK;
+  if (num_seqs == 0 || total_nodes == 0) return PKV_OK;
   if (!tables->block_tables || !cu_nodes || !context_lens || !out || !q || !k_nodes || !v_nodes || !mask)
     return PKV_ERR_INVALID_ARGUMENT;
   auto addr = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
   if ((addr(out) & 3) || ((out_stride_n | out_stride_h) & 1)) return PKV_ERR_INVALID_ARGUMENT;
   // Q and the nodes' K/V are read by TMA: rows and heads on 16 bytes.
   const int64_t strides[6] = {q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h};
+  const int64_t steps[6] = {total_nodes, num_q_heads, total_nodes, hkv, total_nodes, hkv};
   if ((addr(q) | addr(k_nodes) | addr(v_nodes)) & 15) return PKV_ERR_INVALID_ARGUMENT;
-  for (int64_t x : strides)
-    if (x < 0 || x % 8 || x >= (int64_t)1 << 38) return PKV_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] < (steps[i] > 1) || strides[i] % 8 || strides[i] >= (int64_t)1 << 38) return PKV_ERR_INVALID_ARGUMENT;
   if (!workspace || (addr(workspace) & 255)) return PKV_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < pkv_tree_attention_workspace_bytes(num_seqs, d)) return PKV_ERR_WORKSPACE;
   CUtensorMap maps[5];

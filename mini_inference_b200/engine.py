@@ -181,7 +181,8 @@ class ModelRunner:
         self.model = model
         self.cache = cache
         self.device = cache.device
-        self.head = GreedyLMHead(model.lm_head_weight, max_batch=max_batch)
+        # At least what one kernel call takes: a verified batch has several rows per sequence.
+        self.head = GreedyLMHead(model.lm_head_weight, max_batch=max(max_batch, GreedyLMHead.KERNEL_ROWS))
         self.graphs: GraphedDecoder | None = None
         self._ids_host = torch.empty(0, dtype=torch.int64).pin_memory()
 

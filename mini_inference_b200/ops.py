@@ -580,7 +580,8 @@ def tree_attention(pool: PkvPool, layer: int, tables: PkvTables, q: torch.Tensor
     ``max_nodes`` each) attends to the sequence's ``context_lens[b]`` cached keys in the pool
     and to the nodes of its tree whose bits are set in ``mask[n]`` (int64 ``[N, W]``,
     :func:`build_tree_metadata`). The nodes' own keys and values ``[N, Hkv, d]`` (any
-    strides) are not in the pool; :func:`accept_tree` writes the accepted ones there.
+    strides) are not in the pool; :func:`accept_tree` writes the accepted ones there. ``out``
+    must not overlap the inputs.
     """
     result = _speculative.tree_attention(ctypes.addressof(pool), layer, ctypes.addressof(tables), q, k_nodes, v_nodes,
                                          cu_nodes, context_lens, mask, max_nodes, workspace, out,

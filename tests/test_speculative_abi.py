@@ -75,7 +75,7 @@ def test_tree_attention():
     assert call(t=tables(rows=3)) == BAD and call(ws=FAKE + 8) == BAD and call(nbytes=need - 1) == WORKSPACE
     assert call(words=9) == UNSUPPORTED and call(pool(bs=8)) == UNSUPPORTED and call(pool(d=96)) == UNSUPPORTED
     assert call(hq=34) == UNSUPPORTED and call(t=tables(rows=2000), n=1025) == UNSUPPORTED and call(pool(dtype=5)) == UNSUPPORTED
-    assert call(n=0) == OK and call(most=0) == OK and call(total=0, cu=None) == OK
+    assert call(n=0) == OK and call(total=0, cu=None) == OK and call(qs=0) == BAD and call(ks=0) == BAD and call(ks=-128) == BAD
 
 
 def test_accept_tree():

@@ -98,6 +98,7 @@ def test_tree_context_refusals(dev):
                            ([slot], [[-1, -1]]), ([slot], [[-1] * 1 + list(range(64))]), ([slot], [[-1] + [0] * 512])):
         with pytest.raises(ValueError):
             cache.tree_context(slots, parents)
+    assert cache.tree_context([], []).accept(torch.zeros(0, dtype=torch.int64, device=dev), torch.zeros(0, dtype=torch.int64, device=dev)) == []
     with pytest.raises(ValueError, match="no room"):
         cache.tree_context([slot], [[-1] + list(range(40))])
     with pytest.raises(TypeError):

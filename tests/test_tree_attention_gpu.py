@@ -206,6 +206,10 @@ def test_strides_and_views(dev, dtype, hq, hkv, d):
     k = case.kn.transpose(0, 1).contiguous().transpose(0, 1)
     got = case.run(q=rows[:, :hq * d].view(n, hq, d), k_nodes=k, v_nodes=rows[:, (hq + hkv) * d:].view(n, hkv, d))
     assert torch.equal(got, want)
+    # One node's rows, and one head's, for all (stride 0): copied by the wrapper.
+    same = Case(dev, dtype, hq, hkv, d, [100, 31], [9, 20], seed=7)
+    same.kn, same.vn = case.kn[:1].expand(n, hkv, d), case.vn[:, :1].expand(n, hkv, d)
+    same.check(same.run())
     # Rows on 4 bytes only: q and out by pairs, k and v copied by the wrapper.
     def odd(x):
         base = torch.zeros(n, x.shape[1] * d + 2, dtype=dtype, device=dev)
@@ -308,8 +312,9 @@ def test_bad_indexes_are_reported(dev):
     bad(tables=[[0, 1, 2, 99], [3, 4, 0, 0]])
     bad(tables=[[0, -1, 2, 3], [3, 4, 0, 0]])
     case = Case(dev, torch.float16, 14, 2, 64, [50, 20], [4, 6], seed=12)
-    with pytest.raises(IndexError):
-        case.run(max_nodes=5)
+    for most in (5, 0):
+        with pytest.raises(IndexError):
+            case.run(max_nodes=most)
     with pytest.raises(IndexError):
         case.run(seq_rows=torch.tensor([0, 2], dtype=torch.int32, device=dev))
 
