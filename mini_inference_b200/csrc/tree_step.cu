@@ -117,24 +117,27 @@ __global__ void __launch_bounds__(kPlanThreads, 1) extend_tables_kernel(const Pl
     n = max(n, (int64_t)0);
     int64_t fresh = 0;
     if (row >= 0) {
-      const int64_t need = (len + n + p.bs - 1) / p.bs;
+      const int64_t end = max(len, (int64_t)0) + n;
+      const int64_t need = end < 0x7fffffff - p.bs ? p.blocks_before((uint32_t)(end + p.bs - 1)) : 0x7fffffff;
       if (need > p.cols) bad = true;
       fresh = max(need - held, (int64_t)0);
     }
     s_len[b] = (int32_t)max(len, (int64_t)0);
     s_held[b] = (int32_t)held;
     s_row[b] = row;
+    s_cu[b] = (int32_t)n;  // the counts themselves, until what came before is known
+    s_fp[b] = (int32_t)min(fresh, (int64_t)0x7fffffff);
     sum_new += n;
     sum_fresh += fresh;
   }
   int64_t pre_new = sum_new, pre_fresh = sum_fresh, total_new, total_fresh;
   block_scan2(pre_new, pre_fresh, &total_new, &total_fresh);
-  for (int b = b0; b < b1; ++b) {  // the sums once more, now with what came before
-    const int64_t n = max((int64_t)p.new_tokens[b], (int64_t)0);
+  for (int b = b0; b < b1; ++b) {
+    const int64_t n = s_cu[b], fresh = s_fp[b];
     s_cu[b] = (int32_t)min(pre_new, p.total_tokens);
     s_fp[b] = (int32_t)min(pre_fresh, (int64_t)0x7fffffff);
     pre_new += n;
-    if (s_row[b] >= 0) pre_fresh += max(((int64_t)s_len[b] + n + p.bs - 1) / p.bs - s_held[b], (int64_t)0);
+    pre_fresh += fresh;
   }
   if (tid == 0) {
     s_cu[B] = (int32_t)min(total_new, p.total_tokens);
