@@ -323,7 +323,14 @@ __device__ inline uint32_t swz128(uint32_t row, uint32_t col) {
 // x heads_per_box KV heads of one (layer, block).
 int make_pool_tensor_map(CUtensorMap* map, const void* base, const pkv_pool& pool, int heads_per_box,
                          int chunks_per_box = 0);
-// Cached K and V maps of a pool (one encode per pool and box shape).
+// Cached K and V maps of a pool (one encode per pool and box shape). heads_per_box = kRowGroups:
+// the pool viewed as {64, R, D/64, L*NBt*Hkv*(bs/R)}, its groups of R tokens one behind the
+// other, with a box of one head's block: shared-memory layout [bs/R][D/64][R][64], in which
+// groups of 8 tokens stand at an even distance over any number of blocks. That needs R = 8
+// where a row has two chunks; with one any R does, and a block as one group copies faster
+// (64 trees over 8K keys at head_dim 64: 75 us, 81 with R = 8).
+constexpr int kRowGroups = 0;
+__host__ __device__ constexpr int row_group_tokens(int head_dim, int block_size) { return head_dim == 64 ? block_size : 8; }
 bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int heads_per_box = 1,
                    int chunks_per_box = 0);
 // 2-D tensor map over a row-major [rows, inner] matrix of 16-bit elements (row stride in
@@ -337,6 +344,10 @@ int make_matrix_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64
 // Rows past `rows` read as zeros.
 int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
                          int64_t head_stride, int64_t row_stride, int box_heads, int box_rows);
+// The same rows viewed as {64, rows, d/64, heads} with a box of {64, 8, d/64, 1}: eight rows of a
+// head per copy, in the layout [d/64][8][64].
+int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
+                              int64_t head_stride, int64_t row_stride);
 // Streaming multiprocessors of the current device (queried once).
 int num_sms();
 

@@ -107,17 +107,13 @@ int make_matrix_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64
   return PKV_OK;
 }
 
-int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
-                         int64_t head_stride, int64_t row_stride, int box_heads, int box_rows) {
+static int encode_rows(CUtensorMap* map, const void* base, int dtype, const cuuint64_t (&dims)[4],
+                       const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4]) {
   auto fn = encode_fn();
   if (!fn) {
     g_last_cuda_error = "cuTensorMapEncodeTiled is not available from the driver";
     return PKV_ERR_CUDA;
   }
-  cuuint64_t dims[4] = {64, (cuuint64_t)(d / 64), (cuuint64_t)heads, (cuuint64_t)rows};
-  // A dimension of one entry is never stepped over: any valid stride will do.
-  cuuint64_t strides[3] = {128, heads > 1 ? (cuuint64_t)head_stride * 2 : 128, rows > 1 ? (cuuint64_t)row_stride * 2 : 128};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType dt = dtype == PKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUresult r = fn(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -127,6 +123,30 @@ int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, i
     return PKV_ERR_CUDA;
   }
   return PKV_OK;
+}
+
+int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
+                         int64_t head_stride, int64_t row_stride, int box_heads, int box_rows) {
+  // A dimension of one entry is never stepped over: any valid stride will do.
+  return encode_rows(map, base, dtype, {64, (cuuint64_t)(d / 64), (cuuint64_t)heads, (cuuint64_t)rows},
+                     {128, heads > 1 ? (cuuint64_t)head_stride * 2 : 128, rows > 1 ? (cuuint64_t)row_stride * 2 : 128},
+                     {64, 1, (cuuint32_t)box_heads, (cuuint32_t)box_rows});
+}
+
+int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
+                              int64_t head_stride, int64_t row_stride) {
+  return encode_rows(map, base, dtype, {64, (cuuint64_t)rows, (cuuint64_t)(d / 64), (cuuint64_t)heads},
+                     {rows > 1 ? (cuuint64_t)row_stride * 2 : 128, 128, heads > 1 ? (cuuint64_t)head_stride * 2 : 128},
+                     {64, 8, (cuuint32_t)(d / 64), 1});
+}
+
+// Blocks, heads and a block's groups of tokens lie one behind the other in the pool: one dimension.
+static int make_pool_group_tensor_map(CUtensorMap* map, const void* base, const pkv_pool& pool) {
+  const cuuint64_t d = pool.head_dim, rows = row_group_tokens(pool.head_dim, pool.block_size);
+  const cuuint64_t groups = pool.block_size / rows;
+  const cuuint64_t all = (cuuint64_t)pool.num_layers * pool.num_blocks_total * pool.num_kv_heads * groups;
+  return encode_rows(map, base, pool.dtype, {64, rows, d / 64, all}, {d * 2, 128, rows * d * 2},
+                     {64, (cuuint32_t)rows, (cuuint32_t)(d / 64), (cuuint32_t)groups});
 }
 
 bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int heads_per_box, int chunks_per_box) {
@@ -143,8 +163,11 @@ bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int h
   e.pool = pool;
   e.heads_per_box = heads_per_box;
   e.chunks_per_box = chunks_per_box;
-  if (make_pool_tensor_map(&e.k, pool.k, pool, heads_per_box, chunks_per_box) != PKV_OK) return false;
-  if (make_pool_tensor_map(&e.v, pool.v, pool, heads_per_box, chunks_per_box) != PKV_OK) return false;
+  auto make = [&](CUtensorMap* map, const void* base) {
+    return heads_per_box == kRowGroups ? make_pool_group_tensor_map(map, base, pool)
+                                       : make_pool_tensor_map(map, base, pool, heads_per_box, chunks_per_box);
+  };
+  if (make(&e.k, pool.k) != PKV_OK || make(&e.v, pool.v) != PKV_OK) return false;
   if (g_maps.size() >= 64) g_maps.erase(g_maps.begin());
   g_maps.push_back(e);
   *tk = e.k;

@@ -18,9 +18,9 @@
 // lengths; every CTA derives the same ranges from the lengths on the device, so nothing of
 // the plan needs the host to know one. An item inside one range writes its output; one cut
 // between ranges leaves its pieces' states (running maximum, sum, unnormalised output, all
-// float32; a range has at most two cut pieces, its first and its last), which a second small
-// kernel joins. Where every tree has the same number of tiles, the tiles of an item go to as
-// many CTAs side by side over the same range of keys, so that they share its reads in L2.
+// float32; a range has at most two cut pieces, its first and its last), which the CTAs of those
+// pieces join. Where every tree has the same number of tiles, the tiles of an item go to as many
+// CTAs side by side over the same range of keys, so that they share its reads in L2.
 //
 // Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to
 // two streams, each a warp that issues tcgen05 MMAs and four softmax warps (a row per
@@ -55,7 +55,8 @@ static_assert(kRing % (2 * kStreams) == 0, "ring slots per stream and score buff
 
 template <int D> struct TreeShape {
   static constexpr int DC = D / 64;             // 64-wide head_dim chunks
-  static constexpr int KSB = DC * kNK * 128;    // one stage of K (or V): [DC][64 keys][64], 128B-swizzled
+  static constexpr int GB = DC * 1024;          // eight keys of K (or V): [DC][8 keys][64], 128B-swizzled
+  static constexpr int KSB = kNK / 8 * GB;      // a stage of them
   static constexpr int QB = DC * 128 * 128;     // the Q tile: [DC][128 rows][64], 128B-swizzled
   // TMEM columns: two score buffers and an accumulator per stream.
   static constexpr int OCOL = kStreams * 2 * kNK;
@@ -313,17 +314,19 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp < SW + 2) {
     // ---------------------------------------------------------------- TMA copies: a warp for K, one for V
-    // A copy costs the issuing warp about 85 cycles whichever lane issues it (measured): with
-    // one warp for both, 16 copies and two waits made 2000 cycles a stage at head_dim 128 and
-    // set the pace of the whole CTA.
+    // What these warps cost per stage sets the pace of the whole CTA (measured at head_dim 128,
+    // in cycles: waits that find their barrier complete 180, a copy 85 to 110 whichever lane
+    // issues it, the loop's own arithmetic 450), so a block's keys are one copy (the layout in
+    // shared memory takes groups of 8 keys, all of a row's chunks) and the loops over the tree's
+    // own keys and the context's are apart. Two copies a block and one loop: 128 us for 16
+    // trees of 40 nodes over 8K keys, so 118. Four copy warps: 120, for the registers they take
+    // from the softmax warps.
     const bool is_v = warp != SW;
     uint8_t* const ring = is_v ? sV : sK;
     uint64_t* const full = is_v ? v_full : k_full;
     uint64_t* const done = is_v ? o_done : s_done;  // the slot's last reader
     const CUtensorMap* const cmap = is_v ? &tmap_v : &tmap_k;
     const CUtensorMap* const nmap = is_v ? &nmap_v : &nmap_k;
-    constexpr int kCopies = (kNK / kBS) * DC;  // a context stage: one copy per lane
-    const int bl = lane / DC, c = lane % DC;
     bool ok = true;
     int gs = 0, k = 0;
     Piece u;
@@ -331,16 +334,19 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       const int32_t* table = u.ctx > 0 ? p.tables + (int64_t)s_row[u.b] * p.table_stride : nullptr;
       const int nkb = ceil_div(u.ctx, kBS);
       const int own = max(0, u.nns - u.s0);  // leading stages of the tree's own keys
+      const int own_end = min(own, u.nst);
       const int kb0 = max(0, u.s0 - u.nns) * (kNK / kBS);
-      auto lookup = [&](int kb) -> int {  // blocks past the sequence: masked, any block will do
-        int blk = kb < nkb ? table[kb] : p.nbt - 1;
+      // The first of a block's groups of keys in the pool's tensor map; for blocks past the
+      // sequence, which are not copied, any will do.
+      auto lookup = [&](int kb) -> int {
+        int blk = kb < nkb ? table[kb] : 0;
         if (blk < 0 || blk >= p.nbt) {
           report(p.status, PKV_ERR_OUT_OF_RANGE);
-          blk = p.nbt - 1;
+          blk = 0;
         }
-        return blk;
+        return ((p.layer * p.nbt + blk) * p.hkv + u.head) * (kBS / row_group_tokens(D, kBS));
       };
-      constexpr int kPerWindow = 32 / (kNK / kBS);  // stages per window of 32 block ids
+      constexpr int kBlocks = kNK / kBS, kPerWindow = 32 / kBlocks;  // stages per window of 32 block ids
       int win = lookup(kb0 + lane), win_next = lookup(kb0 + 32 + lane);
       if (!is_v) {  // the piece's Q: rows (node, head of the group), those past the tree unused
         if (k >= 2) ok = mbar_wait_until(&q_free[k & 1], ((k >> 1) - 1) & 1, deadline);
@@ -354,31 +360,34 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           tma_load_4d(sQ + (k & 1) * S::QB + lane * 128 * 128, &qmap, 0, lane, u.head * G,
                       s_first[u.b] + u.tile * p.tile_nodes, &q_full[k & 1]);
       }
-      for (int i = 0; i < u.nst; ++i) {
-        const int ci = i - own;  // context stage of the piece
-        int blk = 0;
-        if (ci >= 0) {
-          if (ci > 0 && ci % kPerWindow == 0) {
-            win = win_next;
-            win_next = lookup(kb0 + 32 * (ci / kPerWindow + 1) + lane);
-          }
-          blk = __shfl_sync(0xffffffffu, win, (ci * (kNK / kBS) + bl) % 32);
-        }
+      // Keys past the tree or the sequence come only as far as their group or block reaches: what
+      // a slot holds there is masked (K) or cleared (V) by the softmax warps.
+      for (int i = 0; i < own_end && ok; ++i) {
         const int j = gs + i, st = j % kRing;
         if (j >= kRing) ok = mbar_wait_until(&done[st], ((j / kRing) - 1) & 1, deadline);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], S::KSB);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int node0 = (u.s0 + i) * kNK, copies = min(kNK / 8, ceil_div(u.nodes - node0, 8));
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], copies * S::GB);
         __syncwarp();
-        uint8_t* const slot = ring + st * S::KSB;
-        if (ci >= 0) {
-          if (lane < kCopies)
-            tma_load_5d(slot + c * kNK * 128 + bl * kBS * 128, cmap, 0, 0, c, u.head, p.layer * p.nbt + blk, &full[st]);
-        } else if (lane < DC) {
-          tma_load_4d(slot + lane * kNK * 128, nmap, 0, lane, u.head, s_first[u.b] + (u.s0 + i) * kNK, &full[st]);
+        if (lane < copies)
+          tma_load_4d(ring + st * S::KSB + lane * S::GB, nmap, 0, s_first[u.b] + node0 + lane * 8, 0, u.head, &full[st]);
+      }
+      for (int i = own_end; i < u.nst && ok; ++i) {
+        const int ci = i - own;  // context stage of the piece
+        if (ci > 0 && ci % kPerWindow == 0) {
+          win = win_next;
+          win_next = lookup(kb0 + 32 * (ci / kPerWindow + 1) + lane);
         }
+        const int group = __shfl_sync(0xffffffffu, win, (ci * kBlocks + lane) % 32);
+        const int j = gs + i, st = j % kRing;
+        if (j >= kRing) ok = mbar_wait_until(&done[st], ((j / kRing) - 1) & 1, deadline);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int copies = min(kBlocks, nkb - kb0 - ci * kBlocks);
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], copies * (kBS / 8) * S::GB);
+        __syncwarp();
+        if (lane < copies) tma_load_4d(ring + st * S::KSB + lane * (kBS / 8) * S::GB, cmap, 0, 0, 0, group, &full[st]);
       }
     }
     if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
@@ -391,40 +400,32 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, true, 128, D);
       const uint32_t to = tmem + S::OCOL + stream * D;
       auto ts_of = [&](int j) { return tmem + (stream * 2 + j / kStreams % 2) * kNK; };  // S(j), then P(j)
-      // Descriptors are computed before the waits, so that the MMAs issue back to back.
-      auto pin = [](uint64_t& x) { asm volatile("" : "+l"(x)); };
+      // Shared memory ends below 2^18 bytes: a descriptor's address field takes offsets (in 16
+      // bytes) by addition.
+      const uint64_t dq = umma_desc_sw128(smem_u32(sQ), 16, 1024), dk = umma_desc_sw128(smem_u32(sK), 16, S::GB);
+      const uint64_t dv = umma_desc_sw128(smem_u32(sV), 1024, S::GB);
       auto issue_s = [&](int j, int k) -> bool {  // of piece k
         const int st = j % kRing;
-        uint64_t aq[D / 16], bk[D / 16];
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          aq[kk] = umma_desc_sw128(smem_u32(sQ + (k & 1) * S::QB + (kk / 4) * 128 * 128 + (kk % 4) * 32), 16, 1024);
-          bk[kk] = umma_desc_sw128(smem_u32(sK + st * S::KSB + (kk / 4) * kNK * 128 + (kk % 4) * 32), 16, 1024);
-          pin(aq[kk]);
-          pin(bk[kk]);
-        }
+        const uint64_t aq = dq + (k & 1) * (S::QB / 16), bk = dk + st * (S::KSB / 16);
         if (!mbar_wait_until(&k_full[st], (j / kRing) & 1, deadline)) return false;
         const int jb = j - 2 * kStreams;  // whose P the score buffer holds, until its O has read it
         if (jb >= 0 && !mbar_wait_until(&o_done[jb % kRing], (jb / kRing) & 1, deadline)) return false;
         tc_fence_after_sync();
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) umma_f16_ss(ts_of(j), aq[kk], bk[kk], idesc_s, kk > 0);
+        for (int kk = 0; kk < D / 16; ++kk) 
+          umma_f16_ss(ts_of(j), aq + (kk / 4 * 128 * 128 + kk % 4 * 32) / 16, bk + (kk / 4 * 1024 + kk % 4 * 32) / 16,
+                      idesc_s, kk > 0);
         umma_commit(&s_done[st]);
         return true;
       };
       auto issue_o = [&](int j, bool first) -> bool {
         const int st = j % kRing;
-        uint64_t bv[kNK / 16];
-#pragma unroll
-        for (int kb = 0; kb < kNK / 16; ++kb) {
-          bv[kb] = umma_desc_sw128(smem_u32(sV + st * S::KSB + kb * 16 * 128), kNK * 128, 1024);
-          pin(bv[kb]);
-        }
+        const uint64_t bv = dv + st * (S::KSB / 16);
         if (!mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) return false;
         if (!mbar_wait_until(&p_full[stream * 2 + j / kStreams % 2], (j / (2 * kStreams)) & 1, deadline)) return false;
         tc_fence_after_sync();
 #pragma unroll
-        for (int kb = 0; kb < kNK / 16; ++kb) umma_f16_ts(to, ts_of(j) + kb * 8, bv[kb], idesc_o, !first || kb > 0);
+        for (int kb = 0; kb < kNK / 16; ++kb) umma_f16_ts(to, ts_of(j) + kb * 8, bv + kb * 2 * S::GB / 16, idesc_o, !first || kb > 0);
         umma_commit(&o_done[st]);
         return true;
       };
@@ -492,11 +493,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         // included: 0 x NaN would reach the output, so they are cleared in place.
         if (keys < kNK) {
           if (ok && !mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) ok = false;
-          uint8_t* const gap = sV + st * S::KSB + keys * 128 + r * 16;
-#pragma unroll
-          for (int c = 0; c < DC; ++c) {
-            for (int x = 0; x < (kNK - keys) * 8 - r; x += 128)
-              *reinterpret_cast<uint4*>(gap + c * kNK * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+          for (int x = r; x < (kNK - keys) * DC * 8; x += 128) {
+            const int key = keys + x / (DC * 8);
+            *reinterpret_cast<uint4*>(sV + st * S::KSB + key / 8 * S::GB + x / 8 % DC * 1024 + key % 8 * 128 + x % 8 * 16) =
+                make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
@@ -870,10 +870,10 @@ extern "C" int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv
   if (!workspace || (addr(workspace) & 255)) return PKV_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < pkv_tree_attention_workspace_bytes(num_seqs, d)) return PKV_ERR_WORKSPACE;
   CUtensorMap maps[5];
-  if (!get_pool_maps(*pool, &maps[0], &maps[1], 1, 1)) return PKV_ERR_CUDA;
-  int rc = make_rows_tensor_map(&maps[2], k_nodes, pool->dtype, d, hkv, total_nodes, k_stride_h, k_stride_n, 1, kNK);
+  if (!get_pool_maps(*pool, &maps[0], &maps[1], kRowGroups)) return PKV_ERR_CUDA;
+  int rc = make_row_group_tensor_map(&maps[2], k_nodes, pool->dtype, d, hkv, total_nodes, k_stride_h, k_stride_n);
   if (rc == PKV_OK)
-    rc = make_rows_tensor_map(&maps[3], v_nodes, pool->dtype, d, hkv, total_nodes, v_stride_h, v_stride_n, 1, kNK);
+    rc = make_row_group_tensor_map(&maps[3], v_nodes, pool->dtype, d, hkv, total_nodes, v_stride_h, v_stride_n);
   if (rc == PKV_OK)
     rc = make_rows_tensor_map(&maps[4], q, pool->dtype, d, num_q_heads, total_nodes, q_stride_h, q_stride_n, group,
                               128 / group);
