@@ -372,7 +372,7 @@ PKV_API int pkv_copy_blocks(const pkv_pool* pool, const int32_t* src, const int3
  * accepted path to the cache and advances the lengths on the device. No counterpart in the
  * reference, which decodes one token per sequence and step (engine/engine.py:108-123).
  * In every call table row seq_rows[b] < 0 marks a padding sequence, which has no cached keys
- * and writes nothing; two sequences of a call must not name the same row.
+ * and writes none; two sequences of a call must not name the same row.
  *
  * pkv_extend_tables: block tables and slot maps from request lengths, without the host.
  *   tables->block_tables is written; tables->rows/cols bound it (seq_rows optional)
@@ -443,8 +443,8 @@ PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* q
  *                Calls that share a workspace must not overlap on the GPU. After a call that
  *                reported a timed-out wait, pkv_decode_reset_workspace clears its counters.
  * Rows past cu_nodes[num_seqs] of out are not written. Slots of the pool past
- * context_lens may hold anything, NaN included; K/V that any node of a tree may see must be
- * finite. Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head
+ * context_lens may hold anything, NaN included, and so may the K/V of nodes that no node's mask
+ * names (a padded tree's); K/V that any node of a tree may see must be finite. Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head
  * <= 16, num_seqs <= 1024, scale > 0; anything else returns PKV_ERR_UNSUPPORTED (a scale
  * that is not positive PKV_ERR_INVALID_ARGUMENT).
  */

@@ -32,6 +32,7 @@
 // Rounding P costs each weight half a step of its type, as much as the output's own
 // rounding; the row sum is taken before it, in float32.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -464,13 +465,19 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     };
     int gs = 0, k = 0, pos = pos0;
     Piece u, ahead;
-    // The mask word of a piece's stage, for this row: the tree's own keys that it may see.
-    auto mask_of = [&](const Piece& x, int stage) -> uint64_t {
-      return stage < x.nns && r < x.rows
-                 ? p.mask[((int64_t)s_first[x.b] + x.tile * p.tile_nodes + t) * p.words + stage] : 0;
+    // The mask words of a piece's stage, loaded a stage ahead: the tree's own keys that this
+    // row may see, and those that the lane's share of the tile's nodes may.
+    uint64_t see_next = 0, any_next = 0;
+    auto fetch_masks = [&](const Piece& x, int stage) {
+      see_next = any_next = 0;
+      if (stage >= x.nns) return;
+      const int node0 = x.tile * p.tile_nodes;
+      const uint64_t* const words = p.mask + ((int64_t)s_first[x.b] + node0) * p.words + stage;
+      if (r < x.rows) see_next = words[(int64_t)t * p.words];
+      for (int y = lane; y < min(p.tile_nodes, x.nodes - node0); y += 32) any_next |= words[(int64_t)y * p.words];
     };
     bool more = next_piece(pos, u);
-    uint64_t see_next = more ? mask_of(u, u.s0 + first_of(stream, 0)) : 0;
+    if (more) fetch_masks(u, u.s0 + first_of(stream, 0));
     for (; more; gs += u.nst, ++k, u = ahead) {
       const bool valid = r < u.rows;
       const bool live = (warp % 4) * 32 < u.rows;  // some row of the warp has a query
@@ -478,25 +485,39 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
 
       float m = -INFINITY, l = 0.f;
       const int i0 = first_of(stream, gs);
-      for (int i = i0; i < u.nst; i += kStreams) {
+      // Stage i of the piece: the tree's own keys (OWN) or the context's.
+      auto step = [&](int i, auto own_keys, auto whole) {
+        constexpr bool own = decltype(own_keys)::value;
         const int j = gs + i, sg = u.s0 + i, st = j % kRing;
-        const bool own = sg < u.nns;  // the tree's own keys
         const int keys = own ? u.nodes - sg * kNK : u.ctx - (sg - u.nns) * kNK;  // of the stage, if < kNK
         const int buf = j / kStreams % 2;
         const uint32_t ts = tl + (stream * 2 + buf) * kNK;
-        uint64_t see = own ? see_next : ~0ull;
-        if (i + kStreams < u.nst) see_next = mask_of(u, sg + kStreams);
-        if (keys < kNK) see &= (1ull << keys) - 1;
+        const bool partial = own || !decltype(whole)::value;  // not every row sees all of the stage's keys
+        uint64_t see = ~0ull, seen = ~0ull;      // by this row, by any of the tile's
+        if (partial) {
+          if (own) {
+            see = see_next;
+            seen = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(any_next >> 32)) << 32 |
+                   __reduce_or_sync(0xffffffffu, (uint32_t)any_next);
+            if (i + kStreams < u.nst) fetch_masks(u, sg + kStreams);
+          }
+          if (keys < kNK) {
+            see &= (1ull << keys) - 1;
+            seen &= (1ull << keys) - 1;
+          }
+        }
         if (ok && !mbar_wait_until(&s_done[st], (j / kRing) & 1, deadline)) ok = false;
         tc_fence_after_sync();
-        // Rows of V past the sequence or the tree hold whatever was there, infinities and NaN
-        // included: 0 x NaN would reach the output, so they are cleared in place.
-        if (keys < kNK) {
+        // Rows of V past the sequence or the tree, and those of nodes that no row sees (a padded
+        // tree's), hold whatever was there, infinities and NaN included: 0 x NaN would reach the
+        // output, so they are cleared in place.
+        if (partial && seen != ~0ull) {
           if (ok && !mbar_wait_until(&v_full[st], (j / kRing) & 1, deadline)) ok = false;
-          for (int x = r; x < (kNK - keys) * DC * 8; x += 128) {
-            const int key = keys + x / (DC * 8);
-            *reinterpret_cast<uint4*>(sV + st * S::KSB + key / 8 * S::GB + x / 8 % DC * 1024 + key % 8 * 128 + x % 8 * 16) =
-                make_uint4(0, 0, 0, 0);
+          for (int x = r; x < kNK * DC * 8; x += 128) {
+            const int key = x / (DC * 8);
+            if (!((seen >> key) & 1))
+              *reinterpret_cast<uint4*>(sV + st * S::KSB + key / 8 * S::GB + x / 8 % DC * 1024 + key % 8 * 128 + x % 8 * 16) =
+                  make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
@@ -505,7 +526,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
 #pragma unroll
           for (int c = 0; c < kNK / 32; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sa + c * 32));
           tmem_wait_ld();
-          if (own || keys < kNK) {
+          if (partial) {
             const uint32_t lo32 = (uint32_t)see, hi32 = (uint32_t)(see >> 32);
 #pragma unroll
             for (int e = 0; e < kNK; ++e)
@@ -564,9 +585,14 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[stream * 2 + buf]);
-      }
+      };
+      int i = i0;
+      for (; i < u.nst && u.s0 + i < u.nns; i += kStreams) step(i, std::true_type{}, std::false_type{});
+      const int full = min(u.nst, u.nns - u.s0 + u.ctx / kNK);  // stages before one that the sequence does not fill
+      for (; i < full; i += kStreams) step(i, std::false_type{}, std::true_type{});
+      if (i < u.nst) step(i, std::false_type{}, std::false_type{});
       more = next_piece(pos, ahead);
-      see_next = more ? mask_of(ahead, ahead.s0 + first_of(stream, gs + u.nst)) : 0;
+      if (more) fetch_masks(ahead, ahead.s0 + first_of(stream, gs + u.nst));
       // An item of two pieces is finished by the CTA of the first, at the end of its range: the
       // other piece was its CTA's first, stored long ago. One of more pieces is finished by all
       // of its CTAs, below.
@@ -578,7 +604,6 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       }
       const bool takes = pieces == 2 && u.begins, gives = pieces > 1 && !takes;
       constexpr int kChunks = D / 16 / kStreams;  // a stream's share of the output, in 16 columns
-      float4 taken[kChunks * 4];
       float m2 = -INFINITY, l2 = 0.f;
       if (takes) {
         const int64_t rest = 2 * ((int64_t)blockIdx.x + plan.gang);
@@ -588,9 +613,6 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         ok = __shfl_sync(0xffffffffu, ok, 0);
         m2 = ld_cg(&p.part_ml[rest * 256 + r]);
         l2 = ld_cg(&p.part_ml[rest * 256 + 128 + r]);
-#pragma unroll
-        for (int x = 0; x < kChunks * 4; ++x)
-          taken[x] = ld_cg(p.part_o + (rest * (D / 4) + (stream + x / 4 * kStreams) * 4 + x % 4) * 128 + r);
       }
       // The piece's streams joined: maxima and sums through shared memory, then each stream's
       // warps take their share of the output columns from every accumulator.
@@ -638,9 +660,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = 0.f;
           if (takes) {
+            const float4* const rest = p.part_o + (2 * ((int64_t)blockIdx.x + plan.gang) * (D / 4) + c * 4) * 128 + r;
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-              const float4 v = taken[share * 4 + e / 4];
+              const float4 v = ld_cg(rest + e / 4 * 128);
               acc[e] = w_rest * v.x, acc[e + 1] = w_rest * v.y, acc[e + 2] = w_rest * v.z, acc[e + 3] = w_rest * v.w;
             }
           }

@@ -187,6 +187,28 @@ def test_any_mask_and_rows_that_see_nothing(dev, dtype, hq, hkv, d):
 
 
 @pytest.mark.parametrize("dtype,hq,hkv,d", SHAPES[:2])
+def test_nodes_that_no_one_sees_may_hold_anything(dev, dtype, hq, hkv, d):
+    """Trees padded to one size: the padding's K/V are whatever the buffers held."""
+    nodes, real = [12, 150, 64, 90], [5, 130, 1, 0]
+    vis = []
+    for t, n in zip(nodes, real):
+        see = torch.zeros(t, t, dtype=torch.bool)
+        see[:n, :n] = tree_visible(n, 2)[:n, :n] if n else False
+        vis.append(see)
+    case = Case(dev, dtype, hq, hkv, d, [40, 333, 0, 16], nodes, vis=vis)
+    lo = 0
+    clean_k, clean_v = case.kn.clone(), case.vn.clone()
+    for t, n in zip(nodes, real):
+        case.kn[lo + n:lo + t] = float("nan")
+        case.vn[lo + n:lo + t, :, ::2] = float("inf")
+        case.vn[lo + n:lo + t, :, 1::2] = float("nan")
+        lo += t
+    out = case.run()
+    case.kn, case.vn = clean_k, clean_v  # unseen: the values make no difference
+    case.check(out)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", SHAPES[:2])
 def test_large_scores_move_the_maximum(dev, dtype, hq, hkv, d):
     case = Case(dev, dtype, hq, hkv, d, [900, 64], [20, 3], spread=4.0, seed=5)
     case.check(case.run())
