@@ -244,6 +244,8 @@ class ModelRunner:
         """
         if any(len(t) != len(p) for t, p in trees):
             raise ValueError("a tree has one parent per token")
+        if len(slots) == 0 and len(trees) == 0:
+            return []
         ctx = self.cache.tree_context(slots, [p for _, p in trees])
         ids = self._ids_to_device([t for tokens, _ in trees for t in tokens])
         hidden = self.model(ids.unsqueeze(0), ctx.positions.unsqueeze(0), ctx)[0]

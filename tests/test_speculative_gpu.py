@@ -166,6 +166,7 @@ def test_engine_tokens_are_the_models_greedy_choices(dev, layout, speculative):
                                            speculative_tokens=speculative))
     seqs = engine.generate(prompts, SamplingParams(max_tokens=40, ignore_eos=True))
     steps = len(engine.step_stats)
+    assert engine.runner.verify_tokens([], []) == []
     for s in seqs:
         assert len(s.output_token_ids) == 40
         rows = dense_logits(model, cfg, s.token_ids)[s.prompt_len - 1:-1]
