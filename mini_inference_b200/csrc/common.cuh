@@ -324,13 +324,10 @@ __device__ inline uint32_t swz128(uint32_t row, uint32_t col) {
 int make_pool_tensor_map(CUtensorMap* map, const void* base, const pkv_pool& pool, int heads_per_box,
                          int chunks_per_box = 0);
 // Cached K and V maps of a pool (one encode per pool and box shape). heads_per_box = kRowGroups:
-// the pool viewed as {64, R, D/64, L*NBt*Hkv*(bs/R)}, its groups of R tokens one behind the
-// other, with a box of one head's block: shared-memory layout [bs/R][D/64][R][64], in which
-// groups of 8 tokens stand at an even distance over any number of blocks. That needs R = 8
-// where a row has two chunks; with one any R does, and a block as one group copies faster
-// (64 trees over 8K keys at head_dim 64: 75 us, 81 with R = 8).
+// the pool viewed as {64, 8, D/64, L*NBt*Hkv*(bs/8)}, its groups of 8 tokens one behind the
+// other, with a box of one head's block: shared-memory layout [bs/8][D/64][8][64], in which
+// groups of 8 tokens stand at an even distance over any number of blocks.
 constexpr int kRowGroups = 0;
-__host__ __device__ constexpr int row_group_tokens(int head_dim, int block_size) { return head_dim == 64 ? block_size : 8; }
 bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int heads_per_box = 1,
                    int chunks_per_box = 0);
 // 2-D tensor map over a row-major [rows, inner] matrix of 16-bit elements (row stride in

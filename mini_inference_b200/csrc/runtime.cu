@@ -140,13 +140,12 @@ int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int
                      {64, 8, (cuuint32_t)(d / 64), 1});
 }
 
-// Blocks, heads and a block's groups of tokens lie one behind the other in the pool: one dimension.
+// Blocks, heads and a block's groups of 8 tokens lie one behind the other in the pool: one dimension.
 static int make_pool_group_tensor_map(CUtensorMap* map, const void* base, const pkv_pool& pool) {
-  const cuuint64_t d = pool.head_dim, rows = row_group_tokens(pool.head_dim, pool.block_size);
-  const cuuint64_t groups = pool.block_size / rows;
+  const cuuint64_t d = pool.head_dim, groups = pool.block_size / 8;
   const cuuint64_t all = (cuuint64_t)pool.num_layers * pool.num_blocks_total * pool.num_kv_heads * groups;
-  return encode_rows(map, base, pool.dtype, {64, rows, d / 64, all}, {d * 2, 128, rows * d * 2},
-                     {64, (cuuint32_t)rows, (cuuint32_t)(d / 64), (cuuint32_t)groups});
+  return encode_rows(map, base, pool.dtype, {64, 8, d / 64, all}, {d * 2, 128, 8 * d * 2},
+                     {64, 8, (cuuint32_t)(d / 64), (cuuint32_t)groups});
 }
 
 bool get_pool_maps(const pkv_pool& pool, CUtensorMap* tk, CUtensorMap* tv, int heads_per_box, int chunks_per_box) {

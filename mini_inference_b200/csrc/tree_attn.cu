@@ -31,6 +31,19 @@
 // computes exponentials while the other waits; their states are joined at the end of a piece.
 // Rounding P costs each weight half a step of its type, as much as the output's own
 // rounding; the row sum is taken before it, in float32.
+//
+// Measured (B200, captured calls): 16 trees of 9-18 nodes over 8K-32K keys, 28 / 4 heads of 128,
+// bf16: 122 us = 5.4 TB/s, 0.83 of the copy bandwidth. 64 trees of 1-26 nodes over 128-2048
+// keys, 14 / 2 heads of 64, fp16: 26.9 us (1.46 TB/s; an item has 3 to 33 stages, so starts, ends
+// and the set-up weigh as much as its stages). 4 trees of 129-256 nodes over 1000-4100
+// keys: 53-56 us = 0.55 PFLOP/s, tensor cores and exponentials at a third of their rates. One
+// tree of 8 nodes over 129 keys: 9 us, a launch, the plan, one load and one stage behind one
+// another. What bounds the wide cases is the warps' own instructions, with three warps on
+// a scheduler to hide their latency: without any exponential or all but one MMA of a stage the
+// time stays, with no softmax at all it falls by a tenth. Measured beside it and slower: two
+// softmax warps per row (long 142 us), stages of 128 keys with one score buffer (136 us),
+// four streams at head_dim 64 (88-127 us for 77), a separate launch for the join (7-11 us more on
+// short calls).
 #include <algorithm>
 #include <type_traits>
 
@@ -320,8 +333,8 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     // issues it, the loop's own arithmetic 450), so a block's keys are one copy (the layout in
     // shared memory takes groups of 8 keys, all of a row's chunks) and the loops over the tree's
     // own keys and the context's are apart. Two copies a block and one loop: 128 us for 16
-    // trees of 40 nodes over 8K keys, so 118. Four copy warps: 120, for the registers they take
-    // from the softmax warps.
+    // trees of 40 nodes over 8K keys; so 118. Four copy warps: 113-118 where two take 107, for the
+    // registers and issue slots they take from the softmax warps.
     const bool is_v = warp != SW;
     uint8_t* const ring = is_v ? sV : sK;
     uint64_t* const full = is_v ? v_full : k_full;
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           report(p.status, PKV_ERR_OUT_OF_RANGE);
           blk = 0;
         }
-        return ((p.layer * p.nbt + blk) * p.hkv + u.head) * (kBS / row_group_tokens(D, kBS));
+        return ((p.layer * p.nbt + blk) * p.hkv + u.head) * (kBS / 8);
       };
       constexpr int kBlocks = kNK / kBS, kPerWindow = 32 / kBlocks;  // stages per window of 32 block ids
       int win = lookup(kb0 + lane), win_next = lookup(kb0 + 32 + lane);
@@ -485,7 +498,9 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
 
       float m = -INFINITY, l = 0.f;
       const int i0 = first_of(stream, gs);
-      // Stage i of the piece: the tree's own keys (OWN) or the context's.
+      // Stage i of the piece: of the tree's own keys, or of the context's, whole or not. The three
+      // are apart because every instruction of the loop counts (64 trees over 8K keys at head_dim
+      // 64: 75 us in one loop, 71 so).
       auto step = [&](int i, auto own_keys, auto whole) {
         constexpr bool own = decltype(own_keys)::value;
         const int j = gs + i, sg = u.s0 + i, st = j % kRing;
