@@ -83,7 +83,7 @@ def _bind() -> Path:
     for path in (include, include / "torch" / "csrc" / "api" / "include", cuda):
         cmd += ["-isystem", str(path)]
     cmd += [str(BINDING_SRC), "-o", str(tmp), "-L", str(PKG), "-l:libpkv.so", "-Wl,-rpath,$ORIGIN", "-L",
-            str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+            str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")

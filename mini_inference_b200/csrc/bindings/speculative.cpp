@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -52,6 +53,11 @@ T* handle(PyObject* o) {  // the address of a ctypes structure
   return reinterpret_cast<T*>(integer(o));
 }
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
+
+// A new contiguous tensor of t's type and device, without the dispatcher's part of the call.
+Tensor fresh(at::IntArrayRef sizes, const Tensor& t) {
+  return Tensor(at::detail::empty_cuda(sizes, t.scalar_type(), t.device(), std::nullopt));
+}
 
 int cuda_index(const Tensor& t) {
   if (!t.is_cuda()) throw std::runtime_error("the paged-KV kernels need CUDA tensors (there is no CPU path)");
@@ -184,7 +190,7 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t) {
     auto output = [&](PyObject* o, int64_t heads, bool always) {
       Output x;
       if (o == Py_True || (always && !given(o))) {
-        x.t = at::empty({n, heads, d}, qkv.options());
+        x.t = fresh({n, heads, d}, qkv);
       } else if (given(o) && o != Py_False) {
         x.t = tensor(o);
         if (x.t.dim() != 3 || x.t.size(0) != n || x.t.size(1) != heads || x.t.size(2) != d ||
@@ -252,7 +258,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t) {
         call.refuse("out must match q, last dimension contiguous");
       call.here(out);
     } else {
-      out = at::empty({n, hq, d}, q.options());
+      out = fresh({n, hq, d}, q);
     }
     const int status = pkv_tree_attention(
         &pool, integer32(a[1]), handle<pkv_tables>(a[2]), (int32_t)batch, cu, ctx, integer32(a[9]), n, (int32_t)hq,
