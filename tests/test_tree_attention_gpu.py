@@ -306,6 +306,30 @@ def test_the_same_result_each_time_and_from_a_graph(dev):
     case.check(outs[0])
 
 
+def test_two_calls_at_once(dev):
+    """Calls on two streams, a workspace each, with other work on the GPU between them."""
+    from mini_inference_b200 import ops
+
+    cases = [Case(dev, torch.bfloat16, 28, 4, 128, [3000, 5000, 100, 7000], [16, 40, 16, 7], seed=1),
+             Case(dev, torch.float16, 14, 2, 64, [300] * 40, [9] * 40, seed=2)]
+    spaces = [ops.tree_attention_workspace(ops.make_pool(c.k, c.v), 64, dev) for c in cases]
+    want = [c.run() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(30):
+        for i, c in enumerate(cases):
+            status = torch.zeros(1, dtype=torch.int32, device=dev)
+            streams[i].wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(streams[i]):
+                out = ops.tree_attention(ops.make_pool(c.k, c.v), 0, ops.make_tables(c.tables), c.q, c.kn, c.vn, c.cu, c.lens,
+                                         c.mask, max(c.nodes), spaces[i], status=status)
+            outs[i].append((out, status))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(s.item() == 0 and torch.equal(o, want[i]) for o, s in outs[i])
+
+
 def test_cache_past_32_bit_offsets(dev):
     hkv, d, blocks = 8, 128, 131080  # 2^31 elements and a little more
     k = torch.zeros(1, blocks + 1, hkv, BS, d, dtype=torch.bfloat16, device=dev)
