@@ -21,6 +21,15 @@ namespace {
 constexpr int kMaxHalf = 256;  // pairs of a head: head_dim <= 512
 constexpr int kThreads = 256;   // at most
 
+// n / d for n d < 2^32 by a multiplication with ceil(2^32 / d), whose excess over 2^32 / d is
+// below one: n times it stays below 2^32 / d.
+struct Quotient {
+  uint32_t d = 1, m = 0;
+  Quotient() = default;
+  explicit Quotient(uint32_t x) : d(x), m(x > 1 ? (uint32_t)(((1ull << 32) + x - 1) / x) : 0) {}
+  __device__ int operator()(int n) const { return d > 1 ? (int)__umulhi((uint32_t)n, m) : n; }
+};
+
 struct RotaryParams {
   const void* qkv;
   const int64_t* positions;
@@ -35,6 +44,7 @@ struct RotaryParams {
   int64_t qkv_stride, q_st, q_sh, k_st, k_sh, v_st, v_sh, layer_base;
   float factor;
   int32_t hq, hkv, d, half, bs, nbt;
+  Quotient per_head, per_rest, per_v;  // a head's units: rotated, copied, of V
 };
 
 template <typename T, int EW> struct alignas(EW * sizeof(T)) Vec {
@@ -86,7 +96,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
   };
   for (int u = threadIdx.x; u < units; u += blockDim.x) {
     if (u < rot_units) {
-      const int head = u / per_head, i0 = (u - head * per_head) * EW;  // first pair
+      const int head = p.per_head(u), i0 = (u - head * per_head) * EW;  // first pair
       const int ca = INTER ? 2 * i0 : i0, cb = INTER ? 2 * i0 + EW : i0 + p.half;
       V a = *reinterpret_cast<const V*>(row + head * p.d + ca);
       V b = *reinterpret_cast<const V*>(row + head * p.d + cb);
@@ -103,10 +113,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
       put(head, ca, a);
       put(head, cb, b);
     } else if (u < rot_units + rest_units) {
-      const int w = u - rot_units, head = w / rest, c = 2 * p.half + (w - head * rest) * EW;
+      const int w = u - rot_units, head = p.per_rest(w), c = 2 * p.half + (w - head * rest) * EW;
       put(head, c, *reinterpret_cast<const V*>(row + head * p.d + c));
     } else {
-      const int w = u - rot_units - rest_units, kh = w / per_v, c = (w - kh * per_v) * EW;
+      const int w = u - rot_units - rest_units, kh = p.per_v(w), c = (w - kh * per_v) * EW;
       const V x = *reinterpret_cast<const V*>(row + (heads + kh) * p.d + c);
       if (p.v_out) *reinterpret_cast<V*>(static_cast<T*>(p.v_out) + t * p.v_st + kh * p.v_sh + c) = x;
       if (slot >= 0) *reinterpret_cast<V*>(static_cast<T*>(p.v_pool) + in_block + kh * head_step + c) = x;
@@ -115,12 +125,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
 }
 
 template <typename T>
-int launch(const RotaryParams& p, int64_t n, bool vec16, bool inter, cudaStream_t st) {
+int launch(RotaryParams p, int64_t n, bool vec16, bool inter, cudaStream_t st) {
   // Few tokens: a unit per thread, for latency. More than the SMs hold at once: four units
   // per thread, so that more tokens are under way (a CTA's chain is position, angles, rows).
   // 28 / 4 heads of 128, one and four units: 64 tokens 2.9 and 3.6 us, 592 tokens 4.1 and 4.3, 900
   // tokens 6.1 and 5.2, 8192 tokens 37 and 30.
   const int ew = vec16 ? 8 : 1;
+  p.per_head = Quotient(p.half / ew);
+  p.per_rest = Quotient(std::max(1, (p.d - 2 * p.half) / ew));
+  p.per_v = Quotient(p.d / ew);
   const int units = (p.hq + p.hkv) * (p.d - p.half) / ew + (p.v_out || p.slots ? p.hkv * p.d / ew : 0);
   const int per = n > 4 * num_sms() ? 4 : 1;
   const int threads = std::min(kThreads, std::max(64, (units + per * 32 - 1) / (per * 32) * 32));
@@ -151,7 +164,9 @@ extern "C" int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void
                        pool->num_blocks_total <= 0))
     return PKV_ERR_INVALID_ARGUMENT;
   if ((pool->dtype != PKV_F16 && pool->dtype != PKV_BF16) || rotary_dim / 2 > kMaxHalf) return PKV_ERR_UNSUPPORTED;
-  if (qkv_stride < ((int64_t)num_q_heads + 2 * (int64_t)hkv) * d) return PKV_ERR_INVALID_ARGUMENT;
+  const int64_t row = ((int64_t)num_q_heads + 2 * (int64_t)hkv) * d;
+  if (qkv_stride < row) return PKV_ERR_INVALID_ARGUMENT;
+  if (row > ((int64_t)1 << 31) / d) return PKV_ERR_UNSUPPORTED;  // units are divided in 32 bits
   if (n_tokens == 0) return PKV_OK;
   if (!qkv || !positions || !inv_freq || !q_out) return PKV_ERR_INVALID_ARGUMENT;
   if (!slot_mapping && !k_out) return PKV_ERR_INVALID_ARGUMENT;  // the rotated keys must go somewhere
