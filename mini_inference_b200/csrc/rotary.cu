@@ -54,8 +54,9 @@ template <typename T, int EW> struct alignas(EW * sizeof(T)) Vec {
 // One CTA per token: the pairs' cos and sin once into shared memory, then every head's
 // units from there. Bound by the rows' bytes, or by the chain position, angles, barrier, rows
 // when tokens are few: 8192 tokens of 28 / 4 heads of 128 (bf16, appended as they are rotated)
-// take 30 us = 5.0 TB/s, 0.78 of the copy bandwidth; 64 tokens 2.8 us. Several tokens per
-// CTA or the next unit's loads ahead of this one's stores were slower (43-53 us). A unit is EW pairs: two vectors of EW elements, half a rotation apart
+// take 29.8 us = 5.1 TB/s, 0.78 of the copy bandwidth; 64 tokens 2.8 us. Several tokens per
+// CTA or the next unit's loads ahead of this one's stores were slower (43-53 us), and so were the
+// first unit's loads ahead of the angles (33 us). A unit is EW pairs: two vectors of EW elements, half a rotation apart
 // or side by side; the elements past the rotated part and the V rows are copied.
 template <typename T, int EW, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
@@ -128,8 +129,8 @@ template <typename T>
 int launch(RotaryParams p, int64_t n, bool vec16, bool inter, cudaStream_t st) {
   // Few tokens: a unit per thread, for latency. More than the SMs hold at once: four units
   // per thread, so that more tokens are under way (a CTA's chain is position, angles, rows).
-  // 28 / 4 heads of 128, one and four units: 64 tokens 2.9 and 3.6 us, 592 tokens 4.1 and 4.3, 900
-  // tokens 6.1 and 5.2, 8192 tokens 37 and 30.
+  // 28 / 4 heads of 128, one and four units: 64 tokens 2.8 and 3.4 us, 592 tokens 4.0 and 4.2, 900
+  // tokens 5.8 and 5.1, 8192 tokens 36 and 30.
   const int ew = vec16 ? 8 : 1;
   p.per_head = Quotient(p.half / ew);
   p.per_rest = Quotient(std::max(1, (p.d - 2 * p.half) / ew));
