@@ -54,6 +54,7 @@ def test_rotary_append():
     assert call(stride=17 * 64) == BAD and call(qkv=FAKE + 1) == BAD
     assert call(layer=2, slots=FAKE) == BAD and call(pool(k=None), slots=FAKE) == BAD
     assert call(pool(dtype=7)) == UNSUPPORTED and call(pool(d=1024), stride=18 * 1024, rotary=1024) == UNSUPPORTED
+    assert call(hq=1 << 19, stride=1 << 30) == UNSUPPORTED
     assert call(n=0, qkv=None) == OK
 
 
