@@ -419,7 +419,8 @@ PKV_API int pkv_build_tree_metadata(const int32_t* parents, const int32_t* cu_no
  *   v_out (NULL = not written) : the v columns, token t, kv head j at v_out + t*stride_t + j*stride_h
  *   inv_freq : float64 [rotary_dim / 2] on the device; positions >= 0 (a negative one is
  *                reported and rotates backwards)
- * Any head_dim (rotary_dim <= 512, rows of at most 2^31 / head_dim elements); 16-byte accesses where every row, head and rotary_dim / 2 allow them.
+ * Any head_dim (rotary_dim <= 512, rows of at most 2^31 / head_dim elements); 16-byte
+ * accesses where every row, head and rotary_dim / 2 allow them.
  */
 PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* qkv, int64_t qkv_stride,
                               int64_t n_tokens, int32_t num_q_heads, const int64_t* positions,

@@ -20,7 +20,9 @@
 // between ranges leaves its pieces' states (running maximum, sum, unnormalised output, all
 // float32; a range has at most two cut pieces, its first and its last), which the CTAs of those
 // pieces join. Where every tree has the same number of tiles, the tiles of an item go to as many
-// CTAs side by side over the same range of keys, so that they share its reads in L2.
+// CTAs side by side over the same range of keys, so that they share its reads in L2 (28 / 4 heads
+// of 128: 16 trees of 64 nodes over 16K keys 260-305 us, 335 with each tile an item of its own;
+// 32 of 20 nodes 280 and 310; 16 of 40 over 8K 107 and 118).
 //
 // Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to
 // two streams, each a warp that issues tcgen05 MMAs and four softmax warps (a row per
@@ -60,8 +62,12 @@ constexpr int kRing = 4;         // stages of the K ring and of the V ring
 constexpr int kBars = 4 * kRing + 3 * kStreams + 5;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
-constexpr int kItemCost = 8;     // an item's start and end, in stages
-constexpr int kMinRange = 8;     // no CTA gets less than this
+// An item's start and end, in stages, and the least that a CTA gets, both as measured best over
+// small and large calls. Charge 5: 4 trees over 2K keys 25.1 us for 18.7, wide trees 55.8 for 53.0;
+// 11: serving batch 27.7 for 27.1. Least 4: one tree over 16K keys 24.0 us for 22.6; 12: 4 trees
+// over 2K keys 24.2 for 18.7.
+constexpr int kItemCost = 8;
+constexpr int kMinRange = 8;
 constexpr int kMaxPieces = 160;  // CTAs at most: an item's pieces
 constexpr float kLog2e = 1.4426950408889634f;
 // Every slot of a ring belongs to one stream, so that a wait sees each of its phases.
