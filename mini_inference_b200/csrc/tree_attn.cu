@@ -27,12 +27,13 @@
 // Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to
 // two streams, each a warp that issues tcgen05 MMAs and four softmax warps (a row per
 // thread) with two score buffers and an accumulator of its own in TMEM: S = Q K^T (128 x 64,
-// float32), P = 2^(S - m) rounded to the storage type over S, O += P V against a maximum m
+// float32), P = 2^(S - m) in the storage type over S, O += P V against a maximum m
 // that moves only when a row's maximum grew by more than 8 (in log2). The scores of a
 // stream's next stage are made while its warps work on the present one's, and one stream
 // computes exponentials while the other waits; their states are joined at the end of a piece.
-// Rounding P costs each weight half a step of its type, as much as the output's own
-// rounding; the row sum is taken before it, in float32.
+// P goes to the tensor cores as in this package's other attention kernels: float16 keeps 11
+// bits of a weight; bfloat16 keeps 8, so what that leaves of it follows as a second half (S leaves
+// room for both) and V is multiplied by either. The row sum is taken in float32, before any of it.
 //
 // Measured (B200, captured calls): 16 trees of 9-18 nodes over 8K-32K keys, 28 / 4 heads of 128,
 // bf16: 122 us = 5.4 TB/s, 0.83 of the copy bandwidth. 64 trees of 1-26 nodes over 128-2048
@@ -446,6 +447,11 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         tc_fence_after_sync();
 #pragma unroll
         for (int kb = 0; kb < kNK / 16; ++kb) umma_f16_ts(to, ts_of(j) + kb * 8, bv + kb * 2 * S::GB / 16, idesc_o, !first || kb > 0);
+        if constexpr (!Dt<T>::kExactP) {  // the weights' lo halves
+#pragma unroll
+          for (int kb = 0; kb < kNK / 16; ++kb)
+            umma_f16_ts(to, ts_of(j) + kNK / 2 + kb * 8, bv + kb * 2 * S::GB / 16, idesc_o, true);
+        }
         umma_commit(&o_done[st]);
         return true;
       };
@@ -589,16 +595,27 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           tc_fence_after_sync();
 #pragma unroll
           for (int c = 0; c < kNK / 32; ++c) {
-            uint32_t pk[16];
+            uint32_t pk[16], pl[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               const float2 x = ffma2(make_float2(__uint_as_float(sa[c * 32 + e]), __uint_as_float(sa[c * 32 + e + 1])), scale2,
                                      negm2);
               const float p0 = ex2(x.x), p1 = ex2(x.y);
-              pk[e / 2] = Dt<T>::pack(p0, p1);
+              if constexpr (Dt<T>::kExactP) {
+                pk[e / 2] = Dt<T>::pack(p0, p1);
+              } else {
+                // Cut, not rounded: what is left is below 2^-7 of the weight and the second half holds it
+                // to 2^-8 of itself, 2^-15 in all, and cutting takes one instruction less.
+                const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+                pk[e / 2] = __byte_perm(b0, b1, 0x7632);
+                const float2 rest = ffma2(make_float2(__uint_as_float(b0 & 0xffff0000u), __uint_as_float(b1 & 0xffff0000u)),
+                                          make_float2(-1.f, -1.f), make_float2(p0, p1));
+                pl[e / 2] = Dt<T>::pack(rest.x, rest.y);
+              }
               lsum[(e / 2) % 2] = fadd2(lsum[(e / 2) % 2], make_float2(p0, p1));
             }
             tmem_st16(ts + c * 16, pk);
+            if constexpr (!Dt<T>::kExactP) tmem_st16(ts + kNK / 2 + c * 16, pl);
           }
           tmem_wait_st();
           l += (lsum[0].x + lsum[1].x) + (lsum[0].y + lsum[1].y);

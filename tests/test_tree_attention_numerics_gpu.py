@@ -1,0 +1,60 @@
+"""pkv_tree_attention's softmax weights: the bits they keep.
+
+The tolerances count the roundings of tests/test_tree_attention_gpu.py (u = half a step of the
+storage type, A = sum_j p_j |v_j|, n visible keys, delta the error of a score), but with the weights as
+they are meant to reach the products with V:
+
+* bfloat16: two halves, the first cut (off by less than 2 u), the second that remainder rounded (off by
+  u of it), so a weight is off by 2 u u of itself.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_tree_attention_gpu import BS, Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+    return torch.device("cuda", 0)
+
+
+def expected(case, weight, scale=None):
+    """(out, tolerance) in float64 where a weight is off by `weight` of itself."""
+    u = torch.finfo(case.dtype).eps / 2
+    scale = case.d ** -0.5 if scale is None else scale
+    out = torch.zeros(case.q.shape, dtype=torch.float64, device=case.dev)
+    tol = torch.zeros_like(out)
+    group, lo = case.hq // case.hkv, 0
+    for b, t in enumerate(case.nodes):
+        c = case.ctx[b]
+        blocks = case.tables[b, :-(-c // BS)].long()
+        vis = torch.cat([torch.ones(t, c, dtype=torch.bool), case.vis[b]], 1).to(case.dev)
+        for h in range(case.hq):
+            kv = h // group
+            k = torch.cat([case.k[case.layer, blocks, kv].reshape(-1, case.d)[:c], case.kn[lo:lo + t, kv]]).double()
+            v = torch.cat([case.v[case.layer, blocks, kv].reshape(-1, case.d)[:c], case.vn[lo:lo + t, kv]]).double()
+            q = case.q[lo:lo + t, h].double()
+            p = torch.softmax((q @ k.T * scale).masked_fill(~vis, float("-inf")), -1)
+            size = ((q.abs() @ k.abs().T) * scale).masked_fill(~vis, 0.0).amax(-1, keepdim=True)
+            delta = (case.d + 4) * 2.0 ** -24 * size + 2.0 ** -21
+            n = vis.sum(-1, keepdim=True).double()
+            out[lo:lo + t, h] = o = p @ v
+            tol[lo:lo + t, h] = u * o.abs() + (weight + 2 * delta + 2 * n * 2.0 ** -23) * (p @ v.abs()) + 2.0 ** -25
+        lo += t
+    return out, tol
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("ctx,nodes", [([3, 40, 0], [1, 9, 12]), ([200], [100])])
+def test_bfloat16_weights_keep_two_halves(dev, hq, hkv, d, ctx, nodes):
+    case = Case(dev, torch.bfloat16, hq, hkv, d, ctx, nodes, seed=31)
+    want, tol = expected(case, 2 * (torch.finfo(torch.bfloat16).eps / 2) ** 2)
+    off = (case.run().double() - want).abs() - tol
+    assert off.max().item() <= 0, off.max().item()
