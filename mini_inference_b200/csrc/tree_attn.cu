@@ -28,7 +28,7 @@
 // two streams, each a warp that issues tcgen05 MMAs and four softmax warps (a row per
 // thread) with two score buffers and an accumulator of its own in TMEM: S = Q K^T (128 x 64,
 // float32), P = 2^(S - m) in the storage type over S, O += P V against a maximum m
-// that moves only when a row's maximum grew by more than 8 (in log2). The scores of a
+// that moves only when a row's maximum grew by more than kSlack (in log2). The scores of a
 // stream's next stage are made while its warps work on the present one's, and one stream
 // computes exponentials while the other waits; their states are joined at the end of a piece.
 // P goes to the tensor cores as in this package's other attention kernels: float16 keeps 11
@@ -483,7 +483,11 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     const int t = r / G, gq = r - t * G;   // node of the tile, query head of the group
     const uint32_t tl = tmem + ((uint32_t)((warp % 4) * 32) << 16);
     const uint32_t to = tl + S::OCOL + stream * D;
-    constexpr float kSlack = 8.f;
+    // 2^(S - m) is at most 2^kSlack. In float16 it is made 2^kRaise times as large (so are the row
+    // sums, and it leaves the output again with them): weights down to 2^-25 of m's are normal
+    // numbers with all their bits and the largest are 2^15; unraised, a long tail beside one
+    // dominant key would lose its bits from 2^-14 down and vanish below 2^-25.
+    constexpr float kSlack = Dt<T>::kExactP ? 4.f : 8.f, kRaise = Dt<T>::kExactP ? 11.f : 0.f;
     bool ok = true;
     auto confirm = [&](int j) {  // O += P(j) V(j) has completed
       if (ok && !mbar_wait_until(&o_done[j % kRing], (j / kRing) & 1, deadline)) ok = false;
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
           }
           const float mref = m == -INFINITY ? 0.f : m;
           float2 lsum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), negm2 = make_float2(-mref, -mref);
+          const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), negm2 = make_float2(kRaise - mref, kRaise - mref);
           tc_fence_after_sync();
 #pragma unroll
           for (int c = 0; c < kNK / 32; ++c) {

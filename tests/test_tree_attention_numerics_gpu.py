@@ -1,11 +1,13 @@
-"""pkv_tree_attention's softmax weights: the bits they keep.
+"""pkv_tree_attention's softmax weights: the bits they keep, small ones beside a large one.
 
 The tolerances count the roundings of tests/test_tree_attention_gpu.py (u = half a step of the
 storage type, A = sum_j p_j |v_j|, n visible keys, delta the error of a score), but with the weights as
 they are meant to reach the products with V:
 
 * bfloat16: two halves, the first cut (off by less than 2 u), the second that remainder rounded (off by
-  u of it), so a weight is off by 2 u u of itself.
+  u of it), so a weight is off by 2 u u of itself;
+* float16: one half, off by u of itself down to 2^-25 of the row's running maximum. (The weights
+  are made 2^11 times as large, so the smallest normal number, 2^-14, stands for 2^-25.)
 """
 
 from __future__ import annotations
@@ -13,7 +15,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_tree_attention_gpu import BS, Case
+from tests.test_tree_attention_gpu import BS, Case, SHAPES
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +60,28 @@ def test_bfloat16_weights_keep_two_halves(dev, hq, hkv, d, ctx, nodes):
     want, tol = expected(case, 2 * (torch.finfo(torch.bfloat16).eps / 2) ** 2)
     off = (case.run().double() - want).abs() - tol
     assert off.max().item() <= 0, off.max().item()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("below", [12.5, 15.0, 16.5, 17.25])
+def test_a_long_tail_beside_dominant_keys_of_no_value(dev, dtype, hq, hkv, d, below):
+    """The first key of every other block scores `below` (18 to 24.9 in log2) above all others and has value zero: the others make the output.
+
+    Scores are exact: q is one number in the first column, the keys' first column 0 or -below.
+    """
+    case = Case(dev, dtype, hq, hkv, d, [2000], [3], seed=32, poison=False)
+    case.q.zero_()
+    case.q[..., 0] = 8.0  # times the scale of 1/8: one
+    case.k[..., 1:], case.kn[..., 1:] = 0.0, 0.0
+    case.k[..., 0], case.kn[..., 0] = -below, -below
+    case.k[:, 1::2, :, 0, 0] = 0.0  # the first key of every other block, blocks in any order
+    case.v.abs_().mul_(4096.0)  # so that what is left of them is no subnormal output
+    case.vn.abs_().mul_(4096.0)
+    dominant = case.k[..., 0] == 0
+    assert int(dominant.sum()) // hkv > 50
+    case.v[dominant] = 0.0
+    u = torch.finfo(dtype).eps / 2
+    want, tol = expected(case, u if dtype == torch.float16 else 2 * u * u, scale=0.125)
+    assert (tol < 0.01 * want).all()
+    off = (case.run(scale=0.125).double() - want).abs() - tol
+    assert off.max().item() <= 0, f"{(off / want).max().item():.3e} of the value past the tolerance"
