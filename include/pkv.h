@@ -443,7 +443,8 @@ PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* q
  *                before first use; every call leaves it ready for the next, whatever its sizes.
  *                Calls that share a workspace must not overlap on the GPU. After a call that
  *                reported a timed-out wait, pkv_decode_reset_workspace clears its counters.
- * Rows past cu_nodes[num_seqs] of out are not written. Slots of the pool past
+ * Rows past cu_nodes[num_seqs] of out are not written. Bad lengths, offsets or rows are reported
+ * (PKV_ERR_OUT_OF_RANGE); with cu_nodes out of order nothing is written. Slots of the pool past
  * context_lens may hold anything, NaN included, and so may the K/V of nodes that no node's mask
  * names (a padded tree's); K/V that any node of a tree may see must be finite. Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head
  * <= 16, num_seqs <= 1024, scale > 0; anything else returns PKV_ERR_UNSUPPORTED (a scale

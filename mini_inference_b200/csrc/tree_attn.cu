@@ -163,6 +163,7 @@ __device__ inline int TreePlan::range_of(int x) const {
 // The lengths of sequence b, clamped to what the call's own sizes allow.
 struct SeqLens {
   int first, nodes, ctx, row;
+  bool ordered;  // its offsets do not fall
 };
 __device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) {
   SeqLens s;
@@ -173,6 +174,7 @@ __device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) 
   s.first = (int)min((int64_t)max(lo, 0), p.total_nodes);
   s.nodes = min(max((int)min((int64_t)hi, p.total_nodes) - s.first, 0), p.max_nodes);
   s.row = row;
+  s.ordered = hi >= lo;
   // A padding row has no cached keys.
   s.ctx = row < 0 || row >= p.table_rows ? 0 : (int)min((int64_t)max(n, 0), (int64_t)p.table_cols * kBS);
   if (bad) report(status, PKV_ERR_OUT_OF_RANGE);
@@ -239,14 +241,18 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     prefetch_tensormap(&qmap);
   }
   // ------------------------------------------------------------------ plan
+  bool ordered = true;
   for (int b = tid; b < B; b += S::THREADS) {
     const SeqLens s = seq_lens(p, b, blockIdx.x == 0 ? p.status : nullptr);
     s_first[b] = s.first;
     s_nodes[b] = s.nodes;
     s_ctx[b] = s.ctx;
     s_row[b] = s.row;
+    ordered = ordered && s.ordered;
   }
-  __syncthreads();
+  // Node offsets out of order (reported) would let trees overlap, and the sum of their stages pass
+  // what the host has bounded by the nodes: then nothing is computed.
+  const bool none = __syncthreads_or(!ordered);
   tc_fence_after_sync();
   // The rest by every warp for itself: no further barrier, and all write the same offsets.
   TreePlan plan;
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       const int u = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += u;
     }
-    const int total = __shfl_sync(0xffffffffu, before, 31);
+    const int total = none ? 0 : __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
     for (int b = b0; b < b1; ++b) {
       s_off[b] = before;

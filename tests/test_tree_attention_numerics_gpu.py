@@ -85,3 +85,14 @@ def test_a_long_tail_beside_dominant_keys_of_no_value(dev, dtype, hq, hkv, d, be
     assert (tol < 0.01 * want).all()
     off = (case.run(scale=0.125).double() - want).abs() - tol
     assert off.max().item() <= 0, f"{(off / want).max().item():.3e} of the value past the tolerance"
+
+
+def test_nothing_is_computed_from_node_offsets_out_of_order(dev):
+    """Trees that would overlap are reported and no output is written: their stages are not bounded by the nodes."""
+    case = Case(dev, torch.float16, 14, 2, 64, [50, 20, 9], [4, 6, 2], seed=34)
+    for cu in ([0, 10, 4, 12], [4, 0, 10, 12], [0, 4, 12, 10]):
+        case.cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+        out = torch.full_like(case.q, 3.0)
+        with pytest.raises(IndexError):
+            case.run(out=out, max_nodes=12)
+        assert (out == 3).all()
