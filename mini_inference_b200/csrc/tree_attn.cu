@@ -162,8 +162,7 @@ __device__ inline int TreePlan::range_of(int x) const {
 
 // The lengths of sequence b, clamped to what the call's own sizes allow.
 struct SeqLens {
-  int first, nodes, ctx, row;
-  bool ordered;  // its offsets do not fall
+  int first, nodes, ctx, row;  // nodes -1: its offsets fall
 };
 __device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) {
   SeqLens s;
@@ -172,9 +171,8 @@ __device__ inline SeqLens seq_lens(const TreeParams& p, int b, int32_t* status) 
   const bool bad = lo < 0 || hi < lo || hi > p.total_nodes || hi - lo > p.max_nodes || n < 0 ||
              n > (int64_t)p.table_cols * kBS || row >= p.table_rows;
   s.first = (int)min((int64_t)max(lo, 0), p.total_nodes);
-  s.nodes = min(max((int)min((int64_t)hi, p.total_nodes) - s.first, 0), p.max_nodes);
+  s.nodes = hi < lo ? -1 : min(max((int)min((int64_t)hi, p.total_nodes) - s.first, 0), p.max_nodes);
   s.row = row;
-  s.ordered = hi >= lo;
   // A padding row has no cached keys.
   s.ctx = row < 0 || row >= p.table_rows ? 0 : (int)min((int64_t)max(n, 0), (int64_t)p.table_cols * kBS);
   if (bad) report(status, PKV_ERR_OUT_OF_RANGE);
@@ -241,27 +239,25 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     prefetch_tensormap(&qmap);
   }
   // ------------------------------------------------------------------ plan
-  bool ordered = true;
   for (int b = tid; b < B; b += S::THREADS) {
     const SeqLens s = seq_lens(p, b, blockIdx.x == 0 ? p.status : nullptr);
     s_first[b] = s.first;
     s_nodes[b] = s.nodes;
     s_ctx[b] = s.ctx;
     s_row[b] = s.row;
-    ordered = ordered && s.ordered;
   }
-  // Node offsets out of order (reported) would let trees overlap, and the sum of their stages pass
-  // what the host has bounded by the nodes: then nothing is computed.
-  const bool none = __syncthreads_or(!ordered);
+  __syncthreads();
   tc_fence_after_sync();
   // The rest by every warp for itself: no further barrier, and all write the same offsets.
   TreePlan plan;
   {
     const int per = ceil_div(B, 32), b0 = min(B, lane * per), b1 = min(B, b0 + per);
+    constexpr int kDisorder = 1 << 30;
     int least = 1 << 30, most = 0, alone = 0, ganged = 0;  // stages if a tile is an item; if its item's tiles go together
     for (int b = b0; b < b1; ++b) {
       const int n = s_nodes[b];
-      if (n == 0) continue;
+      if (n < 0) most = kDisorder;
+      if (n <= 0) continue;
       const int tiles = tiles_of(p, n), cost = p.hkv * item_cost(n, s_ctx[b]);
       least = min(least, tiles);
       most = max(most, tiles);
@@ -278,7 +274,9 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       const int u = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += u;
     }
-    const int total = none ? 0 : __shfl_sync(0xffffffffu, before, 31);
+    // Node offsets out of order (reported) would let trees overlap, and the sum of their stages pass
+    // what the host has bounded by the nodes: then nothing is computed.
+    const int total = most == kDisorder ? 0 : __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
     for (int b = b0; b < b1; ++b) {
       s_off[b] = before;
