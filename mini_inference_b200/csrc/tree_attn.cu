@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     const CUtensorMap* const cmap = is_v ? &tmap_v : &tmap_k;
     const CUtensorMap* const nmap = is_v ? &nmap_v : &nmap_k;
     bool ok = true;
-    int gs = 0, k = 0;
+    int gs = 0, k = 0, stopped = 0;  // stages and pieces before this one; the stage a wait ran out at
     Piece u;
     for (int pos = pos0; ok && next_piece(pos, u); gs += u.nst, ++k) {
       const int32_t* table = u.ctx > 0 ? p.tables + (int64_t)s_row[u.b] * p.table_stride : nullptr;
@@ -377,6 +377,7 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         if (k >= 2) ok = mbar_wait_until(&q_free[k & 1], ((k >> 1) - 1) & 1, deadline);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
+          stopped = gs;
           break;
         }
         if (lane == 0) mbar_arrive_expect_tx(&q_full[k & 1], DC * 128 * G * p.tile_nodes);
@@ -391,7 +392,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         const int j = gs + i, st = j % kRing;
         if (j >= kRing) ok = mbar_wait_until(&done[st], ((j / kRing) - 1) & 1, deadline);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) {
+          stopped = j;
+          break;
+        }
         const int node0 = (u.s0 + i) * kNK, copies = min(kNK / 8, ceil_div(u.nodes - node0, 8));
         if (lane == 0) mbar_arrive_expect_tx(&full[st], copies * S::GB);
         __syncwarp();
@@ -408,7 +412,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
         const int j = gs + i, st = j % kRing;
         if (j >= kRing) ok = mbar_wait_until(&done[st], ((j / kRing) - 1) & 1, deadline);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) {
+          stopped = j;
+          break;
+        }
         const int copies = min(kBlocks, nkb - kb0 - ci * kBlocks);
         if (lane == 0) mbar_arrive_expect_tx(&full[st], copies * (kBS / 8) * S::GB);
         __syncwarp();
@@ -416,6 +423,12 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
       }
     }
     if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
+    // No copy may still be under way when the CTA leaves its shared memory. The MMA warps wait for
+    // each of them, unless one gave up: so every ring slot's last copy, and every Q buffer's, again.
+    const int issued = ok ? gs : stopped;
+    const uint64_t until = global_ns() + kWaitBudgetNs;
+    for (int j = max(0, issued - kRing); j < issued; ++j) mbar_wait_until(&full[j % kRing], (j / kRing) & 1, until);
+    for (int x = max(0, k - 2); x < k && !is_v; ++x) mbar_wait_until(&q_full[x & 1], (x >> 1) & 1, until);
   } else {
     // ---------------------------------------------------------------- MMA issue, one warp per stream
     if (lane == 0) {
