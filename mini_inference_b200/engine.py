@@ -251,7 +251,9 @@ class ModelRunner:
         hidden = self.model(ids.unsqueeze(0), ctx.positions.unsqueeze(0), ctx)[0]
         step = self.head.max_batch
         targets = torch.cat([self.head(hidden[a:a + step]).clone() for a in range(0, ctx.total, step)])
-        return ctx.accept(ids, targets)
+        new = ctx.accept(ids, targets)
+        self.head.raise_device_errors()
+        return new
 
 
 @dataclass

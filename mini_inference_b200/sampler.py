@@ -60,9 +60,13 @@ class GreedyLMHead:
         if params is not None and not all(p.greedy for p in params):
             raise ValueError("sampled requests need the logits: use compute_logits and the reference Sampler")
         ids = self(hidden).tolist()
+        self.raise_device_errors()
+        return ids
+
+    def raise_device_errors(self) -> None:
+        """Synchronise and raise what a call recorded since the last check (a timed-out wait)."""
         try:
             ops.raise_device_errors(self.status)
         except RuntimeError:
             self.workspace.zero_()  # a call that gave up may have left maxima or its ticket behind
             raise
-        return ids
