@@ -504,6 +504,13 @@ PKV_API int pkv_bm_allocate(pkv_block_manager* bm, int64_t num_tokens, const int
 PKV_API int pkv_bm_register_prefix(pkv_block_manager* bm, int32_t slot, const int64_t* token_ids, int64_t n_ids);
 /* engine/kv_cache.py:542-551; *out = 0 when the pool (or max_len) cannot hold num_tokens */
 PKV_API int pkv_bm_ensure_capacity(pkv_block_manager* bm, int32_t slot, int64_t num_tokens, int32_t* out);
+/*
+ * Gives back the blocks of a slot behind those of its first num_tokens tokens, the last taken
+ * first, so that growing a table and truncating it again leaves the free pool as it was (but for
+ * prefix keys of blocks it took). PKV_ERR_OUT_OF_RANGE if num_tokens is below the slot's length.
+ * No counterpart in the reference, whose tables only grow.
+ */
+PKV_API int pkv_bm_truncate(pkv_block_manager* bm, int32_t slot, int64_t num_tokens);
 /* engine/kv_cache.py:553-560; PKV_ERR_DOUBLE_FREE for a slot without a table */
 PKV_API int pkv_bm_free(pkv_block_manager* bm, int32_t slot);
 /*

@@ -133,6 +133,7 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_bm_allocate": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, P_I32]),
     "pkv_bm_register_prefix": (c_int32, [c_void_p, c_int32, c_void_p, c_int64]),
     "pkv_bm_ensure_capacity": (c_int32, [c_void_p, c_int32, c_int64, P_I32]),
+    "pkv_bm_truncate": (c_int32, [c_void_p, c_int32, c_int64]),
     "pkv_bm_free": (c_int32, [c_void_p, c_int32]),
     "pkv_bm_fork": (c_int32, [c_void_p, c_int32, P_I32]),
     "pkv_bm_prepare_write": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int32, P_I32]),

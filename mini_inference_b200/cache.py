@@ -98,6 +98,14 @@ class NativeBlockManager:
         check(st, "ensure_capacity")
         return bool(self._i32.value)
 
+    def truncate(self, slot: int, num_tokens: int) -> None:
+        st = lib.pkv_bm_truncate(self._h, slot, num_tokens)
+        if st == PKV_ERR_UNKNOWN_SLOT:
+            raise KeyError(slot)
+        if st == PKV_ERR_OUT_OF_RANGE:
+            raise ValueError(f"slot {slot} holds more than {num_tokens} tokens")
+        check(st, "truncate")
+
     def free(self, slot: int) -> None:
         st = lib.pkv_bm_free(self._h, slot)
         if st == PKV_ERR_DOUBLE_FREE:
@@ -130,6 +138,13 @@ class NativeBlockManager:
             buf = (ctypes.c_int32 * n)()
             check(lib.pkv_bm_get_table(self._h, slot, buf, n, ctypes.byref(self._i32)), "block_tables")
         return list(buf[:n])
+
+    def num_blocks_held(self, slot: int) -> int:
+        st = lib.pkv_bm_get_table(self._h, slot, None, 0, ctypes.byref(self._i32))
+        if st == PKV_ERR_UNKNOWN_SLOT:
+            raise KeyError(slot)
+        check(st, "block_tables")
+        return self._i32.value
 
     def live_slots(self) -> list[int]:
         buf = (ctypes.c_int32 * max(self.max_seqs, 1))()
@@ -354,6 +369,14 @@ class PagedKVCache:
 
     def ensure_capacity(self, slot: int, num_tokens: int) -> bool:
         return self._bm.ensure_capacity(slot, num_tokens)
+
+    def truncate(self, slot: int, num_tokens: int) -> None:
+        """Give back the blocks behind those of the first ``num_tokens`` tokens (no counterpart in the reference)."""
+        self._bm.truncate(slot, num_tokens)
+
+    def num_blocks_held(self, slot: int) -> int:
+        """``len(block_tables[slot])`` without building the list."""
+        return self._bm.num_blocks_held(slot)
 
     def free(self, slot: int) -> None:
         self._bm.free(slot)
@@ -660,7 +683,8 @@ class TreeContext:
     node hangs below an earlier one (``parents``, -1 for node 0) and holds a drafted token.
     The model runs over all nodes packed end to end, node ``n`` at position ``length +
     depth``; each attends to its sequence's cached keys and to its ancestors. The nodes' keys
-    and values stay outside the cache until :meth:`accept` writes the accepted path's.
+    and values stay outside the cache until :meth:`accept` writes the accepted path's. Blocks
+    for the longest path are taken at the start; :meth:`accept` gives back those it left unused.
     """
 
     def __init__(self, cache: PagedKVCache, slots: Sequence[int], parents: Sequence[Sequence[int]]) -> None:
@@ -683,6 +707,7 @@ class TreeContext:
         if max(sizes, default=1) > 512 or max(depth, default=1) > 64:
             raise ValueError("trees of up to 512 nodes and 64 levels")
         self.starts = [cache.lengths[s] for s in self.slots]
+        self._held = [cache.num_blocks_held(s) for s in self.slots]
         for s, start, n in zip(self.slots, self.starts, depth):
             if not cache.ensure_capacity(s, start + n):
                 raise ValueError(f"no room in the KV cache for {start + n} tokens")
@@ -753,6 +778,7 @@ class TreeContext:
                         self.k_nodes[:, :, :, 0], self.v_nodes[:, :, :, 0], self.context_lens, counts, path, tokens,
                         lengths_out=lengths, status=cache.status)
         new = [row[:n] for n, row in zip(counts.tolist(), tokens.tolist())]
-        for slot, start, row in zip(self.slots, self.starts, new):
+        for slot, start, held, row in zip(self.slots, self.starts, self._held, new):
             cache.lengths[slot] = start + len(row)
+            cache.truncate(slot, max(start + len(row), held * cache.block_size))
         return new

@@ -285,6 +285,16 @@ int pkv_bm_ensure_capacity(pkv_block_manager* bm, int32_t slot, int64_t num_toke
   return PKV_OK;
 }
 
+int pkv_bm_truncate(pkv_block_manager* bm, int32_t slot, int64_t num_tokens) {
+  if (!bm) return PKV_ERR_INVALID_ARGUMENT;
+  if (!bm->valid_slot(slot)) return PKV_ERR_UNKNOWN_SLOT;
+  if (num_tokens < bm->lengths[slot]) return PKV_ERR_OUT_OF_RANGE;
+  std::vector<int32_t>& table = bm->tables[slot];
+  for (const int64_t keep = bm->blocks_for(num_tokens); static_cast<int64_t>(table.size()) > keep; table.pop_back())
+    bm->drop_ref(table.back());
+  return PKV_OK;
+}
+
 int pkv_bm_free(pkv_block_manager* bm, int32_t slot) {
   if (!bm) return PKV_ERR_INVALID_ARGUMENT;
   if (!bm->valid_slot(slot)) return PKV_ERR_DOUBLE_FREE;

@@ -369,13 +369,15 @@ class LLMEngine:
         """
         lasts = self.scheduler.decode_last_tokens()
         trees = []
+        free = self.cache.num_free_blocks  # taken by the tree context and, where a draft fails, given back
         for s, last in zip(seqs, lasts):
             ids = s.token_ids[:self.cache.lengths[s.slot]] + [int(last)]  # a chunked prefill may leave one prompt token
             room = min(self.config.speculative_tokens, s.sampling.max_tokens - len(s.output_token_ids) - 1,
                        self.config.max_model_len - len(ids) - 1)
             draft = draft_by_lookup(ids, room) if room > 0 else []
-            if draft and not self.cache.ensure_capacity(s.slot, len(ids) + len(draft)):
-                draft = []
+            held = self.cache.num_blocks_held(s.slot)
+            draft = draft[:max(0, (held + free) * self.cache.block_size - len(ids))]
+            free -= max(0, self.cache.blocks_for(len(ids) + len(draft)) - held)
             trees.append(([int(last), *draft], list(range(-1, len(draft)))))
         rows = self.runner.verify_tokens([s.slot for s in seqs], trees)
         now, finished = time.perf_counter(), 0

@@ -62,3 +62,46 @@ def test_an_error_of_the_lm_head_is_raised(dev):
     with pytest.raises(RuntimeError, match="timed out"):
         engine.runner.verify_tokens([slot], [([6], [-1])])
     assert engine.runner.verify_tokens([slot], [([7], [-1])])  # cleared
+
+
+def test_drafts_take_no_block_that_a_decode_step_needs(dev):
+    """A pool in which plain decoding preempts nothing: nor does drafting, and the tokens are still greedy choices.
+
+    Four sequences end at 71, 71, 50 and 61 tokens, 18 blocks of 16 in all, as many as there are.
+    """
+    from mini_inference_b200.engine import SamplingParams
+
+    model, prompts = make_model(dev), prompts_of()
+    params = SamplingParams(max_tokens=40, ignore_eos=True)
+    for speculative in (0, 40):
+        engine = make_engine(model, max_model_len=80, kv_cache_tokens=18 * 16, speculative_tokens=speculative)
+        for p in prompts:
+            engine.add_request(p, params)
+        while engine.has_unfinished_requests():
+            engine.step()
+            for s in engine.scheduler.running:
+                assert len(engine.cache.block_tables[s.slot]) <= engine.cache.blocks_for(s.num_tokens)
+        engine.check_device_errors()
+        assert engine.scheduler.num_preemptions == 0
+        assert engine.cache.num_free_blocks == 18
+        check_greedy(model, engine.sequences.values())
+
+
+def test_a_tree_gives_back_what_its_path_left_unused(dev):
+    from mini_inference_b200 import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 64, num_blocks=12, block_size=16, max_seqs=3, max_len=160, dtype=torch.float16, device=dev)
+    a, b = cache.allocate(10), cache.allocate(60)  # the second one's spare blocks are its caller's own
+    cache.lengths[a], cache.lengths[b] = 10, 15
+    ctx = cache.tree_context([a, b], [[-1] + list(range(40)), [-1, 0]])
+    assert len(cache.block_tables[a]) == 4 and len(cache.block_tables[b]) == 4
+    x = torch.randn(1, 2, 43, 64, device=dev).half()
+    ctx.attend(0, x, x, x)
+    ids = torch.arange(43, device=dev)
+    assert ctx.accept(ids, ids + 1000) == [[1000], [1041]]  # nothing drafted is right
+    assert len(cache.block_tables[a]) == 1 and len(cache.block_tables[b]) == 4 and cache.num_free_blocks == 7
+    ctx = cache.tree_context([a, b], [[-1] + list(range(40)), [-1, 0]])
+    ctx.attend(0, x, x, x)
+    assert [len(row) for row in ctx.accept(ids, ids + 1)] == [41, 2]  # all of it is
+    assert cache.lengths[a] == 52 and len(cache.block_tables[a]) == 4 and len(cache.block_tables[b]) == 4
+    cache.raise_device_errors()
