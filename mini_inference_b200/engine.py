@@ -115,7 +115,7 @@ class EngineConfig:
     chunked_prefill: bool = False
     # Speculative decoding (opt-in; the reference has none): each decode step also verifies up
     # to this many tokens drafted by draft_by_lookup, and may emit that many more. The tokens
-    # are the model's own greedy choices either way.
+    # are the model's own greedy choices either way. A step without a draft is a plain one.
     speculative_tokens: int = 0
 
     def __post_init__(self) -> None:
@@ -345,9 +345,10 @@ class LLMEngine:
             # The token at each sequence's last position (its last output, or with chunked
             # prefill the last prompt token when the final chunk left exactly that one), as
             # the native scheduler reports it.
-            if self.config.speculative_tokens:
+            drafts = self._draft(batch.decodes) if self.config.speculative_tokens else []
+            if any(drafts):
                 count_context()
-                n_finished += self._verify(batch.decodes, new_tokens)
+                n_finished += self._verify(batch.decodes, drafts, new_tokens)
             else:
                 tokens = self.runner.decode_tokens(self.scheduler.decode_slots(), self.scheduler.decode_last_tokens(),
                                                    while_running=count_context)
@@ -361,24 +362,26 @@ class LLMEngine:
             num_running=self.scheduler.num_running, num_waiting=self.scheduler.num_waiting))
         return new_tokens
 
-    def _verify(self, seqs: list[Sequence], new_tokens: list[tuple[int, int]]) -> int:
-        """A decode step that verifies drafted tokens with each sequence's last; how many finished.
-
-        A draft takes no more than the request's remaining tokens, the model length and the
-        free blocks allow; without one the step is a plain decode.
-        """
-        lasts = self.scheduler.decode_last_tokens()
-        trees = []
+    def _draft(self, seqs: list[Sequence]) -> list[list[int]]:
+        """Tokens to verify after each sequence's last: no more than ``speculative_tokens``, the request's
+        remaining tokens, the model length and the free blocks allow."""
+        drafts = []
         free = self.cache.num_free_blocks  # taken by the tree context and, where a draft fails, given back
-        for s, last in zip(seqs, lasts):
-            ids = s.token_ids[:self.cache.lengths[s.slot]] + [int(last)]  # a chunked prefill may leave one prompt token
+        for s in seqs:
+            n = s.num_tokens
             room = min(self.config.speculative_tokens, s.sampling.max_tokens - len(s.output_token_ids) - 1,
-                       self.config.max_model_len - len(ids) - 1)
-            draft = draft_by_lookup(ids, room) if room > 0 else []
+                       self.config.max_model_len - n - 1)
+            draft = draft_by_lookup(s.token_ids, room) if room > 0 else []
             held = self.cache.num_blocks_held(s.slot)
-            draft = draft[:max(0, (held + free) * self.cache.block_size - len(ids))]
-            free -= max(0, self.cache.blocks_for(len(ids) + len(draft)) - held)
-            trees.append(([int(last), *draft], list(range(-1, len(draft)))))
+            draft = draft[:max(0, (held + free) * self.cache.block_size - n)]
+            free -= max(0, self.cache.blocks_for(n + len(draft)) - held)
+            drafts.append(draft)
+        return drafts
+
+    def _verify(self, seqs: list[Sequence], drafts: list[list[int]], new_tokens: list[tuple[int, int]]) -> int:
+        """A decode step that verifies each sequence's draft with its last token; how many finished."""
+        trees = [([int(last), *draft], list(range(-1, len(draft))))
+                 for last, draft in zip(self.scheduler.decode_last_tokens(), drafts)]
         rows = self.runner.verify_tokens([s.slot for s in seqs], trees)
         now, finished = time.perf_counter(), 0
         for k in range(max(map(len, rows), default=0)):  # the scheduler takes a token per sequence at a time

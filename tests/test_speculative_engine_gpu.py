@@ -105,3 +105,19 @@ def test_a_tree_gives_back_what_its_path_left_unused(dev):
     assert [len(row) for row in ctx.accept(ids, ids + 1)] == [41, 2]  # all of it is
     assert cache.lengths[a] == 52 and len(cache.block_tables[a]) == 4 and len(cache.block_tables[b]) == 4
     cache.raise_device_errors()
+
+
+def test_a_step_without_a_draft_is_a_plain_decode(dev):
+    """It goes through the captured decode graph: the last token of a request leaves no room for a draft."""
+    from mini_inference_b200.engine import SamplingParams
+
+    model = make_model(dev)
+    engine = make_engine(model, speculative_tokens=8)
+    seqs = engine.generate([[7], [9, 8, 7]], SamplingParams(max_tokens=2, ignore_eos=True))
+    assert engine.runner.graphs.replays == 1 and len(engine.step_stats) == 2
+    check_greedy(model, seqs)
+    # Steps with and without drafts in turn, on one cache.
+    engine = make_engine(model, speculative_tokens=3)
+    seqs = engine.generate(prompts_of(6), SamplingParams(max_tokens=50, ignore_eos=True))
+    assert 0 < engine.runner.graphs.replays < len(engine.step_stats)
+    check_greedy(model, seqs)
