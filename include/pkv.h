@@ -617,6 +617,18 @@ PKV_API int pkv_sched_set_chunked_prefill(pkv_scheduler* s, int32_t enable);
  * finish_reasons[i] = PKV_FINISH_*; finished sequences leave running and free their slot. */
 PKV_API int pkv_sched_append_tokens(pkv_scheduler* s, const int64_t* seq_ids, const int64_t* tokens, int32_t n,
                             int32_t* finish_reasons);
+/*
+ * Drafts by lookup, for speculative decoding (no counterpart in the reference): up to `count`
+ * tokens that followed the latest earlier occurrence of a text's last `longest` tokens, or if
+ * there is none of its last longest - 1, ... 1; *n_out of them in out, 0 if even the last token has
+ * not occurred before. pkv_sched_draft does so for n requests, from the tokens the scheduler keeps:
+ * request i's draft of up to counts[i] (0 allowed) <= stride tokens in out[i * stride ...], their
+ * number in n_out[i]. One pass backwards over the text.
+ */
+PKV_API int pkv_draft_by_lookup(const int64_t* tokens, int64_t n, int32_t longest, int32_t count, int64_t* out,
+                                int32_t* n_out);
+PKV_API int pkv_sched_draft(const pkv_scheduler* s, const int64_t* seq_ids, const int32_t* counts, int32_t n,
+                            int32_t longest, int64_t* out, int32_t stride, int32_t* n_out);
 /* Scheduler.abort (engine/scheduler.py:150-159): *where = PKV_SEQ_WAITING or PKV_SEQ_RUNNING
  * (it was there and is now finished) or PKV_SEQ_FINISHED (already done: nothing happened). */
 PKV_API int pkv_sched_abort(pkv_scheduler* s, int64_t seq_id, int32_t* where);

@@ -123,6 +123,8 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_sched_add": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32]),
     "pkv_sched_schedule": (c_int32, [c_void_p, POINTER(PkvSchedStep)]),
     "pkv_sched_set_chunked_prefill": (c_int32, [c_void_p, c_int32]),
+    "pkv_draft_by_lookup": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_void_p, P_I32]),
+    "pkv_sched_draft": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p]),
     "pkv_sched_append_tokens": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
     "pkv_sched_abort": (c_int32, [c_void_p, c_int64, P_I32]),
     "pkv_sched_counts": (c_int32, [c_void_p, P_I32, P_I32, P_I64]),

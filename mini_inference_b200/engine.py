@@ -18,6 +18,7 @@ Token-id prompts only: the tokenizer is not part of this path.
 
 from __future__ import annotations
 
+import ctypes
 import enum
 import time
 from collections.abc import Callable, Sequence as SequenceOf
@@ -26,6 +27,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
+from ._lib import check, lib
 from .cache import PagedKVCache
 from .cuda_graphs import GraphedDecoder
 from .sampler import GreedyLMHead
@@ -160,13 +162,11 @@ def draft_by_lookup(token_ids: SequenceOf[int], count: int, longest: int = 3) ->
     has not occurred before. Text that repeats itself (quotations, code, structured output)
     is continued as it went before.
     """
-    ids, n = list(token_ids), len(token_ids)
-    for size in range(min(longest, n - 1), 0, -1):
-        tail = ids[n - size:]
-        for at in range(n - size - 1, -1, -1):
-            if ids[at:at + size] == tail:
-                return ids[at + size:at + size + count]
-    return []
+    ids = np.asarray(token_ids, dtype=np.int64)
+    out, got = np.empty(max(0, count), np.int64), ctypes.c_int32()
+    check(lib.pkv_draft_by_lookup(ids.ctypes.data, ids.size, max(0, longest), out.size, out.ctypes.data, ctypes.byref(got)),
+          "draft_by_lookup")
+    return out[:got.value].tolist()
 
 
 class ModelRunner:
@@ -365,17 +365,16 @@ class LLMEngine:
     def _draft(self, seqs: list[Sequence]) -> list[list[int]]:
         """Tokens to verify after each sequence's last: no more than ``speculative_tokens``, the request's
         remaining tokens, the model length and the free blocks allow."""
-        drafts = []
+        limit = self.config.max_model_len - 1
+        drafts = self.scheduler.draft(seqs, [min(self.config.speculative_tokens, limit - s.num_tokens,
+                                                 s.sampling.max_tokens - len(s.output_token_ids) - 1) for s in seqs])
         free = self.cache.num_free_blocks  # taken by the tree context and, where a draft fails, given back
-        for s in seqs:
-            n = s.num_tokens
-            room = min(self.config.speculative_tokens, s.sampling.max_tokens - len(s.output_token_ids) - 1,
-                       self.config.max_model_len - n - 1)
-            draft = draft_by_lookup(s.token_ids, room) if room > 0 else []
-            held = self.cache.num_blocks_held(s.slot)
-            draft = draft[:max(0, (held + free) * self.cache.block_size - n)]
+        for i, (s, draft) in enumerate(zip(seqs, drafts)):
+            if not draft:
+                continue
+            n, held = s.num_tokens, self.cache.num_blocks_held(s.slot)
+            drafts[i] = draft = draft[:max(0, (held + free) * self.cache.block_size - n)]
             free -= max(0, self.cache.blocks_for(n + len(draft)) - held)
-            drafts.append(draft)
         return drafts
 
     def _verify(self, seqs: list[Sequence], drafts: list[list[int]], new_tokens: list[tuple[int, int]]) -> int:

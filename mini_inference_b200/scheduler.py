@@ -239,6 +239,19 @@ class Scheduler:
                 n_done += 1
         return n_done
 
+    def draft(self, seqs: SequenceOf, counts: SequenceOf[int], longest: int = 3) -> list[list[int]]:
+        """``draft_by_lookup`` of up to ``counts[i]`` tokens for each sequence, from the scheduler's own copy of its tokens."""
+        n = len(seqs)
+        most = np.fromiter((max(0, c) for c in counts), dtype=np.int32, count=n)
+        stride = int(most.max(initial=0))
+        if stride == 0:
+            return [[] for _ in seqs]
+        ids = np.fromiter((s.seq_id for s in seqs), dtype=np.int64, count=n)
+        out, got = np.empty((n, stride), np.int64), np.empty(n, np.int32)
+        _check(lib.pkv_sched_draft(self._h, ids.ctypes.data, most.ctypes.data, n, longest, out.ctypes.data, stride,
+                                   got.ctypes.data), "scheduler draft")
+        return [row[:k] for row, k in zip(out.tolist(), got.tolist())]
+
     def abort(self, seq, now: float) -> None:
         """Cancel a request wherever it is: drop it from the queue, or finish it and free its slot."""
         if seq.is_finished:
