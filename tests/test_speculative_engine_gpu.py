@@ -121,3 +121,85 @@ def test_a_step_without_a_draft_is_a_plain_decode(dev):
     seqs = engine.generate(prompts_of(6), SamplingParams(max_tokens=50, ignore_eos=True))
     assert 0 < engine.runner.graphs.replays < len(engine.step_stats)
     check_greedy(model, seqs)
+
+
+def true_drafts(engine, streams, wrong_every=0):
+    """A drafter that knows each request's stream; with `wrong_every` the draft's last token is wrong now and then."""
+    calls = [0]
+
+    def draft(seqs, counts, longest=3):
+        rows = []
+        for s, c in zip(seqs, counts):
+            calls[0] += 1
+            n = len(s.output_token_ids)
+            row = list(streams[s.seq_id][n:n + max(0, c)])
+            if wrong_every and row and calls[0] % wrong_every == 0:
+                row[-1] = (row[-1] + 1) % VOCAB
+            rows.append(row)
+        return rows
+
+    engine.scheduler.draft = draft
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_right_drafts_save_steps(dev, dtype):
+    """Drafts of 7 tokens, one in three wrong at its end: the same tokens in a fifth of the steps."""
+    from mini_inference_b200.engine import SamplingParams
+
+    model, params = make_model(dev, dtype), SamplingParams(max_tokens=40, ignore_eos=True)
+    plain = [s.output_token_ids for s in make_engine(model).generate(prompts_of(), params)]
+    engine = make_engine(model, speculative_tokens=7)
+    true_drafts(engine, plain, wrong_every=3)
+    seqs = engine.generate(prompts_of(), params)
+    if dtype == torch.float16:
+        check_greedy(model, seqs)
+    same = 0
+    for s, want in zip(seqs, plain):
+        # Near-ties may part the streams (other batch shapes round differently); from there the drafts are wrong.
+        k = next((i for i, (a, b) in enumerate(zip(s.output_token_ids, want)) if a != b), 40)
+        same += k
+        if k < 40:
+            row = dense_logits(model, model.cfg, s.token_ids[:s.prompt_len + k])[-1]
+            # bfloat16's half step is eight times float16's
+            tol = (0.02 if dtype == torch.float16 else 0.16) * max(1.0, float(row.max()))
+            assert row[s.output_token_ids[k]] >= row.max() - tol and row[want[k]] >= row.max() - tol
+    assert same >= 80
+    if same == 160:
+        assert len(engine.step_stats) <= 8
+
+
+def test_an_end_token_inside_an_accepted_path(dev):
+    """What comes after it is dropped, its request ends there, the others go on, and every block comes back."""
+    from mini_inference_b200.engine import SamplingParams
+
+    model = make_model(dev)
+    params = SamplingParams(max_tokens=40, ignore_eos=True)
+    plain = [s.output_token_ids for s in make_engine(model).generate(prompts_of(), params)]
+    # A token first met in the middle of the first stream: between two ends of drafts of 9.
+    eos = next(t for i, t in enumerate(plain[0]) if i >= 4 and i % 10 in (3, 4, 5) and t not in plain[0][:i])
+    want = [row[:row.index(eos) + 1] if eos in row else row for row in plain]
+    engine = make_engine(model, speculative_tokens=9, eos=[eos])
+    true_drafts(engine, plain)
+    seqs = engine.generate(prompts_of(), SamplingParams(max_tokens=40))
+    assert [s.output_token_ids for s in seqs] == want
+    assert [s.finish_reason.value for s in seqs] == ["eos" if row[-1] == eos else "length" for row in want]
+    assert engine.cache.num_free_blocks == 40 and engine.cache.num_free_slots == 4
+    assert sum(len(r) for r in want) == sum(len(s.output_token_ids) for s in seqs)
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+def test_preemption_chunks_and_prefixes_beside_drafts(dev, chunked):
+    """A pool too small for all, prompts in chunks (one of which leaves a single token), shared prefixes."""
+    from mini_inference_b200.engine import SamplingParams
+
+    model = make_model(dev)
+    rng = random.Random(8)
+    phrase = [rng.randrange(VOCAB) for _ in range(17)]
+    prompts = [phrase + [rng.randrange(VOCAB) for _ in range(rng.randint(1, 20))] for _ in range(7)] + [phrase * 2 + [5], [3]]
+    engine = make_engine(model, max_num_seqs=5, max_model_len=96, kv_cache_tokens=192, speculative_tokens=6, enable_prefix_caching=True,
+                         chunked_prefill=chunked, max_num_batched_tokens=34 if chunked else 256)
+    seqs = engine.generate(prompts, SamplingParams(max_tokens=30, ignore_eos=True))
+    assert engine.scheduler.num_preemptions > 0 and engine.cache.prefix_hit_tokens > 0
+    assert all(len(s.output_token_ids) == 30 for s in seqs)
+    assert engine.cache.num_free_blocks == 12
+    check_greedy(model, seqs)

@@ -1,4 +1,4 @@
-"""pkv_tree_attention's softmax weights: the bits they keep, small ones beside a large one.
+"""pkv_tree_attention's softmax weights: the bits they keep, small ones beside a large one, every key once.
 
 The tolerances count the roundings of tests/test_tree_attention_gpu.py (u = half a step of the
 storage type, A = sum_j p_j |v_j|, n visible keys, delta the error of a score), but with the weights as
@@ -85,6 +85,36 @@ def test_a_long_tail_beside_dominant_keys_of_no_value(dev, dtype, hq, hkv, d, be
     assert (tol < 0.01 * want).all()
     off = (case.run(scale=0.125).double() - want).abs() - tol
     assert off.max().item() <= 0, f"{(off / want).max().item():.3e} of the value past the tolerance"
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", SHAPES[:2])
+@pytest.mark.parametrize("ctx,nodes", [([20000], [5]), ([20000], [64]), ([9000, 8999, 8961], [3, 1, 7]), ([500] * 60, [2] * 60)])
+def test_every_stage_of_keys_counts_once(dev, dtype, hq, hkv, d, ctx, nodes):
+    """Equal scores, and a value of one at the keys of one stage of 64 alone, another stage for each column and head.
+
+    The sums are whole numbers, exact in float32; the exponentials and the quotient are
+    within 2^-20 of it, and it is stored with one rounding.
+    """
+    case = Case(dev, dtype, hq, hkv, d, ctx, nodes, seed=33, poison=False)
+    case.q.zero_()
+    case.v.zero_()
+    case.vn.zero_()
+    per = hkv * d
+    for b, c in enumerate(ctx):
+        at = torch.arange(c, device=dev)
+        blocks = case.tables[b].long()[at // BS]
+        mark = at // 64 % per
+        case.v[0, blocks, mark // d, at % BS, mark % d] = 1.0
+    out = case.run().double()
+    u, lo = torch.finfo(dtype).eps / 2, 0
+    for b, (c, t) in enumerate(zip(ctx, nodes)):
+        count = torch.zeros(per, dtype=torch.float64, device=dev)
+        count.index_add_(0, torch.arange(c, device=dev) // 64 % per, torch.ones(c, dtype=torch.float64, device=dev))
+        seen = c + case.vis[b].sum(-1).double().to(dev)
+        want = count.view(1, hkv, 1, d) / seen.view(t, 1, 1, 1)
+        got = out[lo:lo + t].view(t, hkv, hq // hkv, d)
+        assert ((got - want).abs() <= (u + 2.0 ** -20) * want + 2.0 ** -25).all()
+        lo += t
 
 
 def test_nothing_is_computed_from_node_offsets_out_of_order(dev):
