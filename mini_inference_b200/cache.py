@@ -502,7 +502,8 @@ class PagedKVCache:
         """Workspace of :class:`TreeContext`'s attention (zeroed once, reused)."""
         ws = self._workspaces.get("tree")
         if ws is None:
-            ws = self._workspaces["tree"] = ops.tree_attention_workspace(self.pool, self.max_seqs, self.device)
+            most = min(self.max_seqs, ops.TREE_MAX_SEQS)
+            ws = self._workspaces["tree"] = ops.tree_attention_workspace(self.pool, most, self.device)
         return ws
 
 
@@ -693,6 +694,8 @@ class TreeContext:
         self.slots = list(slots)
         if len(parents) != len(self.slots) or len(set(self.slots)) != len(self.slots):
             raise ValueError("one tree per slot, each slot once")
+        if len(self.slots) > ops.TREE_MAX_SEQS:
+            raise ValueError(f"at most {ops.TREE_MAX_SEQS} trees")
         sizes = [len(p) for p in parents]
         depth: list[int] = []  # of each tree's longest path, in nodes
         for tree in parents:

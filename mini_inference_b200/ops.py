@@ -558,6 +558,9 @@ def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch
     return out
 
 
+TREE_MAX_SEQS = 1024  # sequences of one tree_attention call
+
+
 def tree_attention_workspace(pool: PkvPool, max_seqs: int, device: torch.device | str) -> torch.Tensor:
     """A zeroed workspace for :func:`tree_attention` of up to ``max_seqs`` sequences (each call leaves it ready).
 

@@ -203,3 +203,19 @@ def test_preemption_chunks_and_prefixes_beside_drafts(dev, chunked):
     assert all(len(s.output_token_ids) == 30 for s in seqs)
     assert engine.cache.num_free_blocks == 12
     check_greedy(model, seqs)
+
+
+def test_caches_of_more_sequences_than_a_tree_step_takes(dev):
+    """1,024 trees at a time (as many as a decode step takes), whatever the cache holds."""
+    from mini_inference_b200 import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 64, num_blocks=1100, block_size=16, max_seqs=1100, max_len=32, dtype=torch.float16, device=dev)
+    slots = [cache.allocate(2) for _ in range(1025)]
+    with pytest.raises(ValueError, match="1024"):
+        cache.tree_context(slots, [[-1]] * 1025)
+    ctx = cache.tree_context(slots[1:], [[-1]] * 1024)
+    x = torch.randn(1, 2, 1024, 64, device=dev).half()
+    assert torch.equal(ctx.attend(0, x, x, x), x)  # one key each: its value
+    ids = torch.arange(1024, device=dev)
+    assert ctx.accept(ids, ids + 7) == [[i + 7] for i in range(1024)]
+    cache.raise_device_errors()
