@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import sysconfig
 from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_void_p
 from pathlib import Path
 
@@ -171,20 +172,32 @@ def _load() -> ctypes.CDLL:
 lib = _load()
 
 
-def _load_binding():
-    """The compiled binding of the speculative step's calls (``_speculative.so``), as loud when it is missing."""
-    path = LIB_PATH.with_name("_speculative.so")
-    if not path.exists():
-        raise ImportError(f"{path.name} is not built; run `python mini_inference_b200/build.py`")
-    import torch  # noqa: F401  (the binding's own libraries)
+class _Binding:
+    """The compiled binding of the speculative step's calls (``_speculative``), loaded by the first of them.
 
-    spec = importlib.util.spec_from_file_location("_speculative", path)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
-    return module
+    It is built against one Python and one torch, which ``libpkv.so`` is not: where it is missing or
+    does not load, those calls raise and every other operator works.
+    """
+
+    def __getattr__(self, name: str):
+        if name.startswith("__"):
+            raise AttributeError(name)
+        import torch  # noqa: F401  (the binding's own libraries)
+
+        path = LIB_PATH.with_name("_speculative" + sysconfig.get_config_var("EXT_SUFFIX"))
+        if not path.exists():
+            raise ImportError(f"{path.name} is not built; run `python mini_inference_b200/build.py`")
+        spec = importlib.util.spec_from_file_location("_speculative", path)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise ImportError(f"{path.name} does not load ({e}); run `python mini_inference_b200/build.py`") from e
+        self.__dict__.update({k: v for k, v in vars(module).items() if not k.startswith("__")})  # found without this from now on
+        return getattr(module, name)
 
 
-speculative = _load_binding()
+speculative = _Binding()
 
 
 class PkvError(RuntimeError):

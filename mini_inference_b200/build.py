@@ -7,8 +7,8 @@ Every ``csrc/*.cu`` and ``csrc/*.cpp`` is compiled for
 is rebuilt only when it or a header changed) and linked with the static CUDA
 runtime into ``mini_inference_b200/libpkv.so``. nvcc cross-compiles, so no GPU
 is needed to build. ``csrc/bindings/speculative.cpp`` (tensors to the C ABI for the calls
-of a speculative decoding step) becomes ``mini_inference_b200/_speculative.so``, compiled
-by g++ against the installed torch's headers and linked to ``libpkv.so``.
+of a speculative decoding step) becomes ``mini_inference_b200/_speculative.<python tag>.so``,
+compiled by g++ against the installed torch's headers and linked to ``libpkv.so``.
 """
 
 from __future__ import annotations
@@ -28,7 +28,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB = PKG / "libpkv.so"
-BINDING = PKG / "_speculative.so"
+BINDING = PKG / ("_speculative" + sysconfig.get_config_var("EXT_SUFFIX"))  # of this Python
 BINDING_SRC = CSRC / "bindings" / "speculative.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -69,13 +69,16 @@ def _compile(src: Path, verbose_ptxas: bool) -> Path:
 
 
 def _bind() -> Path:
-    """The compiled binding: rebuilt when its source, the C ABI or the installed torch changed."""
+    """The compiled binding: rebuilt when its source, the C ABI or the torch it was built against changed."""
     spec = importlib.util.find_spec("torch")  # found, not imported: that takes seconds
     if spec is None or not spec.submodule_search_locations:
         raise RuntimeError("torch not found: its headers are needed to build the binding")
     torch_dir = Path(spec.submodule_search_locations[0])
     include = torch_dir / "include"
-    if not _stale(BINDING, [BINDING_SRC, INCLUDE / "pkv.h", torch_dir / "version.py"]):
+    # By torch's version and place: its files may be older than the binding of another torch.
+    against = f"{torch_dir}\n{(torch_dir / 'version.py').read_text()}"
+    stamp = BUILD / (BINDING.name + ".torch")
+    if not _stale(BINDING, [BINDING_SRC, INCLUDE / "pkv.h"]) and stamp.exists() and stamp.read_text() == against:
         return BINDING
     cuda = Path(nvcc()).resolve().parent.parent / "include"
     tmp = BINDING.with_suffix(".so.tmp")
@@ -88,6 +91,7 @@ def _bind() -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, BINDING)
+    stamp.write_text(against)
     return BINDING
 
 
