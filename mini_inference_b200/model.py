@@ -188,12 +188,14 @@ class Qwen2Model:
                                 weights[p + "mlp.down_proj.weight"]))
         self.norm = weights["norm.weight"]
         # The reference's RoPE tables (float32, cast to the model dtype per lookup), built once.
-        # Other layouts take no tables: ops.rotary_append makes the angles.
+        # Other layouts and scaled frequencies go through ops.rotary_append, which makes the
+        # angles in float64 and rounds once; a context without it takes scaled tables.
         self.cos = self.sin = self.rotary = None
-        if cfg.rope_interleaved or cfg.rotary_dim not in (None, cfg.head_dim):
+        whole = not cfg.rope_interleaved and cfg.rotary_dim in (None, cfg.head_dim)
+        if not whole or cfg.rope_scaling is not None:
             self.rotary = ops.Rotary.build(cfg.rotary_dim or cfg.head_dim, cfg.rope_theta, cfg.rope_interleaved,
                                            cfg.rope_scaling, self.device)
-        else:
+        if whole:
             self.cos, self.sin = ops.rope_tables(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta, self.dtype,
                                                  self.device, cfg.rope_scaling)
 
@@ -204,7 +206,7 @@ class Qwen2Model:
         cfg = self.cfg
         b, t, _ = x.shape
         qkv = F.linear(x, wqkv, bqkv)
-        if self.rotary is not None:  # this package's contexts only
+        if self.rotary is not None and (self.cos is None or hasattr(ctx, "attend_rotary")):  # this package's contexts
             out = ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads)
         elif hasattr(ctx, "attend_qkv"):
             out = ctx.attend_qkv(layer, qkv, self.cos, self.sin, cfg.num_heads)  # [B, Hq, T, d]
