@@ -711,10 +711,15 @@ class TreeContext:
             raise ValueError("trees of up to 512 nodes and 64 levels")
         self.starts = [cache.lengths[s] for s in self.slots]
         self._held = [cache.num_blocks_held(s) for s in self.slots]
-        for s, start, n in zip(self.slots, self.starts, depth):
-            if not cache.ensure_capacity(s, start + n):
-                raise ValueError(f"no room in the KV cache for {start + n} tokens")
-        cache.copy_on_write(list(zip(self.slots, self.starts, depth)))
+        try:
+            for s, start, n in zip(self.slots, self.starts, depth):
+                if not cache.ensure_capacity(s, start + n):
+                    raise ValueError(f"no room in the KV cache for {start + n} tokens")
+            cache.copy_on_write(list(zip(self.slots, self.starts, depth)))
+        except (ValueError, RuntimeError):  # nothing stays taken
+            for s, held in zip(self.slots, self._held):
+                cache.truncate(s, held * cache.block_size)
+            raise
         cache.sync_tables()
         dev, b = cache.device, len(self.slots)
         cu = np.zeros(b + 1, np.int32)

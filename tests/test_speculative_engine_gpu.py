@@ -219,3 +219,22 @@ def test_caches_of_more_sequences_than_a_tree_step_takes(dev):
     ids = torch.arange(1024, device=dev)
     assert ctx.accept(ids, ids + 7) == [[i + 7] for i in range(1024)]
     cache.raise_device_errors()
+
+
+def test_a_refused_tree_context_takes_no_block(dev):
+    """The first sequence's tree fits, the second's does not (no blocks, or none for its copy of a shared one)."""
+    from mini_inference_b200 import PagedKVCache
+
+    chain = [-1] + list(range(40))
+    for fork in (False, True):
+        cache = PagedKVCache(1, 2, 64, num_blocks=6 if fork else 5, block_size=16, max_seqs=4, max_len=80, dtype=torch.float16, device=dev,
+                             enable_copy_on_write=fork)
+        a, b = cache.allocate(10), cache.allocate(10)
+        cache.lengths[a] = cache.lengths[b] = 10
+        c = cache.fork(b) if fork else b
+        before = cache._bm.state()
+        with pytest.raises(RuntimeError if fork else ValueError):
+            cache.tree_context([a, c], [chain, [-1] + list(range(21)) if fork else chain])  # 32 tokens: two blocks, and the copy
+        after = cache._bm.state()
+        assert {s: len(t) for s, t in after["block_tables"].items()} == {s: len(t) for s, t in before["block_tables"].items()}
+        assert sorted(after["free_blocks"]) == sorted(before["free_blocks"]) and after["lengths"] == before["lengths"]
