@@ -401,10 +401,14 @@ class PagedKVCache:
         """
         if not self.enable_copy_on_write:
             return 0
-        pairs = [pr for slot, a, n in writes for pr in self._bm.prepare_write(slot, a, n)]
-        if pairs and self.on_gpu:
-            dev = torch.from_numpy(np.asarray(pairs, np.int32).T.copy()).pin_memory().to(self.device, non_blocking=True)
-            ops.copy_blocks(self.pool, dev[0], dev[1], self.status)
+        pairs: list[tuple[int, int]] = []
+        try:
+            for slot, a, n in writes:
+                pairs += self._bm.prepare_write(slot, a, n)
+        finally:  # when the pool runs out midway, the blocks already exchanged still need their contents
+            if pairs and self.on_gpu:
+                dev = torch.from_numpy(np.asarray(pairs, np.int32).T.copy()).pin_memory().to(self.device, non_blocking=True)
+                ops.copy_blocks(self.pool, dev[0], dev[1], self.status)
         return len(pairs)
 
     def write_index(self, slots: Sequence[int], starts: Sequence[int], counts: Sequence[int]

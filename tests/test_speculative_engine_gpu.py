@@ -238,3 +238,22 @@ def test_a_refused_tree_context_takes_no_block(dev):
         after = cache._bm.state()
         assert {s: len(t) for s, t in after["block_tables"].items()} == {s: len(t) for s, t in before["block_tables"].items()}
         assert sorted(after["free_blocks"]) == sorted(before["free_blocks"]) and after["lengths"] == before["lengths"]
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_a_copy_on_write_that_runs_out_keeps_what_it_exchanged(dev, tree):
+    """Two forks and one free block: the step is refused, and the first fork's own block has the shared one's rows."""
+    from mini_inference_b200 import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 64, num_blocks=3, block_size=16, max_seqs=4, max_len=16, dtype=torch.float16, device=dev,
+                         enable_copy_on_write=True)
+    a, b = cache.allocate(10), cache.allocate(10)
+    cache.lengths[a] = cache.lengths[b] = 10
+    cache.k.normal_()
+    cache.v.normal_()
+    c, d = cache.fork(a), cache.fork(b)
+    with pytest.raises(RuntimeError, match="not enough free"):
+        cache.tree_context([c, d], [[-1], [-1]]) if tree else cache.decode_context([c, d])
+    mine, shared = cache.block_tables[c][0], cache.block_tables[a][0]
+    assert mine != shared
+    assert torch.equal(cache.k[:, mine], cache.k[:, shared]) and torch.equal(cache.v[:, mine], cache.v[:, shared])
