@@ -191,10 +191,12 @@ class Qwen2Model:
         # Other layouts and scaled frequencies go through ops.rotary_append, which makes the
         # angles in float64 and rounds once; a context without it takes scaled tables.
         self.cos = self.sin = self.rotary = None
-        whole = not cfg.rope_interleaved and cfg.rotary_dim in (None, cfg.head_dim)
+        rotary_dim = cfg.head_dim if cfg.rotary_dim is None else cfg.rotary_dim
+        if rotary_dim > cfg.head_dim:
+            raise ValueError(f"rotary_dim {rotary_dim} is past head_dim {cfg.head_dim}")
+        whole = not cfg.rope_interleaved and rotary_dim == cfg.head_dim
         if not whole or cfg.rope_scaling is not None:
-            self.rotary = ops.Rotary.build(cfg.rotary_dim or cfg.head_dim, cfg.rope_theta, cfg.rope_interleaved,
-                                           cfg.rope_scaling, self.device)
+            self.rotary = ops.Rotary.build(rotary_dim, cfg.rope_theta, cfg.rope_interleaved, cfg.rope_scaling, self.device)
         if whole:
             self.cos, self.sin = ops.rope_tables(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta, self.dtype,
                                                  self.device, cfg.rope_scaling)
