@@ -446,9 +446,12 @@ PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* q
  * Rows past cu_nodes[num_seqs] of out are not written. Bad lengths, offsets or rows are reported
  * (PKV_ERR_OUT_OF_RANGE); with cu_nodes out of order nothing is written. Slots of the pool past
  * context_lens may hold anything, NaN included, and so may the K/V of nodes that no node's mask
- * names (a padded tree's); K/V that any node of a tree may see must be finite. Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head
- * <= 16, num_seqs <= 1024, scale > 0; anything else returns PKV_ERR_UNSUPPORTED (a scale
- * that is not positive PKV_ERR_INVALID_ARGUMENT).
+ * names (a padded tree's); K/V that any node of a tree may see must be finite.
+ * Softmax weights enter the product with V within 2^-15 (bf16) or 2^-11 (fp16) of themselves;
+ * fp16 weights below 2^-25 of the row's running maximum keep fewer bits, below 2^-36 none.
+ * Supported: fp16 / bf16, block_size 16, head_dim 64 or 128, query heads per KV head <= 16,
+ * num_seqs <= 1024, scale > 0; anything else returns PKV_ERR_UNSUPPORTED (a scale that is not
+ * positive PKV_ERR_INVALID_ARGUMENT).
  */
 PKV_API int64_t pkv_tree_attention_workspace_bytes(int32_t batch, int32_t head_dim);
 PKV_API int pkv_tree_attention(const pkv_pool* pool, int32_t layer, const pkv_tables* tables, int32_t num_seqs,

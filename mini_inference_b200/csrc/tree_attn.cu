@@ -20,9 +20,9 @@
 // between ranges leaves its pieces' states (running maximum, sum, unnormalised output, all
 // float32; a range has at most two cut pieces, its first and its last), which the CTAs of those
 // pieces join. Where every tree has the same number of tiles, the tiles of an item go to as many
-// CTAs side by side over the same range of keys, so that they share its reads in L2 (28 / 4 heads
-// of 128: 16 trees of 64 nodes over 16K keys 260-305 us, 335 with each tile an item of its own;
-// 32 of 20 nodes 280 and 310; 16 of 40 over 8K 107 and 118).
+// CTAs side by side over the same range of keys, so that they share its reads in L2 (bf16, 28 / 4
+// heads of 128: 16 trees of 64 nodes over 16K keys 342 us, 382 with each tile an item of its own;
+// 16 of 40 over 8K 137 and 145; 32 of 20 over 16K 338 either way).
 //
 // Inside a CTA: one warp issues the TMA copies of K, one those of V. The stages go in turn to
 // two streams, each a warp that issues tcgen05 MMAs and four softmax warps (a row per
@@ -36,17 +36,18 @@
 // room for both) and V is multiplied by either. The row sum is taken in float32, before any of it.
 //
 // Measured (B200, captured calls): 16 trees of 9-18 nodes over 8K-32K keys, 28 / 4 heads of 128,
-// bf16: 122 us = 5.4 TB/s, 0.83 of the copy bandwidth. 64 trees of 1-26 nodes over 128-2048
-// keys, 14 / 2 heads of 64, fp16: 26.9 us (1.46 TB/s; an item has 3 to 33 stages, so starts, ends
-// and the set-up weigh as much as its stages). 4 trees of 129-256 nodes over 1000-4100
-// keys: 53-56 us = 0.55 PFLOP/s, tensor cores and exponentials at a third of their rates. One
-// tree of 8 nodes over 129 keys: 9 us, a launch, the plan, one load and one stage behind one
-// another. What bounds the wide cases is the warps' own instructions, with three warps on
-// a scheduler to hide their latency: without any exponential or all but one MMA of a stage the
-// time stays, with no softmax at all it falls by a tenth. Measured beside it and slower: two
-// softmax warps per row (long 142 us), stages of 128 keys with one score buffer (136 us),
-// four streams at head_dim 64 (88-127 us for 77), a separate launch for the join (7-11 us more on
-// short calls).
+// bf16: 134 us = 4.9 TB/s, 0.76 of the copy bandwidth; 156-167 us for a lone call on a flushed
+// L2. 64 trees of 1-26 nodes over 128-2048 keys, 14 / 2 heads of 64, fp16: 27.6 us (1.4 TB/s; an
+// item has 3 to 33 stages, so starts, ends and the set-up weigh as much as its stages). 4 trees
+// of 129-256 nodes over 1000-4100 keys, bf16: 60-65 us = 0.5 PFLOP/s, tensor cores busy 40 % of
+// the time, exponentials 27 %. One tree of 8 nodes over 129 keys: 9 us, a launch, the plan, one
+// load and one stage behind one another. What bounds the wide cases is the warps' own
+// instructions, with three warps on a scheduler to hide their latency.
+// The second halves of bfloat16's weights cost 123 -> 134 us, 56 -> 62 us, and 262 -> 342 us for
+// 16 trees of 64 nodes over 16K keys, by their products and the softmax warps' arithmetic.
+// Slower, measured before them (long case then 122-128 us): two softmax warps per row (142),
+// stages of 128 keys with one score buffer (136), four streams at head_dim 64 (88-127 us for 77),
+// a separate launch for the join (7-11 us more on short calls).
 #include <algorithm>
 #include <type_traits>
 
@@ -63,10 +64,9 @@ constexpr int kRing = 4;         // stages of the K ring and of the V ring
 constexpr int kBars = 4 * kRing + 3 * kStreams + 5;
 constexpr int kMaxSeqs = 1024;   // sequences per call: their tables live in shared memory
 constexpr int kMaxWords = 8;     // mask words of 64 nodes
-// An item's start and end, in stages, and the least that a CTA gets, both as measured best over
-// small and large calls. Charge 5: 4 trees over 2K keys 25.1 us for 18.7, wide trees 55.8 for 53.0;
-// 11: serving batch 27.7 for 27.1. Least 4: one tree over 16K keys 24.0 us for 22.6; 12: 4 trees
-// over 2K keys 24.2 for 18.7.
+// An item's start and end, in stages, and the least that a CTA gets, each as good as any on small
+// and large calls. Charge 5: serving batch 29.5 us for 27.7; 11: 28.0, wide trees alike. Least 4:
+// no different; 12: one tree over 16K keys 28.2 us for 25.2.
 constexpr int kItemCost = 8;
 constexpr int kMinRange = 8;
 constexpr int kMaxPieces = 160;  // CTAs at most: an item's pieces
@@ -343,9 +343,10 @@ __global__ void __launch_bounds__(TreeShape<D>::THREADS, 1)
     // in cycles: waits that find their barrier complete 180, a copy 85 to 110 whichever lane
     // issues it, the loop's own arithmetic 450), so a block's keys are one copy (the layout in
     // shared memory takes groups of 8 keys, all of a row's chunks) and the loops over the tree's
-    // own keys and the context's are apart. Two copies a block and one loop: 128 us for 16
-    // trees of 40 nodes over 8K keys; so 118. Four copy warps: 113-118 where two take 107, for the
-    // registers and issue slots they take from the softmax warps.
+    // own keys and the context's are apart. (Before bfloat16's weights had second halves: two copies
+    // a block and one loop 128 us for 16 trees of 40 nodes over 8K keys, so 118; four copy warps
+    // 113-118 where two took 107, for the registers and issue slots they take from the softmax
+    // warps.)
     const bool is_v = warp != SW;
     uint8_t* const ring = is_v ? sV : sK;
     uint64_t* const full = is_v ? v_full : k_full;

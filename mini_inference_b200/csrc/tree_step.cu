@@ -30,8 +30,9 @@ namespace cg = cooperative_groups;
 // scan's two barriers, a table lookup and the stores. As many CTAs run as the tokens fill (2048
 // each). Where outputs continue an input in place, every CTA must have read it first: up to
 // 16 K tokens by a cluster's barrier, beyond that by a second launch of one CTA that writes
-// them. Measured: 250 requests of one token 4.7 us; 61 requests with 8 K tokens 5.1 us, 5.8 as a
-// cluster, with 122 K tokens (2 MB written) 5.4 us, 15 if one cluster took them.
+// them. Measured, apart and in place: 250 requests of one token 3.8 and 4.1 us; 61 requests with
+// 8 K tokens 4.5 and 5.0, with 16 K 4.9 and 5.5, with 122 K (2 MB written) 5.1 and 7.8, 15 if one
+// cluster took them.
 constexpr int kPlanSeqs = 4096;   // requests per call
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;      // the portable cluster size
