@@ -163,7 +163,7 @@ def draft_by_lookup(token_ids: SequenceOf[int], count: int, longest: int = 3) ->
     is continued as it went before.
     """
     ids = np.asarray(token_ids, dtype=np.int64)
-    out, got = np.empty(max(0, count), np.int64), ctypes.c_int32()
+    out, got = np.empty(max(0, min(count, ids.size)), np.int64), ctypes.c_int32()
     check(lib.pkv_draft_by_lookup(ids.ctypes.data, ids.size, max(0, longest), out.size, out.ctypes.data, ctypes.byref(got)),
           "draft_by_lookup")
     return out[:got.value].tolist()

@@ -34,7 +34,7 @@ def test_against_the_plain_form():
         count, longest = rng.randint(0, 9), rng.randint(0, 5)
         assert draft_by_lookup(ids, count, longest) == plain(ids, count, longest), (ids, count, longest)
     assert draft_by_lookup([5, 1 << 40, 7, 1 << 40], 2) == [7, 1 << 40]
-    assert draft_by_lookup([1, 1], -3) == []
+    assert draft_by_lookup([1, 1], -3) == [] and draft_by_lookup([1, 2, 1], 1 << 60) == [2, 1]
 
 
 def make_scheduler(texts, max_tokens=50):
