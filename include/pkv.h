@@ -430,6 +430,73 @@ PKV_API int pkv_rotary_append(const pkv_pool* pool, int32_t layer, const void* q
                               int64_t v_out_stride_t, int64_t v_out_stride_h, const int64_t* slot_mapping,
                               int32_t* status_dev, pkv_stream_t stream);
 /*
+ * pkv_rotary_append with the queries' and keys' norms in the same pass and positions on several
+ * axes. Each q and k head is first normalised over its head_dim elements, x -> x / sqrt(mean(x^2)
+ * + eps) * weight (q_weight for q heads, k_weight for k heads, [head_dim] of the pool's dtype;
+ * both NULL: no norm), then rotated: pair i by the angle positions[axes[i]][t] * inv_freq[i].
+ * The norm and the rotation are float32 and each element is rounded once.
+ *   positions : int64 [num_axes][n_tokens], axis a at positions + a * positions_stride
+ *   axes      : int32 [rotary_dim / 2] on the device, 0 <= axes[i] < num_axes (an entry outside is
+ *               reported and taken as 0); NULL: axis 0 for every pair
+ * The rest as pkv_rotary_append; slot_mapping names no slot twice. num_axes <= 4.
+ */
+PKV_API int pkv_norm_rotary_append(const pkv_pool* pool, int32_t layer, const void* qkv, int64_t qkv_stride,
+                                   int64_t n_tokens, int32_t num_q_heads, const int64_t* positions,
+                                   int64_t positions_stride, const int32_t* axes, int32_t num_axes,
+                                   const double* inv_freq, int32_t rotary_dim, int32_t interleaved,
+                                   float attention_factor, const void* q_weight, const void* k_weight, float eps,
+                                   void* q_out, int64_t q_out_stride_t, int64_t q_out_stride_h, void* k_out,
+                                   int64_t k_out_stride_t, int64_t k_out_stride_h, void* v_out,
+                                   int64_t v_out_stride_t, int64_t v_out_stride_h, const int64_t* slot_mapping,
+                                   int32_t* status_dev, pkv_stream_t stream);
+/*
+ * Positions on three axes (time, height, width) of tokens whose sequences hold images and video.
+ * A sequence's media are spans of its tokens, in order and apart: a span (start, frames, height,
+ * width, step) holds frames * height * width tokens from index start on, frame by frame and row by
+ * row. With p the position where a span starts, its token (f, y, x) stands at (p + f * step, p + y,
+ * p + x), and the text behind it goes on at p + max((frames - 1) * step + 1, height, width). Text
+ * stands at the same position on every axis, and counts on by one.
+ *   positions  : int64 [n_tokens], each token's index in its sequence (pkv_build_*_metadata's)
+ *   cu_seqlens : int32 [num_seqs + 1], sequence b's tokens are cu_seqlens[b] .. cu_seqlens[b + 1] - 1;
+ *                NULL: one token per sequence (n_tokens == num_seqs). Tokens of no sequence are left
+ *                as they were in out
+ *   seq_rows   : int32 [num_seqs], each sequence's row of the media table (negative: no media); NULL:
+ *                row b. A row outside the table is reported and taken as no media
+ *   media      : int32 [rows][max_spans][5]; media_counts int32 [rows], the spans of each row
+ *   out        : int64 [3][n_tokens], axis a at out + a * out_stride
+ * A count outside 0 .. max_spans, a span that starts before the last one's end, a size below 1 or a step
+ * below 0 is reported (PKV_ERR_OUT_OF_RANGE), and the spans from there on are left out.
+ */
+PKV_API int pkv_media_positions(const int64_t* positions, int64_t n_tokens, const int32_t* cu_seqlens,
+                                int32_t num_seqs, const int32_t* seq_rows, const int32_t* media,
+                                const int32_t* media_counts, int32_t rows, int32_t max_spans, int64_t* out,
+                                int64_t out_stride, int32_t* status_dev, pkv_stream_t stream);
+/*
+ * A mixture-of-experts MLP, router included: for each token x the num_experts logits router . x, the
+ * top_k largest of them (the first among equals), and
+ *   out = sum_k w_k * down[e_k] . (silu(gate[e_k] . x) * (up[e_k] . x)),
+ * with w the softmax of the chosen logits (renormalize != 0) or their part of the softmax over all.
+ * Products, weights and sums are float32; the activations between the two products are rounded to
+ * dtype once, and so is out. The choice is that of exact logits: where float32 sums leave it open,
+ * the logits beside the border are computed in float64.
+ *   x       : [n_tokens, hidden], token t at x + t * x_stride (16-byte aligned, a multiple of 8)
+ *   router  : [num_experts, hidden]
+ *   gate_up : [num_experts, 2 * intermediate, hidden], an expert's gate rows before its up rows
+ *   down    : [num_experts, hidden, intermediate]; all three contiguous and 16-byte aligned
+ *   out     : as x; it may not overlap any input
+ *   workspace : pkv_expert_mlp_workspace_bytes of at least these sizes, 256-byte aligned, zeroed once
+ *             before first use; every call leaves it ready for the next, whatever its sizes. Calls that
+ *             share a workspace must not overlap on the GPU. After a call that reported a timed-out
+ *             wait, zero it.
+ * hidden and intermediate are multiples of 8; num_experts <= 512, top_k <= 16.
+ */
+PKV_API int64_t pkv_expert_mlp_workspace_bytes(int64_t n_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                                               int32_t intermediate);
+PKV_API int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, int64_t n_tokens, int32_t hidden,
+                           int32_t intermediate, int32_t num_experts, int32_t top_k, int32_t renormalize,
+                           const void* router, const void* gate_up, const void* down, void* out, int64_t out_stride,
+                           void* workspace, int64_t workspace_bytes, int32_t* status_dev, pkv_stream_t stream);
+/*
  * Attention of the trees' nodes over the paged cache: node n attends to its sequence's
  * cached keys 0 .. context_lens[b] - 1 (0 allowed), read from the pool through tables, and
  * to the nodes of its tree whose bit is set in its mask row (any mask, as

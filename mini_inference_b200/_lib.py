@@ -103,6 +103,16 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_rotary_append": (c_int32, [P_POOL, c_int32, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32,
                                     c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                     c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "pkv_norm_rotary_append": (c_int32, [P_POOL, c_int32, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                         c_int32, c_void_p, c_int32, c_int32, c_float, c_void_p, c_void_p, c_float,
+                                         c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                         c_int64, c_void_p, c_void_p, c_void_p]),
+    "pkv_media_positions": (c_int32, [c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
+                                      c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
+    "pkv_expert_mlp_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32]),
+    "pkv_expert_mlp": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                 c_void_p]),
     "pkv_tree_attention_workspace_bytes": (c_int64, [c_int32, c_int32]),
     "pkv_tree_attention": (c_int32, [P_POOL, c_int32, P_TABLES, c_int32, c_void_p, c_void_p, c_int32, c_int64, c_int32,
                                      c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
@@ -173,21 +183,23 @@ lib = _load()
 
 
 class _Binding:
-    """The compiled binding of the speculative step's calls (``_speculative``), loaded by the first of them.
+    """A compiled binding of some of the calls, loaded by the first of them.
 
     It is built against one Python and one torch, which ``libpkv.so`` is not: where it is missing or
     does not load, those calls raise and every other operator works.
     """
+
+    _module = "_speculative"
 
     def __getattr__(self, name: str):
         if name.startswith("__"):
             raise AttributeError(name)
         import torch  # noqa: F401  (the binding's own libraries)
 
-        path = LIB_PATH.with_name("_speculative" + sysconfig.get_config_var("EXT_SUFFIX"))
+        path = LIB_PATH.with_name(self._module + sysconfig.get_config_var("EXT_SUFFIX"))
         if not path.exists():
             raise ImportError(f"{path.name} is not built; run `python mini_inference_b200/build.py`")
-        spec = importlib.util.spec_from_file_location("_speculative", path)
+        spec = importlib.util.spec_from_file_location(self._module, path)
         try:
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
@@ -197,7 +209,12 @@ class _Binding:
         return getattr(module, name)
 
 
-speculative = _Binding()
+class _LayerBinding(_Binding):
+    _module = "_layer"
+
+
+speculative = _Binding()  # the speculative step's calls
+layer = _LayerBinding()  # norms with rotation, positions on several axes, experts
 
 
 class PkvError(RuntimeError):

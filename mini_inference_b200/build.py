@@ -28,8 +28,10 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB = PKG / "libpkv.so"
-BINDING = PKG / ("_speculative" + sysconfig.get_config_var("EXT_SUFFIX"))  # of this Python
+SUFFIX = sysconfig.get_config_var("EXT_SUFFIX")  # of this Python
+BINDING = PKG / ("_speculative" + SUFFIX)
 BINDING_SRC = CSRC / "bindings" / "speculative.cpp"
+BINDINGS = [(BINDING, BINDING_SRC), (PKG / ("_layer" + SUFFIX), CSRC / "bindings" / "layer.cpp")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-I", str(INCLUDE)]
@@ -68,8 +70,8 @@ def _compile(src: Path, verbose_ptxas: bool) -> Path:
     return obj
 
 
-def _bind() -> Path:
-    """The compiled binding: rebuilt when its source, the C ABI or the torch it was built against changed."""
+def _bind(binding: Path, source: Path) -> Path:
+    """A compiled binding: rebuilt when its source, the C ABI or the torch it was built against changed."""
     spec = importlib.util.find_spec("torch")  # found, not imported: that takes seconds
     if spec is None or not spec.submodule_search_locations:
         raise RuntimeError("torch not found: its headers are needed to build the binding")
@@ -77,22 +79,23 @@ def _bind() -> Path:
     include = torch_dir / "include"
     # By torch's version and place: its files may be older than the binding of another torch.
     against = f"{torch_dir}\n{(torch_dir / 'version.py').read_text()}"
-    stamp = BUILD / (BINDING.name + ".torch")
-    if not _stale(BINDING, [BINDING_SRC, INCLUDE / "pkv.h"]) and stamp.exists() and stamp.read_text() == against:
-        return BINDING
+    stamp = BUILD / (binding.name + ".torch")
+    deps = [source, source.with_name("common.h"), INCLUDE / "pkv.h"]
+    if not _stale(binding, deps) and stamp.exists() and stamp.read_text() == against:
+        return binding
     cuda = Path(nvcc()).resolve().parent.parent / "include"
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"]]
     for path in (include, include / "torch" / "csrc" / "api" / "include", cuda):
         cmd += ["-isystem", str(path)]
-    cmd += [str(BINDING_SRC), "-o", str(tmp), "-L", str(PKG), "-l:libpkv.so", "-Wl,-rpath,$ORIGIN", "-L",
+    cmd += [str(source), "-o", str(tmp), "-L", str(PKG), "-l:libpkv.so", "-Wl,-rpath,$ORIGIN", "-L",
             str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, BINDING)
+        raise RuntimeError(f"g++ failed on {source.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, binding)
     stamp.write_text(against)
-    return BINDING
+    return binding
 
 
 def build(verbose_ptxas: bool = False) -> Path:
@@ -107,7 +110,8 @@ def build(verbose_ptxas: bool = False) -> Path:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
-    _bind()
+    with cf.ThreadPoolExecutor(max_workers=len(BINDINGS)) as ex:
+        list(ex.map(lambda b: _bind(*b), BINDINGS))
     return LIB
 
 

@@ -197,6 +197,27 @@ __device__ inline void tma_load_2d(void* smem_dst, const CUtensorMap* map, int c
       : "memory");
 }
 
+// 4-D bulk tensor copy global -> shared (no multicast) with an L2 cache policy.
+__device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar,
+                                   uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+// Four rows r0 .. r3 of a 2-D tensor, their elements from column c0 on, one behind the other in
+// shared memory (no multicast). The map's box is one row high.
+__device__ inline void tma_gather4(void* smem_dst, const CUtensorMap* map, int c0, int r0, int r1, int r2, int r3,
+                                   uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
 // Bulk (non-tensor) copy of `bytes` (a multiple of 16, both addresses 16-byte aligned)
 // global -> shared, completing on an mbarrier (no multicast).
 __device__ inline void bulk_load(void* smem_dst, const void* gmem_src, uint32_t bytes, uint64_t* bar) {
@@ -345,6 +366,10 @@ int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, i
 // head per copy, in the layout [d/64][8][64].
 int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
                               int64_t head_stride, int64_t row_stride);
+// Contiguous [stacks, rows, inner] of 16-bit elements with a box of {64, box_rows, box_stacks, 1} (a
+// fourth dimension of one entry), 128-byte swizzle. Rows past a stack's end read as zeros.
+int make_stack_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
+                          uint32_t box_rows, uint32_t box_stacks);
 // Streaming multiprocessors of the current device (queried once).
 int num_sms();
 

@@ -1,0 +1,735 @@
+// A mixture-of-experts MLP, router included, in two launches:
+//   out = sum_k w_k * down[e_k] . (silu(gate[e_k] . x) * (up[e_k] . x))
+// over the top_k experts e_k with the largest logits router . x, w their softmax.
+//
+// Few tokens are bound by the touched experts' weights (6 hidden intermediate bytes each, read
+// once); many by the products. Both run as the same tiles: the weights are the 128-row operand A
+// of tcgen05.mma (M), an expert's tokens operand B (N, 16 to 256 of them), so that the few tokens
+// of a decode step cost no more than their share of the tensor core's columns.
+//
+// 1. router_kernel: logits in float32, the choice of experts (exact, see choose()), each choice
+//    noted in its expert's list.
+// 2. expert_kernel: a persistent cooperative grid, one CTA per SM. Its items are first every
+//    (expert, token tile, weight rows) of gate and up, then every one of down, dealt out in
+//    turn. The rings of weight and token stages run on from item to item and from the first
+//    product to the second: the weights of down stream in while the activations are still being
+//    made, and only the tokens' side waits for them (a counter per token tile). Then the
+//    weighted sum over each token's experts, in their order.
+//
+// No counterpart in the reference, whose MLP is dense (engine/model.py:254-264).
+#include <algorithm>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace pkv {
+namespace {
+
+constexpr int kMaxExperts = 512;
+constexpr int kMaxTopK = 16;
+constexpr int kKB = 64;            // K elements per stage: one 128-byte swizzled row
+constexpr int kMaxStages = 32;
+constexpr int kThreads = 256;      // weight copies, token copies, MMA, (idle), 4 epilogue warps
+constexpr int kRouterTokens = 4;   // tokens of a router CTA
+constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
+constexpr int kRing = 200 * 1024;  // bytes of the stages
+
+// What persists between calls, zero outside them; the rest of the workspace is written before it is read.
+struct Header {
+  int32_t counts[kMaxExperts];   // tokens of each expert
+  int32_t tickets[kMaxTickets];  // router CTAs done of each group of tokens
+  int32_t arrived;               // CTAs that finished their items
+  int32_t left;                  // CTAs that finished
+};
+
+struct ExpertParams {
+  const void* x;
+  const void* router;
+  Header* head;
+  float* logits;    // [tokens][experts]
+  int32_t* perm;    // [experts][tokens]: an expert's choices, token * top_k + k each
+  float* weight;    // [tokens][top_k]
+  int32_t* done;    // [token tiles]: row tiles of gate and up that are finished
+  void* act;        // [tokens * top_k][inter], an expert's rows one behind the other
+  float* y;         // [splits][tokens * top_k][hidden]
+  void* out;
+  int32_t* status;
+  int64_t x_stride, out_stride;
+  int tokens, hidden, inter, experts, top_k, renormalize;
+  int max_tiles;    // entries of done
+  int rows1, rows2; // weight rows of an item (gate and up; down): 32, 64 or 128
+  int tile_n;       // tokens of a tile, at most
+  int stages, slot_a, slot_b, splits;
+  uint32_t tmem_cols;
+};
+
+// ---------------------------------------------------------------- router
+
+__device__ __forceinline__ uint32_t order_key(float f) {  // larger is later; NaN last, -0 = 0; never 0
+  f += 0.f;
+  const uint32_t u = __float_as_uint(f);
+  return f != f ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = Dt<T>::unpack(w[i]);
+    f[2 * i] = v.x, f[2 * i + 1] = v.y;
+  }
+}
+
+// router[e] . x[t] in float64, by a warp (every lane gets it).
+template <typename T>
+__device__ double exact_logit(const ExpertParams& p, int t, int e) {
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + t * p.x_stride);
+  const uint4* w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden);
+  double s = 0;
+  for (int c = threadIdx.x & 31; c < p.hidden / 8; c += 32) {
+    float a[8], b[8];
+    unpack8<T>(x[c], a);
+    unpack8<T>(w[c], b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += (double)a[i] * (double)b[i];
+  }
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// The top_k experts of a token and their weights, by a warp. Lane l holds experts l, l + 32, ... The
+// float32 logits are off by about 1e-7 of the largest; where the last expert in and the first one
+// out are within 2^-15 of it, those within that of the border are chosen by their float64 logits, so
+// that the choice does not hang on the order of a sum. `exact`: float64 scratch of the warp.
+template <typename T, int NV>
+__device__ void choose(const ExpertParams& p, int t, double* exact) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t all = 0xffffffffu;
+  float v[NV];
+  uint32_t big = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = e < p.experts ? __ldcg(&p.logits[(int64_t)t * p.experts + e]) : 0.f;
+    big = max(big, __float_as_uint(fabsf(v[i])));
+  }
+  const float tol = __uint_as_float(__reduce_max_sync(all, big)) * 0x1p-15f;
+  uint32_t taken = 0;
+  int mine_e = 0;
+  float mine_v = 0.f, last = 0.f;
+  for (int j = 0; j <= p.top_k; ++j) {  // one more than are taken: the first one out
+    if (j == p.experts) break;
+    uint32_t best = 0;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t k = lane + 32 * i < p.experts && !(taken >> i & 1) ? order_key(v[i]) : 0u;
+      if (k > best) best = k, at = lane + 32 * i;
+    }
+    const uint32_t m = __reduce_max_sync(all, best);
+    const int e = __reduce_min_sync(all, best == m ? at : 0x7fffffff);
+    const float val = key_value(m);
+    if (j == p.top_k) {
+      // Finite, unlike and near: infinities and NaN compare false.
+      if (tol > 0.f && tol < INFINITY && last - val <= tol) {
+        int sure = 0;
+        taken = 0;
+        uint32_t border = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const bool here = lane + 32 * i < p.experts;
+          if (here && v[i] > last + tol) taken |= 1u << i, ++sure;
+          if (here && fabsf(v[i] - last) <= tol) border |= 1u << i;
+        }
+        sure = __reduce_add_sync(all, sure);
+        for (int i = 0; i < NV; ++i)
+          for (uint32_t b = __ballot_sync(all, border >> i & 1); b; b &= b - 1) {
+            const int c = 32 * i + __ffs(b) - 1;
+            const double s = exact_logit<T>(p, t, c);
+            if (lane == 0) exact[c] = s;
+          }
+        __syncwarp();
+        for (int n = sure; n < p.top_k; ++n) {
+          double top = -INFINITY;
+          int c = 0x7fffffff;
+          for (int i = 0; i < NV; ++i)
+            if ((border & ~taken) >> i & 1) {
+              const double s = exact[lane + 32 * i];
+              if (c == 0x7fffffff || s > top) top = s, c = lane + 32 * i;
+            }
+          for (int o = 16; o; o >>= 1) {
+            const double s = __shfl_xor_sync(all, top, o);
+            const int d = __shfl_xor_sync(all, c, o);
+            if (d != 0x7fffffff && (c == 0x7fffffff || s > top || (s == top && d < c))) top = s, c = d;
+          }
+          if (lane == (c & 31)) taken |= 1u << (c >> 5);
+        }
+        __syncwarp();
+        // The taken ones to the lanes 0 .. top_k - 1, in the order of their index.
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const uint32_t b = __ballot_sync(all, taken >> i & 1);
+          for (uint32_t left = b; left; left &= left - 1, ++n) {
+            const int src = __ffs(left) - 1;
+            const float val_c = __shfl_sync(all, v[i], src);
+            if (lane == n) mine_e = 32 * i + src, mine_v = val_c;
+          }
+        }
+      }
+      break;
+    }
+    last = val;
+    if (lane == (e & 31)) taken |= 1u << (e >> 5);
+    if (lane == j) mine_e = e, mine_v = val;
+  }
+  const bool on = lane < p.top_k;
+  const uint32_t top = __reduce_max_sync(all, on ? order_key(mine_v) : 0u);
+  const float m = key_value(top);
+  float sum = 0.f;
+  if (p.renormalize) {
+    sum = on ? expf(mine_v - m) : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) sum += lane + 32 * i < p.experts ? expf(v[i] - m) : 0.f;
+  }
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(all, sum, o);
+  if (on) {
+    const int a = t * p.top_k + lane;
+    p.weight[a] = expf(mine_v - m) / sum;
+    // Places are handed out in no fixed order: a row's products do not depend on its place.
+    const int at = atomicAdd(&p.head->counts[mine_e], 1);
+    p.perm[(int64_t)mine_e * p.tokens + at] = a;
+  }
+}
+
+// A CTA takes kRouterTokens tokens and, of the experts, 8 EPW (one warp EPW of them at a time); grid y
+// is the number of such shares. The last CTA of a group of tokens chooses.
+template <typename T, int EPW, int NV>
+__global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
+  __shared__ double exact[kRouterTokens][32 * NV];
+  __shared__ int s_last;
+  const int group = blockIdx.x, t0 = group * kRouterTokens;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The expert kernel's counters of finished tiles start at zero.
+  for (int i = (blockIdx.y * gridDim.x + group) * 256 + threadIdx.x; i < p.max_tiles; i += 256 * gridDim.x * gridDim.y)
+    p.done[i] = 0;
+  const uint4* x[kRouterTokens];
+#pragma unroll
+  for (int q = 0; q < kRouterTokens; ++q)
+    x[q] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + min(t0 + q, p.tokens - 1) * p.x_stride);
+  const int step = 8 * EPW * gridDim.y;
+  for (int e0 = (blockIdx.y * 8 + warp) * EPW; e0 < p.experts; e0 += step) {
+    float acc[EPW][kRouterTokens];
+#pragma unroll
+    for (int j = 0; j < EPW; ++j)
+#pragma unroll
+      for (int q = 0; q < kRouterTokens; ++q) acc[j][q] = 0.f;
+    for (int c = lane; c < p.hidden / 8; c += 32) {
+      float a[kRouterTokens][8];
+#pragma unroll
+      for (int q = 0; q < kRouterTokens; ++q) unpack8<T>(x[q][c], a[q]);
+#pragma unroll
+      for (int j = 0; j < EPW; ++j) {
+        const int e = min(e0 + j, p.experts - 1);
+        float w[8];
+        unpack8<T>(reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden)[c], w);
+#pragma unroll
+        for (int q = 0; q < kRouterTokens; ++q)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[j][q] += a[q][i] * w[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < EPW; ++j)
+#pragma unroll
+      for (int q = 0; q < kRouterTokens; ++q) {
+        float s = acc[j][q];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0 && e0 + j < p.experts && t0 + q < p.tokens) p.logits[(int64_t)(t0 + q) * p.experts + e0 + j] = s;
+      }
+  }
+  __syncthreads();
+  if (gridDim.y > 1) {
+    if (threadIdx.x == 0) {
+      const bool last = atom_add_acq_rel_gpu(&p.head->tickets[group], 1) == (int)gridDim.y - 1;
+      if (last) st_relaxed_gpu(&p.head->tickets[group], 0);
+      s_last = last;
+    }
+    __syncthreads();
+    if (!s_last) return;
+  }
+  if (warp < kRouterTokens && t0 + warp < p.tokens) choose<T, NV>(p, t0 + warp, exact[warp]);
+}
+
+// ---------------------------------------------------------------- experts
+
+struct Item {
+  bool second;            // down; else gate and up
+  int tile, e, n0, n;     // token tile, its expert, its first and number of tokens
+  int row;                // row tile
+  int split, k0, k1;      // stages
+};
+
+struct Shared {
+  uint64_t full[kMaxStages];   // a stage's weight rows and token rows landed
+  uint64_t freed[kMaxStages];  // its MMAs completed
+  uint64_t acc_full[2], acc_empty[2], mma_done;
+  uint32_t tmem;
+  int last;
+  int offset[kMaxExperts + 1];  // rows of act before each expert's
+  int tile[kMaxExperts + 1];    // token tiles before each expert's
+};
+
+__device__ __forceinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
+  const int per1 = (2 * p.inter + p.rows1 - 1) / p.rows1, per2 = (p.hidden + p.rows2 - 1) / p.rows2;
+  const int tiles = s.tile[p.experts], first = tiles * per1;
+  int k = 0;
+  it.second = i >= first;
+  if (!it.second) {
+    it.tile = i / per1, it.row = i - it.tile * per1, it.split = 0;
+    it.k0 = 0, it.k1 = (p.hidden + kKB - 1) / kKB;
+  } else {
+    i -= first;
+    if (i >= tiles * per2 * p.splits) return false;
+    it.tile = i / (per2 * p.splits);
+    k = i - it.tile * per2 * p.splits;
+    it.split = k / per2, it.row = k - it.split * per2;
+    const int stages = (p.inter + kKB - 1) / kKB;
+    it.k0 = stages * it.split / p.splits, it.k1 = stages * (it.split + 1) / p.splits;
+  }
+  int lo = 0, hi = p.experts - 1;  // the expert whose tiles hold it.tile
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.tile[mid] <= it.tile) lo = mid; else hi = mid - 1;
+  }
+  it.e = lo;
+  it.n0 = (it.tile - s.tile[lo]) * p.tile_n;
+  it.n = min(p.tile_n, s.offset[lo + 1] - s.offset[lo] - it.n0);
+  return true;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    expert_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_gu,
+                  const __grid_constant__ CUtensorMap map_act, const __grid_constant__ CUtensorMap map_down,
+                  const ExpertParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared s;
+  uint8_t* ring_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring_b = ring_a + p.stages * p.slot_a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = gridDim.x;
+
+  if (tid == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&s.full[i], 2);
+      mbar_init(&s.freed[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.acc_full[i], 1);
+      mbar_init(&s.acc_empty[i], 4);
+    }
+    mbar_init(&s.mma_done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {  // where each expert's rows and tiles start
+    int rows = 0, tiles = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+      const int c = e0 + lane < p.experts ? __ldcg(&p.head->counts[e0 + lane]) : 0;
+      int r = c, n = (c + p.tile_n - 1) / p.tile_n;
+      const int own_n = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) r += a, n += b;
+      }
+      if (e0 + lane < p.experts) s.offset[e0 + lane] = rows + r - c, s.tile[e0 + lane] = tiles + n - own_n;
+      rows += __shfl_sync(0xffffffffu, r, 31);
+      tiles += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) s.offset[p.experts] = rows, s.tile[p.experts] = tiles;
+  }
+  if (warp == 2) {
+    tmem_alloc(&s.tmem, p.tmem_cols);
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s.tmem;
+  const uint64_t deadline = global_ns() + kWaitBudgetNs;
+  const int per1 = (2 * p.inter + p.rows1 - 1) / p.rows1;
+  Item it;
+  bool ok = true;
+
+  if (warp == 0 || warp == 1) {
+    // ---------------------------------------------------------------- copies: weights, tokens
+    const bool weights = warp == 0;
+    const uint64_t once = policy_evict_first(), reused = policy_evict_last();
+    const uint64_t w_policy = p.tokens > p.tile_n ? reused : once;
+    int j = 0;  // stage
+    for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G) {
+      const int pad = (it.n + 15) & ~15;
+      int token[2][4];
+      if (!weights && !it.second) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = (lane + 32 * g) * 4 + q;  // rows past the tile's tokens: its first token again
+            token[g][q] = __ldg(&p.perm[(int64_t)it.e * p.tokens + it.n0 + (c < it.n ? c : 0)]) / p.top_k;
+          }
+      }
+      if (!weights && it.second) {  // the tile's activations
+        if (lane == 0)
+          while (ld_acquire_gpu(&p.done[it.tile]) < per1)
+            if (global_ns() > deadline) {
+              ok = false;
+              break;
+            }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        fence_proxy_async_global();
+      }
+      for (int ks = it.k0; ks < it.k1; ++ks, ++j) {
+        const int slot = j % p.stages;
+        if (j >= p.stages) {
+          if (lane == 0) ok = mbar_wait_until(&s.freed[slot], (j / p.stages - 1) & 1, deadline);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+        }
+        uint64_t* bar = &s.full[slot];
+        if (weights) {
+          const int rows = it.second ? p.rows2 : p.rows1;
+          if (lane == 0) mbar_arrive_expect_tx(bar, rows * 128);
+          __syncwarp();
+          if (lane < rows / 32) {
+            uint8_t* dst = ring_a + slot * p.slot_a + lane * 4096;
+            if (it.second)
+              tma_load_4d(dst, &map_down, ks * kKB, it.row * p.rows2 + lane * 32, it.e, 0, bar, w_policy);
+            else  // 16 gate rows, then their 16 up rows
+              tma_load_4d(dst, &map_gu, ks * kKB, it.row * (p.rows1 / 2) + lane * 16, 2 * it.e, 0, bar, w_policy);
+          }
+        } else {
+          if (lane == 0) mbar_arrive_expect_tx(bar, pad * 128);
+          __syncwarp();
+          uint8_t* dst = ring_b + slot * p.slot_b;
+          if (it.second) {
+            if (lane < pad / 16)
+              tma_load_2d(dst + lane * 2048, &map_act, ks * kKB, s.offset[it.e] + it.n0 + lane * 16, bar, reused);
+          } else {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+              if ((lane + 32 * g) * 4 < pad)
+                tma_gather4(dst + (lane + 32 * g) * 512, &map_x, ks * kKB, token[g][0], token[g][1], token[g][2],
+                            token[g][3], bar, reused);
+          }
+        }
+      }
+    }
+    if (!ok) {  // this warp's copies have landed before its CTA may leave
+      if (lane == 0) {
+        report(p.status, PKV_ERR_TIMEOUT);
+        const uint64_t end = global_ns() + kWaitBudgetNs / 4;
+        for (int q = max(0, j - p.stages); q < j; ++q) mbar_wait_until(&s.full[q % p.stages], (q / p.stages) & 1, end);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- MMA issue
+    if (lane == 0) {
+      constexpr bool kBf16 = Dt<T>::code == PKV_BF16;
+      int j = 0, c = 0;
+      for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G, ++c) {
+        const int b = c & 1;
+        if (c >= 2 && !mbar_wait_until(&s.acc_empty[b], ((c >> 1) - 1) & 1, deadline)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, (it.n + 15) & ~15);
+        const uint32_t d = tmem + (uint32_t)(b * p.tile_n);
+        for (int ks = it.k0; ks < it.k1; ++ks, ++j) {
+          const int slot = j % p.stages;
+          if (!mbar_wait_until(&s.full[slot], (j / p.stages) & 1, deadline)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          // An item of fewer than 128 weight rows reads on into the next slots: those lanes of the
+          // accumulator are not read.
+          const uint32_t a = smem_u32(ring_a + slot * p.slot_a), bb = smem_u32(ring_b + slot * p.slot_b);
+#pragma unroll
+          for (int kk = 0; kk < kKB / 16; ++kk)
+            umma_f16_ss(d, umma_desc_sw128(a + kk * 32, 16, 1024), umma_desc_sw128(bb + kk * 32, 16, 1024), idesc,
+                        ks > it.k0 || kk > 0);
+          umma_commit(&s.freed[slot]);
+        }
+        if (ok) umma_commit(&s.acc_full[b]);
+      }
+      if (!ok) report(p.status, PKV_ERR_TIMEOUT);
+      umma_commit(&s.mma_done);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- epilogue
+    const int q = warp - 4;  // TMEM lane quarter
+    const uint32_t tl = tmem + ((uint32_t)(q * 32) << 16);
+    T* act = static_cast<T*>(p.act);
+    int c = 0;
+    for (int i = blockIdx.x; find_item(p, s, i, it); i += G, ++c) {
+      const int b = c & 1;
+      // After a wait that ran out the warp goes on to its barriers, without data: the others wait there.
+      ok = ok && mbar_wait_until(&s.acc_full[b], (c >> 1) & 1, deadline);
+      tc_fence_after_sync();
+      const uint32_t d = tl + (uint32_t)(b * p.tile_n);
+      if (!it.second) {
+        // Lanes 0..15 hold gate rows, 16..31 the same up rows: of two columns a lane finishes one.
+        const bool low = lane < 16;
+        const int r = it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
+        const bool in = q * 32 < p.rows1 && r < p.inter;
+        T* row = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
+        if (q * 32 < p.rows1)
+          for (int c0 = 0; c0 < it.n; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16(d + c0, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, low ? v[k + 1] : v[k], 16));
+              const float g = low ? __uint_as_float(v[k]) : other;
+              const float u = low ? other : __uint_as_float(v[k + 1]);
+              const int col = c0 + k + (low ? 0 : 1);
+              if (in && col < it.n) row[(int64_t)col * p.inter] = Dt<T>::from_f(g / (1.f + __expf(-g)) * u);
+            }
+          }
+        tc_fence_before_sync();
+        fence_proxy_async_global();  // the rows are read by bulk copies
+        fence_acq_rel_gpu();
+        named_barrier_sync(1, 128);
+        if (warp == 4 && lane == 0) atom_add_acq_rel_gpu(&p.done[it.tile], 1);
+      } else {
+        const int r = it.row * p.rows2 + q * 32 + lane;
+        if (q * 32 < p.rows2) {
+          float* y = p.y + (int64_t)it.split * p.tokens * p.top_k * p.hidden + r;
+          const int32_t* perm = p.perm + (int64_t)it.e * p.tokens + it.n0;
+          for (int c0 = 0; c0 < it.n; c0 += 16) {
+            const int a = lane < 16 && c0 + lane < it.n ? __ldg(&perm[c0 + lane]) : 0;
+            uint32_t v[16];
+            tmem_ld16(d + c0, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int at = __shfl_sync(0xffffffffu, a, k);
+              if (c0 + k < it.n && r < p.hidden) y[(int64_t)at * p.hidden] = __uint_as_float(v[k]);
+            }
+          }
+        }
+        tc_fence_before_sync();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+    }
+    if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
+  }
+  __syncthreads();
+  if (warp == 2) {
+    if (!mbar_wait_until(&s.mma_done, 0, global_ns() + kWaitBudgetNs) && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, p.tmem_cols);
+  }
+
+  // ---------------------------------------------------------------- weighted sum over each token's experts
+  if (tid == 0) {
+    atom_add_acq_rel_gpu(&p.head->arrived, 1);
+    const uint64_t end = global_ns() + 2 * kWaitBudgetNs;  // past every CTA's own waits
+    while (ld_acquire_gpu(&p.head->arrived) < G)
+      if (global_ns() > end) {
+        report(p.status, PKV_ERR_TIMEOUT);
+        break;
+      }
+  }
+  __syncthreads();
+  const int per_row = p.hidden / 8;
+  const int64_t units = (int64_t)p.tokens * per_row, plane = (int64_t)p.tokens * p.top_k * p.hidden;
+  for (int64_t u = (int64_t)blockIdx.x * kThreads + tid; u < units; u += (int64_t)G * kThreads) {
+    const int t = (int)(u / per_row), c = (int)(u - (int64_t)t * per_row) * 8;
+    float sum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+    for (int k = 0; k < p.top_k; ++k) {
+      const float w = __ldg(&p.weight[t * p.top_k + k]);
+      const float* y = p.y + ((int64_t)t * p.top_k + k) * p.hidden + c;
+      float part[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[e] = 0.f;
+      for (int z = 0; z < p.splits; ++z, y += plane) {
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(y)), b = __ldcg(reinterpret_cast<const float4*>(y) + 1);
+        part[0] += a.x, part[1] += a.y, part[2] += a.z, part[3] += a.w;
+        part[4] += b.x, part[5] += b.y, part[6] += b.z, part[7] += b.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += w * part[e];
+    }
+    uint4 o;
+    o.x = Dt<T>::pack(sum[0], sum[1]), o.y = Dt<T>::pack(sum[2], sum[3]);
+    o.z = Dt<T>::pack(sum[4], sum[5]), o.w = Dt<T>::pack(sum[6], sum[7]);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_stride + c) = o;
+  }
+  if (tid == 0) s.last = atom_add_acq_rel_gpu(&p.head->left, 1) == G - 1;
+  __syncthreads();
+  if (s.last) {  // every CTA has read the counters: ready for the next call
+    for (int e = tid; e < p.experts; e += kThreads) p.head->counts[e] = 0;
+    if (tid == 0) p.head->arrived = p.head->left = 0;
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+struct Layout {
+  int64_t logits, perm, weight, done, act, y, bytes;
+  int max_tiles, tile_n, rows1, rows2, splits, stages, slot_a, slot_b;
+};
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// The tiling, from sizes alone, and where each part of the workspace lies.
+Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter, int sms) {
+  Layout l = {};
+  l.tile_n = (int)std::min<int64_t>(256, up(std::max<int64_t>(tokens, 1), 16));
+  const int64_t rows = tokens * top_k;
+  l.max_tiles = (int)(std::min<int64_t>(experts, rows) + rows / l.tile_n);
+  // Weight rows of an item: the size whose dealing out over the SMs leaves the least idle.
+  auto pick = [&](int64_t n) {
+    int best = 128;
+    double least = 1e300;
+    for (int r : {128, 64, 32}) {
+      const double rounds = (double)((l.max_tiles * ((n + r - 1) / r) + sms - 1) / sms) * r;
+      if (rounds < 0.93 * least) least = rounds, best = r;
+    }
+    return best;
+  };
+  l.rows1 = pick(2 * (int64_t)inter);
+  l.rows2 = pick(hidden);
+  l.splits = 1;
+  l.slot_a = std::max(l.rows1, l.rows2) * 128;
+  l.slot_b = l.tile_n * 128;
+  l.stages = std::min(kMaxStages, kRing / (l.slot_a + l.slot_b));
+  int64_t at = up(sizeof(Header), 256);
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  l.logits = take(tokens * experts * 4);
+  l.perm = take(tokens * experts * 4);
+  l.weight = take(rows * 4);
+  l.done = take((int64_t)l.max_tiles * 4);
+  l.act = take(rows * inter * 2);
+  l.y = take((int64_t)l.splits * rows * hidden * 4);
+  l.bytes = at;
+  return l;
+}
+
+bool sizes_ok(int64_t tokens, int experts, int top_k, int hidden, int inter) {
+  return tokens >= 0 && experts > 0 && experts <= kMaxExperts && top_k > 0 && top_k <= kMaxTopK && top_k <= experts &&
+         hidden > 0 && inter > 0 && hidden % 8 == 0 && inter % 8 == 0 && tokens <= (1 << 24) && hidden <= (1 << 20) &&
+         inter <= (1 << 20);
+}
+
+template <typename T, int EPW>
+void launch_router(const ExpertParams& p, int groups, int shares, cudaStream_t st) {
+  const dim3 grid(groups, shares);
+  if (p.experts <= 64) router_kernel<T, EPW, 2><<<grid, 256, 0, st>>>(p);
+  else if (p.experts <= 128) router_kernel<T, EPW, 4><<<grid, 256, 0, st>>>(p);
+  else router_kernel<T, EPW, 16><<<grid, 256, 0, st>>>(p);
+}
+
+template <typename T>
+int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, cudaStream_t st) {
+  const int groups = (p.tokens + kRouterTokens - 1) / kRouterTokens;
+  // Few tokens: an expert per warp, its logits' CTAs spread over the SMs. Many: eight experts per warp
+  // for each load of the tokens.
+  const int shares = (p.experts + 7) / 8;
+  if (groups * (int64_t)shares <= 4 * num_sms() && groups <= kMaxTickets) launch_router<T, 1>(p, groups, shares, st);
+  else launch_router<T, 8>(p, groups, 1, st);
+  int rc = launch_status();
+  if (rc != PKV_OK) return rc;
+  static SmemAttribute attribute;
+  const int smem = 1024 + p.stages * (p.slot_a + p.slot_b);
+  const cudaError_t e = attribute.set(reinterpret_cast<const void*>(expert_kernel<T>), 1024 + kRing);
+  if (e != cudaSuccess) return cuda_status(e);
+  // Cooperative: the CTAs wait for one another's activations, so they must all be resident.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms());
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, expert_kernel<T>, maps[0], maps[1], maps[2], maps[3], p));
+}
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int64_t pkv_expert_mlp_workspace_bytes(int64_t n_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                                                  int32_t intermediate) {
+  if (!sizes_ok(n_tokens, num_experts, top_k, hidden, intermediate)) return 0;
+  return make_layout(n_tokens, num_experts, top_k, hidden, intermediate, 148).bytes;
+}
+
+extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, int64_t n_tokens, int32_t hidden,
+                              int32_t intermediate, int32_t num_experts, int32_t top_k, int32_t renormalize,
+                              const void* router, const void* gate_up, const void* down, void* out, int64_t out_stride,
+                              void* workspace, int64_t workspace_bytes, int32_t* status_dev, pkv_stream_t stream) {
+  if (!router || !gate_up || !down || !workspace) return PKV_ERR_INVALID_ARGUMENT;
+  if (n_tokens < 0 || hidden <= 0 || intermediate <= 0 || num_experts <= 0 || top_k <= 0 || top_k > num_experts)
+    return PKV_ERR_INVALID_ARGUMENT;
+  if (dtype != PKV_F16 && dtype != PKV_BF16) return PKV_ERR_UNSUPPORTED;
+  if (!sizes_ok(n_tokens, num_experts, top_k, hidden, intermediate)) return PKV_ERR_UNSUPPORTED;
+  if (n_tokens == 0) return PKV_OK;
+  if (!x || !out) return PKV_ERR_INVALID_ARGUMENT;
+  if (x_stride < hidden || out_stride < hidden || x_stride % 8 || out_stride % 8) return PKV_ERR_INVALID_ARGUMENT;
+  auto bits = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+  if (((bits(x) | bits(router) | bits(gate_up) | bits(down) | bits(out)) & 15) || (bits(workspace) & 255))
+    return PKV_ERR_INVALID_ARGUMENT;
+  const Layout l = make_layout(n_tokens, num_experts, top_k, hidden, intermediate, 148);
+  if (workspace_bytes < l.bytes) return PKV_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  ExpertParams p = {};
+  p.x = x, p.router = router, p.out = out, p.status = status_dev;
+  p.head = reinterpret_cast<Header*>(ws);
+  p.logits = reinterpret_cast<float*>(ws + l.logits);
+  p.perm = reinterpret_cast<int32_t*>(ws + l.perm);
+  p.weight = reinterpret_cast<float*>(ws + l.weight);
+  p.done = reinterpret_cast<int32_t*>(ws + l.done);
+  p.act = ws + l.act;
+  p.y = reinterpret_cast<float*>(ws + l.y);
+  p.x_stride = x_stride, p.out_stride = out_stride;
+  p.tokens = (int)n_tokens, p.hidden = hidden, p.inter = intermediate, p.experts = num_experts, p.top_k = top_k;
+  p.renormalize = renormalize;
+  p.max_tiles = l.max_tiles, p.rows1 = l.rows1, p.rows2 = l.rows2, p.tile_n = l.tile_n;
+  p.stages = l.stages, p.slot_a = l.slot_a, p.slot_b = l.slot_b, p.splits = l.splits;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
+  CUtensorMap maps[4];
+  int rc = make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB, 1);
+  if (rc == PKV_OK) rc = make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
+  if (rc == PKV_OK)
+    rc = make_matrix_tensor_map(&maps[2], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB,
+                                16);
+  if (rc == PKV_OK) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, 32, 1);
+  if (rc != PKV_OK) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == PKV_F16 ? launch<__half>(maps, p, st) : launch<__nv_bfloat16>(maps, p, st);
+}

@@ -140,6 +140,13 @@ int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int
                      {64, 8, (cuuint32_t)(d / 64), 1});
 }
 
+int make_stack_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
+                          uint32_t box_rows, uint32_t box_stacks) {
+  const uint64_t row = inner * 2, stack = rows * row;
+  return encode_rows(map, base, dtype, {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)stacks, 1},
+                     {(cuuint64_t)row, (cuuint64_t)stack, (cuuint64_t)(stacks * stack)}, {64, box_rows, box_stacks, 1});
+}
+
 // Blocks, heads and a block's groups of 8 tokens lie one behind the other in the pool: one dimension.
 static int make_pool_group_tensor_map(CUtensorMap* map, const void* base, const pkv_pool& pool) {
   const cuuint64_t d = pool.head_dim, groups = pool.block_size / 8;

@@ -10,12 +10,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections.abc import Sequence
 from dataclasses import dataclass
 
 import torch
 
 from ._lib import (PKV_BF16, PKV_DECODE_INPUTS_READY, PKV_DECODE_STATIC_SCRATCH_BYTES, PKV_ERR_WORKSPACE, PKV_F16,
                    PKV_LM_WEIGHT_READY, PkvError, PkvPool, PkvTables, check, lib)
+from ._lib import layer as _layer
 from ._lib import speculative as _speculative
 
 _DTYPES = {torch.float16: PKV_F16, torch.bfloat16: PKV_BF16}
@@ -556,6 +558,101 @@ def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch
     if type(out) is int:
         check(out, "rotary_append")
     return out
+
+
+def norm_rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                       num_q_heads: int, axes: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                       k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                       attention_factor: float = 1.0, q_out: torch.Tensor | None = None,
+                       k_out: torch.Tensor | bool = False, v_out: torch.Tensor | bool = False,
+                       slot_mapping: torch.Tensor | None = None, status: torch.Tensor | None = None
+                       ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """:func:`rotary_append` of heads that are normalised first, by positions on one axis or several.
+
+    Each q head becomes ``x / sqrt(mean(x^2) + eps) * q_weight`` (``[head_dim]`` of qkv's dtype),
+    each k head the same with ``k_weight`` (neither given: no norm), then pair ``i`` is rotated by
+    ``positions[axes[i]] * inv_freq[i]``: ``positions`` int64 ``[N]``, or ``[axes, N]`` (up to 4,
+    :func:`media_positions`) with ``axes`` int32, one entry per pair (:func:`pair_axes`). Norm and
+    rotation are float32, each element is rounded once. Outputs, append and errors are
+    :func:`rotary_append`'s; no slot may stand in ``slot_mapping`` twice.
+    """
+    out = _layer.norm_rotary_append(ctypes.addressof(pool), layer, qkv, positions, inv_freq, num_q_heads, axes, q_weight,
+                                    k_weight, eps, interleaved, attention_factor, q_out, k_out, v_out, slot_mapping, status)
+    if type(out) is int:
+        check(out, "norm_rotary_append")
+    return out
+
+
+def pair_axes(sections: Sequence[int], alternate: bool = False, device: torch.device | str = "cuda") -> torch.Tensor:
+    """``axes`` of :func:`norm_rotary_append`: int32, one entry per pair, ``sections[a]`` pairs of them axis ``a``'s.
+
+    The sections follow one another, or with ``alternate`` the axes take turns pair by pair for as
+    long as each has pairs left (what an axis lacks, the first axis takes).
+    """
+    if not 1 <= len(sections) <= 4 or any(n < 0 for n in sections) or sum(sections) < 1:
+        raise ValueError("sections must be one to four counts of pairs, not all zero")
+    if not alternate:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    else:
+        axes, left = [], list(sections)
+        for i in range(sum(sections)):
+            a = i % len(sections)
+            a = a if left[a] else next(j for j, n in enumerate(left) if n)
+            left[a] -= 1
+            axes.append(a)
+    return torch.tensor(axes, dtype=torch.int32, device=device)
+
+
+def media_positions(positions: torch.Tensor, media: torch.Tensor, media_counts: torch.Tensor,
+                    seq_rows: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Positions on three axes (time, height, width) of tokens whose sequences hold images and video: int64 ``[3, N]``.
+
+    ``positions`` (int64 ``[N]``) are the tokens' indexes in their sequences, ``cu_seqlens`` (int32
+    ``[B + 1]``) which are whose (None: one token per sequence), ``seq_rows`` (int32 ``[B]``) each
+    sequence's row of ``media`` (negative: none; None: row ``b``). Row ``r`` holds
+    ``media_counts[r]`` spans ``(start, frames, height, width, step)`` (int32 ``[rows, spans, 5]``)
+    in order: ``frames * height * width`` tokens from index ``start`` on. With ``p`` the position
+    where a span starts, its token ``(f, y, x)`` stands at ``(p + f * step, p + y, p + x)`` and the
+    text behind it goes on at ``p + max((frames - 1) * step + 1, height, width)``; text stands at
+    one position on all axes. Tokens of no sequence are left as they were in ``out``.
+    """
+    result = _layer.media_positions(positions, media, media_counts, seq_rows, cu_seqlens, out, status)
+    if type(result) is int:
+        check(result, "media_positions")
+    return result
+
+
+def expert_mlp_workspace(max_tokens: int, num_experts: int, top_k: int, hidden: int, intermediate: int,
+                         device: torch.device | str) -> torch.Tensor:
+    """A zeroed workspace for :func:`expert_mlp` of up to ``max_tokens`` tokens (each call leaves it ready).
+
+    Calls that share one must not overlap on the GPU. After a call whose status reports a timed-out
+    wait, zero it.
+    """
+    nbytes = int(lib.pkv_expert_mlp_workspace_bytes(max_tokens, num_experts, top_k, hidden, intermediate))
+    if nbytes == 0:
+        raise ValueError("expert_mlp takes 1 to 512 experts, top_k of 1 to 16 of them, and hidden and intermediate sizes "
+                         "that are multiples of 8")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+def expert_mlp(x: torch.Tensor, router: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, top_k: int,
+               workspace: torch.Tensor, renormalize: bool = True, out: torch.Tensor | None = None,
+               status: torch.Tensor | None = None) -> torch.Tensor:
+    """A mixture-of-experts MLP of ``x`` ``[..., hidden]``, router included, -> ``[..., hidden]``.
+
+    Each token's ``top_k`` experts are those of its largest logits ``router . x`` (``router``
+    ``[E, hidden]``; the first among equals), and the result is the sum over them of ``w * down[e] .
+    (silu(gate) * up)`` with ``gate | up = gate_up[e] . x`` (``gate_up`` ``[E, 2 * intermediate,
+    hidden]``, ``down`` ``[E, hidden, intermediate]``) and ``w`` the softmax of the chosen logits
+    (``renormalize=False``: of all of them). float32 throughout but for one rounding of ``silu(gate) *
+    up`` and one of the result; the choice of experts is that of exact logits.
+    """
+    result = _layer.expert_mlp(x, router, gate_up, down, top_k, renormalize, workspace, out, status)
+    if type(result) is int:
+        check(result, "expert_mlp")
+    return result
 
 
 TREE_MAX_SEQS = 1024  # sequences of one tree_attention call
