@@ -9,7 +9,8 @@
 //
 // 1. router_kernel: logits in float32, the choice of experts (exact, see choose()), each choice
 //    noted in its expert's list.
-// 2. expert_kernel: a persistent cooperative grid, one CTA per SM. Its items are first every
+// 2. (past 256 tokens) gather_kernel: each expert's token rows one behind the other.
+// 3. expert_kernel: a persistent cooperative grid, one CTA per SM. Its items are first every
 //    (expert, token tile, weight rows) of gate and up, then every one of down, dealt out in
 //    turn. The rings of weight and token stages run on from item to item and from the first
 //    product to the second: the weights of down stream in while the activations are still being
@@ -27,8 +28,10 @@ namespace {
 
 constexpr int kMaxExperts = 512;
 constexpr int kMaxTopK = 16;
-constexpr int kKB = 64;            // K elements per stage: one 128-byte swizzled row
-constexpr int kMaxStages = 32;
+constexpr int kKB = 64;            // K elements of a chunk: one 128-byte swizzled row
+constexpr int kSlotA = 16384;      // weight bytes of a stage: 32, 64 or 128 rows of 4, 2 or 1 chunks
+constexpr int kBox = 4096;         // of them per copy: 32 rows of a chunk
+constexpr int kMaxStages = 16;
 constexpr int kThreads = 256;      // weight copies, token copies, MMA, (idle), 4 epilogue warps
 constexpr int kRouterTokens = 4;   // tokens of a router CTA
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
@@ -50,6 +53,7 @@ struct ExpertParams {
   int32_t* perm;    // [experts][tokens]: an expert's choices, token * top_k + k each
   float* weight;    // [tokens][top_k]
   int32_t* done;    // [token tiles]: row tiles of gate and up that are finished
+  void* xs;         // [tokens * top_k][hidden], past 256 tokens: x by expert
   void* act;        // [tokens * top_k][inter], an expert's rows one behind the other
   float* y;         // [splits][tokens * top_k][hidden]
   void* out;
@@ -59,9 +63,16 @@ struct ExpertParams {
   int max_tiles;    // entries of done
   int rows1, rows2; // weight rows of an item (gate and up; down): 32, 64 or 128
   int tile_n;       // tokens of a tile, at most
-  int stages, slot_a, slot_b, splits;
+  int stages, slot_b, splits;
+  int source;       // of gate and up's token rows: kDirect, kGather, kSorted
+  int rows_b;       // token rows of a copy, but for kGather
   uint32_t tmem_cols;
 };
+
+// Where gate and up's tokens come from. Up to 16 tokens are all loaded for every expert (its columns are
+// looked up afterwards); up to 256 are gathered four rows a copy; more are laid out by expert first:
+// a tile of 256 rows would be 64 copies a chunk.
+enum Source { kDirect, kGather, kSorted };
 
 // ---------------------------------------------------------------- router
 
@@ -269,11 +280,18 @@ __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
 
 // ---------------------------------------------------------------- experts
 
+// As mbar_wait_until, with the clock read every 64th poll.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t deadline) {
+  for (int i = 1; !mbar_try_wait(bar, parity); ++i)
+    if ((i & 63) == 0 && global_ns() > deadline) return false;
+  return true;
+}
+
 struct Item {
   bool second;            // down; else gate and up
   int tile, e, n0, n;     // token tile, its expert, its first and number of tokens
   int row;                // row tile
-  int split, k0, k1;      // stages
+  int split, k0, k1;      // chunks of 64
 };
 
 struct Shared {
@@ -282,9 +300,49 @@ struct Shared {
   uint64_t acc_full[2], acc_empty[2], mma_done;
   uint32_t tmem;
   int last;
+  alignas(16) int token[256];   // the tokens of the tile being copied
   int offset[kMaxExperts + 1];  // rows of act before each expert's
   int tile[kMaxExperts + 1];    // token tiles before each expert's
 };
+
+// Rows and token tiles before each expert's, by a warp.
+__device__ __forceinline__ void scan_experts(const ExpertParams& p, int* offset, int* tile) {
+  const int lane = threadIdx.x & 31;
+  int rows = 0, tiles = 0;
+  for (int e0 = 0; e0 < p.experts; e0 += 32) {
+    const int c = e0 + lane < p.experts ? __ldcg(&p.head->counts[e0 + lane]) : 0;
+    const int own = (c + p.tile_n - 1) / p.tile_n;
+    int r = c, n = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) r += a, n += b;
+    }
+    if (e0 + lane < p.experts) offset[e0 + lane] = rows + r - c, tile[e0 + lane] = tiles + n - own;
+    rows += __shfl_sync(0xffffffffu, r, 31);
+    tiles += __shfl_sync(0xffffffffu, n, 31);
+  }
+  if (lane == 0) offset[p.experts] = rows, tile[p.experts] = tiles;
+}
+
+// x's rows by expert. A warp copies a row at a time; bound by the rows' bytes.
+__global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
+  __shared__ int offset[kMaxExperts + 1], tile[kMaxExperts + 1];
+  if (threadIdx.x < 32) scan_experts(p, offset, tile);
+  __syncthreads();
+  const int rows = p.tokens * p.top_k, lane = threadIdx.x & 31, vecs = p.hidden / 8;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+    int lo = 0, hi = p.experts - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (offset[mid] <= r) lo = mid; else hi = mid - 1;
+    }
+    const int t = p.perm[(int64_t)lo * p.tokens + r - offset[lo]] / p.top_k;
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t * p.x_stride);
+    uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.xs) + (int64_t)r * p.hidden);
+#pragma unroll 4
+    for (int c = lane; c < vecs; c += 32) to[c] = from[c];
+  }
+}
 
 __device__ __forceinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
   const int per1 = (2 * p.inter + p.rows1 - 1) / p.rows1, per2 = (p.hidden + p.rows2 - 1) / p.rows2;
@@ -300,8 +358,8 @@ __device__ __forceinline__ bool find_item(const ExpertParams& p, const Shared& s
     it.tile = i / (per2 * p.splits);
     k = i - it.tile * per2 * p.splits;
     it.split = k / per2, it.row = k - it.split * per2;
-    const int stages = (p.inter + kKB - 1) / kKB;
-    it.k0 = stages * it.split / p.splits, it.k1 = stages * (it.split + 1) / p.splits;
+    const int chunks = (p.inter + kKB - 1) / kKB;
+    it.k0 = chunks * it.split / p.splits, it.k1 = chunks * (it.split + 1) / p.splits;
   }
   int lo = 0, hi = p.experts - 1;  // the expert whose tiles hold it.tile
   while (lo < hi) {
@@ -322,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared s;
   uint8_t* ring_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring_b = ring_a + p.stages * p.slot_a;
+  uint8_t* ring_b = ring_a + p.stages * kSlotA;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = gridDim.x;
 
@@ -338,22 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.mma_done, 1);
     fence_mbar_init();
   }
-  if (warp == 1) {  // where each expert's rows and tiles start
-    int rows = 0, tiles = 0;
-    for (int e0 = 0; e0 < p.experts; e0 += 32) {
-      const int c = e0 + lane < p.experts ? __ldcg(&p.head->counts[e0 + lane]) : 0;
-      int r = c, n = (c + p.tile_n - 1) / p.tile_n;
-      const int own_n = n;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) r += a, n += b;
-      }
-      if (e0 + lane < p.experts) s.offset[e0 + lane] = rows + r - c, s.tile[e0 + lane] = tiles + n - own_n;
-      rows += __shfl_sync(0xffffffffu, r, 31);
-      tiles += __shfl_sync(0xffffffffu, n, 31);
-    }
-    if (lane == 0) s.offset[p.experts] = rows, s.tile[p.experts] = tiles;
-  }
+  if (warp == 1) scan_experts(p, s.offset, s.tile);
   if (warp == 2) {
     tmem_alloc(&s.tmem, p.tmem_cols);
     tc_fence_before_sync();
@@ -368,26 +411,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0 || warp == 1) {
     // ---------------------------------------------------------------- copies: weights, tokens
+    // The whole warp runs the loop and one lane issues: a copy's operands are uniform registers, and
+    // in a branch of one lane each would be moved there anew for every copy.
     const bool weights = warp == 0;
     const uint64_t once = policy_evict_first(), reused = policy_evict_last();
     const uint64_t w_policy = p.tokens > p.tile_n ? reused : once;
-    int j = 0;  // stage
+    const bool leader = elect_one();
+    int issued = 0, slot = 0;
+    uint32_t round = 0;  // of the ring
     for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G) {
-      const int pad = (it.n + 15) & ~15;
-      int token[2][4];
-      if (!weights && !it.second) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = (lane + 32 * g) * 4 + q;  // rows past the tile's tokens: its first token again
-            token[g][q] = __ldg(&p.perm[(int64_t)it.e * p.tokens + it.n0 + (c < it.n ? c : 0)]) / p.top_k;
-          }
+      const int e = uniform(it.e), rows = it.second ? p.rows2 : p.rows1, wide = 128 / rows;
+      const int k0 = uniform(it.k0), k1 = uniform(it.k1), pad = uniform((it.n + 15) & ~15);
+      const int row = uniform(it.row) * (it.second ? p.rows2 : p.rows1 / 2), row_step = it.second ? 32 : 16;
+      const bool direct = !it.second && p.source == kDirect, gather = !it.second && p.source == kGather;
+      const int first = direct ? 0 : uniform(s.offset[it.e] + it.n0);
+      if (!weights && gather) {
+        __syncwarp();
+        for (int c = lane; c < pad; c += 32)  // rows past the tile's tokens: its first token again
+          s.token[c] = __ldg(&p.perm[(int64_t)it.e * p.tokens + it.n0 + (c < it.n ? c : 0)]) / p.top_k;
+        __syncwarp();
       }
       if (!weights && it.second) {  // the tile's activations
         if (lane == 0)
-          while (ld_acquire_gpu(&p.done[it.tile]) < per1)
-            if (global_ns() > deadline) {
+          for (int n = 1; ld_acquire_gpu(&p.done[it.tile]) < per1; ++n)
+            if ((n & 63) == 0 && global_ns() > deadline) {
               ok = false;
               break;
             }
@@ -395,82 +442,93 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         fence_proxy_async_global();
       }
-      for (int ks = it.k0; ks < it.k1; ++ks, ++j) {
-        const int slot = j % p.stages;
-        if (j >= p.stages) {
-          if (lane == 0) ok = mbar_wait_until(&s.freed[slot], (j / p.stages - 1) & 1, deadline);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
+      const CUtensorMap* map_w = it.second ? &map_down : &map_gu;
+      const CUtensorMap* map_b = it.second ? &map_act : &map_x;
+      const int stack = it.second ? e : 2 * e;
+      for (int ks = k0; ks < k1; ks += wide) {
+        if (round > 0 && !__all_sync(0xffffffffu, wait_for(&s.freed[slot], (round - 1) & 1, deadline))) {
+          ok = false;
+          break;
         }
         uint64_t* bar = &s.full[slot];
+        const int chunks = min(wide, k1 - ks);
         if (weights) {
-          const int rows = it.second ? p.rows2 : p.rows1;
-          if (lane == 0) mbar_arrive_expect_tx(bar, rows * 128);
-          __syncwarp();
-          if (lane < rows / 32) {
-            uint8_t* dst = ring_a + slot * p.slot_a + lane * 4096;
-            if (it.second)
-              tma_load_4d(dst, &map_down, ks * kKB, it.row * p.rows2 + lane * 32, it.e, 0, bar, w_policy);
-            else  // 16 gate rows, then their 16 up rows
-              tma_load_4d(dst, &map_gu, ks * kKB, it.row * (p.rows1 / 2) + lane * 16, 2 * it.e, 0, bar, w_policy);
-          }
+          uint8_t* dst = ring_a + slot * kSlotA;
+          if (leader) mbar_arrive_expect_tx(bar, chunks * rows * 128);
+          for (int c = 0; c < chunks; ++c)
+            for (int b = 0; b < rows; b += 32, dst += kBox)  // gate and up: 16 gate rows, then their 16 up rows
+              if (leader) tma_load_4d(dst, map_w, (ks + c) * kKB, row + (b >> 5) * row_step, stack, 0, bar, w_policy);
         } else {
-          if (lane == 0) mbar_arrive_expect_tx(bar, pad * 128);
-          __syncwarp();
           uint8_t* dst = ring_b + slot * p.slot_b;
-          if (it.second) {
-            if (lane < pad / 16)
-              tma_load_2d(dst + lane * 2048, &map_act, ks * kKB, s.offset[it.e] + it.n0 + lane * 16, bar, reused);
-          } else {
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-              if ((lane + 32 * g) * 4 < pad)
-                tma_gather4(dst + (lane + 32 * g) * 512, &map_x, ks * kKB, token[g][0], token[g][1], token[g][2],
-                            token[g][3], bar, reused);
+          const int loaded = gather ? pad : (pad + p.rows_b - 1) / p.rows_b * p.rows_b;
+          if (leader) mbar_arrive_expect_tx(bar, chunks * loaded * 128);
+          for (int c = 0; c < chunks; ++c, dst += loaded * 128) {
+            if (gather) {
+              for (int b = 0; b < pad; b += 4) {
+                const int4 t = *reinterpret_cast<const int4*>(&s.token[b]);
+                if (leader) tma_gather4(dst + b * 128, &map_x, (ks + c) * kKB, t.x, t.y, t.z, t.w, bar, reused);
+              }
+            } else {
+              for (int b = 0; b < pad; b += p.rows_b)
+                if (leader) tma_load_2d(dst + b * 128, map_b, (ks + c) * kKB, first + b, bar, reused);
+            }
           }
         }
+        ++issued;
+        if (++slot == p.stages) slot = 0, ++round;
       }
     }
-    if (!ok) {  // this warp's copies have landed before its CTA may leave
-      if (lane == 0) {
-        report(p.status, PKV_ERR_TIMEOUT);
-        const uint64_t end = global_ns() + kWaitBudgetNs / 4;
-        for (int q = max(0, j - p.stages); q < j; ++q) mbar_wait_until(&s.full[q % p.stages], (q / p.stages) & 1, end);
-      }
-      __syncwarp();
+    if (!ok && lane == 0) {  // this warp's copies have landed before its CTA may leave
+      report(p.status, PKV_ERR_TIMEOUT);
+      const uint64_t end = global_ns() + kWaitBudgetNs / 4;
+      for (int q = max(0, issued - p.stages); q < issued; ++q) wait_for(&s.full[q % p.stages], (q / p.stages) & 1, end);
     }
+    __syncwarp();
   } else if (warp == 2) {
     // ---------------------------------------------------------------- MMA issue
-    if (lane == 0) {
-      constexpr bool kBf16 = Dt<T>::code == PKV_BF16;
-      int j = 0, c = 0;
-      for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G, ++c) {
-        const int b = c & 1;
-        if (c >= 2 && !mbar_wait_until(&s.acc_empty[b], ((c >> 1) - 1) & 1, deadline)) {
+    constexpr bool kBf16 = Dt<T>::code == PKV_BF16;
+    const bool leader = elect_one();
+    const uint64_t a0 = umma_desc_sw128(smem_u32(ring_a), 16, 1024), b0 = umma_desc_sw128(smem_u32(ring_b), 16, 1024);
+    int c = 0, slot = 0;
+    uint32_t round = 0;
+    for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G, ++c) {
+      const int b = c & 1;
+      if (c >= 2 && !__all_sync(0xffffffffu, wait_for(&s.acc_empty[b], ((c >> 1) - 1) & 1, deadline))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      const int rows = it.second ? p.rows2 : p.rows1, wide = 128 / rows;
+      const int k0 = uniform(it.k0), k1 = uniform(it.k1), pad = uniform((it.n + 15) & ~15);
+      const bool gather = !it.second && p.source == kGather;
+      const int loaded = gather ? pad : (pad + p.rows_b - 1) / p.rows_b * p.rows_b;
+      const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, pad);
+      const uint32_t d = tmem + (uint32_t)(b * p.tile_n);
+      bool more = false;
+      for (int ks = k0; ks < k1; ks += wide) {
+        if (!__all_sync(0xffffffffu, wait_for(&s.full[slot], round & 1, deadline))) {
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, (it.n + 15) & ~15);
-        const uint32_t d = tmem + (uint32_t)(b * p.tile_n);
-        for (int ks = it.k0; ks < it.k1; ++ks, ++j) {
-          const int slot = j % p.stages;
-          if (!mbar_wait_until(&s.full[slot], (j / p.stages) & 1, deadline)) {
-            ok = false;
-            break;
+        // An item of fewer than 128 weight rows reads on into what is behind them: those lanes of the
+        // accumulator are not read. Descriptors count in 16 bytes.
+        uint64_t ad = a0 + slot * (kSlotA >> 4), bd = b0 + (uint32_t)(slot * (p.slot_b >> 4));
+        for (int n = min(wide, k1 - ks); n; --n, ad += rows * 8, bd += loaded * 8) {
+          if (leader) {
+            umma_f16_ss(d, ad, bd, idesc, more);
+            umma_f16_ss(d, ad + 2, bd + 2, idesc, true);
+            umma_f16_ss(d, ad + 4, bd + 4, idesc, true);
+            umma_f16_ss(d, ad + 6, bd + 6, idesc, true);
           }
-          tc_fence_after_sync();
-          // An item of fewer than 128 weight rows reads on into the next slots: those lanes of the
-          // accumulator are not read.
-          const uint32_t a = smem_u32(ring_a + slot * p.slot_a), bb = smem_u32(ring_b + slot * p.slot_b);
-#pragma unroll
-          for (int kk = 0; kk < kKB / 16; ++kk)
-            umma_f16_ss(d, umma_desc_sw128(a + kk * 32, 16, 1024), umma_desc_sw128(bb + kk * 32, 16, 1024), idesc,
-                        ks > it.k0 || kk > 0);
-          umma_commit(&s.freed[slot]);
+          more = true;
         }
-        if (ok) umma_commit(&s.acc_full[b]);
+        if (leader) umma_commit(&s.freed[slot]);
+        if (++slot == p.stages) slot = 0, ++round;
       }
+      if (ok && leader) umma_commit(&s.acc_full[b]);
+    }
+    if (leader) {
       if (!ok) report(p.status, PKV_ERR_TIMEOUT);
       umma_commit(&s.mma_done);
     }
@@ -484,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = blockIdx.x; find_item(p, s, i, it); i += G, ++c) {
       const int b = c & 1;
       // After a wait that ran out the warp goes on to its barriers, without data: the others wait there.
-      ok = ok && mbar_wait_until(&s.acc_full[b], (c >> 1) & 1, deadline);
+      ok = ok && wait_for(&s.acc_full[b], (c >> 1) & 1, deadline);
       tc_fence_after_sync();
       const uint32_t d = tl + (uint32_t)(b * p.tile_n);
       if (!it.second) {
@@ -493,8 +551,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int r = it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
         const bool in = q * 32 < p.rows1 && r < p.inter;
         T* row = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
-        if (q * 32 < p.rows1)
-          for (int c0 = 0; c0 < it.n; c0 += 16) {
+        const bool direct = p.source == kDirect;
+        if (q * 32 < p.rows1) {
+          const int token = direct && lane < it.n ? __ldg(&p.perm[(int64_t)it.e * p.tokens + lane]) / p.top_k : -1;
+          for (int c0 = 0; c0 < (direct ? p.tokens : it.n); c0 += 16) {
             uint32_t v[16];
             tmem_ld16(d + c0, v);
             tmem_wait_ld();
@@ -503,10 +563,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, low ? v[k + 1] : v[k], 16));
               const float g = low ? __uint_as_float(v[k]) : other;
               const float u = low ? other : __uint_as_float(v[k + 1]);
-              const int col = c0 + k + (low ? 0 : 1);
-              if (in && col < it.n) row[(int64_t)col * p.inter] = Dt<T>::from_f(g / (1.f + __expf(-g)) * u);
+              int col = c0 + k + (low ? 0 : 1);
+              if (direct) {  // the column of token `col`: its place in the expert's list
+                const uint32_t even = __ballot_sync(0xffffffffu, token == k), odd = __ballot_sync(0xffffffffu, token == k + 1);
+                col = __ffs(low ? even : odd) - 1;
+              }
+              if (in && col >= 0 && col < it.n) row[(int64_t)col * p.inter] = Dt<T>::from_f(g / (1.f + __expf(-g)) * u);
             }
           }
+        }
         tc_fence_before_sync();
         fence_proxy_async_global();  // the rows are read by bulk copies
         fence_acq_rel_gpu();
@@ -538,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (warp == 2) {
-    if (!mbar_wait_until(&s.mma_done, 0, global_ns() + kWaitBudgetNs) && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
+    if (!wait_for(&s.mma_done, 0, global_ns() + kWaitBudgetNs) && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
     tc_fence_after_sync();
     tmem_dealloc(tmem, p.tmem_cols);
   }
@@ -591,8 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------- host
 
 struct Layout {
-  int64_t logits, perm, weight, done, act, y, bytes;
-  int max_tiles, tile_n, rows1, rows2, splits, stages, slot_a, slot_b;
+  int64_t logits, perm, weight, done, xs, act, y, bytes;
+  int max_tiles, tile_n, rows1, rows2, splits, stages, slot_b, source, rows_b;
 };
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -608,6 +673,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
     int best = 128;
     double least = 1e300;
     for (int r : {128, 64, 32}) {
+      if (r < 128 && l.tile_n > 64) break;  // too many token rows a stage
       const double rounds = (double)((l.max_tiles * ((n + r - 1) / r) + sms - 1) / sms) * r;
       if (rounds < 0.93 * least) least = rounds, best = r;
     }
@@ -616,9 +682,11 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.rows1 = pick(2 * (int64_t)inter);
   l.rows2 = pick(hidden);
   l.splits = 1;
-  l.slot_a = std::max(l.rows1, l.rows2) * 128;
-  l.slot_b = l.tile_n * 128;
-  l.stages = std::min(kMaxStages, kRing / (l.slot_a + l.slot_b));
+  l.source = tokens <= 16 ? kDirect : tokens <= 256 ? kGather : kSorted;
+  l.rows_b = l.tile_n <= 64 ? 16 : 64;
+  // A stage's token rows, of as many chunks as its weights have.
+  l.slot_b = (l.tile_n + l.rows_b - 1) / l.rows_b * l.rows_b * 128 * (128 / std::min(l.rows1, l.rows2));
+  l.stages = std::min(kMaxStages, kRing / (kSlotA + l.slot_b));
   int64_t at = up(sizeof(Header), 256);
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -629,6 +697,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.perm = take(tokens * experts * 4);
   l.weight = take(rows * 4);
   l.done = take((int64_t)l.max_tiles * 4);
+  l.xs = take(l.source == kSorted ? rows * hidden * 2 : 0);
   l.act = take(rows * inter * 2);
   l.y = take((int64_t)l.splits * rows * hidden * 4);
   l.bytes = at;
@@ -657,10 +726,11 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, cudaStream_t st)
   const int shares = (p.experts + 7) / 8;
   if (groups * (int64_t)shares <= 4 * num_sms() && groups <= kMaxTickets) launch_router<T, 1>(p, groups, shares, st);
   else launch_router<T, 8>(p, groups, 1, st);
+  if (p.source == kSorted) gather_kernel<<<4 * num_sms(), 256, 0, st>>>(p);
   int rc = launch_status();
   if (rc != PKV_OK) return rc;
   static SmemAttribute attribute;
-  const int smem = 1024 + p.stages * (p.slot_a + p.slot_b);
+  const int smem = 1024 + p.stages * (kSlotA + p.slot_b);
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(expert_kernel<T>), 1024 + kRing);
   if (e != cudaSuccess) return cuda_status(e);
   // Cooperative: the CTAs wait for one another's activations, so they must all be resident.
@@ -713,21 +783,25 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.perm = reinterpret_cast<int32_t*>(ws + l.perm);
   p.weight = reinterpret_cast<float*>(ws + l.weight);
   p.done = reinterpret_cast<int32_t*>(ws + l.done);
+  p.xs = ws + l.xs;
   p.act = ws + l.act;
   p.y = reinterpret_cast<float*>(ws + l.y);
   p.x_stride = x_stride, p.out_stride = out_stride;
   p.tokens = (int)n_tokens, p.hidden = hidden, p.inter = intermediate, p.experts = num_experts, p.top_k = top_k;
   p.renormalize = renormalize;
   p.max_tiles = l.max_tiles, p.rows1 = l.rows1, p.rows2 = l.rows2, p.tile_n = l.tile_n;
-  p.stages = l.stages, p.slot_a = l.slot_a, p.slot_b = l.slot_b, p.splits = l.splits;
+  p.stages = l.stages, p.slot_b = l.slot_b, p.splits = l.splits, p.source = l.source, p.rows_b = l.rows_b;
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
   CUtensorMap maps[4];
-  int rc = make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB, 1);
+  int rc = l.source == kSorted
+               ? make_matrix_tensor_map(&maps[0], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, l.rows_b)
+               : make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB,
+                                        l.source == kDirect ? l.rows_b : 1);
   if (rc == PKV_OK) rc = make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
   if (rc == PKV_OK)
     rc = make_matrix_tensor_map(&maps[2], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB,
-                                16);
+                                l.rows_b);
   if (rc == PKV_OK) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, 32, 1);
   if (rc != PKV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
