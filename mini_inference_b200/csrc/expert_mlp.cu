@@ -48,6 +48,8 @@ struct Header {
 struct ExpertParams {
   const void* x;
   const void* router;
+  const void* gate_up;
+  const void* down;
   Header* head;
   float* logits;    // [tokens][experts]
   int32_t* perm;    // [experts][tokens]: an expert's choices, token * top_k + k each
@@ -115,9 +117,10 @@ __device__ double exact_logit(const ExpertParams& p, int t, int e) {
 // The top_k experts of a token and their weights, by a warp. Lane l holds experts l, l + 32, ... The
 // float32 logits are off by about 1e-7 of the largest; where the last expert in and the first one
 // out are within 2^-15 of it, those within that of the border are chosen by their float64 logits, so
-// that the choice does not hang on the order of a sum. `exact`: float64 scratch of the warp.
+// that the choice does not hang on the order of a sum. `exact`: float64 scratch of the warp. Lane k < top_k
+// gets the k-th expert and its weight.
 template <typename T, int NV>
-__device__ void choose(const ExpertParams& p, int t, double* exact) {
+__device__ void choose(const ExpertParams& p, int t, double* exact, int& expert, float& weight) {
   const int lane = threadIdx.x & 31;
   const uint32_t all = 0xffffffffu;
   float v[NV];
@@ -209,13 +212,8 @@ __device__ void choose(const ExpertParams& p, int t, double* exact) {
     for (int i = 0; i < NV; ++i) sum += lane + 32 * i < p.experts ? expf(v[i] - m) : 0.f;
   }
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(all, sum, o);
-  if (on) {
-    const int a = t * p.top_k + lane;
-    p.weight[a] = expf(mine_v - m) / sum;
-    // Places are handed out in no fixed order: a row's products do not depend on its place.
-    const int at = atomicAdd(&p.head->counts[mine_e], 1);
-    p.perm[(int64_t)mine_e * p.tokens + at] = a;
-  }
+  expert = mine_e;
+  weight = on ? expf(mine_v - m) / sum : 0.f;
 }
 
 // A CTA takes kRouterTokens tokens and, of the experts, 8 EPW (one warp EPW of them at a time); grid y
@@ -240,19 +238,36 @@ __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
     for (int j = 0; j < EPW; ++j)
 #pragma unroll
       for (int q = 0; q < kRouterTokens; ++q) acc[j][q] = 0.f;
-    for (int c = lane; c < p.hidden / 8; c += 32) {
-      float a[kRouterTokens][8];
+    // A warp with one expert has few loads to hide their latency behind: four steps' go ahead together.
+    constexpr int kAhead = EPW == 1 ? 4 : 1;
+    const int vecs = p.hidden / 8;
+    for (int c0 = lane; c0 < vecs; c0 += 32 * kAhead) {
+      uint4 xs[kAhead][kRouterTokens], ws[kAhead];
 #pragma unroll
-      for (int q = 0; q < kRouterTokens; ++q) unpack8<T>(x[q][c], a[q]);
+      for (int n = 0; n < kAhead; ++n) {
+        const int c = min(c0 + 32 * n, vecs - 1);
+        if constexpr (EPW == 1)
+          ws[n] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e0 * p.hidden)[c];
 #pragma unroll
-      for (int j = 0; j < EPW; ++j) {
-        const int e = min(e0 + j, p.experts - 1);
-        float w[8];
-        unpack8<T>(reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden)[c], w);
+        for (int q = 0; q < kRouterTokens; ++q) xs[n][q] = x[q][c];
+      }
 #pragma unroll
-        for (int q = 0; q < kRouterTokens; ++q)
+      for (int n = 0; n < kAhead; ++n) {
+        const bool in = c0 + 32 * n < vecs;
+        float a[kRouterTokens][8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[j][q] += a[q][i] * w[i];
+        for (int q = 0; q < kRouterTokens; ++q) unpack8<T>(xs[n][q], a[q]);
+#pragma unroll
+        for (int j = 0; j < EPW; ++j) {
+          const int e = min(e0 + j, p.experts - 1);
+          float w[8];
+          unpack8<T>(EPW == 1 ? ws[n]
+                              : reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden)[c0], w);
+#pragma unroll
+          for (int q = 0; q < kRouterTokens; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[j][q] += in ? a[q][i] * w[i] : 0.f;
+        }
       }
     }
 #pragma unroll
@@ -275,7 +290,17 @@ __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
     __syncthreads();
     if (!s_last) return;
   }
-  if (warp < kRouterTokens && t0 + warp < p.tokens) choose<T, NV>(p, t0 + warp, exact[warp]);
+  if (warp < kRouterTokens && t0 + warp < p.tokens) {
+    int e;
+    float w;
+    choose<T, NV>(p, t0 + warp, exact[warp], e, w);
+    if (lane < p.top_k) {
+      const int a = (t0 + warp) * p.top_k + lane;
+      p.weight[a] = w;
+      // Places are handed out in no fixed order: a row's products do not depend on its place.
+      p.perm[(int64_t)e * p.tokens + atomicAdd(&p.head->counts[e], 1)] = a;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- experts
@@ -370,6 +395,62 @@ __device__ __forceinline__ bool find_item(const ExpertParams& p, const Shared& s
   it.n0 = (it.tile - s.tile[lo]) * p.tile_n;
   it.n = min(p.tile_n, s.offset[lo + 1] - s.offset[lo] - it.n0);
   return true;
+}
+
+// Every CTA of the grid has come here `times` times; what it wrote before is visible.
+__device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    atom_add_acq_rel_gpu(&p.head->arrived, 1);
+    const uint64_t end = global_ns() + 2 * kWaitBudgetNs;  // past the waits of every CTA
+    for (int n = 1; ld_acquire_gpu(&p.head->arrived) < times * (int)gridDim.x; ++n)
+      if ((n & 63) == 0 && global_ns() > end) {
+        report(p.status, PKV_ERR_TIMEOUT);
+        break;
+      }
+  }
+  __syncthreads();
+}
+
+// out = the sum over each token's experts, in their order, of its products; by the whole grid.
+template <typename T>
+__device__ __forceinline__ void combine(const ExpertParams& p, const float* weight) {
+  const int per_row = p.hidden / 8;
+  const int64_t units = (int64_t)p.tokens * per_row, plane = (int64_t)p.tokens * p.top_k * p.hidden;
+  for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (int64_t)gridDim.x * blockDim.x) {
+    const int t = (int)(u / per_row), c = (int)(u - (int64_t)t * per_row) * 8;
+    float sum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+    for (int k = 0; k < p.top_k; ++k) {
+      const float w = weight[t * p.top_k + k];
+      const float* y = p.y + ((int64_t)t * p.top_k + k) * p.hidden + c;
+      float part[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[e] = 0.f;
+      for (int z = 0; z < p.splits; ++z, y += plane) {
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(y)), b = __ldcg(reinterpret_cast<const float4*>(y) + 1);
+        part[0] += a.x, part[1] += a.y, part[2] += a.z, part[3] += a.w;
+        part[4] += b.x, part[5] += b.y, part[6] += b.z, part[7] += b.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += w * part[e];
+    }
+    uint4 o;
+    o.x = Dt<T>::pack(sum[0], sum[1]), o.y = Dt<T>::pack(sum[2], sum[3]);
+    o.z = Dt<T>::pack(sum[4], sum[5]), o.w = Dt<T>::pack(sum[6], sum[7]);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_stride + c) = o;
+  }
+}
+
+// The last CTA to come here leaves the workspace ready for the next call.
+__device__ __forceinline__ void leave(const ExpertParams& p, int* s_last) {
+  if (threadIdx.x == 0) *s_last = atom_add_acq_rel_gpu(&p.head->left, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (*s_last) {
+    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.head->counts[e] = 0;
+    if (threadIdx.x == 0) p.head->arrived = p.head->left = 0;
+  }
 }
 
 template <typename T>
@@ -608,49 +689,248 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, p.tmem_cols);
   }
 
-  // ---------------------------------------------------------------- weighted sum over each token's experts
-  if (tid == 0) {
-    atom_add_acq_rel_gpu(&p.head->arrived, 1);
-    const uint64_t end = global_ns() + 2 * kWaitBudgetNs;  // past every CTA's own waits
-    while (ld_acquire_gpu(&p.head->arrived) < G)
-      if (global_ns() > end) {
-        report(p.status, PKV_ERR_TIMEOUT);
-        break;
-      }
-  }
-  __syncthreads();
-  const int per_row = p.hidden / 8;
-  const int64_t units = (int64_t)p.tokens * per_row, plane = (int64_t)p.tokens * p.top_k * p.hidden;
-  for (int64_t u = (int64_t)blockIdx.x * kThreads + tid; u < units; u += (int64_t)G * kThreads) {
-    const int t = (int)(u / per_row), c = (int)(u - (int64_t)t * per_row) * 8;
-    float sum[8];
+  grid_barrier(p, 1);
+  combine<T>(p, p.weight);
+  leave(p, &s.last);
+}
+
+// ---------------------------------------------------------------- experts, few tokens
+
+// Up to kFewTokens tokens, in one launch with the router: the latency of a decode step of one request.
+//
+// A unit is 16 weight rows by an expert's tokens (the 8 columns of mma.sync m16n8k16), and a warp's own.
+// The warp streams its units' rows through a ring of its own in shared memory by cp.async, kDepth - 1
+// chunks ahead of the products, on from unit to unit and from gate and up to down: no CTA-wide step
+// but the grid's barriers. Rows 0 .. 7 of a unit are gate and 8 .. 15 the same up rows, so that a
+// thread holds both. The K order of a product is free: a lane takes 16 consecutive elements of its
+// rows, and of its token.
+constexpr int kFewTokens = 8;
+constexpr int kFewChoices = kFewTokens * kMaxTopK;
+constexpr int kFewThreads = 256;
+constexpr int kDepth = 3;
+constexpr int kChunkK = 256;                // elements of a row in a chunk
+constexpr int kChunk = 16 * kChunkK * 2;  // bytes: 16 rows
+constexpr int kFewSmem = kFewThreads / 32 * kDepth * kChunk;
+
+struct FewShared {
+  float part[8][kFewTokens];       // a logit's parts, by warp
+  float weight[kFewChoices];       // of each choice, token * top_k + k
+  alignas(16) int expert[kFewChoices];
+  uint32_t lead[kFewChoices / 32]; // choices that are their expert's first
+  int group_e[kFewChoices];        // the chosen experts
+  int group_n[kFewChoices];        // their tokens' number
+  int group_a[kFewChoices][kFewTokens];  // and choices
+  int last;
+};
+
+// Where a warp's copies are: its unit of which product, and the chunk.
+template <typename T>
+struct Copies {
+  const T* low;         // row 0
+  int64_t high;         // from row 0 to row 8
+  int second, u, k, K;  // u past the last unit: none left
+};
+
+__device__ __forceinline__ void cp_async_16_or_0(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Logits of every expert, an expert per CTA at a time, its warps a part of hidden each.
+template <typename T>
+__device__ __forceinline__ void few_logits(const ExpertParams& p, FewShared& s) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vecs = p.hidden / 8;
+  for (int e = blockIdx.x; e < p.experts; e += gridDim.x) {
+    float acc[kFewTokens];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    for (int k = 0; k < p.top_k; ++k) {
-      const float w = __ldg(&p.weight[t * p.top_k + k]);
-      const float* y = p.y + ((int64_t)t * p.top_k + k) * p.hidden + c;
-      float part[8];
+    for (int t = 0; t < kFewTokens; ++t) acc[t] = 0.f;
+    const uint4* w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden);
+    for (int c = threadIdx.x; c < vecs; c += kFewThreads) {
+      float a[8], b[8];
+      unpack8<T>(w[c], a);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[e] = 0.f;
-      for (int z = 0; z < p.splits; ++z, y += plane) {
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(y)), b = __ldcg(reinterpret_cast<const float4*>(y) + 1);
-        part[0] += a.x, part[1] += a.y, part[2] += a.z, part[3] += a.w;
-        part[4] += b.x, part[5] += b.y, part[6] += b.z, part[7] += b.w;
-      }
+      for (int t = 0; t < kFewTokens; ++t)
+        if (t < p.tokens) {
+          unpack8<T>(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + t * p.x_stride)[c], b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += w * part[e];
+          for (int i = 0; i < 8; ++i) acc[t] += a[i] * b[i];
+        }
     }
-    uint4 o;
-    o.x = Dt<T>::pack(sum[0], sum[1]), o.y = Dt<T>::pack(sum[2], sum[3]);
-    o.z = Dt<T>::pack(sum[4], sum[5]), o.w = Dt<T>::pack(sum[6], sum[7]);
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_stride + c) = o;
+#pragma unroll
+    for (int t = 0; t < kFewTokens; ++t) {
+      if (t < p.tokens)
+        for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
+      if (lane == 0) s.part[warp][t] = acc[t];
+    }
+    __syncthreads();
+    if (threadIdx.x < p.tokens) {
+      float sum = 0.f;
+      for (int k = 0; k < kFewThreads / 32; ++k) sum += s.part[k][threadIdx.x];
+      p.logits[(int64_t)threadIdx.x * p.experts + e] = sum;
+    }
+    __syncthreads();
   }
-  if (tid == 0) s.last = atom_add_acq_rel_gpu(&p.head->left, 1) == G - 1;
+}
+
+// Every CTA chooses for all tokens, a warp each, and lists the chosen experts in the order of their first
+// choice: the same lists everywhere. Returns their number.
+template <typename T, int NV>
+__device__ __forceinline__ int few_groups(const ExpertParams& p, FewShared& s, double* exact) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n = p.tokens * p.top_k;
+  if (tid < kFewChoices) s.expert[tid] = -1;
   __syncthreads();
-  if (s.last) {  // every CTA has read the counters: ready for the next call
-    for (int e = tid; e < p.experts; e += kThreads) p.head->counts[e] = 0;
-    if (tid == 0) p.head->arrived = p.head->left = 0;
+  if (warp < p.tokens) {
+    int e;
+    float w;
+    choose<T, NV>(p, warp, exact + warp * kMaxExperts, e, w);
+    if (lane < p.top_k) s.expert[warp * p.top_k + lane] = e, s.weight[warp * p.top_k + lane] = w;
   }
+  __syncthreads();
+  int first = -1, rank = 0, count = 0;
+  const int mine = tid < n ? s.expert[tid] : -2;
+  if (tid < kFewChoices) {
+    for (int a = 0; a < n; a += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(&s.expert[a]);
+      const int e4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (e4[i] == mine) {
+          if (first < 0) first = a + i;
+          ++count;
+          if (a + i < tid) ++rank;
+        }
+    }
+    const uint32_t lead = __ballot_sync(0xffffffffu, tid < n && first == tid);
+    if (lane == 0) s.lead[warp] = lead;
+  }
+  __syncthreads();
+  int groups = 0;
+  for (int w = 0; w < kFewChoices / 32; ++w) groups += __popc(s.lead[w]);
+  if (tid < n) {
+    int at = __popc(s.lead[first >> 5] & ((1u << (first & 31)) - 1));
+    for (int w = 0; w < first >> 5; ++w) at += __popc(s.lead[w]);
+    s.group_a[at][rank] = tid;
+    if (rank == 0) s.group_e[at] = mine, s.group_n[at] = count;
+  }
+  __syncthreads();
+  return groups;
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const ExpertParams p) {
+  extern __shared__ __align__(128) uint8_t rings[];
+  __shared__ FewShared s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  few_logits<T>(p, s);
+  grid_barrier(p, 1);
+  const int groups = few_groups<T, NV>(p, s, reinterpret_cast<double*>(rings));  // nothing is copied yet
+  const int per1 = p.inter / 8, per2 = (p.hidden + 15) / 16;
+  const int units1 = groups * per1, units2 = groups * per2;
+  const int warps = gridDim.x * (kFewThreads / 32), me = warp * gridDim.x + blockIdx.x;  // neighbours on other SMs
+  const uint32_t ring = smem_u32(rings + warp * kDepth * kChunk);
+
+  Copies<T> w;
+  auto open = [&](int second, int u) {
+    if (!second && u >= units1) second = 1, u = me;
+    w.second = second, w.u = u, w.k = 0;
+    w.K = second ? p.inter : p.hidden;
+    if (second && u >= units2) return;
+    const int group = u / (second ? per2 : per1), row = u - group * (second ? per2 : per1), e = s.group_e[group];
+    w.low = second ? static_cast<const T*>(p.down) + ((int64_t)e * p.hidden + row * 16) * p.inter
+                   : static_cast<const T*>(p.gate_up) + ((int64_t)e * 2 * p.inter + row * 8) * p.hidden;
+    w.high = !second ? (int64_t)p.inter * p.hidden  // past hidden there are no rows of down: the first eight again
+             : row * 16 + 8 < p.hidden ? (int64_t)8 * p.inter : 0;
+  };
+  int put_slot = 0;
+  auto copy = [&] {  // one chunk, or an empty group: a row's 512 bytes by each instruction
+    if (!(w.second && w.u >= units2)) {
+      const int k = w.k + lane * 8;
+      const bool there = k < w.K;
+      const T* from = w.low + (there ? k : 0);
+      const uint32_t to = ring + put_slot * kChunk + (lane >> 3) * 128;
+#pragma unroll
+      for (int r = 0; r < 8; ++r, from += w.K) {
+        const uint32_t at = to + r * kChunkK * 2 + (((lane & 7) ^ r) << 4);
+        cp_async_16_or_0(at, from, there);
+        cp_async_16_or_0(at + 8 * kChunkK * 2, from + w.high, there);
+      }
+      w.k += kChunkK;
+      if (w.k >= w.K) open(w.second, w.u + warps);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++put_slot == kDepth) put_slot = 0;
+  };
+  open(0, me);
+  for (int i = 0; i < kDepth - 1; ++i) copy();
+
+  // This lane's 16-byte units of rows g and g + 8, and its 16 elements of 64.
+  const uint32_t get0 = ring + g * kChunkK * 2 + (((2 * q) ^ g) << 4), get1 = ring + g * kChunkK * 2 + (((2 * q + 1) ^ g) << 4);
+  int get_slot = 0;
+  float acc[4];
+  auto product = [&](const T* col, int K) {
+    acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+    for (int c = 0; c < K; c += kChunkK) {
+      uint4 b[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = c + i * 64 + q * 16;
+        b[i][0] = k < K ? *reinterpret_cast<const uint4*>(col + k) : make_uint4(0, 0, 0, 0);
+        b[i][1] = k + 8 < K ? *reinterpret_cast<const uint4*>(col + k + 8) : make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 a[4];  // rows g and g + 8, two units each
+        const uint32_t at = get_slot * kChunk + i * 128;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(a[h].x), "=r"(a[h].y), "=r"(a[h].z), "=r"(a[h].w)
+                       : "r"((h & 1 ? get1 : get0) + at + (h >> 1) * 8 * kChunkK * 2)
+                       : "memory");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t a0[4] = {a[h].x, a[2 + h].x, a[h].y, a[2 + h].y};
+          const uint32_t a1[4] = {a[h].z, a[2 + h].z, a[h].w, a[2 + h].w};
+          mma16816<T>(acc, a0, b[i][h].x, b[i][h].y);
+          mma16816<T>(acc, a1, b[i][h].z, b[i][h].w);
+        }
+      }
+      if (++get_slot == kDepth) get_slot = 0;
+      __syncwarp();
+      copy();
+    }
+  };
+
+  T* act = static_cast<T*>(p.act);
+  for (int u = me; u < units1; u += warps) {
+    const int group = u / per1, row = u - group * per1, n = s.group_n[group];
+    // A column past the group's tokens: its first token again.
+    product(static_cast<const T*>(p.x) + s.group_a[group][g < n ? g : 0] / p.top_k * p.x_stride, p.hidden);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (2 * q + k < n) {
+        const float gate = acc[k], up = acc[2 + k];
+        act[(int64_t)s.group_a[group][2 * q + k] * p.inter + row * 8 + g] = Dt<T>::from_f(gate / (1.f + __expf(-gate)) * up);
+      }
+  }
+  grid_barrier(p, 2);  // the first of down's rows are on their way meanwhile
+  for (int u = me; u < units2; u += warps) {
+    const int group = u / per2, row = u - group * per2, n = s.group_n[group];
+    product(act + (int64_t)s.group_a[group][g < n ? g : 0] * p.inter, p.inter);
+    const int r = row * 16 + g;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (2 * q + k < n) {
+        float* y = p.y + (int64_t)s.group_a[group][2 * q + k] * p.hidden + r;
+        y[0] = acc[k];
+        if (r + 8 < p.hidden) y[8] = acc[2 + k];
+      }
+  }
+  grid_barrier(p, 3);
+  combine<T>(p, s.weight);
+  leave(p, &s.last);
 }
 
 // ---------------------------------------------------------------- host
@@ -658,6 +938,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 struct Layout {
   int64_t logits, perm, weight, done, xs, act, y, bytes;
   int max_tiles, tile_n, rows1, rows2, splits, stages, slot_b, source, rows_b;
+  bool few;
 };
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -665,7 +946,8 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 // The tiling, from sizes alone, and where each part of the workspace lies.
 Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter, int sms) {
   Layout l = {};
-  l.tile_n = (int)std::min<int64_t>(256, up(std::max<int64_t>(tokens, 1), 16));
+  l.few = tokens <= kFewTokens;
+  l.tile_n = l.few ? 16 : (int)std::min<int64_t>(256, up(tokens, 16));
   const int64_t rows = tokens * top_k;
   l.max_tiles = (int)(std::min<int64_t>(experts, rows) + rows / l.tile_n);
   // Weight rows of an item: the size whose dealing out over the SMs leaves the least idle.
@@ -719,10 +1001,30 @@ void launch_router(const ExpertParams& p, int groups, int shares, cudaStream_t s
 }
 
 template <typename T>
-int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, cudaStream_t st) {
+int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms());
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  // Cooperative: the CTAs wait for one another's activations, so they must all be resident.
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (few) {
+    static SmemAttribute attributes[3];
+    const int n = p.experts <= 64 ? 0 : p.experts <= 128 ? 1 : 2;
+    auto kernel = n == 0 ? expert_few_kernel<T, 2> : n == 1 ? expert_few_kernel<T, 4> : expert_few_kernel<T, 16>;
+    const cudaError_t e = attributes[n].set(reinterpret_cast<const void*>(kernel), kFewSmem);
+    if (e != cudaSuccess) return cuda_status(e);
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = kFewSmem;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
+  }
   const int groups = (p.tokens + kRouterTokens - 1) / kRouterTokens;
-  // Few tokens: an expert per warp, its logits' CTAs spread over the SMs. Many: eight experts per warp
-  // for each load of the tokens.
+  // An expert per warp, and the logits' CTAs spread over the SMs; more tokens than that: eight experts
+  // per warp for each load of the tokens.
   const int shares = (p.experts + 7) / 8;
   if (groups * (int64_t)shares <= 4 * num_sms() && groups <= kMaxTickets) launch_router<T, 1>(p, groups, shares, st);
   else launch_router<T, 8>(p, groups, 1, st);
@@ -733,17 +1035,7 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, cudaStream_t st)
   const int smem = 1024 + p.stages * (kSlotA + p.slot_b);
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(expert_kernel<T>), 1024 + kRing);
   if (e != cudaSuccess) return cuda_status(e);
-  // Cooperative: the CTAs wait for one another's activations, so they must all be resident.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_sms());
-  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeCooperative;
-  at[0].val.cooperative = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, expert_kernel<T>, maps[0], maps[1], maps[2], maps[3], p));
 }
 
@@ -777,7 +1069,7 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   if (workspace_bytes < l.bytes) return PKV_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   ExpertParams p = {};
-  p.x = x, p.router = router, p.out = out, p.status = status_dev;
+  p.x = x, p.router = router, p.gate_up = gate_up, p.down = down, p.out = out, p.status = status_dev;
   p.head = reinterpret_cast<Header*>(ws);
   p.logits = reinterpret_cast<float*>(ws + l.logits);
   p.perm = reinterpret_cast<int32_t*>(ws + l.perm);
@@ -794,16 +1086,17 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
   CUtensorMap maps[4];
-  int rc = l.source == kSorted
+  int rc = l.few ? PKV_OK
+           : l.source == kSorted
                ? make_matrix_tensor_map(&maps[0], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, l.rows_b)
                : make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB,
                                         l.source == kDirect ? l.rows_b : 1);
-  if (rc == PKV_OK) rc = make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
-  if (rc == PKV_OK)
+  if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
+  if (rc == PKV_OK && !l.few)
     rc = make_matrix_tensor_map(&maps[2], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB,
                                 l.rows_b);
-  if (rc == PKV_OK) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, 32, 1);
+  if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, 32, 1);
   if (rc != PKV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == PKV_F16 ? launch<__half>(maps, p, st) : launch<__nv_bfloat16>(maps, p, st);
+  return dtype == PKV_F16 ? launch<__half>(maps, p, l.few, st) : launch<__nv_bfloat16>(maps, p, l.few, st);
 }
