@@ -33,7 +33,7 @@ constexpr int kSlotA = 16384;      // weight bytes of a stage: 32, 64 or 128 row
 constexpr int kBox = 4096;         // of them per copy: 32 rows of a chunk
 constexpr int kMaxStages = 16;
 constexpr int kThreads = 256;      // weight copies, token copies, MMA, (idle), 4 epilogue warps
-constexpr int kRouterTokens = 4;   // tokens of a router CTA
+constexpr int kRouterTokens = 8;   // tokens of a router CTA, a warp's choice each
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
 constexpr int kRing = 200 * 1024;  // bytes of the stages
 
@@ -103,20 +103,29 @@ __device__ double exact_logit(const ExpertParams& p, int t, int e) {
   const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + t * p.x_stride);
   const uint4* w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden);
   double s = 0;
-  for (int c = threadIdx.x & 31; c < p.hidden / 8; c += 32) {
-    float a[8], b[8];
-    unpack8<T>(x[c], a);
-    unpack8<T>(w[c], b);
+  const int vecs = p.hidden / 8;
+  for (int c0 = threadIdx.x & 31; c0 < vecs; c0 += 32 * 8) {
+    uint4 u[8], v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += (double)a[i] * (double)b[i];
+    for (int n = 0; n < 8; ++n) u[n] = x[min(c0 + 32 * n, vecs - 1)], v[n] = w[min(c0 + 32 * n, vecs - 1)];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      float a[8], b[8];
+      unpack8<T>(u[n], a);
+      unpack8<T>(v[n], b);
+      if (c0 + 32 * n < vecs) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += (double)a[i] * (double)b[i];
+      }
+    }
   }
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
 // The top_k experts of a token and their weights, by a warp. Lane l holds experts l, l + 32, ... The
-// float32 logits are off by about 1e-7 of the largest; where the last expert in and the first one
-// out are within 2^-15 of it, those within that of the border are chosen by their float64 logits, so
+// float32 logits are off by about 2^-23 of the largest; where the last expert in and the first one
+// out are within 2^-17 of it, those within that of the border are chosen by their float64 logits, so
 // that the choice does not hang on the order of a sum. `exact`: float64 scratch of the warp. Lane k < top_k
 // gets the k-th expert and its weight.
 template <typename T, int NV>
@@ -131,7 +140,7 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
     v[i] = e < p.experts ? __ldcg(&p.logits[(int64_t)t * p.experts + e]) : 0.f;
     big = max(big, __float_as_uint(fabsf(v[i])));
   }
-  const float tol = __uint_as_float(__reduce_max_sync(all, big)) * 0x1p-15f;
+  const float tol = __uint_as_float(__reduce_max_sync(all, big)) * 0x1p-17f;
   uint32_t taken = 0;
   int mine_e = 0;
   float mine_v = 0.f, last = 0.f;
@@ -216,73 +225,81 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
   weight = on ? expf(mine_v - m) / sum : 0.f;
 }
 
-// A CTA takes kRouterTokens tokens and, of the experts, 8 EPW (one warp EPW of them at a time); grid y
-// is the number of such shares. The last CTA of a group of tokens chooses.
-template <typename T, int EPW, int NV>
+// A CTA takes kRouterTokens tokens and EPC experts at a time, its threads a part of hidden each, so that
+// every load is one of few a thread waits for; grid y shares out the experts. The last CTA of a group
+// of tokens chooses, a warp for each.
+template <typename T, int EPC, int NV>
 __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
   __shared__ double exact[kRouterTokens][32 * NV];
+  __shared__ float part[8][EPC * kRouterTokens];
   __shared__ int s_last;
   const int group = blockIdx.x, t0 = group * kRouterTokens;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, vecs = p.hidden / 8;
   // The expert kernel's counters of finished tiles start at zero.
-  for (int i = (blockIdx.y * gridDim.x + group) * 256 + threadIdx.x; i < p.max_tiles; i += 256 * gridDim.x * gridDim.y)
-    p.done[i] = 0;
-  const uint4* x[kRouterTokens];
+  for (int i = (blockIdx.y * gridDim.x + group) * 256 + tid; i < p.max_tiles; i += 256 * gridDim.x * gridDim.y) p.done[i] = 0;
+  for (int e0 = blockIdx.y * EPC; e0 < p.experts; e0 += EPC * gridDim.y) {
+    float acc[EPC][kRouterTokens];
 #pragma unroll
-  for (int q = 0; q < kRouterTokens; ++q)
-    x[q] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + min(t0 + q, p.tokens - 1) * p.x_stride);
-  const int step = 8 * EPW * gridDim.y;
-  for (int e0 = (blockIdx.y * 8 + warp) * EPW; e0 < p.experts; e0 += step) {
-    float acc[EPW][kRouterTokens];
-#pragma unroll
-    for (int j = 0; j < EPW; ++j)
+    for (int j = 0; j < EPC; ++j)
 #pragma unroll
       for (int q = 0; q < kRouterTokens; ++q) acc[j][q] = 0.f;
-    // A warp with one expert has few loads to hide their latency behind: four steps' go ahead together.
-    constexpr int kAhead = EPW == 1 ? 4 : 1;
-    const int vecs = p.hidden / 8;
-    for (int c0 = lane; c0 < vecs; c0 += 32 * kAhead) {
-      uint4 xs[kAhead][kRouterTokens], ws[kAhead];
+    for (int c = tid; c < vecs; c += 256) {
+      uint4 ws[EPC], xs[kRouterTokens];
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int c = min(c0 + 32 * n, vecs - 1);
-        if constexpr (EPW == 1)
-          ws[n] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e0 * p.hidden)[c];
+      for (int j = 0; j < EPC; ++j)
+        ws[j] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)min(e0 + j, p.experts - 1) * p.hidden)[c];
 #pragma unroll
-        for (int q = 0; q < kRouterTokens; ++q) xs[n][q] = x[q][c];
-      }
+      for (int q = 0; q < kRouterTokens; ++q)
+        xs[q] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + min(t0 + q, p.tokens - 1) * p.x_stride)[c];
+      float w[EPC][8];
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const bool in = c0 + 32 * n < vecs;
-        float a[kRouterTokens][8];
-#pragma unroll
-        for (int q = 0; q < kRouterTokens; ++q) unpack8<T>(xs[n][q], a[q]);
-#pragma unroll
-        for (int j = 0; j < EPW; ++j) {
-          const int e = min(e0 + j, p.experts - 1);
-          float w[8];
-          unpack8<T>(EPW == 1 ? ws[n]
-                              : reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden)[c0], w);
-#pragma unroll
-          for (int q = 0; q < kRouterTokens; ++q)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[j][q] += in ? a[q][i] * w[i] : 0.f;
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < EPW; ++j)
+      for (int j = 0; j < EPC; ++j) unpack8<T>(ws[j], w[j]);
 #pragma unroll
       for (int q = 0; q < kRouterTokens; ++q) {
-        float s = acc[j][q];
+        float a[8];
+        unpack8<T>(xs[q], a);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0 && e0 + j < p.experts && t0 + q < p.tokens) p.logits[(int64_t)(t0 + q) * p.experts + e0 + j] = s;
+        for (int j = 0; j < EPC; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[j][q] += a[i] * w[j][i];
       }
+    }
+    if constexpr (EPC * kRouterTokens == 32) {  // a warp's 32 sums to its 32 lanes, halving what is held each time
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = acc[i / kRouterTokens][i % kRouterTokens];
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+          const bool high = lane & o;
+          const float other = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[i + o], o);
+          v[i] = (high ? v[i + o] : v[i]) + other;
+        }
+      part[warp][lane] = v[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < EPC; ++j)
+#pragma unroll
+        for (int q = 0; q < kRouterTokens; ++q) {
+          float v = acc[j][q];
+#pragma unroll
+          for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          if (lane == 0) part[warp][j * kRouterTokens + q] = v;
+        }
+    }
+    __syncthreads();
+    if (tid < EPC * kRouterTokens) {
+      const int e = e0 + tid / kRouterTokens, t = t0 + tid % kRouterTokens;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += part[k][tid];
+      if (e < p.experts && t < p.tokens) p.logits[(int64_t)t * p.experts + e] = sum;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (gridDim.y > 1) {
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       const bool last = atom_add_acq_rel_gpu(&p.head->tickets[group], 1) == (int)gridDim.y - 1;
       if (last) st_relaxed_gpu(&p.head->tickets[group], 0);
       s_last = last;
@@ -290,7 +307,7 @@ __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
     __syncthreads();
     if (!s_last) return;
   }
-  if (warp < kRouterTokens && t0 + warp < p.tokens) {
+  if (t0 + warp < p.tokens) {
     int e;
     float w;
     choose<T, NV>(p, t0 + warp, exact[warp], e, w);
@@ -992,12 +1009,14 @@ bool sizes_ok(int64_t tokens, int experts, int top_k, int hidden, int inter) {
          inter <= (1 << 20);
 }
 
-template <typename T, int EPW>
-void launch_router(const ExpertParams& p, int groups, int shares, cudaStream_t st) {
-  const dim3 grid(groups, shares);
-  if (p.experts <= 64) router_kernel<T, EPW, 2><<<grid, 256, 0, st>>>(p);
-  else if (p.experts <= 128) router_kernel<T, EPW, 4><<<grid, 256, 0, st>>>(p);
-  else router_kernel<T, EPW, 16><<<grid, 256, 0, st>>>(p);
+template <typename T, int EPC>
+void launch_router(const ExpertParams& p, int groups, cudaStream_t st) {
+  // With more groups than tickets a CTA takes all experts of its group.
+  const int shares = std::min((p.experts + EPC - 1) / EPC, std::max(1, 2 * num_sms() / groups));
+  const dim3 grid(groups, groups <= kMaxTickets ? shares : 1);
+  if (p.experts <= 64) router_kernel<T, EPC, 2><<<grid, 256, 0, st>>>(p);
+  else if (p.experts <= 128) router_kernel<T, EPC, 4><<<grid, 256, 0, st>>>(p);
+  else router_kernel<T, EPC, 16><<<grid, 256, 0, st>>>(p);
 }
 
 template <typename T>
@@ -1023,11 +1042,9 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaSt
     return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
   }
   const int groups = (p.tokens + kRouterTokens - 1) / kRouterTokens;
-  // An expert per warp, and the logits' CTAs spread over the SMs; more tokens than that: eight experts
-  // per warp for each load of the tokens.
-  const int shares = (p.experts + 7) / 8;
-  if (groups * (int64_t)shares <= 4 * num_sms() && groups <= kMaxTickets) launch_router<T, 1>(p, groups, shares, st);
-  else launch_router<T, 8>(p, groups, 1, st);
+  // An expert per CTA for few tokens; four for each load of the tokens when that still fills the SMs.
+  if (groups * (int64_t)((p.experts + 3) / 4) < 4 * num_sms()) launch_router<T, 1>(p, groups, st);
+  else launch_router<T, 4>(p, groups, st);
   if (p.source == kSorted) gather_kernel<<<4 * num_sms(), 256, 0, st>>>(p);
   int rc = launch_status();
   if (rc != PKV_OK) return rc;
