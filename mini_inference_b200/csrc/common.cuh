@@ -207,17 +207,6 @@ __device__ inline void tma_load_4d(void* smem_dst, const CUtensorMap* map, int c
       : "memory");
 }
 
-// Four rows r0 .. r3 of a 2-D tensor, their elements from column c0 on, one behind the other in
-// shared memory (no multicast). The map's box is one row high.
-__device__ inline void tma_gather4(void* smem_dst, const CUtensorMap* map, int c0, int r0, int r1, int r2, int r3,
-                                   uint64_t* bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
-
 // Bulk (non-tensor) copy of `bytes` (a multiple of 16, both addresses 16-byte aligned)
 // global -> shared, completing on an mbarrier (no multicast).
 __device__ inline void bulk_load(void* smem_dst, const void* gmem_src, uint32_t bytes, uint64_t* bar) {
@@ -379,6 +368,10 @@ int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int
 // fourth dimension of one entry), 128-byte swizzle. Rows past a stack's end read as zeros.
 int make_stack_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
                           uint32_t box_rows, uint32_t box_stacks);
+// The same with rows, a multiple of `group`, in groups: dimensions {inner, group, stacks, rows / group} and a
+// box of {64, group, box_stacks, box_groups}: a group's rows of each stack, group by group.
+int make_split_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
+                          uint32_t group, uint32_t box_stacks, uint32_t box_groups);
 // Streaming multiprocessors of the current device (queried once).
 int num_sms();
 

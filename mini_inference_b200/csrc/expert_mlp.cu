@@ -9,7 +9,7 @@
 //
 // 1. router_kernel: logits in float32, the choice of experts (exact, see choose()), each choice
 //    noted in its expert's list.
-// 2. (past 256 tokens) gather_kernel: each expert's token rows one behind the other.
+// 2. (past kDirectTokens) gather_kernel: each expert's token rows one behind the other.
 // 3. expert_kernel: a persistent cooperative grid, one CTA per SM. Its items are first every
 //    (expert, token tile, weight rows) of gate and up, then every one of down, dealt out in
 //    turn. The rings of weight and token stages run on from item to item and from the first
@@ -30,7 +30,6 @@ constexpr int kMaxExperts = 512;
 constexpr int kMaxTopK = 16;
 constexpr int kKB = 64;            // K elements of a chunk: one 128-byte swizzled row
 constexpr int kSlotA = 16384;      // weight bytes of a stage: 32, 64 or 128 rows of 4, 2 or 1 chunks
-constexpr int kBox = 4096;         // of them per copy: 32 rows of a chunk
 constexpr int kMaxStages = 16;
 constexpr int kThreads = 256;      // weight copies, token copies, MMA, (idle), 4 epilogue warps
 constexpr int kRouterTokens = 8;   // tokens of a router CTA, a warp's choice each
@@ -57,7 +56,7 @@ struct ExpertParams {
   int32_t* done;    // [token tiles]: row tiles of gate and up that are finished
   void* xs;         // [tokens * top_k][hidden], past 256 tokens: x by expert
   void* act;        // [tokens * top_k][inter], an expert's rows one behind the other
-  float* y;         // [splits][tokens * top_k][hidden]
+  float* y;         // [tokens * top_k][hidden]
   void* out;
   int32_t* status;
   int64_t x_stride, out_stride;
@@ -65,16 +64,17 @@ struct ExpertParams {
   int max_tiles;    // entries of done
   int rows1, rows2; // weight rows of an item (gate and up; down): 32, 64 or 128
   int tile_n;       // tokens of a tile, at most
-  int stages, slot_b, splits;
-  int source;       // of gate and up's token rows: kDirect, kGather, kSorted
-  int rows_b;       // token rows of a copy, but for kGather
+  int stages, slot_b;
+  bool in16;        // intermediate is a multiple of 16
+  bool direct;      // gate and up's token rows: all of x, or the expert's of xs
+  int rows_x, rows_act;  // token rows of a copy of either product
   uint32_t tmem_cols;
 };
 
-// Where gate and up's tokens come from. Up to 16 tokens are all loaded for every expert (its columns are
-// looked up afterwards); up to 256 are gathered four rows a copy; more are laid out by expert first:
-// a tile of 256 rows would be 64 copies a chunk.
-enum Source { kDirect, kGather, kSorted };
+// Where gate and up's tokens come from: up to kDirectTokens are all loaded for every expert, which takes
+// its columns of the accumulator; more are laid out by expert first (gathering four rows a copy cost
+// as much as a copy of 32: 503 of a stage's 830 cycles at 64 tokens of 8 in 64 experts).
+constexpr int kDirectTokens = 64;
 
 // ---------------------------------------------------------------- router
 
@@ -333,7 +333,7 @@ struct Item {
   bool second;            // down; else gate and up
   int tile, e, n0, n;     // token tile, its expert, its first and number of tokens
   int row;                // row tile
-  int split, k0, k1;      // chunks of 64
+  int chunks;             // of 64 elements of K
 };
 
 struct Shared {
@@ -342,7 +342,6 @@ struct Shared {
   uint64_t acc_full[2], acc_empty[2], mma_done;
   uint32_t tmem;
   int last;
-  alignas(16) int token[256];   // the tokens of the tile being copied
   int offset[kMaxExperts + 1];  // rows of act before each expert's
   int tile[kMaxExperts + 1];    // token tiles before each expert's
 };
@@ -389,19 +388,15 @@ __global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
 __device__ __forceinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
   const int per1 = (2 * p.inter + p.rows1 - 1) / p.rows1, per2 = (p.hidden + p.rows2 - 1) / p.rows2;
   const int tiles = s.tile[p.experts], first = tiles * per1;
-  int k = 0;
   it.second = i >= first;
   if (!it.second) {
-    it.tile = i / per1, it.row = i - it.tile * per1, it.split = 0;
-    it.k0 = 0, it.k1 = (p.hidden + kKB - 1) / kKB;
+    it.tile = i / per1, it.row = i - it.tile * per1;
+    it.chunks = (p.hidden + kKB - 1) / kKB;
   } else {
     i -= first;
-    if (i >= tiles * per2 * p.splits) return false;
-    it.tile = i / (per2 * p.splits);
-    k = i - it.tile * per2 * p.splits;
-    it.split = k / per2, it.row = k - it.split * per2;
-    const int chunks = (p.inter + kKB - 1) / kKB;
-    it.k0 = chunks * it.split / p.splits, it.k1 = chunks * (it.split + 1) / p.splits;
+    if (i >= tiles * per2) return false;
+    it.tile = i / per2, it.row = i - it.tile * per2;
+    it.chunks = (p.inter + kKB - 1) / kKB;
   }
   int lo = 0, hi = p.experts - 1;  // the expert whose tiles hold it.tile
   while (lo < hi) {
@@ -429,29 +424,33 @@ __device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times) {
   __syncthreads();
 }
 
-// out = the sum over each token's experts, in their order, of its products; by the whole grid.
+// out = the sum over each token's experts, in their order, of its products; by the whole grid. Four
+// products' loads go ahead together.
 template <typename T>
 __device__ __forceinline__ void combine(const ExpertParams& p, const float* weight) {
   const int per_row = p.hidden / 8;
-  const int64_t units = (int64_t)p.tokens * per_row, plane = (int64_t)p.tokens * p.top_k * p.hidden;
+  const int64_t units = (int64_t)p.tokens * per_row;
   for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (int64_t)gridDim.x * blockDim.x) {
     const int t = (int)(u / per_row), c = (int)(u - (int64_t)t * per_row) * 8;
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    for (int k = 0; k < p.top_k; ++k) {
-      const float w = weight[t * p.top_k + k];
-      const float* y = p.y + ((int64_t)t * p.top_k + k) * p.hidden + c;
-      float part[8];
+    for (int k0 = 0; k0 < p.top_k; k0 += 4) {
+      float4 v[4][2];
+      float w[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[e] = 0.f;
-      for (int z = 0; z < p.splits; ++z, y += plane) {
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(y)), b = __ldcg(reinterpret_cast<const float4*>(y) + 1);
-        part[0] += a.x, part[1] += a.y, part[2] += a.z, part[3] += a.w;
-        part[4] += b.x, part[5] += b.y, part[6] += b.z, part[7] += b.w;
+      for (int k = 0; k < 4; ++k) {
+        const int a = t * p.top_k + min(k0 + k, p.top_k - 1);
+        const float4* y = reinterpret_cast<const float4*>(p.y + (int64_t)a * p.hidden + c);
+        v[k][0] = __ldcg(y), v[k][1] = __ldcg(y + 1);
+        w[k] = weight[a];
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += w * part[e];
+      for (int k = 0; k < 4; ++k)
+        if (k0 + k < p.top_k) {
+          sum[0] += w[k] * v[k][0].x, sum[1] += w[k] * v[k][0].y, sum[2] += w[k] * v[k][0].z, sum[3] += w[k] * v[k][0].w;
+          sum[4] += w[k] * v[k][1].x, sum[5] += w[k] * v[k][1].y, sum[6] += w[k] * v[k][1].z, sum[7] += w[k] * v[k][1].w;
+        }
     }
     uint4 o;
     o.x = Dt<T>::pack(sum[0], sum[1]), o.y = Dt<T>::pack(sum[2], sum[3]);
@@ -519,16 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t round = 0;  // of the ring
     for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G) {
       const int e = uniform(it.e), rows = it.second ? p.rows2 : p.rows1, wide = 128 / rows;
-      const int k0 = uniform(it.k0), k1 = uniform(it.k1), pad = uniform((it.n + 15) & ~15);
-      const int row = uniform(it.row) * (it.second ? p.rows2 : p.rows1 / 2), row_step = it.second ? 32 : 16;
-      const bool direct = !it.second && p.source == kDirect, gather = !it.second && p.source == kGather;
-      const int first = direct ? 0 : uniform(s.offset[it.e] + it.n0);
-      if (!weights && gather) {
-        __syncwarp();
-        for (int c = lane; c < pad; c += 32)  // rows past the tile's tokens: its first token again
-          s.token[c] = __ldg(&p.perm[(int64_t)it.e * p.tokens + it.n0 + (c < it.n ? c : 0)]) / p.top_k;
-        __syncwarp();
-      }
+      const int k1 = uniform(it.chunks), pad = uniform((it.n + 15) & ~15);
+      const int row = uniform(it.row) * (it.second ? p.rows2 : p.rows1 / 2), box = it.second ? p.rows2 : 32;
+      const bool direct = !it.second && p.direct;
+      const int first = direct ? 0 : uniform(s.offset[it.e] + it.n0), columns = direct ? p.tile_n : pad;
+      const int rows_b = it.second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
       if (!weights && it.second) {  // the tile's activations
         if (lane == 0)
           for (int n = 1; ld_acquire_gpu(&p.done[it.tile]) < per1; ++n)
@@ -543,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const CUtensorMap* map_w = it.second ? &map_down : &map_gu;
       const CUtensorMap* map_b = it.second ? &map_act : &map_x;
       const int stack = it.second ? e : 2 * e;
-      for (int ks = k0; ks < k1; ks += wide) {
+      for (int ks = 0; ks < k1; ks += wide) {
         if (round > 0 && !__all_sync(0xffffffffu, wait_for(&s.freed[slot], (round - 1) & 1, deadline))) {
           ok = false;
           break;
@@ -553,24 +547,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (weights) {
           uint8_t* dst = ring_a + slot * kSlotA;
           if (leader) mbar_arrive_expect_tx(bar, chunks * rows * 128);
-          for (int c = 0; c < chunks; ++c)
-            for (int b = 0; b < rows; b += 32, dst += kBox)  // gate and up: 16 gate rows, then their 16 up rows
-              if (leader) tma_load_4d(dst, map_w, (ks + c) * kKB, row + (b >> 5) * row_step, stack, 0, bar, w_policy);
-        } else {
-          uint8_t* dst = ring_b + slot * p.slot_b;
-          const int loaded = gather ? pad : (pad + p.rows_b - 1) / p.rows_b * p.rows_b;
-          if (leader) mbar_arrive_expect_tx(bar, chunks * loaded * 128);
-          for (int c = 0; c < chunks; ++c, dst += loaded * 128) {
-            if (gather) {
-              for (int b = 0; b < pad; b += 4) {
-                const int4 t = *reinterpret_cast<const int4*>(&s.token[b]);
-                if (leader) tma_gather4(dst + b * 128, &map_x, (ks + c) * kKB, t.x, t.y, t.z, t.w, bar, reused);
-              }
+          for (int c = 0; c < chunks; ++c, dst += rows * 128) {
+            if (it.second || !p.in16) {
+              for (int b = 0; b < rows; b += box)
+                if (leader)
+                  tma_load_4d(dst + b * 128, map_w, (ks + c) * kKB, row + (it.second ? b : b / 2), stack, 0, bar, w_policy);
             } else {
-              for (int b = 0; b < pad; b += p.rows_b)
-                if (leader) tma_load_2d(dst + b * 128, map_b, (ks + c) * kKB, first + b, bar, reused);
+              if (leader) tma_load_4d(dst, map_w, (ks + c) * kKB, 0, stack, row / 16, bar, w_policy);
             }
           }
+        } else {
+          uint8_t* dst = ring_b + slot * p.slot_b;
+          if (leader) mbar_arrive_expect_tx(bar, chunks * loaded * 128);
+          for (int c = 0; c < chunks; ++c, dst += loaded * 128)
+            for (int b = 0; b < columns; b += rows_b)
+              if (leader) tma_load_2d(dst + b * 128, map_b, (ks + c) * kKB, first + b, bar, reused);
         }
         ++issued;
         if (++slot == p.stages) slot = 0, ++round;
@@ -597,13 +588,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after_sync();
       const int rows = it.second ? p.rows2 : p.rows1, wide = 128 / rows;
-      const int k0 = uniform(it.k0), k1 = uniform(it.k1), pad = uniform((it.n + 15) & ~15);
-      const bool gather = !it.second && p.source == kGather;
-      const int loaded = gather ? pad : (pad + p.rows_b - 1) / p.rows_b * p.rows_b;
-      const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, pad);
+      const int k1 = uniform(it.chunks), pad = uniform((it.n + 15) & ~15);
+      const int columns = !it.second && p.direct ? p.tile_n : pad;
+      const int rows_b = it.second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
+      const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, columns);
       const uint32_t d = tmem + (uint32_t)(b * p.tile_n);
       bool more = false;
-      for (int ks = k0; ks < k1; ks += wide) {
+      for (int ks = 0; ks < k1; ks += wide) {
         if (!__all_sync(0xffffffffu, wait_for(&s.full[slot], round & 1, deadline))) {
           ok = false;
           break;
@@ -649,24 +640,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int r = it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
         const bool in = q * 32 < p.rows1 && r < p.inter;
         T* row = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
-        const bool direct = p.source == kDirect;
+        const bool direct = p.direct;
         if (q * 32 < p.rows1) {
-          const int token = direct && lane < it.n ? __ldg(&p.perm[(int64_t)it.e * p.tokens + lane]) / p.top_k : -1;
-          for (int c0 = 0; c0 < (direct ? p.tokens : it.n); c0 += 16) {
+          // The column of the tile's token c: itself, or the token's place in x.
+          const int32_t* perm = p.perm + (int64_t)it.e * p.tokens + it.n0;
+          int token = 0;
+          for (int c0 = 0; c0 < it.n; c0 += 16) {
             uint32_t v[16];
-            tmem_ld16(d + c0, v);
+            if (direct) {
+              if ((c0 & 31) == 0) token = c0 + lane < it.n ? __ldg(&perm[c0 + lane]) / p.top_k : 0;
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const int at = __shfl_sync(0xffffffffu, token, (c0 & 31) + k);
+                v[k] = tmem_ld1(d + at);
+              }
+            } else {
+              tmem_ld16(d + c0, v);
+            }
             tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
               const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, low ? v[k + 1] : v[k], 16));
               const float g = low ? __uint_as_float(v[k]) : other;
               const float u = low ? other : __uint_as_float(v[k + 1]);
-              int col = c0 + k + (low ? 0 : 1);
-              if (direct) {  // the column of token `col`: its place in the expert's list
-                const uint32_t even = __ballot_sync(0xffffffffu, token == k), odd = __ballot_sync(0xffffffffu, token == k + 1);
-                col = __ffs(low ? even : odd) - 1;
-              }
-              if (in && col >= 0 && col < it.n) row[(int64_t)col * p.inter] = Dt<T>::from_f(g / (1.f + __expf(-g)) * u);
+              const int col = c0 + k + (low ? 0 : 1);
+              if (in && col < it.n) row[(int64_t)col * p.inter] = Dt<T>::from_f(g / (1.f + __expf(-g)) * u);
             }
           }
         }
@@ -678,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         const int r = it.row * p.rows2 + q * 32 + lane;
         if (q * 32 < p.rows2) {
-          float* y = p.y + (int64_t)it.split * p.tokens * p.top_k * p.hidden + r;
+          float* y = p.y + r;
           const int32_t* perm = p.perm + (int64_t)it.e * p.tokens + it.n0;
           for (int c0 = 0; c0 < it.n; c0 += 16) {
             const int a = lane < 16 && c0 + lane < it.n ? __ldg(&perm[c0 + lane]) : 0;
@@ -954,8 +952,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
 
 struct Layout {
   int64_t logits, perm, weight, done, xs, act, y, bytes;
-  int max_tiles, tile_n, rows1, rows2, splits, stages, slot_b, source, rows_b;
-  bool few;
+  int max_tiles, tile_n, rows1, rows2, stages, slot_b, rows_x, rows_act;
+  bool few, direct;
 };
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -964,7 +962,11 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter, int sms) {
   Layout l = {};
   l.few = tokens <= kFewTokens;
-  l.tile_n = l.few ? 16 : (int)std::min<int64_t>(256, up(tokens, 16));
+  l.direct = tokens <= kDirectTokens;
+  // Twice an expert's share of the tokens, so that few take a second tile; not all slots of a stage's rows
+  // for tokens that most experts do not have.
+  l.tile_n = (int)(l.few ? 16 : l.direct ? up(tokens, 16)
+                   : std::min<int64_t>(std::min<int64_t>(256, up(tokens, 16)), std::max<int64_t>(32, up(2 * tokens * top_k / experts, 32))));
   const int64_t rows = tokens * top_k;
   l.max_tiles = (int)(std::min<int64_t>(experts, rows) + rows / l.tile_n);
   // Weight rows of an item: the size whose dealing out over the SMs leaves the least idle.
@@ -980,11 +982,10 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   };
   l.rows1 = pick(2 * (int64_t)inter);
   l.rows2 = pick(hidden);
-  l.splits = 1;
-  l.source = tokens <= 16 ? kDirect : tokens <= 256 ? kGather : kSorted;
-  l.rows_b = l.tile_n <= 64 ? 16 : 64;
+  l.rows_act = l.tile_n <= 64 ? 16 : 32;
+  l.rows_x = l.direct ? l.tile_n : l.rows_act;
   // A stage's token rows, of as many chunks as its weights have.
-  l.slot_b = (l.tile_n + l.rows_b - 1) / l.rows_b * l.rows_b * 128 * (128 / std::min(l.rows1, l.rows2));
+  l.slot_b = (int)up(l.tile_n, l.rows_act) * 128 * (128 / std::min(l.rows1, l.rows2));
   l.stages = std::min(kMaxStages, kRing / (kSlotA + l.slot_b));
   int64_t at = up(sizeof(Header), 256);
   auto take = [&](int64_t bytes) {
@@ -996,9 +997,9 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.perm = take(tokens * experts * 4);
   l.weight = take(rows * 4);
   l.done = take((int64_t)l.max_tiles * 4);
-  l.xs = take(l.source == kSorted ? rows * hidden * 2 : 0);
+  l.xs = take(l.direct ? 0 : rows * hidden * 2);
   l.act = take(rows * inter * 2);
-  l.y = take((int64_t)l.splits * rows * hidden * 4);
+  l.y = take(rows * hidden * 4);
   l.bytes = at;
   return l;
 }
@@ -1045,7 +1046,7 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaSt
   // An expert per CTA for few tokens; four for each load of the tokens when that still fills the SMs.
   if (groups * (int64_t)((p.experts + 3) / 4) < 4 * num_sms()) launch_router<T, 1>(p, groups, st);
   else launch_router<T, 4>(p, groups, st);
-  if (p.source == kSorted) gather_kernel<<<4 * num_sms(), 256, 0, st>>>(p);
+  if (!p.direct) gather_kernel<<<4 * num_sms(), 256, 0, st>>>(p);
   int rc = launch_status();
   if (rc != PKV_OK) return rc;
   static SmemAttribute attribute;
@@ -1099,20 +1100,24 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.tokens = (int)n_tokens, p.hidden = hidden, p.inter = intermediate, p.experts = num_experts, p.top_k = top_k;
   p.renormalize = renormalize;
   p.max_tiles = l.max_tiles, p.rows1 = l.rows1, p.rows2 = l.rows2, p.tile_n = l.tile_n;
-  p.stages = l.stages, p.slot_b = l.slot_b, p.splits = l.splits, p.source = l.source, p.rows_b = l.rows_b;
+  p.stages = l.stages, p.slot_b = l.slot_b, p.direct = l.direct, p.rows_x = l.rows_x, p.rows_act = l.rows_act;
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
   CUtensorMap maps[4];
-  int rc = l.few ? PKV_OK
-           : l.source == kSorted
-               ? make_matrix_tensor_map(&maps[0], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, l.rows_b)
-               : make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB,
-                                        l.source == kDirect ? l.rows_b : 1);
-  if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
+  int rc = PKV_OK;
+  if (!l.few && l.direct) rc = make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB, l.rows_x);
+  else if (!l.few)
+    rc = make_matrix_tensor_map(&maps[0], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, l.rows_x);
+  // Operand A of the first product alternates 16 gate rows and their 16 up rows: in one copy where an
+  // expert's rows are whole groups of 16, else a copy for each 32.
+  p.in16 = intermediate % 16 == 0;
+  if (rc == PKV_OK && !l.few)
+    rc = p.in16 ? make_split_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2, l.rows1 / 32)
+                : make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
   if (rc == PKV_OK && !l.few)
     rc = make_matrix_tensor_map(&maps[2], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB,
-                                l.rows_b);
-  if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, 32, 1);
+                                l.rows_act);
+  if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, l.rows2, 1);
   if (rc != PKV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == PKV_F16 ? launch<__half>(maps, p, l.few, st) : launch<__nv_bfloat16>(maps, p, l.few, st);

@@ -147,6 +147,13 @@ int make_stack_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_
                      {(cuuint64_t)row, (cuuint64_t)stack, (cuuint64_t)(stacks * stack)}, {64, box_rows, box_stacks, 1});
 }
 
+int make_split_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
+                          uint32_t group, uint32_t box_stacks, uint32_t box_groups) {
+  const uint64_t row = inner * 2;
+  return encode_rows(map, base, dtype, {(cuuint64_t)inner, (cuuint64_t)group, (cuuint64_t)stacks, (cuuint64_t)(rows / group)},
+                     {(cuuint64_t)row, (cuuint64_t)(rows * row), (cuuint64_t)(group * row)}, {64, group, box_stacks, box_groups});
+}
+
 // Blocks, heads and a block's groups of 8 tokens lie one behind the other in the pool: one dimension.
 static int make_pool_group_tensor_map(CUtensorMap* map, const void* base, const pkv_pool& pool) {
   const cuuint64_t d = pool.head_dim, groups = pool.block_size / 8;
