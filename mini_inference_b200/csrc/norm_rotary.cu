@@ -48,108 +48,129 @@ template <typename T, int EW> struct alignas(EW * sizeof(T)) Vec {
   T v[EW];
 };
 
-// The token's slot (-1: none) and its pairs' cos and sin in shared memory, by all threads.
-template <typename T>
-__device__ __forceinline__ int64_t token_angles(const NormRotaryParams& p, int64_t t, float2* cs) {
-  int64_t slot = p.slots ? p.slots[t] : -1;
-  if (slot >= (int64_t)p.nbt * p.bs) {
-    if (threadIdx.x == 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
-    slot = -1;
-  }
-  for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
-    int axis = p.axes ? p.axes[i] : 0;
-    if ((unsigned)axis >= (unsigned)p.num_axes) {
-      report(p.status, PKV_ERR_OUT_OF_RANGE);
-      axis = 0;
-    }
-    const int64_t pos = p.positions[axis * p.pos_stride + t];
-    if (pos < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
-    const double turns = (double)pos * p.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
-    const float r = (float)(turns - rint(turns));                             // [-1/2, 1/2]
-    float s, c;
-    sincospif(2.f * r, &s, &c);
-    cs[i] = make_float2(c * p.factor, s * p.factor);
-  }
-  return slot;
+// A token's slot, or -1: none.
+__device__ __forceinline__ int64_t token_slot(const NormRotaryParams& p, int64_t t) {
+  const int64_t slot = p.slots ? p.slots[t] : -1;
+  if (slot < (int64_t)p.nbt * p.bs) return slot;
+  report(p.status, PKV_ERR_OUT_OF_RANGE);
+  return -1;
 }
 
-// One CTA per token: the pairs' cos and sin once into shared memory, then its heads, each on a
-// group of 2 to 32 lanes that holds it in registers: a lane's unit is 16 elements, two vectors of
-// 8 that rotate together (half a rotation apart, or side by side) or, past the rotated part, two
-// that do not. The group sums the squares by shuffles, so a head is read once and written once.
+// Cos and sin of a token's pair i, times the factor.
+__device__ __forceinline__ float2 pair_angle(const NormRotaryParams& p, int64_t t, int i) {
+  int axis = p.axes ? p.axes[i] : 0;
+  if ((unsigned)axis >= (unsigned)p.num_axes) {
+    report(p.status, PKV_ERR_OUT_OF_RANGE);
+    axis = 0;
+  }
+  const int64_t pos = p.positions[axis * p.pos_stride + t];
+  if (pos < 0) report(p.status, PKV_ERR_OUT_OF_RANGE);
+  const double turns = (double)pos * p.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
+  const float r = (float)(turns - rint(turns));                             // [-1/2, 1/2]
+  float s, c;
+  sincospif(2.f * r, &s, &c);
+  return make_float2(c * p.factor, s * p.factor);
+}
+
+// One CTA per token. A head is held by a group of 2 to 32 lanes: a lane's unit is 16 elements a[8] and
+// b[8], pairs that rotate together (half a rotation apart, or side by side), or past the rotated
+// part two vectors that do not. The group sums the squares by shuffles, so a head is read once and
+// written once. Norm weight, cos, sin and factor are multiplied once per token and pair, into four
+// numbers for q and four for k:
+//   a' = (a A - b B) rs,  b' = (b C + a D) rs,  A = wa cos, B = wb sin, C = wb cos, D = wa sin
+// (A = wa, C = wb, B = D = 0 past the rotated part), so that a head costs three products an element
+// and no weights: the kernel is bound by instructions as much as by bytes. 8192 tokens of 28 / 4 heads
+// of 128 (bf16, three axes, appended) take 31 us = 4.9 TB/s, 0.74 of the copy bandwidth; with weights, cos
+// and sin applied one after another they took 45. Two elements at a time by paired fp32
+// instructions. Four tokens per CTA with their loads ahead of the angles were slower (61-120 us).
 template <typename T, bool INTER, bool NORM>
 __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryParams p) {
-  __shared__ float2 cs[kMaxHalf];
+  __shared__ float4 table[NORM ? 2 : 1][8][32];  // q and k: {A A B B}, {C C D D} of two pairs, by unit
   using V = Vec<T, 8>;
   const int64_t t = blockIdx.x;
-  const int64_t slot = token_angles<T>(p, t, cs);
-  __syncthreads();
-  const T* row = static_cast<const T*>(p.qkv) + t * p.qkv_stride;
   const int heads = p.hq + p.hkv;
+  const T* row = static_cast<const T*>(p.qkv) + t * p.qkv_stride;
+  const int rot_units = p.half / 8, rest = p.d - 2 * p.half;
+  const int64_t slot = token_slot(p, t);
+  // The elements of unit u's pair e.
+  auto first = [&](int u, int e) { return u < rot_units ? INTER ? 16 * u + 2 * e : 8 * u + e : 2 * p.half + 16 * (u - rot_units) + e; };
+  auto second = [&](int u, int e) { return first(u, e) + (u < rot_units ? INTER ? 1 : p.half : 8); };
+  const int units = rot_units + (rest + 15) / 16;
+  for (int i = threadIdx.x; i < 8 * units; i += blockDim.x) {
+    const int u = i >> 3, e = i & 7;
+    const float2 cs = u < rot_units ? pair_angle(p, t, i) : make_float2(1.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < (NORM ? 2 : 1); ++k) {
+      float wa = 1.f, wb = 1.f;
+      if (NORM) {
+        const T* w = static_cast<const T*>(k ? p.k_weight : p.q_weight);
+        const int cb = second(u, e);
+        wa = Dt<T>::to_f(w[first(u, e)]);
+        wb = cb < p.d ? Dt<T>::to_f(w[cb]) : 0.f;
+      }
+      float* ab = reinterpret_cast<float*>(&table[k][e & 6][u]) + (e & 1);
+      float* cd = reinterpret_cast<float*>(&table[k][e | 1][u]) + (e & 1);
+      ab[0] = wa * cs.x, ab[2] = wb * cs.y;
+      cd[0] = wb * cs.x, cd[2] = wa * cs.y;
+    }
+  }
+  __syncthreads();
   const int64_t in_block = slot >= 0 ? ((p.layer_base + slot / p.bs) * p.hkv * p.bs + slot % p.bs) * p.d : 0;
   const int64_t head_step = (int64_t)p.bs * p.d;
 
   const int lanes = 1 << p.lanes_log2, sub = threadIdx.x & (lanes - 1);
   const int groups = blockDim.x >> p.lanes_log2;
-  const int rot_units = p.half / 8, rest = p.d - 2 * p.half;
-  const bool turns = sub < rot_units;
-  const bool has_a = turns || (sub - rot_units) * 16 < rest;
-  const int ca = turns ? (INTER ? 16 * sub : 8 * sub) : 2 * p.half + 16 * (sub - rot_units);
-  const int cb = turns && !INTER ? ca + p.half : ca + 8;
+  const bool has_a = sub < units;
+  const int ca = first(sub, 0);
+  const int cb = INTER && sub < rot_units ? ca + 8 : second(sub, 0);
   const bool has_b = has_a && cb < p.d;
-  const int first = threadIdx.x >> p.lanes_log2;
   for (int h0 = 0; h0 < heads; h0 += groups) {  // the same count for every lane: the shuffles need them all
-    const int head = h0 + first;
+    const int head = h0 + (threadIdx.x >> p.lanes_log2);
     const bool on_a = has_a && head < heads, on_b = has_b && head < heads;
-    float a[8], b[8];
-    V va, vb;
+    uint4 va = make_uint4(0, 0, 0, 0), vb = va;
+    if (on_a) va = *reinterpret_cast<const uint4*>(row + head * p.d + ca);
+    if (on_b) vb = *reinterpret_cast<const uint4*>(row + head * p.d + cb);
+    const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+    float2 a[4], b[4];  // pairs 2 j and 2 j + 1
+    const bool side = INTER && sub < rot_units;  // pair e is word e of the two vectors
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.f;
-    if (on_a) va = *reinterpret_cast<const V*>(row + head * p.d + ca);
-    if (on_b) vb = *reinterpret_cast<const V*>(row + head * p.d + cb);
-    if (on_a) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] = Dt<T>::to_f(va.v[e]);
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = Dt<T>::unpack(INTER && side ? (j < 2 ? wa[(2 * j) & 3] : wb[(2 * j) & 3]) : wa[j]);
+      const float2 y = Dt<T>::unpack(INTER && side ? (j < 2 ? wa[(2 * j + 1) & 3] : wb[(2 * j + 1) & 3]) : wb[j]);
+      a[j] = INTER && side ? make_float2(x.x, y.x) : x;
+      b[j] = INTER && side ? make_float2(x.y, y.y) : y;
     }
-    if (on_b) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = Dt<T>::to_f(vb.v[e]);
-    }
+    float rs = 1.f;
     if constexpr (NORM) {
-      float ss = 0.f;
+      float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
-      for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float rs = rsqrtf(ss / (float)p.d + p.eps);
-      const T* w = static_cast<const T*>(head < p.hq ? p.q_weight : p.k_weight);
-      if (on_a) {
-        const V wa = *reinterpret_cast<const V*>(w + ca);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] *= rs * Dt<T>::to_f(wa.v[e]);
-      }
-      if (on_b) {
-        const V wb = *reinterpret_cast<const V*>(w + cb);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] *= rs * Dt<T>::to_f(wb.v[e]);
-      }
+      for (int j = 0; j < 4; ++j) ss = ffma2(b[j], b[j], ffma2(a[j], a[j], ss));
+      float sum = ss.x + ss.y;
+      for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      rs = rsqrtf(sum / (float)p.d + p.eps);
     }
     if (!on_a) continue;  // the group's own lanes only: shuffles are above
-    if (turns) {
+    const float2 rs2 = make_float2(rs, rs);
+    const int which = NORM && head >= p.hq ? 1 : 0;
+    uint32_t oa[4], ob[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float& x = INTER ? (2 * e < 8 ? a[(2 * e) % 8] : b[(2 * e) % 8]) : a[e];
-        float& y = INTER ? (2 * e + 1 < 8 ? a[(2 * e + 1) % 8] : b[(2 * e + 1) % 8]) : b[e];
-        const float2 w = cs[8 * sub + e];
-        const float fx = x, fy = y;
-        x = fx * w.x - fy * w.y;
-        y = fy * w.x + fx * w.y;
+    for (int j = 0; j < 4; ++j) {
+      const float4 ab = table[which][2 * j][sub], cd = table[which][2 * j + 1][sub];
+      float2 x = ffma2(a[j], make_float2(ab.x, ab.y), fmul2(make_float2(-b[j].x, -b[j].y), make_float2(ab.z, ab.w)));
+      float2 y = INTER ? ffma2(a[j], make_float2(cd.z, cd.w), fmul2(b[j], make_float2(cd.x, cd.y)))
+                       : ffma2(b[j], make_float2(cd.x, cd.y), fmul2(a[j], make_float2(cd.z, cd.w)));
+      if (NORM) x = fmul2(x, rs2), y = fmul2(y, rs2);
+      if (INTER && side) {
+        (j < 2 ? oa : ob)[(2 * j) & 3] = Dt<T>::pack(x.x, y.x);
+        (j < 2 ? oa : ob)[(2 * j + 1) & 3] = Dt<T>::pack(x.y, y.y);
+      } else {
+        oa[j] = Dt<T>::pack(x.x, x.y);
+        ob[j] = Dt<T>::pack(y.x, y.y);
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) va.v[e] = Dt<T>::from_f(a[e]), vb.v[e] = Dt<T>::from_f(b[e]);
     auto put = [&](T* base) {
-      *reinterpret_cast<V*>(base + ca) = va;
-      if (on_b) *reinterpret_cast<V*>(base + cb) = vb;
+      *reinterpret_cast<uint4*>(base + ca) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+      if (on_b) *reinterpret_cast<uint4*>(base + cb) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
     };
     if (head < p.hq) {
       put(static_cast<T*>(p.q_out) + t * p.q_st + head * p.q_sh);
@@ -160,9 +181,8 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryP
     }
   }
   if (p.v_out || slot >= 0) {
-    const int per = 1 << p.v_log2;
     for (int u = threadIdx.x; u < p.hkv << p.v_log2; u += blockDim.x) {
-      const int kh = u >> p.v_log2, c = (u & (per - 1)) * 8;
+      const int kh = u >> p.v_log2, c = (u & ((1 << p.v_log2) - 1)) * 8;
       if (c >= p.d) continue;
       const V x = *reinterpret_cast<const V*>(row + (heads + kh) * p.d + c);
       if (p.v_out) *reinterpret_cast<V*>(static_cast<T*>(p.v_out) + t * p.v_st + kh * p.v_sh + c) = x;
@@ -177,7 +197,8 @@ template <typename T, bool INTER, bool NORM>
 __global__ void __launch_bounds__(kThreads) norm_rotary_any_kernel(const NormRotaryParams p) {
   __shared__ float2 cs[kMaxHalf];
   const int64_t t = blockIdx.x;
-  const int64_t slot = token_angles<T>(p, t, cs);
+  const int64_t slot = token_slot(p, t);
+  for (int i = threadIdx.x; i < p.half; i += blockDim.x) cs[i] = pair_angle(p, t, i);
   __syncthreads();
   const T* row = static_cast<const T*>(p.qkv) + t * p.qkv_stride;
   const int heads = p.hq + p.hkv, lane = threadIdx.x & 31;
@@ -245,7 +266,10 @@ int launch(NormRotaryParams p, int64_t n, bool vec16, bool inter, cudaStream_t s
     return launch_status();
   }
   const int work = ((p.hq + p.hkv) << p.lanes_log2) + (p.v_out || p.slots ? p.hkv << p.v_log2 : 0);
-  const int per = n > 4 * num_sms() ? 4 : 1;
+  // Few tokens: a unit per thread, for latency. More than the SMs hold at once: several units per thread,
+  // so that more tokens are under way. 28 / 4 heads of 128, one, three and five units per thread:
+  // 8192 tokens 57, 35 and 31 us; 1013 tokens of 32 / 8 heads 13, 9.1 and 10.8 us.
+  const int per = n > 16 * num_sms() ? 5 : n > 4 * num_sms() ? 3 : 1;
   const int threads = std::min(kThreads, std::max(64, (work + per * 32 - 1) / (per * 32) * 32));
   auto kernel = norm ? inter ? norm_rotary_kernel<T, true, true> : norm_rotary_kernel<T, false, true>
                      : inter ? norm_rotary_kernel<T, true, false> : norm_rotary_kernel<T, false, false>;
