@@ -296,7 +296,7 @@ class PagedKVCache:
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, block_size: int,
                  max_seqs: int, max_len: int, dtype: torch.dtype, device: torch.device | str,
-                 enable_prefix_caching: bool = False, enable_copy_on_write: bool = False) -> None:
+                 enable_prefix_caching: bool = False, enable_copy_on_write: bool = False, max_media: int = 0) -> None:
         shape = (num_layers, num_blocks + 1, num_kv_heads, block_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
@@ -335,6 +335,11 @@ class PagedKVCache:
             self._edits_sent = torch.cuda.Event()
             self._bm.set_journal(True)
             self._workspaces: dict[tuple[int, int] | str, torch.Tensor] = {}
+            # Images and video of each slot's sequence (set_media), for positions on several axes.
+            self.media_dev = torch.zeros(max_seqs, max_media, 5, dtype=torch.int32, device=self.device)
+            self.media_counts = torch.zeros(max_seqs, dtype=torch.int32, device=self.device)
+        self.max_media = max_media
+        self._media: dict[int, tuple[tuple[int, ...], ...]] = {}
 
     @classmethod
     def for_model(cls, cfg, num_blocks: int, block_size: int, max_seqs: int, max_len: int, dtype: torch.dtype,
@@ -362,7 +367,10 @@ class PagedKVCache:
         return self._bm.can_allocate(num_tokens)
 
     def allocate(self, num_tokens: int = 0, token_ids: Sequence[int] | None = None) -> int:
-        return self._bm.allocate(num_tokens, token_ids)
+        slot = self._bm.allocate(num_tokens, token_ids)
+        if self._media.get(slot):  # an earlier sequence's
+            self.set_media(slot, ())
+        return slot
 
     def register_prefix(self, slot: int, token_ids: Sequence[int]) -> None:
         self._bm.register_prefix(slot, token_ids)
@@ -390,7 +398,47 @@ class PagedKVCache:
         """
         if not self.enable_copy_on_write:
             raise RuntimeError("fork needs a cache built with enable_copy_on_write=True")
-        return self._bm.fork(slot)
+        child = self._bm.fork(slot)
+        if self.max_media:
+            self.set_media(child, self._media.get(slot, ()))
+        return child
+
+    def set_media(self, slot: int, spans: Sequence[Sequence[int]]) -> None:
+        """The images and video of ``slot``'s sequence: ``(start, frames, height, width, step)`` each, in order.
+
+        No counterpart in the reference. Contexts made afterwards place the sequence's tokens on
+        three axes by them (``ops.media_positions``), for models that rotate by several. Needs a
+        cache built with ``max_media``, the most spans of a sequence. They stay until they are set
+        again or the slot is allocated again; slots that the native scheduler hands out are set by
+        the engine at each prefill.
+        """
+        rows, end = tuple(tuple(int(v) for v in s) for s in spans), 0
+        for row in rows:
+            if len(row) != 5:
+                raise ValueError("a span is (start, frames, height, width, step)")
+            start, frames, height, width, step = row
+            if start < end or min(frames, height, width) < 1 or step < 0 or max(row) > 2**31 - 1:
+                raise ValueError("spans are in order and apart, their sizes positive")
+            end = start + frames * height * width
+        if len(rows) > self.max_media:
+            raise ValueError(f"{len(rows)} spans in a cache of at most {self.max_media}")
+        if not 0 <= slot < self.max_seqs:
+            raise KeyError(slot)
+        if rows == self._media.get(slot, ()):
+            return
+        if self.on_gpu:
+            if rows:
+                host = torch.tensor(rows, dtype=torch.int32).pin_memory()
+                self.media_dev[slot, :len(rows)].copy_(host, non_blocking=True)
+            self.media_counts[slot].fill_(len(rows))
+        self._media[slot] = rows
+
+    def axis_positions(self, slots: Sequence[int], positions: torch.Tensor, seq_rows: torch.Tensor,
+                       cu_seqlens: torch.Tensor | None) -> torch.Tensor | None:
+        """``positions`` on three axes (int64 ``[3, N]``), or None where no slot has media: all axes alike."""
+        if not any(self._media.get(s) for s in slots):
+            return None
+        return ops.media_positions(positions, self.media_dev, self.media_counts, seq_rows, cu_seqlens, status=self.status)
 
     def copy_on_write(self, writes: Sequence[tuple[int, int, int]]) -> int:
         """Give every (slot, first position, tokens) about to be written its own copy of any shared block.
@@ -539,6 +587,7 @@ class PagedDecodeContext:
         self.tables = ops.make_tables(cache.tables_dev, self.seq_rows)
         ops.build_decode_metadata(self.tables, self.lengths_in, cache.block_size, cache.scratch_block,
                                   self.positions, self.slot_mapping, self.context_lens, cache.status)
+        self.axis_positions = cache.axis_positions(self.slots, self.positions, self.seq_rows, None)
         self._attends = 0
 
     @property
@@ -585,13 +634,16 @@ class PagedDecodeContext:
         self._attends += 1
         return out.transpose(1, 2)
 
-    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
-        """:meth:`attend_qkv` for the rotary layouts of ``ops.rotary_append``: the rotation, then the append and attention."""
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int,
+                      norm: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
+        """:meth:`attend_qkv` for the rotary layouts of ``ops.Rotary``: the rotation, then the append and attention.
+
+        ``norm`` (q weight, k weight, eps): the heads' norms before it (``ops.norm_rotary_append``).
+        """
         batch = qkv.shape[0]
         rows = qkv.reshape(batch, -1)
-        q, k, v = ops.rotary_append(self.cache.pool, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
-                                    interleaved=rotary.interleaved, attention_factor=rotary.attention_factor, k_out=True,
-                                    v_out=True, status=self.cache.status)
+        q, k, v = rotary.append(self.cache.pool, layer_idx, rows, self.positions, num_q_heads, norm, self.axis_positions,
+                                k_out=True, v_out=True, status=self.cache.status)
         return self.attend(layer_idx, q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
 
     def commit(self) -> None:
@@ -631,6 +683,7 @@ class PackedPrefillContext:
         self.slot_mapping = torch.empty(self.total, dtype=torch.int64, device=dev)
         ops.build_prefill_metadata(self.tables, self.cu_seqlens, self.starts_dev, cache.block_size, self.total,
                                    self.positions, self.slot_mapping, cache.status)
+        self.axis_positions = cache.axis_positions(self.slots, self.positions, self.seq_rows, self.cu_seqlens)
         self.has_prefix = any(self.starts)
         self.last_index = self.cu_seqlens[1:].to(torch.int64) - 1
 
@@ -664,12 +717,12 @@ class PackedPrefillContext:
                               self.max_new, out=out, status=self.cache.status)
         return out.unsqueeze(0).transpose(1, 2)
 
-    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
-        """:meth:`attend_qkv` for the rotary layouts of ``ops.rotary_append`` (appended as it is rotated)."""
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int,
+                      norm: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
+        """:meth:`attend_qkv` for the rotary layouts of ``ops.Rotary`` (appended as it is rotated); ``norm`` as in a decode step."""
         rows = qkv.reshape(-1, qkv.shape[-1])
-        q_rot, _, _ = ops.rotary_append(self.cache.pool, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
-                                        interleaved=rotary.interleaved, attention_factor=rotary.attention_factor,
-                                        slot_mapping=self.slot_mapping, status=self.cache.status)
+        q_rot, _, _ = rotary.append(self.cache.pool, layer_idx, rows, self.positions, num_q_heads, norm, self.axis_positions,
+                                    slot_mapping=self.slot_mapping, status=self.cache.status)
         out = torch.empty(rows.shape[0], num_q_heads, self.cache.head_dim, dtype=qkv.dtype, device=qkv.device)
         ops.prefill_attention(self.cache.pool, layer_idx, self.tables, q_rot, self.cu_seqlens, self.starts_dev,
                               self.max_new, out=out, status=self.cache.status)
@@ -737,6 +790,7 @@ class TreeContext:
         self.mask = torch.empty(self.total, max(1, -(-self.max_nodes // 64)), dtype=torch.int64, device=dev)
         self.positions = torch.empty(self.total, dtype=torch.int64, device=dev)
         ops.build_tree_metadata(self.parents, self.cu_nodes, self.context_lens, self.mask, self.positions, cache.status)
+        self.axis_positions = cache.axis_positions(self.slots, self.positions, self.seq_rows, self.cu_nodes)
         # The nodes' keys and values of every layer, as a pool of one-token blocks: node n is slot n.
         shape = (cache.num_layers, self.total, cache.num_kv_heads, 1, cache.head_dim)
         self.k_nodes = torch.empty(shape, dtype=cache.k.dtype, device=dev)
@@ -766,12 +820,12 @@ class TreeContext:
                                slot_mapping=self.node_slots, status=self.cache.status)
         return self._attention(layer_idx, q)
 
-    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
-        """:meth:`attend_qkv` for the rotary layouts of ``ops.rotary_append``."""
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int,
+                      norm: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
+        """:meth:`attend_qkv` for the rotary layouts of ``ops.Rotary``; ``norm`` as in a decode step."""
         rows = qkv.reshape(-1, qkv.shape[-1])
-        q, _, _ = ops.rotary_append(self.nodes, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
-                                    interleaved=rotary.interleaved, attention_factor=rotary.attention_factor,
-                                    slot_mapping=self.node_slots, status=self.cache.status)
+        q, _, _ = rotary.append(self.nodes, layer_idx, rows, self.positions, num_q_heads, norm, self.axis_positions,
+                                slot_mapping=self.node_slots, status=self.cache.status)
         return self._attention(layer_idx, q)
 
     def accept(self, draft_tokens: torch.Tensor, target_tokens: torch.Tensor) -> list[list[int]]:

@@ -47,12 +47,17 @@ class _GraphDecodeContext:
         self.positions = torch.empty(batch, dtype=torch.int64, device=dev)
         self.slot_mapping = torch.empty(batch, dtype=torch.int64, device=dev)
         self.context_lens = torch.empty(batch, dtype=torch.int32, device=dev)
+        # The three axes' positions, where sequences may hold media (padding rows have none).
+        self.axis_positions = torch.empty(3, batch, dtype=torch.int64, device=dev) if cache.max_media else None
         self._attends = 0
 
     def prepare(self) -> None:
         """Recorded once per step, before the layers: positions, write slots and lengths on the GPU."""
         ops.build_decode_metadata(self.tables, self.lengths_in, self.cache.block_size, self.cache.scratch_block,
                                   self.positions, self.slot_mapping, self.context_lens, self.cache.status)
+        if self.axis_positions is not None:
+            ops.media_positions(self.positions, self.cache.media_dev, self.cache.media_counts, self.seq_rows,
+                                out=self.axis_positions, status=self.cache.status)
         self._attends = 0
 
     def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
@@ -78,12 +83,12 @@ class _GraphDecodeContext:
         self._attends += 1
         return out.transpose(1, 2)
 
-    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int) -> torch.Tensor:
+    def attend_rotary(self, layer_idx: int, qkv: torch.Tensor, rotary: ops.Rotary, num_q_heads: int,
+                      norm: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
         """As ``PagedDecodeContext.attend_rotary``."""
         rows = qkv.reshape(qkv.shape[0], -1)
-        q, k, v = ops.rotary_append(self.cache.pool, layer_idx, rows, self.positions, rotary.inv_freq, num_q_heads,
-                                    interleaved=rotary.interleaved, attention_factor=rotary.attention_factor, k_out=True,
-                                    v_out=True, status=self.cache.status)
+        q, k, v = rotary.append(self.cache.pool, layer_idx, rows, self.positions, num_q_heads, norm, self.axis_positions,
+                                k_out=True, v_out=True, status=self.cache.status)
         return self.attend(layer_idx, q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
 
 

@@ -55,6 +55,31 @@ class SamplingParams:
         return self.temperature == 0
 
 
+@dataclass(frozen=True)
+class Media:
+    """An image (one frame) or video in a prompt: ``frames * height * width`` of its tokens from index ``start`` on.
+
+    No counterpart in the reference. Its tokens are placed on three axes (``ops.media_positions``;
+    ``step`` is how far two frames are apart in time), and ``rows`` ``[frames * height * width,
+    hidden]``, where given, take the place of their embeddings.
+    """
+
+    start: int
+    frames: int
+    height: int
+    width: int
+    step: int = 1
+    rows: torch.Tensor | None = None
+
+    @property
+    def size(self) -> int:
+        return self.frames * self.height * self.width
+
+    @property
+    def span(self) -> tuple[int, int, int, int, int]:
+        return self.start, self.frames, self.height, self.width, self.step
+
+
 @dataclass(eq=False)
 class Sequence:
     """One request moving through the engine (the fields of engine/sequence.py:58-100)."""
@@ -71,6 +96,7 @@ class Sequence:
     finish_time: float | None = None
     num_preemptions: int = 0
     num_cached_tokens: int = 0
+    media: tuple[Media, ...] = ()
 
     @property
     def prompt_len(self) -> int:
@@ -119,6 +145,8 @@ class EngineConfig:
     # to this many tokens drafted by draft_by_lookup, and may emit that many more. The tokens
     # are the model's own greedy choices either way. A step without a draft is a plain one.
     speculative_tokens: int = 0
+    # Images and videos in a request, at most (models that rotate by several position axes).
+    max_media: int = 0
 
     def __post_init__(self) -> None:
         if self.max_num_seqs < 1:
@@ -135,6 +163,10 @@ class EngineConfig:
             raise ValueError("max_num_batched_tokens must be >= max_model_len")
         if not 0 <= self.speculative_tokens <= 63:
             raise ValueError("speculative_tokens must be between 0 and 63")
+        if self.max_media < 0:
+            raise ValueError("max_media must not be negative")
+        if self.max_media and self.enable_prefix_caching:
+            raise ValueError("prefixes are cached by token ids, which do not tell one image from another: no media with them")
         if self.max_num_batched_tokens < 1:
             raise ValueError("max_num_batched_tokens must be at least 1")
         if self.cuda_graph_max_batch is None:
@@ -201,11 +233,16 @@ class ModelRunner:
         return self.head.tokens(hidden_rows)
 
     @torch.inference_mode()
-    def prefill_tokens(self, slots: SequenceOf[int], prompts: SequenceOf[SequenceOf[int]]) -> list[int]:
-        """Prefill several prompts in one pass; the next token of each (engine/engine.py:99-106)."""
+    def prefill_tokens(self, slots: SequenceOf[int], prompts: SequenceOf[SequenceOf[int]],
+                       media: list[tuple[int, torch.Tensor]] | None = None) -> list[int]:
+        """Prefill several prompts in one pass; the next token of each (engine/engine.py:99-106).
+
+        ``media``: rows in the place of embeddings, by packed token (``Qwen2Model.forward``).
+        """
         ctx = self.cache.packed_prefill_context(slots, [len(p) for p in prompts])
         ids = self._ids_to_device([t for p in prompts for t in p]).unsqueeze(0)
-        hidden = self.model(ids, ctx.positions.unsqueeze(0), ctx)
+        positions = ctx.positions.unsqueeze(0)
+        hidden = self.model(ids, positions, ctx, media) if media else self.model(ids, positions, ctx)
         ctx.commit()
         return self._tokens(hidden[0, ctx.last_index])
 
@@ -286,7 +323,7 @@ class LLMEngine:
                                   num_blocks=config.kv_cache_tokens // config.block_size,
                                   block_size=config.block_size, max_seqs=config.max_num_seqs,
                                   max_len=config.max_model_len, dtype=model.dtype, device=model.device,
-                                  enable_prefix_caching=config.enable_prefix_caching)
+                                  enable_prefix_caching=config.enable_prefix_caching, max_media=config.max_media)
         self.runner = ModelRunner(model, self.cache, max_batch=config.max_num_seqs)
         if config.cuda_graphs:
             self.runner.enable_cuda_graphs(min(config.max_num_seqs, config.cuda_graph_max_batch))
@@ -297,19 +334,53 @@ class LLMEngine:
         self._next_id = 0
 
     def add_request(self, prompt: SequenceOf[int], sampling_params: SamplingParams | None = None,
-                    arrival_time: float | None = None) -> int:
-        """Queue a request of token ids; returns its id (engine/engine.py:251-272)."""
+                    arrival_time: float | None = None, media: SequenceOf[Media] = ()) -> int:
+        """Queue a request of token ids; returns its id (engine/engine.py:251-272).
+
+        ``media``: the images and videos among the prompt's tokens, in order; the last token is text.
+        """
         if isinstance(prompt, str):
             raise TypeError("this engine takes token ids; the tokenizer is not part of the paged-KV path")
         sp = sampling_params or SamplingParams()
         if not sp.greedy:
             raise NotImplementedError("only greedy requests are served (the LM head is fused with argmax)")
+        self._check_media(media, len(prompt))
         seq = Sequence(seq_id=self._next_id, prompt_token_ids=list(prompt), sampling=sp,
-                       arrival_time=time.perf_counter() if arrival_time is None else arrival_time)
+                       arrival_time=time.perf_counter() if arrival_time is None else arrival_time, media=tuple(media))
         self.scheduler.add(seq)  # raises if the prompt can never fit
         self.sequences[seq.seq_id] = seq
         self._next_id += 1
         return seq.seq_id
+
+    def _check_media(self, media: SequenceOf[Media], prompt_len: int) -> None:
+        if not media:
+            return
+        if getattr(self.model.cfg, "rope_sections", None) is None:
+            raise ValueError("this model's positions have one axis: it takes no media (rope_sections)")
+        if len(media) > self.config.max_media:
+            raise ValueError(f"{len(media)} images and videos, max_media is {self.config.max_media}")
+        end = 0
+        for m in media:
+            if m.start < end or min(m.frames, m.height, m.width) < 1 or m.step < 0:
+                raise ValueError("media are in order and apart, their sizes positive")
+            end = m.start + m.size
+            if m.rows is not None and tuple(m.rows.shape) != (m.size, self.model.cfg.hidden_size):
+                raise ValueError(f"rows must be [{m.size}, {self.model.cfg.hidden_size}]")
+        if end >= prompt_len:
+            raise ValueError("a prompt ends in text")
+
+    def _media_rows(self, seqs: list[Sequence], starts: list[int], counts: list[int]) -> list[tuple[int, torch.Tensor]]:
+        """What takes the place of embeddings in a pack of tokens ``start .. start + count - 1`` of each sequence."""
+        out: list[tuple[int, torch.Tensor]] = []
+        base = 0
+        for s, start, n in zip(seqs, starts, counts):
+            for m in s.media:
+                a, b = max(start, m.start), min(start + n, m.start + m.size)
+                if m.rows is not None and a < b:
+                    rows = m.rows[a - m.start:b - m.start]
+                    out.append((base + a - start, rows.to(self.model.device, self.model.dtype, non_blocking=True)))
+            base += n
+        return out
 
     def has_unfinished_requests(self) -> bool:
         return self.scheduler.has_work()
@@ -328,7 +399,11 @@ class LLMEngine:
         n_prefill_tokens = sum(counts)
         for group in pack_by_budget(counts, budget):
             seqs = [batch.prefills[i] for i in group]
-            tokens = self.runner.prefill_tokens([s.slot for s in seqs], [news[i] for i in group])
+            if self.config.max_media:
+                for s in seqs:
+                    self.cache.set_media(s.slot, [m.span for m in s.media])
+            rows = self._media_rows(seqs, [starts[i] for i in group], [counts[i] for i in group])
+            tokens = self.runner.prefill_tokens([s.slot for s in seqs], [news[i] for i in group], *([rows] if rows else []))
             for s in seqs:
                 self.cache.register_prefix(s.slot, s.token_ids)
             done = [(s, t) for i, s, t in zip(group, seqs, tokens) if starts[i] + counts[i] == s.num_tokens]
@@ -394,7 +469,12 @@ class LLMEngine:
 
     def check_device_errors(self) -> None:
         """Synchronise and raise any error a kernel recorded (bad index, timed-out wait)."""
-        self.cache.raise_device_errors()
+        try:
+            self.cache.raise_device_errors()
+        except (RuntimeError, IndexError):
+            if hasattr(self.model, "reset_workspaces"):
+                self.model.reset_workspaces()
+            raise
 
     def generate(self, prompts: SequenceOf[SequenceOf[int]],
                  sampling_params: SamplingParams | SequenceOf[SamplingParams] | None = None) -> list[Sequence]:

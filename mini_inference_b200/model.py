@@ -51,6 +51,18 @@ class Qwen2Config:
     rope_scaling: ops.RopeScaling | None = None
     rope_interleaved: bool = False
     rotary_dim: int | None = None
+    # Decoder layers the reference does not have. qk_norm: each q and k head is RMS-normalised before its
+    # rotation. rope_sections: pairs of a head that are turned by each of up to three position axes
+    # (time, height, width; see ops.media_positions), one section after another or in turns. num_experts:
+    # the MLP is a mixture of that many experts of expert_intermediate_size, experts_per_token of them
+    # for each token, weighted by the softmax over the chosen ones (or over all: renormalize_experts=False).
+    qk_norm: bool = False
+    rope_sections: tuple[int, ...] | None = None
+    rope_sections_alternate: bool = False
+    num_experts: int = 0
+    experts_per_token: int = 2
+    expert_intermediate_size: int | None = None
+    renormalize_experts: bool = True
 
     @property
     def q_size(self) -> int:
@@ -88,10 +100,19 @@ def parameter_shapes(cfg: Qwen2Config) -> list[tuple[str, tuple[int, ...]]]:
         out.append((p + "attn.qkv_proj.weight", (q + 2 * kv, h)))
         if cfg.attention_bias:
             out.append((p + "attn.qkv_proj.bias", (q + 2 * kv,)))
+        if cfg.qk_norm:
+            out.append((p + "attn.q_norm.weight", (cfg.head_dim,)))
+            out.append((p + "attn.k_norm.weight", (cfg.head_dim,)))
         out.append((p + "attn.o_proj.weight", (h, q)))
         out.append((p + "post_attn_norm.weight", (h,)))
-        out.append((p + "mlp.gate_up_proj.weight", (2 * inter, h)))
-        out.append((p + "mlp.down_proj.weight", (h, inter)))
+        if cfg.num_experts:
+            e, mid = cfg.num_experts, cfg.expert_intermediate_size or inter
+            out.append((p + "mlp.router.weight", (e, h)))
+            out.append((p + "mlp.experts.gate_up_proj.weight", (e, 2 * mid, h)))
+            out.append((p + "mlp.experts.down_proj.weight", (e, h, mid)))
+        else:
+            out.append((p + "mlp.gate_up_proj.weight", (2 * inter, h)))
+            out.append((p + "mlp.down_proj.weight", (h, inter)))
     out.append(("norm.weight", (h,)))
     if not cfg.tie_word_embeddings:
         out.append(("lm_head.weight", (cfg.vocab_size, h)))
@@ -180,12 +201,26 @@ class Qwen2Model:
         self.device = self.embed.device
         self.lm_head_weight = self.embed if cfg.tie_word_embeddings else weights["lm_head.weight"]
         self.layers = []
+        mlp = "mlp.experts." if cfg.num_experts else "mlp."
+        self.routers: list[torch.Tensor] = []  # with experts: each layer's, its last two weights then being the experts'
+        self.head_norms: list[tuple[torch.Tensor, torch.Tensor, float] | None] = []
         for i in range(cfg.num_layers):
             p = f"layers.{i}."
             self.layers.append((weights[p + "input_norm.weight"], weights[p + "attn.qkv_proj.weight"],
                                 weights.get(p + "attn.qkv_proj.bias"), weights[p + "attn.o_proj.weight"],
-                                weights[p + "post_attn_norm.weight"], weights[p + "mlp.gate_up_proj.weight"],
-                                weights[p + "mlp.down_proj.weight"]))
+                                weights[p + "post_attn_norm.weight"], weights[p + mlp + "gate_up_proj.weight"],
+                                weights[p + mlp + "down_proj.weight"]))
+            if cfg.num_experts:
+                self.routers.append(weights[p + "mlp.router.weight"])
+            self.head_norms.append((weights[p + "attn.q_norm.weight"], weights[p + "attn.k_norm.weight"], cfg.rms_norm_eps)
+                                   if cfg.qk_norm else None)
+        if cfg.num_experts and not 1 <= cfg.experts_per_token <= min(16, cfg.num_experts):
+            raise ValueError(f"experts_per_token {cfg.experts_per_token} of {cfg.num_experts} experts (at most 16)")
+        if cfg.rope_sections is not None and not 1 <= len(cfg.rope_sections) <= 3:
+            raise ValueError("rope_sections are pairs of one to three axes")
+        # One workspace for the experts of all layers, of the largest step so far (zeroed once, reused):
+        # steps of one model must not overlap on the GPU, as with the cache's workspaces.
+        self._expert_workspace: torch.Tensor | None = None
         self.norm = weights["norm.weight"]
         # The reference's RoPE tables (float32, cast to the model dtype per lookup), built once.
         # Other layouts and scaled frequencies go through ops.rotary_append, which makes the
@@ -195,9 +230,11 @@ class Qwen2Model:
         if rotary_dim > cfg.head_dim:
             raise ValueError(f"rotary_dim {rotary_dim} is past head_dim {cfg.head_dim}")
         whole = not cfg.rope_interleaved and rotary_dim == cfg.head_dim
-        if not whole or cfg.rope_scaling is not None:
-            self.rotary = ops.Rotary.build(rotary_dim, cfg.rope_theta, cfg.rope_interleaved, cfg.rope_scaling, self.device)
-        if whole:
+        own = cfg.qk_norm or cfg.rope_sections is not None  # only ops.norm_rotary_append does these
+        if not whole or own or cfg.rope_scaling is not None:
+            self.rotary = ops.Rotary.build(rotary_dim, cfg.rope_theta, cfg.rope_interleaved, cfg.rope_scaling, self.device,
+                                           cfg.rope_sections, cfg.rope_sections_alternate)
+        if whole and not own:
             self.cos, self.sin = ops.rope_tables(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta, self.dtype,
                                                  self.device, cfg.rope_scaling)
 
@@ -209,7 +246,9 @@ class Qwen2Model:
         b, t, _ = x.shape
         qkv = F.linear(x, wqkv, bqkv)
         if self.rotary is not None and (self.cos is None or hasattr(ctx, "attend_rotary")):  # this package's contexts
-            out = ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads)
+            norm = self.head_norms[layer]
+            out = (ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads) if norm is None else
+                   ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads, norm))
         elif hasattr(ctx, "attend_qkv"):
             out = ctx.attend_qkv(layer, qkv, self.cos, self.sin, cfg.num_heads)  # [B, Hq, T, d]
         else:  # engine/model.py:241-250 for a context that only has attend()
@@ -222,27 +261,57 @@ class Qwen2Model:
             out = ctx.attend(layer, q, k, v)
         return F.linear(out.transpose(1, 2).reshape(b, t, cfg.q_size), wo)
 
-    def __call__(self, input_ids: torch.Tensor, positions: torch.Tensor, ctx) -> torch.Tensor:
-        return self.forward(input_ids, positions, ctx)
+    def expert_workspace(self, rows: int) -> torch.Tensor:
+        """The experts' workspace, of at least ``rows`` tokens: a larger one is made outside graph captures only."""
+        cfg, ws = self.cfg, self._expert_workspace
+        args = (cfg.num_experts, cfg.experts_per_token, cfg.hidden_size, cfg.expert_intermediate_size or cfg.intermediate_size)
+        if ws is None or ws.numel() < ops.expert_mlp_workspace_bytes(rows, *args):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"run a step of {rows} tokens before capturing one: the experts' workspace has to grow")
+            ws = self._expert_workspace = ops.expert_mlp_workspace(max(64, 1 << (rows - 1).bit_length()), *args, self.device)
+        return ws
 
-    def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, ctx) -> torch.Tensor:
+    def reset_workspaces(self) -> None:
+        """Ready the workspaces again after a step that reported a timed-out wait."""
+        if self._expert_workspace is not None:
+            self._expert_workspace.zero_()
+
+    def _experts(self, layer: int, x: torch.Tensor, ctx) -> torch.Tensor:
+        cfg = self.cfg
+        cache = getattr(ctx, "cache", None)
+        return ops.expert_mlp(x, self.routers[layer], *self.layers[layer][5:], cfg.experts_per_token,
+                              self.expert_workspace(x.numel() // x.shape[-1]), renormalize=cfg.renormalize_experts,
+                              status=getattr(cache, "status", None))
+
+    def __call__(self, input_ids: torch.Tensor, positions: torch.Tensor, ctx,
+                 media: list[tuple[int, torch.Tensor]] | None = None) -> torch.Tensor:
+        return self.forward(input_ids, positions, ctx, media)
+
+    def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, ctx,
+                media: list[tuple[int, torch.Tensor]] | None = None) -> torch.Tensor:
         """engine/model.py:266-318: ``x = x + attn(norm(x)); x = x + mlp(norm(x))`` per layer, then the norm.
 
         ``h`` is the residual stream ``x``; each block's output ``y`` is added into it by the
         next norm's launch (``ops.add_rms_norm``, the reference's rounding), and the MLP's
         ``silu(gate) * up`` is one launch (``ops.silu_mul``). For decode batches of the 0.5B
         shape ``down_proj`` leaves float32 split-K partials that the next norm sums and rounds
-        (see :func:`_split_k`).
+        (see :func:`_split_k`). ``media``: rows ``[n, hidden]`` that take the place of the
+        embeddings from the packed token ``a`` on, as ``(a, rows)`` pairs.
         """
         eps = self.cfg.rms_norm_eps
         h = F.embedding(input_ids, self.embed)  # a fresh tensor: updated in place below
+        for a, rows in media or ():
+            h.view(-1, h.shape[-1])[a:a + rows.shape[0]] = rows
         y = None
         rows = h.numel() // h.shape[-1]
-        splits = _split_k(rows, self.layers[0][6]) if self.layers else 0
+        splits = _split_k(rows, self.layers[0][6]) if self.layers and not self.routers else 0
         for i, (n1, wqkv, bqkv, wo, n2, wgu, wd) in enumerate(self.layers):
             x = ops.add_rms_norm(h, n1, eps) if y is None else ops.add_rms_norm(y, n1, eps, residual=h)
             y = self._attention(i, x.view_as(h), positions, ctx, wqkv, bqkv, wo)
             x = ops.add_rms_norm(y, n2, eps, residual=h)
+            if self.routers:
+                y = self._experts(i, x, ctx)
+                continue
             act = ops.silu_mul(F.linear(x, wgu))
             # down_proj: float32 split-K partials for decode batches, summed by the next norm
             y = _linear_split_k(act, wd, splits) if splits else F.linear(act, wd)

@@ -525,17 +525,41 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: RopeScaling | Non
 
 @dataclass(frozen=True)
 class Rotary:
-    """What :func:`rotary_append` rotates by: the frequencies, the pairs' layout and the factor on q and k."""
+    """What :func:`rotary_append` rotates by: the frequencies, the pairs' layout and the factor on q and k.
+
+    ``axes`` (:func:`pair_axes`) names each pair's axis where positions have several.
+    """
 
     inv_freq: torch.Tensor
     interleaved: bool = False
     attention_factor: float = 1.0
+    axes: torch.Tensor | None = None
 
     @classmethod
     def build(cls, rotary_dim: int, theta: float, interleaved: bool = False, scaling: RopeScaling | None = None,
-              device: torch.device | str = "cuda") -> "Rotary":
+              device: torch.device | str = "cuda", sections: Sequence[int] | None = None,
+              alternate: bool = False) -> "Rotary":
         freq, factor = rotary_frequencies(rotary_dim, theta, scaling, device)
-        return cls(freq, interleaved, factor)
+        if sections is not None and sum(sections) != rotary_dim // 2:
+            raise ValueError(f"the sections' pairs must be the {rotary_dim // 2} that are rotated, got {tuple(sections)}")
+        return cls(freq, interleaved, factor, None if sections is None else pair_axes(sections, alternate, device))
+
+    def append(self, pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch.Tensor, num_q_heads: int,
+               norm: tuple[torch.Tensor, torch.Tensor, float] | None = None, axis_positions: torch.Tensor | None = None,
+               **kw) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+        """:func:`rotary_append`, or :func:`norm_rotary_append` for ``norm`` (q weight, k weight, eps) or several axes.
+
+        ``axis_positions`` (``[axes, N]``) count where ``axes`` is set; None: every axis is at ``positions``.
+        """
+        kw |= dict(interleaved=self.interleaved, attention_factor=self.attention_factor)
+        several = self.axes is not None and axis_positions is not None
+        if norm is None and not several:
+            return rotary_append(pool, layer, qkv, positions, self.inv_freq, num_q_heads, **kw)
+        if norm is not None:
+            kw |= dict(q_weight=norm[0], k_weight=norm[1], eps=norm[2])
+        if several:
+            kw["axes"] = self.axes
+        return norm_rotary_append(pool, layer, qkv, axis_positions if several else positions, self.inv_freq, num_q_heads, **kw)
 
 
 def rotary_append(pool: PkvPool, layer: int, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -623,6 +647,15 @@ def media_positions(positions: torch.Tensor, media: torch.Tensor, media_counts: 
     return result
 
 
+def expert_mlp_workspace_bytes(max_tokens: int, num_experts: int, top_k: int, hidden: int, intermediate: int) -> int:
+    """Bytes of :func:`expert_mlp_workspace`; sizes that :func:`expert_mlp` does not take raise."""
+    nbytes = int(lib.pkv_expert_mlp_workspace_bytes(max_tokens, num_experts, top_k, hidden, intermediate))
+    if nbytes == 0:
+        raise ValueError("expert_mlp takes 1 to 512 experts, top_k of 1 to 16 of them, and hidden and intermediate sizes "
+                         "that are multiples of 8")
+    return nbytes
+
+
 def expert_mlp_workspace(max_tokens: int, num_experts: int, top_k: int, hidden: int, intermediate: int,
                          device: torch.device | str) -> torch.Tensor:
     """A zeroed workspace for :func:`expert_mlp` of up to ``max_tokens`` tokens (each call leaves it ready).
@@ -630,10 +663,7 @@ def expert_mlp_workspace(max_tokens: int, num_experts: int, top_k: int, hidden: 
     Calls that share one must not overlap on the GPU. After a call whose status reports a timed-out
     wait, zero it.
     """
-    nbytes = int(lib.pkv_expert_mlp_workspace_bytes(max_tokens, num_experts, top_k, hidden, intermediate))
-    if nbytes == 0:
-        raise ValueError("expert_mlp takes 1 to 512 experts, top_k of 1 to 16 of them, and hidden and intermediate sizes "
-                         "that are multiples of 8")
+    nbytes = expert_mlp_workspace_bytes(max_tokens, num_experts, top_k, hidden, intermediate)
     return torch.zeros(nbytes, dtype=torch.uint8, device=device)
 
 
