@@ -256,6 +256,16 @@ __device__ __forceinline__ bool elect_one() {
 // A value that every lane of a converged warp has, for the compiler to keep it in a uniform register.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
+// A counter in shared memory that one thread of the CTA raises and others poll.
+__device__ inline int ld_acquire_cta(const int* ptr) {
+  int v;
+  asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(v) : "r"(smem_u32(ptr)) : "memory");
+  return v;
+}
+__device__ inline void st_release_cta(int* ptr, int v) {
+  asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(ptr)), "r"(v) : "memory");
+}
+
 __device__ inline void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }

@@ -31,7 +31,7 @@ constexpr int kMaxTopK = 16;
 constexpr int kKB = 64;            // K elements of a chunk: one 128-byte swizzled row
 constexpr int kSlotA = 16384;      // weight bytes of a stage: 32, 64 or 128 rows of 4, 2 or 1 chunks
 constexpr int kMaxStages = 16;
-constexpr int kThreads = 256;      // weight copies, token copies, MMA, (idle), 4 epilogue warps
+constexpr int kThreads = 384;      // weight copies, token copies, MMA, finished activations, 8 epilogue warps
 constexpr int kRouterTokens = 8;   // tokens of a router CTA, a warp's choice each
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
 constexpr int kRing = 200 * 1024;  // bytes of the stages
@@ -341,6 +341,7 @@ struct Shared {
   uint64_t freed[kMaxStages];  // its MMAs completed
   uint64_t acc_full[2], acc_empty[2], mma_done;
   uint32_t tmem;
+  int stored[8];                // items of gate and up whose activations each epilogue warp has stored
   int last;
   int offset[kMaxExperts + 1];  // rows of act before each expert's
   int tile[kMaxExperts + 1];    // token tiles before each expert's
@@ -424,7 +425,7 @@ __device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times) {
   __syncthreads();
 }
 
-// out = the sum over each token's experts, in their order, of its products; by the whole grid. Four
+// out = the sum over each token's experts, in their order, of its products; by the whole grid. Eight
 // products' loads go ahead together.
 template <typename T>
 __device__ __forceinline__ void combine(const ExpertParams& p, const float* weight) {
@@ -435,18 +436,18 @@ __device__ __forceinline__ void combine(const ExpertParams& p, const float* weig
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    for (int k0 = 0; k0 < p.top_k; k0 += 4) {
-      float4 v[4][2];
-      float w[4];
+    for (int k0 = 0; k0 < p.top_k; k0 += 8) {
+      float4 v[8][2];
+      float w[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k) {
         const int a = t * p.top_k + min(k0 + k, p.top_k - 1);
         const float4* y = reinterpret_cast<const float4*>(p.y + (int64_t)a * p.hidden + c);
         v[k][0] = __ldcg(y), v[k][1] = __ldcg(y + 1);
         w[k] = weight[a];
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 8; ++k)
         if (k0 + k < p.top_k) {
           sum[0] += w[k] * v[k][0].x, sum[1] += w[k] * v[k][0].y, sum[2] += w[k] * v[k][0].z, sum[3] += w[k] * v[k][0].w;
           sum[4] += w[k] * v[k][1].x, sum[5] += w[k] * v[k][1].y, sum[6] += w[k] * v[k][1].z, sum[7] += w[k] * v[k][1].w;
@@ -488,9 +489,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.acc_full[i], 1);
-      mbar_init(&s.acc_empty[i], 4);
+      mbar_init(&s.acc_empty[i], 8);
     }
     mbar_init(&s.mma_done, 1);
+    for (int i = 0; i < 8; ++i) s.stored[i] = 0;
     fence_mbar_init();
   }
   if (warp == 1) scan_experts(p, s.offset, s.tile);
@@ -622,78 +624,108 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(&s.mma_done);
     }
     __syncwarp();
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- finished activations
+    // A fence takes 8 to 12 thousand cycles behind the weights' stream: the epilogue does not wait for it.
+    int ready = 0;  // items that every epilogue warp has stored, and that the fence covers
+    int n = 0;
+    for (int i = blockIdx.x; ok && find_item(p, s, i, it) && !it.second; i += G, ++n) {
+      if (n >= ready) {
+        for (int k = 1; ok; ++k) {
+          ready = (int)__reduce_min_sync(0xffffffffu, lane < 8 ? (unsigned)ld_acquire_cta(&s.stored[lane]) : 0x7fffffffu);
+          if (ready > n) break;
+          if ((k & 63) == 0) ok = __all_sync(0xffffffffu, global_ns() <= deadline);
+        }
+        if (!ok) break;
+        fence_proxy_async_global();  // the rows are read by bulk copies
+        fence_acq_rel_gpu();
+      }
+      if (lane == 0) atom_add_acq_rel_gpu(&p.done[it.tile], 1);
+    }
+    if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
+    __syncwarp();
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- epilogue
-    const int q = warp - 4;  // TMEM lane quarter
+    // Two warps a lane quarter, each every other 16 columns. A block of columns is read while the last
+    // one is worked on, and the accumulator is given back once the last block has been read.
+    const int q = warp & 3, half = (warp - 4) >> 2;
     const uint32_t tl = tmem + ((uint32_t)(q * 32) << 16);
+    const bool low = lane < 16;
     T* act = static_cast<T*>(p.act);
     int c = 0;
     for (int i = blockIdx.x; find_item(p, s, i, it); i += G, ++c) {
       const int b = c & 1;
+      const bool second = it.second, direct = !second && p.direct;
+      const int n = q * 32 < (second ? p.rows2 : p.rows1) ? it.n : 0;  // columns to finish
+      int list[8];  // the choices of this warp's columns, lane l & 15 of each block
+      if (second || direct) {
+        const int32_t* perm = p.perm + (int64_t)it.e * p.tokens + it.n0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int col = 16 * (2 * j + half) + (lane & 15);
+          list[j] = col < n ? __ldg(&perm[col]) : 0;
+          if (direct) list[j] /= p.top_k;
+        }
+      }
+      // Gate and up: lanes 0 .. 15 hold gate rows, 16 .. 31 the same up rows; of two columns a lane finishes one.
+      const int r = second ? it.row * p.rows2 + q * 32 + lane : it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
+      const bool in = r < (second ? p.hidden : p.inter);
+      T* to_act = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
+      float* to_y = p.y + r;
       // After a wait that ran out the warp goes on to its barriers, without data: the others wait there.
       ok = ok && wait_for(&s.acc_full[b], (c >> 1) & 1, deadline);
       tc_fence_after_sync();
       const uint32_t d = tl + (uint32_t)(b * p.tile_n);
-      if (!it.second) {
-        // Lanes 0..15 hold gate rows, 16..31 the same up rows: of two columns a lane finishes one.
-        const bool low = lane < 16;
-        const int r = it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
-        const bool in = q * 32 < p.rows1 && r < p.inter;
-        T* row = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
-        const bool direct = p.direct;
-        if (q * 32 < p.rows1) {
-          // The column of the tile's token c: itself, or the token's place in x.
-          const int32_t* perm = p.perm + (int64_t)it.e * p.tokens + it.n0;
-          int token = 0;
-          for (int c0 = 0; c0 < it.n; c0 += 16) {
-            uint32_t v[16];
-            if (direct) {
-              if ((c0 & 31) == 0) token = c0 + lane < it.n ? __ldg(&perm[c0 + lane]) / p.top_k : 0;
+      uint32_t v[2][16];
+      auto fetch = [&](int j) {
+        if (direct) {  // the columns of the tokens themselves
 #pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const int at = __shfl_sync(0xffffffffu, token, (c0 & 31) + k);
-                v[k] = tmem_ld1(d + at);
-              }
-            } else {
-              tmem_ld16(d + c0, v);
-            }
-            tmem_wait_ld();
+          for (int k = 0; k < 16; ++k) v[j & 1][k] = tmem_ld1(d + __shfl_sync(0xffffffffu, list[j], k));
+        } else {
+          tmem_ld16(d + 16 * (2 * j + half), v[j & 1]);
+        }
+      };
+      if (16 * half < n) fetch(0);
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, low ? v[k + 1] : v[k], 16));
-              const float g = low ? __uint_as_float(v[k]) : other;
-              const float u = low ? other : __uint_as_float(v[k + 1]);
-              const int col = c0 + k + (low ? 0 : 1);
-              if (in && col < it.n) row[(int64_t)col * p.inter] = Dt<T>::from_f(g / (1.f + __expf(-g)) * u);
-            }
+      for (int j = 0; j < 8; ++j) {
+        const int c0 = 16 * (2 * j + half);
+        if (c0 >= n) break;
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) asm volatile("" : "+r"(v[j & 1][k]));  // read from here on
+        if (j < 7 && c0 + 32 < n) fetch(j + 1);
+        if (j == 7 || c0 + 32 >= n) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+        }
+        if (second) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int at = __shfl_sync(0xffffffffu, list[j], k);
+            if (c0 + k < n && in) to_y[(int64_t)at * p.hidden] = __uint_as_float(v[j & 1][k]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            const uint32_t x = v[j & 1][k], y = v[j & 1][k + 1];
+            const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, low ? y : x, 16));
+            const float g = low ? __uint_as_float(x) : other;
+            const float u = low ? other : __uint_as_float(y);
+            const int col = c0 + k + (low ? 0 : 1);
+            if (in && col < n) to_act[(int64_t)col * p.inter] = Dt<T>::from_f(__fdividef(g, 1.f + __expf(-g)) * u);
           }
         }
-        tc_fence_before_sync();
-        fence_proxy_async_global();  // the rows are read by bulk copies
-        fence_acq_rel_gpu();
-        named_barrier_sync(1, 128);
-        if (warp == 4 && lane == 0) atom_add_acq_rel_gpu(&p.done[it.tile], 1);
-      } else {
-        const int r = it.row * p.rows2 + q * 32 + lane;
-        if (q * 32 < p.rows2) {
-          float* y = p.y + r;
-          const int32_t* perm = p.perm + (int64_t)it.e * p.tokens + it.n0;
-          for (int c0 = 0; c0 < it.n; c0 += 16) {
-            const int a = lane < 16 && c0 + lane < it.n ? __ldg(&perm[c0 + lane]) : 0;
-            uint32_t v[16];
-            tmem_ld16(d + c0, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int at = __shfl_sync(0xffffffffu, a, k);
-              if (c0 + k < it.n && r < p.hidden) y[(int64_t)at * p.hidden] = __uint_as_float(v[k]);
-            }
-          }
-        }
-        tc_fence_before_sync();
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+      if (16 * half >= n) {  // nothing of this tile
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+      }
+      if (!second) {
+        __syncwarp();
+        if (lane == 0) st_release_cta(&s.stored[warp - 4], c + 1);
+      }
     }
     if (!ok && lane == 0) report(p.status, PKV_ERR_TIMEOUT);
   }
@@ -882,16 +914,21 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
   const uint32_t get0 = ring + g * kChunkK * 2 + (((2 * q) ^ g) << 4), get1 = ring + g * kChunkK * 2 + (((2 * q + 1) ^ g) << 4);
   int get_slot = 0;
   float acc[4];
-  auto product = [&](const T* col, int K) {
+  // acc = rows x this lane's token from col on, K of them, and with `left` their second halves that far behind.
+  auto product = [&](const T* col, int64_t left, int K) {
     acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
     for (int c = 0; c < K; c += kChunkK) {
-      uint4 b[4][2];
+      uint4 b[4][2], rest[4][2];
+      auto load = [&](uint4 (&to)[4][2], const T* from) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = c + i * 64 + q * 16;
-        b[i][0] = k < K ? *reinterpret_cast<const uint4*>(col + k) : make_uint4(0, 0, 0, 0);
-        b[i][1] = k + 8 < K ? *reinterpret_cast<const uint4*>(col + k + 8) : make_uint4(0, 0, 0, 0);
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int k = c + i * 64 + q * 16;
+          to[i][0] = k < K ? *reinterpret_cast<const uint4*>(from + k) : make_uint4(0, 0, 0, 0);
+          to[i][1] = k + 8 < K ? *reinterpret_cast<const uint4*>(from + k + 8) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      load(b, col);
+      if (left) load(rest, col + left);
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
       __syncwarp();
 #pragma unroll
@@ -910,6 +947,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
           const uint32_t a1[4] = {a[h].z, a[2 + h].z, a[h].w, a[2 + h].w};
           mma16816<T>(acc, a0, b[i][h].x, b[i][h].y);
           mma16816<T>(acc, a1, b[i][h].z, b[i][h].w);
+          if (left) {
+            mma16816<T>(acc, a0, rest[i][h].x, rest[i][h].y);
+            mma16816<T>(acc, a1, rest[i][h].z, rest[i][h].w);
+          }
         }
       }
       if (++get_slot == kDepth) get_slot = 0;
@@ -918,22 +959,30 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
     }
   };
 
+  // The activations in two halves, the value rounded and what the rounding left: the second costs
+  // products that the weights' stream hides.
   T* act = static_cast<T*>(p.act);
+  const int64_t left = (int64_t)p.tokens * p.top_k * p.inter;
   for (int u = me; u < units1; u += warps) {
     const int group = u / per1, row = u - group * per1, n = s.group_n[group];
     // A column past the group's tokens: its first token again.
-    product(static_cast<const T*>(p.x) + s.group_a[group][g < n ? g : 0] / p.top_k * p.x_stride, p.hidden);
+    product(static_cast<const T*>(p.x) + s.group_a[group][g < n ? g : 0] / p.top_k * p.x_stride, 0, p.hidden);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (2 * q + k < n) {
         const float gate = acc[k], up = acc[2 + k];
-        act[(int64_t)s.group_a[group][2 * q + k] * p.inter + row * 8 + g] = Dt<T>::from_f(gate / (1.f + __expf(-gate)) * up);
+        const float v = __fdividef(gate, 1.f + __expf(-gate)) * up;
+        T* to = act + (int64_t)s.group_a[group][2 * q + k] * p.inter + row * 8 + g;
+        const T high = Dt<T>::from_f(v);
+        const float low = v - Dt<T>::to_f(high);
+        to[0] = high;
+        to[left] = Dt<T>::from_f(fabsf(low) < INFINITY ? low : 0.f);  // an infinity's rest would be NaN
       }
   }
   grid_barrier(p, 2);  // the first of down's rows are on their way meanwhile
   for (int u = me; u < units2; u += warps) {
     const int group = u / per2, row = u - group * per2, n = s.group_n[group];
-    product(act + (int64_t)s.group_a[group][g < n ? g : 0] * p.inter, p.inter);
+    product(act + (int64_t)s.group_a[group][g < n ? g : 0] * p.inter, left, p.inter);
     const int r = row * 16 + g;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -998,7 +1047,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.weight = take(rows * 4);
   l.done = take((int64_t)l.max_tiles * 4);
   l.xs = take(l.direct ? 0 : rows * hidden * 2);
-  l.act = take(rows * inter * 2);
+  l.act = take(rows * inter * (l.few ? 4 : 2));  // few: two halves
   l.y = take(rows * hidden * 4);
   l.bytes = at;
   return l;
