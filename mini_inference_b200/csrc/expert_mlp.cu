@@ -63,6 +63,7 @@ struct ExpertParams {
   int tokens, hidden, inter, experts, top_k, renormalize;
   int max_tiles;    // entries of done
   int rows1, rows2; // weight rows of an item (gate and up; down): 32, 64 or 128
+  int per1, per2;   // items of a tile
   int tile_n;       // tokens of a tile, at most
   int stages, slot_b;
   bool in16;        // intermediate is a multiple of 16
@@ -74,7 +75,7 @@ struct ExpertParams {
 // Where gate and up's tokens come from: up to kDirectTokens are all loaded for every expert, which takes
 // its columns of the accumulator; more are laid out by expert first (gathering four rows a copy cost
 // as much as a copy of 32: 503 of a stage's 830 cycles at 64 tokens of 8 in 64 experts).
-constexpr int kDirectTokens = 64;
+constexpr int kDirectTokens = 128;
 
 // ---------------------------------------------------------------- router
 
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
   __shared__ int s_last;
   const int group = blockIdx.x, t0 = group * kRouterTokens;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, vecs = p.hidden / 8;
+  grid_dep_launch_dependents();  // the next kernel sets itself up, and waits
   // The expert kernel's counters of finished tiles start at zero.
   for (int i = (blockIdx.y * gridDim.x + group) * 256 + tid; i < p.max_tiles; i += 256 * gridDim.x * gridDim.y) p.done[i] = 0;
   for (int e0 = blockIdx.y * EPC; e0 < p.experts; e0 += EPC * gridDim.y) {
@@ -369,6 +371,8 @@ __device__ __forceinline__ void scan_experts(const ExpertParams& p, int* offset,
 // x's rows by expert. A warp copies a row at a time; bound by the rows' bytes.
 __global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
   __shared__ int offset[kMaxExperts + 1], tile[kMaxExperts + 1];
+  grid_dep_launch_dependents();
+  grid_dep_wait();
   if (threadIdx.x < 32) scan_experts(p, offset, tile);
   __syncthreads();
   const int rows = p.tokens * p.top_k, lane = threadIdx.x & 31, vecs = p.hidden / 8;
@@ -386,27 +390,24 @@ __global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
   }
 }
 
-__device__ __forceinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
-  const int per1 = (2 * p.inter + p.rows1 - 1) / p.rows1, per2 = (p.hidden + p.rows2 - 1) / p.rows2;
-  const int tiles = s.tile[p.experts], first = tiles * per1;
+// Item i, by a converged warp; false past the last. Not inlined: the roles share its instructions, which
+// a launch has to fetch anew (they took 6000 cycles before the first copy when each role had its own).
+__device__ __noinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
+  const int lane = threadIdx.x & 31, first = s.tile[p.experts] * p.per1;
   it.second = i >= first;
-  if (!it.second) {
-    it.tile = i / per1, it.row = i - it.tile * per1;
-    it.chunks = (p.hidden + kKB - 1) / kKB;
-  } else {
-    i -= first;
-    if (i >= tiles * per2) return false;
-    it.tile = i / per2, it.row = i - it.tile * per2;
-    it.chunks = (p.inter + kKB - 1) / kKB;
-  }
-  int lo = 0, hi = p.experts - 1;  // the expert whose tiles hold it.tile
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s.tile[mid] <= it.tile) lo = mid; else hi = mid - 1;
-  }
-  it.e = lo;
-  it.n0 = (it.tile - s.tile[lo]) * p.tile_n;
-  it.n = min(p.tile_n, s.offset[lo + 1] - s.offset[lo] - it.n0);
+  const int per = it.second ? p.per2 : p.per1;
+  if (it.second) i -= first;
+  it.tile = i / per, it.row = i - it.tile * per;
+  if (it.second && it.tile >= s.tile[p.experts]) return false;
+  it.chunks = ((it.second ? p.inter : p.hidden) + kKB - 1) / kKB;
+  // The last expert whose tiles start at or before it.tile, among 32 marks and then between two.
+  const int stride = (p.experts + 31) / 32;
+  int at = lane * stride;
+  const int mark = (__popc(__ballot_sync(0xffffffffu, at < p.experts && s.tile[at] <= it.tile)) - 1) * stride;
+  at = mark + lane;
+  it.e = mark + __popc(__ballot_sync(0xffffffffu, lane < stride && at < p.experts && s.tile[at] <= it.tile)) - 1;
+  it.n0 = (it.tile - s.tile[it.e]) * p.tile_n;
+  it.n = min(p.tile_n, s.offset[it.e + 1] - s.offset[it.e] - it.n0);
   return true;
 }
 
@@ -474,7 +475,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     expert_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_gu,
                   const __grid_constant__ CUtensorMap map_act, const __grid_constant__ CUtensorMap map_down,
-                  const ExpertParams p) {
+                  const __grid_constant__ ExpertParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared s;
   uint8_t* ring_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -494,17 +495,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.mma_done, 1);
     for (int i = 0; i < 8; ++i) s.stored[i] = 0;
     fence_mbar_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_gu);
+    prefetch_tensormap(&map_act);
+    prefetch_tensormap(&map_down);
   }
-  if (warp == 1) scan_experts(p, s.offset, s.tile);
   if (warp == 2) {
     tmem_alloc(&s.tmem, p.tmem_cols);
     tc_fence_before_sync();
   }
+  grid_dep_wait();
+  if (warp == 1) scan_experts(p, s.offset, s.tile);
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s.tmem;
   const uint64_t deadline = global_ns() + kWaitBudgetNs;
-  const int per1 = (2 * p.inter + p.rows1 - 1) / p.rows1;
   Item it;
   bool ok = true;
 
@@ -527,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows_b = it.second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
       if (!weights && it.second) {  // the tile's activations
         if (lane == 0)
-          for (int n = 1; ld_acquire_gpu(&p.done[it.tile]) < per1; ++n)
+          for (int n = 1; ld_acquire_gpu(&p.done[it.tile]) < p.per1; ++n)
             if ((n & 63) == 0 && global_ns() > deadline) {
               ok = false;
               break;
@@ -1025,7 +1030,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
     for (int r : {128, 64, 32}) {
       if (r < 128 && l.tile_n > 64) break;  // too many token rows a stage
       const double rounds = (double)((l.max_tiles * ((n + r - 1) / r) + sms - 1) / sms) * r;
-      if (rounds < 0.93 * least) least = rounds, best = r;
+      if (rounds < 0.65 * least) least = rounds, best = r;
     }
     return best;
   };
@@ -1075,12 +1080,15 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaSt
   cfg.gridDim = dim3(num_sms());
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   // Cooperative: the CTAs wait for one another's activations, so they must all be resident.
   at[0].id = cudaLaunchAttributeCooperative;
   at[0].val.cooperative = 1;
+  // The kernel starts up while the one before it ends.
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = few ? 1 : 2;
   if (few) {
     static SmemAttribute attributes[3];
     const int n = p.experts <= 64 ? 0 : p.experts <= 128 ? 1 : 2;
@@ -1095,9 +1103,18 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaSt
   // An expert per CTA for few tokens; four for each load of the tokens when that still fills the SMs.
   if (groups * (int64_t)((p.experts + 3) / 4) < 4 * num_sms()) launch_router<T, 1>(p, groups, st);
   else launch_router<T, 4>(p, groups, st);
-  if (!p.direct) gather_kernel<<<4 * num_sms(), 256, 0, st>>>(p);
   int rc = launch_status();
   if (rc != PKV_OK) return rc;
+  if (!p.direct) {
+    cudaLaunchConfig_t gather = {};
+    gather.gridDim = dim3(4 * num_sms());
+    gather.blockDim = dim3(256);
+    gather.stream = st;
+    gather.attrs = at + 1;
+    gather.numAttrs = 1;
+    rc = cuda_status(cudaLaunchKernelEx(&gather, gather_kernel, p));
+    if (rc != PKV_OK) return rc;
+  }
   static SmemAttribute attribute;
   const int smem = 1024 + p.stages * (kSlotA + p.slot_b);
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(expert_kernel<T>), 1024 + kRing);
@@ -1148,7 +1165,9 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.x_stride = x_stride, p.out_stride = out_stride;
   p.tokens = (int)n_tokens, p.hidden = hidden, p.inter = intermediate, p.experts = num_experts, p.top_k = top_k;
   p.renormalize = renormalize;
-  p.max_tiles = l.max_tiles, p.rows1 = l.rows1, p.rows2 = l.rows2, p.tile_n = l.tile_n;
+  p.max_tiles = l.max_tiles, p.rows1 = l.rows1, p.rows2 = l.rows2;
+  p.per1 = (2 * intermediate + l.rows1 - 1) / l.rows1, p.per2 = (hidden + l.rows2 - 1) / l.rows2;
+  p.tile_n = l.tile_n;
   p.stages = l.stages, p.slot_b = l.slot_b, p.direct = l.direct, p.rows_x = l.rows_x, p.rows_act = l.rows_act;
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
