@@ -32,7 +32,7 @@ constexpr int kKB = 64;            // K elements of a chunk: one 128-byte swizzl
 constexpr int kSlotA = 16384;      // weight bytes of a stage: 32, 64 or 128 rows of 4, 2 or 1 chunks
 constexpr int kMaxStages = 16;
 constexpr int kThreads = 384;      // weight copies, token copies, MMA, finished activations, 8 epilogue warps
-constexpr int kRouterTokens = 8;   // tokens of a router CTA, a warp's choice each
+constexpr int kRouterTokens = 16;  // tokens of a router CTA
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
 constexpr int kRing = 200 * 1024;  // bytes of the stages
 
@@ -226,77 +226,81 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
   weight = on ? expf(mine_v - m) / sum : 0.f;
 }
 
-// A CTA takes kRouterTokens tokens and EPC experts at a time, its threads a part of hidden each, so that
-// every load is one of few a thread waits for; grid y shares out the experts. The last CTA of a group
-// of tokens chooses, a warp for each.
-template <typename T, int EPC, int NV>
-__global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
-  __shared__ double exact[kRouterTokens][32 * NV];
-  __shared__ float part[8][EPC * kRouterTokens];
+// A CTA takes kRouterTokens tokens and 16 MT experts at a time by mma.sync (m16n8k16: 16 experts by 8
+// tokens, the K order free as below), its warps a part of hidden each; grid y shares out the experts.
+// The last CTA of a group of tokens chooses, a warp for a token at a time. 2048 tokens of 2048 in 64
+// experts took 38 us by fp32 products.
+template <typename T, int MT, int NV>
+__global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const ExpertParams p) {
+  constexpr int kWarps = MT == 1 ? 16 : 8, kChoosers = NV > 4 ? 8 : kWarps;
+  constexpr int kSteps = MT == 1 ? 4 : 1;  // of 64 elements, whose loads go ahead together
+  __shared__ union {
+    float part[kWarps][16 * MT][kRouterTokens];
+    double exact[kChoosers][32 * NV];
+  } s;
   __shared__ int s_last;
   const int group = blockIdx.x, t0 = group * kRouterTokens;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, vecs = p.hidden / 8;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   grid_dep_launch_dependents();  // the next kernel sets itself up, and waits
   // The expert kernel's counters of finished tiles start at zero.
-  for (int i = (blockIdx.y * gridDim.x + group) * 256 + tid; i < p.max_tiles; i += 256 * gridDim.x * gridDim.y) p.done[i] = 0;
-  for (int e0 = blockIdx.y * EPC; e0 < p.experts; e0 += EPC * gridDim.y) {
-    float acc[EPC][kRouterTokens];
+  for (int i = (blockIdx.y * gridDim.x + group) * 32 * kWarps + tid; i < p.max_tiles; i += 32 * kWarps * gridDim.x * gridDim.y)
+    p.done[i] = 0;
+  const T* col[2];
 #pragma unroll
-    for (int j = 0; j < EPC; ++j)
+  for (int j = 0; j < 2; ++j) col[j] = static_cast<const T*>(p.x) + min(t0 + 8 * j + g, p.tokens - 1) * p.x_stride;
+  auto load16 = [&](uint4 (&to)[2], const T* from, int k) {  // 16 elements, zeros past hidden
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    to[0] = k < p.hidden ? *reinterpret_cast<const uint4*>(from + k) : zero;
+    to[1] = k + 8 < p.hidden ? *reinterpret_cast<const uint4*>(from + k + 8) : zero;
+  };
+  for (int e0 = blockIdx.y * 16 * MT; e0 < p.experts; e0 += 16 * MT * gridDim.y) {
+    const T* row[MT][2];
+    float acc[MT][2][4];
 #pragma unroll
-      for (int q = 0; q < kRouterTokens; ++q) acc[j][q] = 0.f;
-    for (int c = tid; c < vecs; c += 256) {
-      uint4 ws[EPC], xs[kRouterTokens];
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int j = 0; j < EPC; ++j)
-        ws[j] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)min(e0 + j, p.experts - 1) * p.hidden)[c];
+      for (int h = 0; h < 2; ++h)
+        row[m][h] = static_cast<const T*>(p.router) + (int64_t)min(e0 + 16 * m + 8 * h + g, p.experts - 1) * p.hidden;
 #pragma unroll
-      for (int q = 0; q < kRouterTokens; ++q)
-        xs[q] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + min(t0 + q, p.tokens - 1) * p.x_stride)[c];
-      float w[EPC][8];
+      for (int j = 0; j < 2; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+    }
+    for (int c = warp * 64; c < p.hidden; c += kWarps * 64 * kSteps) {
+      uint4 a[kSteps][MT][2][2], b[kSteps][2][2];
 #pragma unroll
-      for (int j = 0; j < EPC; ++j) unpack8<T>(ws[j], w[j]);
+      for (int n = 0; n < kSteps; ++n) {
+        const int k = c + n * kWarps * 64 + q * 16;
 #pragma unroll
-      for (int q = 0; q < kRouterTokens; ++q) {
-        float a[8];
-        unpack8<T>(xs[q], a);
-#pragma unroll
-        for (int j = 0; j < EPC; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[j][q] += a[i] * w[j][i];
+        for (int m = 0; m < MT; ++m) load16(a[n][m][0], row[m][0], k), load16(a[n][m][1], row[m][1], k);
+        load16(b[n][0], col[0], k), load16(b[n][1], col[1], k);
       }
+#pragma unroll
+      for (int n = 0; n < kSteps; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 &lo = a[n][m][0][h], &hi = a[n][m][1][h];
+            const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              mma16816<T>(acc[m][j], a0, b[n][j][h].x, b[n][j][h].y);
+              mma16816<T>(acc[m][j], a1, b[n][j][h].z, b[n][j][h].w);
+            }
+          }
     }
-    if constexpr (EPC * kRouterTokens == 32) {  // a warp's 32 sums to its 32 lanes, halving what is held each time
-      float v[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = acc[i / kRouterTokens][i % kRouterTokens];
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int o = 16; o; o >>= 1)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < o; ++i) {
-          const bool high = lane & o;
-          const float other = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[i + o], o);
-          v[i] = (high ? v[i + o] : v[i]) + other;
-        }
-      part[warp][lane] = v[0];
-    } else {
-#pragma unroll
-      for (int j = 0; j < EPC; ++j)
-#pragma unroll
-        for (int q = 0; q < kRouterTokens; ++q) {
-          float v = acc[j][q];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (lane == 0) part[warp][j * kRouterTokens + q] = v;
-        }
-    }
+        for (int i = 0; i < 4; ++i) s.part[warp][16 * m + g + 8 * (i >> 1)][8 * j + 2 * q + (i & 1)] = acc[m][j][i];
     __syncthreads();
-    if (tid < EPC * kRouterTokens) {
-      const int e = e0 + tid / kRouterTokens, t = t0 + tid % kRouterTokens;
+    for (int i = tid; i < 16 * MT * kRouterTokens; i += 32 * kWarps) {
+      const int e = i % (16 * MT), t = i / (16 * MT);
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += part[k][tid];
-      if (e < p.experts && t < p.tokens) p.logits[(int64_t)t * p.experts + e] = sum;
+      for (int k = 0; k < kWarps; ++k) sum += s.part[k][e][t];
+      if (e0 + e < p.experts && t0 + t < p.tokens) p.logits[(int64_t)(t0 + t) * p.experts + e0 + e] = sum;
     }
     __syncthreads();
   }
@@ -309,12 +313,12 @@ __global__ void __launch_bounds__(256) router_kernel(const ExpertParams p) {
     __syncthreads();
     if (!s_last) return;
   }
-  if (t0 + warp < p.tokens) {
+  for (int t = t0 + warp; warp < kChoosers && t < min(t0 + kRouterTokens, p.tokens); t += kChoosers) {
     int e;
     float w;
-    choose<T, NV>(p, t0 + warp, exact[warp], e, w);
+    choose<T, NV>(p, t, s.exact[warp], e, w);
     if (lane < p.top_k) {
-      const int a = (t0 + warp) * p.top_k + lane;
+      const int a = t * p.top_k + lane;
       p.weight[a] = w;
       // Places are handed out in no fixed order: a row's products do not depend on its place.
       p.perm[(int64_t)e * p.tokens + atomicAdd(&p.head->counts[e], 1)] = a;
@@ -412,11 +416,11 @@ __device__ __noinline__ bool find_item(const ExpertParams& p, const Shared& s, i
 }
 
 // Every CTA of the grid has come here `times` times; what it wrote before is visible.
-__device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times) {
+__device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times, uint64_t deadline = 0) {
   __syncthreads();
   if (threadIdx.x == 0) {
     atom_add_acq_rel_gpu(&p.head->arrived, 1);
-    const uint64_t end = global_ns() + 2 * kWaitBudgetNs;  // past the waits of every CTA
+    const uint64_t end = max(deadline, (uint64_t)global_ns()) + 2 * kWaitBudgetNs;  // past the waits of every CTA
     for (int n = 1; ld_acquire_gpu(&p.head->arrived) < times * (int)gridDim.x; ++n)
       if ((n & 63) == 0 && global_ns() > end) {
         report(p.status, PKV_ERR_TIMEOUT);
@@ -509,7 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s.tmem;
-  const uint64_t deadline = global_ns() + kWaitBudgetNs;
+  // Past the time that the kernel's own work takes (4 us a chunk and CTA are four times what it does).
+  const int64_t chunks = (int64_t)s.tile[p.experts] * ((int64_t)p.per1 * (p.hidden / kKB + 1) + (int64_t)p.per2 * (p.inter / kKB + 1));
+  const uint64_t deadline = global_ns() + kWaitBudgetNs + (uint64_t)(chunks / G) * 4000;
   Item it;
   bool ok = true;
 
@@ -642,6 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((k & 63) == 0) ok = __all_sync(0xffffffffu, global_ns() <= deadline);
         }
         if (!ok) break;
+        __syncwarp();
         fence_proxy_async_global();  // the rows are read by bulk copies
         fence_acq_rel_gpu();
       }
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, p.tmem_cols);
   }
 
-  grid_barrier(p, 1);
+  grid_barrier(p, 1, deadline);
   combine<T>(p, p.weight);
   leave(p, &s.last);
 }
@@ -1064,14 +1071,14 @@ bool sizes_ok(int64_t tokens, int experts, int top_k, int hidden, int inter) {
          inter <= (1 << 20);
 }
 
-template <typename T, int EPC>
+template <typename T, int MT>
 void launch_router(const ExpertParams& p, int groups, cudaStream_t st) {
   // With more groups than tickets a CTA takes all experts of its group.
-  const int shares = std::min((p.experts + EPC - 1) / EPC, std::max(1, 2 * num_sms() / groups));
-  const dim3 grid(groups, groups <= kMaxTickets ? shares : 1);
-  if (p.experts <= 64) router_kernel<T, EPC, 2><<<grid, 256, 0, st>>>(p);
-  else if (p.experts <= 128) router_kernel<T, EPC, 4><<<grid, 256, 0, st>>>(p);
-  else router_kernel<T, EPC, 16><<<grid, 256, 0, st>>>(p);
+  const dim3 grid(groups, groups <= kMaxTickets ? (p.experts + 16 * MT - 1) / (16 * MT) : 1);
+  const int threads = MT == 1 ? 512 : 256;
+  if (p.experts <= 64) router_kernel<T, MT, 2><<<grid, threads, 0, st>>>(p);
+  else if (p.experts <= 128) router_kernel<T, MT, 4><<<grid, threads, 0, st>>>(p);
+  else router_kernel<T, MT, 16><<<grid, threads, 0, st>>>(p);
 }
 
 template <typename T>
@@ -1100,8 +1107,8 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaSt
     return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
   }
   const int groups = (p.tokens + kRouterTokens - 1) / kRouterTokens;
-  // An expert per CTA for few tokens; four for each load of the tokens when that still fills the SMs.
-  if (groups * (int64_t)((p.experts + 3) / 4) < 4 * num_sms()) launch_router<T, 1>(p, groups, st);
+  // 16 experts per CTA; 64 for each load of the tokens once those fill the SMs.
+  if (groups * (int64_t)((p.experts + 63) / 64) < num_sms() / 2) launch_router<T, 1>(p, groups, st);
   else launch_router<T, 4>(p, groups, st);
   int rc = launch_status();
   if (rc != PKV_OK) return rc;
