@@ -760,7 +760,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // A unit is 16 weight rows by an expert's tokens (the 8 columns of mma.sync m16n8k16), and a warp's own.
 // The warp streams its units' rows through a ring of its own in shared memory by cp.async, kDepth - 1
 // chunks ahead of the products, on from unit to unit and from gate and up to down: no CTA-wide step
-// but the grid's barriers. Rows 0 .. 7 of a unit are gate and 8 .. 15 the same up rows, so that a
+// but the grid's barriers. A chunk has 512 bytes of each row: 256 cost 4 to 25 percent, 128 30 to 70.
+// Teams of two or four warps to a unit, a part of K each, won 6 percent and lost 10 as often. Rows 0 .. 7 of a unit are gate and 8 .. 15 the same up rows, so that a
 // thread holds both. The K order of a product is free: a lane takes 16 consecutive elements of its
 // rows, and of its token.
 constexpr int kFewTokens = 8;
@@ -926,9 +927,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
   const uint32_t get0 = ring + g * kChunkK * 2 + (((2 * q) ^ g) << 4), get1 = ring + g * kChunkK * 2 + (((2 * q + 1) ^ g) << 4);
   int get_slot = 0;
   float acc[4];
-  // acc = rows x this lane's token from col on, K of them, and with `left` their second halves that far behind.
+  // acc = rows x this lane's token from col on, K of them, and with `left` their second halves that far
+  // behind. Four sums side by side: a product that waits for the last one's sum takes its whole latency.
   auto product = [&](const T* col, int64_t left, int K) {
-    acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+    float part[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
     for (int c = 0; c < K; c += kChunkK) {
       uint4 b[4][2], rest[4][2];
       auto load = [&](uint4 (&to)[4][2], const T* from) {
@@ -957,11 +961,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
         for (int h = 0; h < 2; ++h) {
           const uint32_t a0[4] = {a[h].x, a[2 + h].x, a[h].y, a[2 + h].y};
           const uint32_t a1[4] = {a[h].z, a[2 + h].z, a[h].w, a[2 + h].w};
-          mma16816<T>(acc, a0, b[i][h].x, b[i][h].y);
-          mma16816<T>(acc, a1, b[i][h].z, b[i][h].w);
+          mma16816<T>(part[0], a0, b[i][h].x, b[i][h].y);
+          mma16816<T>(part[1], a1, b[i][h].z, b[i][h].w);
           if (left) {
-            mma16816<T>(acc, a0, rest[i][h].x, rest[i][h].y);
-            mma16816<T>(acc, a1, rest[i][h].z, rest[i][h].w);
+            mma16816<T>(part[2], a0, rest[i][h].x, rest[i][h].y);
+            mma16816<T>(part[3], a1, rest[i][h].z, rest[i][h].w);
           }
         }
       }
@@ -969,6 +973,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
       __syncwarp();
       copy();
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
   };
 
   // The activations in two halves, the value rounded and what the rounding left: the second costs
@@ -1022,7 +1028,9 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 // The tiling, from sizes alone, and where each part of the workspace lies.
 Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter, int sms) {
   Layout l = {};
-  l.few = tokens <= kFewTokens;
+  // Few tokens and few weights: the latency of the chain. From some 300 MB of weights on the tcgen05 tiles are
+  // faster (7 tokens of 896, 183 MB at most: 37 us, 42 by tiles; 8 of 2048, 604 MB at most: 85 and 82 us).
+  l.few = tokens <= kFewTokens && std::min<int64_t>(experts, tokens * top_k) * 6 * hidden * inter <= (300ll << 20);
   l.direct = tokens <= kDirectTokens;
   // Twice an expert's share of the tokens, so that few take a second tile; not all slots of a stage's rows
   // for tokens that most experts do not have.
