@@ -19,6 +19,7 @@
 //
 // No counterpart in the reference, whose MLP is dense (engine/model.py:254-264).
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -1025,6 +1026,35 @@ struct Layout {
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// About how long the tiles of `tile_n` tokens take, in cycles, and the weight rows of an item that take least.
+// A stage of 16 KB of weights and its token rows comes at some 52 bytes a cycle from L2 and costs 45 cycles a
+// product at least, an item some 2500 besides; items are dealt out in rounds over the SMs.
+struct Tiling {
+  double cycles;
+  int rows1, rows2;
+};
+Tiling make_tiling(int64_t tokens, int64_t experts, int top_k, int hidden, int inter, int tile_n, bool direct, int sms) {
+  const double rows = (double)tokens * top_k, active = std::min<double>(experts, rows), share = rows / experts;
+  // An expert's tokens are its share, more or less: half of those that nearly fill a tile take another.
+  const double tiles = direct ? active : active * std::max(1.0, share / tile_n + (share > 0.7 * tile_n ? 0.5 : 0.0));
+  auto pick = [&](int64_t n, int k, int columns, int& best) {
+    double least = 1e300;
+    for (int r : {128, 64, 32}) {
+      const int wide = 128 / r;
+      if (tile_n * wide > 272) break;  // at least four stages
+      const double stage = std::max({(kSlotA + 128.0 * columns * wide) / 52, 4.0 * wide * std::max(45.0, columns / 2.0), 500.0});
+      const double item = 2500 + ((k + kKB - 1) / kKB + wide - 1) / wide * stage;
+      const double time = std::ceil(tiles * (double)((n + r - 1) / r) / sms) * item;
+      if (time < 0.95 * least) least = time, best = r;
+    }
+    return least;
+  };
+  Tiling t = {};
+  const int columns = (int)std::min<double>(tile_n, std::max(16.0, share * 1.2));  // of most tiles
+  t.cycles = pick(2 * (int64_t)inter, hidden, direct ? tile_n : columns, t.rows1) + pick(hidden, inter, columns, t.rows2);
+  return t;
+}
+
 // The tiling, from sizes alone, and where each part of the workspace lies.
 Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter, int sms) {
   Layout l = {};
@@ -1032,25 +1062,23 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   // faster (7 tokens of 896, 183 MB at most: 37 us, 42 by tiles; 8 of 2048, 604 MB at most: 85 and 82 us).
   l.few = tokens <= kFewTokens && std::min<int64_t>(experts, tokens * top_k) * 6 * hidden * inter <= (300ll << 20);
   l.direct = tokens <= kDirectTokens;
-  // Twice an expert's share of the tokens, so that few take a second tile; not all slots of a stage's rows
-  // for tokens that most experts do not have.
-  l.tile_n = (int)(l.few ? 16 : l.direct ? up(tokens, 16)
-                   : std::min<int64_t>(std::min<int64_t>(256, up(tokens, 16)), std::max<int64_t>(32, up(2 * tokens * top_k / experts, 32))));
   const int64_t rows = tokens * top_k;
-  l.max_tiles = (int)(std::min<int64_t>(experts, rows) + rows / l.tile_n);
-  // Weight rows of an item: the size whose dealing out over the SMs leaves the least idle.
-  auto pick = [&](int64_t n) {
-    int best = 128;
-    double least = 1e300;
-    for (int r : {128, 64, 32}) {
-      if (r < 128 && l.tile_n > 64) break;  // too many token rows a stage
-      const double rounds = (double)((l.max_tiles * ((n + r - 1) / r) + sms - 1) / sms) * r;
-      if (rounds < 0.65 * least) least = rounds, best = r;
+  Tiling best = {1e300, 128, 128};
+  if (l.few) {
+    l.tile_n = 16;
+  } else if (l.direct) {  // a tile per expert
+    l.tile_n = (int)up(tokens, 16);
+    best = make_tiling(tokens, experts, top_k, hidden, inter, l.tile_n, true, sms);
+  } else {
+    const double share = (double)rows / experts, most = share + 3 * std::sqrt(share);  // of nearly every expert
+    for (int n : {32, 64, 96, 128, 192, 256}) {  // small ones leave the ring more stages
+      if (n >= share && n < most && most <= 256) continue;  // some would spill over into a tile of their own
+      const Tiling t = make_tiling(tokens, experts, top_k, hidden, inter, n, false, sms);
+      if (t.cycles < 0.98 * best.cycles) best = t, l.tile_n = n;
     }
-    return best;
-  };
-  l.rows1 = pick(2 * (int64_t)inter);
-  l.rows2 = pick(hidden);
+  }
+  l.rows1 = best.rows1, l.rows2 = best.rows2;
+  l.max_tiles = (int)(std::min<int64_t>(experts, rows) + (l.direct ? 0 : rows / l.tile_n));
   l.rows_act = l.tile_n <= 64 ? 16 : 32;
   l.rows_x = l.direct ? l.tile_n : l.rows_act;
   // A stage's token rows, of as many chunks as its weights have.
@@ -1065,7 +1093,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.logits = take(tokens * experts * 4);
   l.perm = take(tokens * experts * 4);
   l.weight = take(rows * 4);
-  l.done = take((int64_t)l.max_tiles * 4);
+  l.done = take((std::min<int64_t>(experts, rows) + rows / 32) * 4);  // of the smallest tiles
   l.xs = take(l.direct ? 0 : rows * hidden * 2);
   l.act = take(rows * inter * (l.few ? 4 : 2));  // few: two halves
   l.y = take(rows * hidden * 4);
@@ -1146,7 +1174,11 @@ using namespace pkv;
 extern "C" int64_t pkv_expert_mlp_workspace_bytes(int64_t n_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
                                                   int32_t intermediate) {
   if (!sizes_ok(n_tokens, num_experts, top_k, hidden, intermediate)) return 0;
-  return make_layout(n_tokens, num_experts, top_k, hidden, intermediate, 148).bytes;
+  // What holds n_tokens holds every smaller call: the layouts change at a few tokens.
+  int64_t most = 0;
+  for (int64_t t : {(int64_t)1, (int64_t)2, (int64_t)3, (int64_t)4, (int64_t)5, (int64_t)6, (int64_t)7, (int64_t)8, (int64_t)kDirectTokens, n_tokens})
+    most = std::max(most, make_layout(std::min(t, n_tokens), num_experts, top_k, hidden, intermediate, 148).bytes);
+  return most;
 }
 
 extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, int64_t n_tokens, int32_t hidden,
