@@ -477,8 +477,8 @@ PKV_API int pkv_media_positions(const int64_t* positions, int64_t n_tokens, cons
  *   out = sum_k w_k * down[e_k] . (silu(gate[e_k] . x) * (up[e_k] . x)),
  * with w the softmax of the chosen logits (renormalize != 0) or their part of the softmax over all.
  * Products, weights and sums are float32; the activations between the two products are rounded to
- * dtype once, and so is out. The choice is that of exact logits: where float32 sums leave it open,
- * the logits beside the border are computed in float64.
+ * dtype once, and so is out. Logits are float32 sums; those within 2^-17 of the largest's size of the
+ * border between chosen and not are computed in float64, and the choice among them is by these.
  *   x       : [n_tokens, hidden], token t at x + t * x_stride (16-byte aligned, a multiple of 8)
  *   router  : [num_experts, hidden]
  *   gate_up : [num_experts, 2 * intermediate, hidden], an expert's gate rows before its up rows
@@ -488,7 +488,8 @@ PKV_API int pkv_media_positions(const int64_t* positions, int64_t n_tokens, cons
  *             before first use; every call leaves it ready for the next, whatever its sizes. Calls that
  *             share a workspace must not overlap on the GPU. After a call that reported a timed-out
  *             wait, zero it.
- * hidden and intermediate are multiples of 8; num_experts <= 512, top_k <= 16.
+ * hidden and intermediate are multiples of 8; num_experts <= 512, top_k <= 16. Needs an sm_100 GPU whose SMs
+ * are all free to the process (a cooperative launch of one CTA per SM).
  */
 PKV_API int64_t pkv_expert_mlp_workspace_bytes(int64_t n_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
                                                int32_t intermediate);

@@ -1,21 +1,29 @@
-// A mixture-of-experts MLP, router included, in two launches:
+// A mixture-of-experts MLP, router included:
 //   out = sum_k w_k * down[e_k] . (silu(gate[e_k] . x) * (up[e_k] . x))
 // over the top_k experts e_k with the largest logits router . x, w their softmax.
 //
 // Few tokens are bound by the touched experts' weights (6 hidden intermediate bytes each, read
-// once); many by the products. Both run as the same tiles: the weights are the 128-row operand A
-// of tcgen05.mma (M), an expert's tokens operand B (N, 16 to 256 of them), so that the few tokens
-// of a decode step cost no more than their share of the tensor core's columns.
+// once) and by the chain from the logits to the sum; many by the products.
 //
+// Up to 8 tokens of few weights: one launch, expert_few_kernel below. Else two or three:
 // 1. router_kernel: logits in float32, the choice of experts (exact, see choose()), each choice
 //    noted in its expert's list.
 // 2. (past kDirectTokens) gather_kernel: each expert's token rows one behind the other.
-// 3. expert_kernel: a persistent cooperative grid, one CTA per SM. Its items are first every
-//    (expert, token tile, weight rows) of gate and up, then every one of down, dealt out in
-//    turn. The rings of weight and token stages run on from item to item and from the first
+// 3. expert_kernel: the weights are the 128-row operand A of tcgen05.mma (M), an expert's tokens
+//    operand B (N, 16 to 256 of them), so that a decode step's few tokens cost no more than their share
+//    of the tensor core's columns. A persistent cooperative grid, one CTA per SM; its items are
+//    first every (expert, token tile, weight rows) of gate and up, then every one of down, dealt out
+//    in turn. The rings of weight and token stages run on from item to item and from the first
 //    product to the second: the weights of down stream in while the activations are still being
 //    made, and only the tokens' side waits for them (a counter per token tile). Then the
 //    weighted sum over each token's experts, in their order.
+// On one B200: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 140 us =
+// 5.8 TB/s, 0.88 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 130 us = 5.5 TB/s;
+// 2048 tokens of 2048 through 8 of 64 experts of 768 310-340 us = 0.50 PFLOP/s, bound by what L2
+// gives the SMs (a stage's 48 KB in some 1000 cycles, the products take 512) and by the 134 MB of
+// float32 products written and read back; 333 tokens of 896 through 4 of 60 experts of 616 66 us and one
+// token of 2048 through 8 of 64 of 768 27 us, bound by the chain: launches and cold instructions 5 us,
+// logits and choice 4-8, first data 4, the wait between the products 3, the last sums 3.
 //
 // No counterpart in the reference, whose MLP is dense (engine/model.py:254-264).
 #include <algorithm>
@@ -32,6 +40,7 @@ constexpr int kMaxTopK = 16;
 constexpr int kKB = 64;            // K elements of a chunk: one 128-byte swizzled row
 constexpr int kSlotA = 16384;      // weight bytes of a stage: 32, 64 or 128 rows of 4, 2 or 1 chunks
 constexpr int kMaxStages = 16;
+constexpr int64_t kMaxItems = 1 << 30;
 constexpr int kThreads = 384;      // weight copies, token copies, MMA, finished activations, 8 epilogue warps
 constexpr int kRouterTokens = 16;  // tokens of a router CTA
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
@@ -55,7 +64,7 @@ struct ExpertParams {
   int32_t* perm;    // [experts][tokens]: an expert's choices, token * top_k + k each
   float* weight;    // [tokens][top_k]
   int32_t* done;    // [token tiles]: row tiles of gate and up that are finished
-  void* xs;         // [tokens * top_k][hidden], past 256 tokens: x by expert
+  void* xs;         // [tokens * top_k][hidden], past kDirectTokens: x by expert
   void* act;        // [tokens * top_k][inter], an expert's rows one behind the other
   float* y;         // [tokens * top_k][hidden]
   void* out;
@@ -762,9 +771,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // The warp streams its units' rows through a ring of its own in shared memory by cp.async, kDepth - 1
 // chunks ahead of the products, on from unit to unit and from gate and up to down: no CTA-wide step
 // but the grid's barriers. A chunk has 512 bytes of each row: 256 cost 4 to 25 percent, 128 30 to 70.
-// Teams of two or four warps to a unit, a part of K each, won 6 percent and lost 10 as often. Rows 0 .. 7 of a unit are gate and 8 .. 15 the same up rows, so that a
-// thread holds both. The K order of a product is free: a lane takes 16 consecutive elements of its
-// rows, and of its token.
+// Teams of two or four warps to a unit, a part of K each, won 6 percent and lost 10 as often. Rows
+// 0 .. 7 of a unit are gate and 8 .. 15 the same up rows, so that a thread holds both. The K order of a
+// product is free: a lane takes 16 consecutive elements of its rows, and of its token.
 constexpr int kFewTokens = 8;
 constexpr int kFewChoices = kFewTokens * kMaxTopK;
 constexpr int kFewThreads = 256;
@@ -1101,6 +1110,12 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   return l;
 }
 
+// Items are counted in 32 bits.
+bool items_ok(const Layout& l, int hidden, int inter) {
+  const int64_t per = (2 * (int64_t)inter + l.rows1 - 1) / l.rows1 + ((int64_t)hidden + l.rows2 - 1) / l.rows2;
+  return l.max_tiles * per <= kMaxItems;
+}
+
 bool sizes_ok(int64_t tokens, int experts, int top_k, int hidden, int inter) {
   return tokens >= 0 && experts > 0 && experts <= kMaxExperts && top_k > 0 && top_k <= kMaxTopK && top_k <= experts &&
          hidden > 0 && inter > 0 && hidden % 8 == 0 && inter % 8 == 0 && tokens <= (1 << 24) && hidden <= (1 << 20) &&
@@ -1174,6 +1189,7 @@ using namespace pkv;
 extern "C" int64_t pkv_expert_mlp_workspace_bytes(int64_t n_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
                                                   int32_t intermediate) {
   if (!sizes_ok(n_tokens, num_experts, top_k, hidden, intermediate)) return 0;
+  if (!items_ok(make_layout(n_tokens, num_experts, top_k, hidden, intermediate, 148), hidden, intermediate)) return 0;
   // What holds n_tokens holds every smaller call: the layouts change at a few tokens.
   int64_t most = 0;
   for (int64_t t : {(int64_t)1, (int64_t)2, (int64_t)3, (int64_t)4, (int64_t)5, (int64_t)6, (int64_t)7, (int64_t)8, (int64_t)kDirectTokens, n_tokens})
@@ -1197,6 +1213,7 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   if (((bits(x) | bits(router) | bits(gate_up) | bits(down) | bits(out)) & 15) || (bits(workspace) & 255))
     return PKV_ERR_INVALID_ARGUMENT;
   const Layout l = make_layout(n_tokens, num_experts, top_k, hidden, intermediate, 148);
+  if (!items_ok(l, hidden, intermediate)) return PKV_ERR_UNSUPPORTED;
   if (workspace_bytes < l.bytes) return PKV_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   ExpertParams p = {};

@@ -219,8 +219,9 @@ class Qwen2Model:
         if cfg.rope_sections is not None and not 1 <= len(cfg.rope_sections) <= 3:
             raise ValueError("rope_sections are pairs of one to three axes")
         # One workspace for the experts of all layers, of the largest step so far (zeroed once, reused):
-        # steps of one model must not overlap on the GPU, as with the cache's workspaces.
-        self._expert_workspace: torch.Tensor | None = None
+        # steps of one model must not overlap on the GPU, as with the cache's workspaces. Smaller ones
+        # stay: captured steps hold their addresses.
+        self._expert_workspaces: list[torch.Tensor] = []
         self.norm = weights["norm.weight"]
         # The reference's RoPE tables (float32, cast to the model dtype per lookup), built once.
         # Other layouts and scaled frequencies go through ops.rotary_append, which makes the
@@ -246,6 +247,8 @@ class Qwen2Model:
         b, t, _ = x.shape
         qkv = F.linear(x, wqkv, bqkv)
         if self.rotary is not None and (self.cos is None or hasattr(ctx, "attend_rotary")):  # this package's contexts
+            if not hasattr(ctx, "attend_rotary"):
+                raise TypeError("this model's rotation and norms need a context of this package (attend_rotary)")
             norm = self.head_norms[layer]
             out = (ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads) if norm is None else
                    ctx.attend_rotary(layer, qkv, self.rotary, cfg.num_heads, norm))
@@ -263,18 +266,19 @@ class Qwen2Model:
 
     def expert_workspace(self, rows: int) -> torch.Tensor:
         """The experts' workspace, of at least ``rows`` tokens: a larger one is made outside graph captures only."""
-        cfg, ws = self.cfg, self._expert_workspace
+        cfg, ws = self.cfg, self._expert_workspaces[-1] if self._expert_workspaces else None
         args = (cfg.num_experts, cfg.experts_per_token, cfg.hidden_size, cfg.expert_intermediate_size or cfg.intermediate_size)
         if ws is None or ws.numel() < ops.expert_mlp_workspace_bytes(rows, *args):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"run a step of {rows} tokens before capturing one: the experts' workspace has to grow")
-            ws = self._expert_workspace = ops.expert_mlp_workspace(max(64, 1 << (rows - 1).bit_length()), *args, self.device)
+            ws = ops.expert_mlp_workspace(max(64, 1 << (rows - 1).bit_length()), *args, self.device)
+            self._expert_workspaces.append(ws)
         return ws
 
     def reset_workspaces(self) -> None:
         """Ready the workspaces again after a step that reported a timed-out wait."""
-        if self._expert_workspace is not None:
-            self._expert_workspace.zero_()
+        for ws in self._expert_workspaces:
+            ws.zero_()
 
     def _experts(self, layer: int, x: torch.Tensor, ctx) -> torch.Tensor:
         cfg = self.cfg

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mini_inference_b200 import ops
+from mini_inference_b200 import PkvError, ops
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -86,6 +86,7 @@ def test_few_tokens(dtype, tokens, hidden, inter, experts, top_k):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", [
+    (20, 8, 16, 5, 2), (9, 64, 8, 3, 1), (128, 512, 104, 7, 3), (129, 512, 112, 7, 3), (200, 40, 24, 2, 2), (300, 8, 8, 9, 9),
     (256, 512, 256, 4, 1), (257, 512, 264, 4, 4), (333, 896, 616, 60, 4), (1025, 256, 200, 3, 2), (2048, 1024, 384, 128, 8),
 ])
 def test_many_tokens(dtype, tokens, hidden, inter, experts, top_k):
@@ -107,9 +108,10 @@ def test_all_tokens_to_one_expert():
     check(x, router, gate_up, down, 1)
 
 
-def test_equal_logits_go_to_the_first():
+@pytest.mark.parametrize("tokens", [5, 40, 150])
+def test_equal_logits_go_to_the_first(tokens):
     """Twin experts and tokens of zeros: the lowest indexes are taken."""
-    x, router, gate_up, down = make(torch.float16, 40, 128, 64, 12)
+    x, router, gate_up, down = make(torch.float16, tokens, 128, 64, 12)
     x[::3] = 0
     router[7] = router[2]
     router[11] = router[2]
@@ -132,15 +134,16 @@ def test_near_ties_are_decided_by_exact_logits():
     check(x, router, gate_up, down, 4)
 
 
-def test_one_tokens_nan_and_infinity_stay_its_own():
-    x, router, gate_up, down = make(torch.float16, 40, 256, 128, 8)
+@pytest.mark.parametrize("tokens", [8, 40, 150])
+def test_one_tokens_nan_and_infinity_stay_its_own(tokens):
+    x, router, gate_up, down = make(torch.float16, tokens, 256, 128, 8)
     clean = check(x, router, gate_up, down, 2)
     bad = x.clone()
     bad[3, 5] = float("nan")
-    bad[20, 7] = float("inf")
-    ws = ops.expert_mlp_workspace(40, 8, 2, 256, 128, "cuda")
+    bad[6, 7] = float("inf")
+    ws = ops.expert_mlp_workspace(tokens, 8, 2, 256, 128, "cuda")
     got = ops.expert_mlp(bad, router, gate_up, down, 2, ws)
-    keep = [i for i in range(40) if i not in (3, 20)]
+    keep = [i for i in range(tokens) if i not in (3, 6)]
     assert torch.equal(got[keep], clean[keep])
     assert got[3].isnan().all()
 
@@ -174,9 +177,24 @@ def test_a_workspace_serves_calls_of_every_size():
     assert torch.equal(check(*big, 4, workspace=ws), first)
 
 
-def test_captured_and_replayed_on_other_inputs():
-    x, router, gate_up, down = make(torch.bfloat16, 32, 512, 256, 16)
-    ws = ops.expert_mlp_workspace(32, 16, 4, 512, 256, "cuda")
+def test_values_past_float16_overflow_as_they_are_rounded():
+    """Activations past the type's range are infinite, as silu(gate) * up is when it is rounded; nothing else is."""
+    x, router, gate_up, down = make(torch.float16, 6, 64, 32, 4)
+    gate_up[:, 0] = 60  # gate row 0 and up row 0 of every expert: about 60 |x| each, their product far past 65504
+    gate_up[:, 32] = 60
+    x = x.abs() * 4
+    for t in (1, 6):
+        ws = ops.expert_mlp_workspace(t, 4, 2, 64, 32, "cuda")
+        got = ops.expert_mlp(x[:t], router, gate_up, down, 2, ws)
+        assert not got.isfinite().any()
+    down[:, :, 0] = 0  # infinity times nothing
+    assert ops.expert_mlp(x, router, gate_up, down, 2, ws).isnan().all()
+
+
+@pytest.mark.parametrize("tokens", [6, 32, 200])
+def test_captured_and_replayed_on_other_inputs(tokens):
+    x, router, gate_up, down = make(torch.bfloat16, tokens, 512, 256, 16)
+    ws = ops.expert_mlp_workspace(tokens, 16, 4, 512, 256, "cuda")
     out = torch.empty_like(x)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -186,9 +204,9 @@ def test_captured_and_replayed_on_other_inputs():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         ops.expert_mlp(x, router, gate_up, down, 4, ws, out=out)
-        ops.expert_mlp(out, router, gate_up, down, 4, ws, out=out.clone())
+        ops.expert_mlp(out, router, gate_up, down, 4, ws)
     for seed in (1, 2, 3):
-        x.copy_(make(torch.bfloat16, 32, 512, 256, 16, seed=seed)[0])
+        x.copy_(make(torch.bfloat16, tokens, 512, 256, 16, seed=seed)[0])
         graph.replay()
         assert torch.equal(out, check(x, router, gate_up, down, 4))
 
@@ -209,3 +227,23 @@ def test_two_calls_at_once_on_two_streams():
             got[1].append(ops.expert_mlp(*b, 2, ws_b))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want_a) for g in got[0]) and all(torch.equal(g, want_b) for g in got[1])
+
+
+def test_refusals():
+    x, router, gate_up, down = make(torch.float16, 12, 128, 64, 4)
+    ws = ops.expert_mlp_workspace(12, 4, 2, 128, 64, "cuda")
+    ok = dict(x=x, router=router, gate_up=gate_up, down=down, top_k=2, workspace=ws)
+    for kw in (dict(router=router[:, :64].contiguous()), dict(router=router.float()), dict(gate_up=gate_up[:, :64].contiguous()),
+               dict(down=down[:2].contiguous()), dict(down=down.transpose(1, 2)), dict(x=x.bfloat16()), dict(workspace=ws.cpu()),
+               dict(out=torch.empty(12, 64, dtype=x.dtype, device="cuda")), dict(out=torch.empty(128, 12, dtype=x.dtype, device="cuda").T),
+               dict(workspace=ws.view(-1, 2)[:, 0]), dict(router=router.cpu())):
+        with pytest.raises(ValueError):
+            ops.expert_mlp(**{**ok, **kw})
+    with pytest.raises(NotImplementedError):
+        ops.expert_mlp(**{**ok, "x": x.float()})
+    for kw in (dict(top_k=5), dict(top_k=0), dict(workspace=ws[:-256])):
+        with pytest.raises(PkvError):
+            ops.expert_mlp(**{**ok, **kw})
+    odd = make(torch.float16, 4, 100, 64, 4)
+    with pytest.raises(PkvError):
+        ops.expert_mlp(*odd, 2, ws)

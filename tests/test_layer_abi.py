@@ -64,6 +64,8 @@ def test_expert_mlp():
     assert call(out=None) == BAD and call(ws=None) == BAD and call(n=-1) == BAD and call(top_k=9) == BAD and call(top_k=0) == BAD
     assert call(xs=120) == BAD and call(xs=130) == BAD and call(os=127) == BAD and call(x=FAKE + 8) == BAD
     assert call(gu=FAKE + 2) == BAD and call(ws=FAKE + 128) == BAD and call(hidden=0) == BAD and call(experts=-1) == BAD
+    assert call(n=1 << 24, hidden=1 << 20, xs=1 << 20, os=1 << 20, inter=1 << 20, nbytes=1 << 62) == UNSUPPORTED
+    assert L.pkv_expert_mlp_workspace_bytes(1 << 24, 8, 2, 1 << 20, 1 << 20) == 0
     assert call(dtype=5) == UNSUPPORTED and call(hidden=124) == UNSUPPORTED and call(inter=60) == UNSUPPORTED
     assert call(experts=600) == UNSUPPORTED and call(experts=64, top_k=17) == UNSUPPORTED
     assert call(nbytes=need - 1) == WORKSPACE and call(n=0, x=None, out=None) == OK

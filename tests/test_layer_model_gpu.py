@@ -259,3 +259,28 @@ def test_an_experts_step_too_large_for_its_workspace_is_not_captured():
         with torch.cuda.graph(graph):
             x.add_(1)
             model.expert_workspace(5000)
+
+
+@torch.inference_mode()
+def test_a_captured_step_keeps_its_workspace():
+    """A larger step takes a larger workspace; the captured one's stays where its graph writes."""
+    model = make_model()
+    cache = new_cache(model)
+    engine_like = [cache.allocate(40), cache.allocate(40)]
+    ids = torch.tensor(ids_of(2, 3), device="cuda")
+    from mini_inference_b200.cuda_graphs import GraphedDecoder
+    graphs = GraphedDecoder(model, cache, 2)
+    graphs.capture()
+    first = model._expert_workspaces[-1]
+    model.expert_workspace(5000)
+    assert model._expert_workspaces[-1] is not first and model._expert_workspaces[0] is first
+    model._expert_workspaces[-1].fill_(0)
+    for s in engine_like:
+        cache.lengths[s] = 0
+    logits = graphs.decode(engine_like, ids.tolist())
+    for s in engine_like:
+        cache.lengths[s] = 0
+    ctx = cache.decode_context(engine_like)
+    want = model.compute_logits(model(ids[:, None], ctx.positions[:, None], ctx)[:, -1]).float()
+    assert torch.equal(logits, want)
+    assert not first[:6200].any()
