@@ -420,8 +420,11 @@ __device__ __noinline__ bool find_item(const ExpertParams& p, const Shared& s, i
   const int mark = (__popc(__ballot_sync(0xffffffffu, at < p.experts && s.tile[at] <= it.tile)) - 1) * stride;
   at = mark + lane;
   it.e = mark + __popc(__ballot_sync(0xffffffffu, lane < stride && at < p.experts && s.tile[at] <= it.tile)) - 1;
-  it.n0 = (it.tile - s.tile[it.e]) * p.tile_n;
-  it.n = min(p.tile_n, s.offset[it.e + 1] - s.offset[it.e] - it.n0);
+  // An expert's tiles are alike: one full and one of a few tokens would take SMs unequal times.
+  const int count = s.offset[it.e + 1] - s.offset[it.e], tiles = s.tile[it.e + 1] - s.tile[it.e];
+  const int size = ((count + tiles - 1) / tiles + 15) & ~15;  // at most tile_n, a multiple of 16: no tile is empty
+  it.n0 = (it.tile - s.tile[it.e]) * size;
+  it.n = min(size, count - it.n0);
   return true;
 }
 
