@@ -327,15 +327,23 @@ __global__ void __launch_bounds__(kThreads) media_positions_kernel(const MediaPa
       break;
     }
     if (start > at) break;
-    const int64_t plane = height * width;
-    const int64_t r = at - start;
-    if (r / plane < frames) {
-      const int64_t f = r / plane, in = r - f * plane, y = in / width;
-      x0 = start - lag + f * step, x1 = start - lag + y, x2 = start - lag + (in - y * width);
+    const int64_t plane = height * width, r = at - start;
+    // In 64 bits only planes and spans past 32: a division of 64 bits is some hundred instructions.
+    const bool small = plane <= 0x7fffffff;
+    const int64_t size = small ? frames * plane : r / plane < frames ? r + 1 : frames * plane;  // past r is enough
+    if (r < size) {
+      int64_t f, y, x;
+      if (small && size <= 0xffffffffll) {
+        const uint32_t in = (uint32_t)r % (uint32_t)plane;
+        f = (uint32_t)r / (uint32_t)plane, y = in / (uint32_t)width, x = in % (uint32_t)width;
+      } else {
+        const int64_t in = r % plane;
+        f = r / plane, y = in / width, x = in % width;
+      }
+      x0 = start - lag + f * step, x1 = start - lag + y, x2 = start - lag + x;
       inside = true;
       break;
     }
-    const int64_t size = frames * plane;  // at most r: no overflow
     end = start + size;
     lag += size - max(max((frames - 1) * step + 1, height), width);
   }
