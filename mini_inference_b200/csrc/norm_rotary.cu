@@ -289,63 +289,100 @@ struct MediaParams {
   int num_seqs, rows, max_spans;
 };
 
-// A thread per token: its sequence by bisection, then its sequence's spans one after another up to
-// the token (a warp's tokens mostly read the same ones). 32 bytes a token; bound by latency.
+constexpr int kStaged = 1024;  // sequences whose starts fit the CTA's shared memory
+
+// A thread per token: its sequence by bisection, then its sequence's spans one after another up to the
+// token (a warp's tokens mostly read the same ones). 32 bytes a token; bound by the chain of loads, so
+// the sequences' starts come in one round, a thread's first four spans with their count, and each
+// further four before the last are worked on: 64 sequences of
+// one token 3.9 -> 3.4 us captured, 32 K packed tokens of up to 12 spans 5.1 -> 4.9.
 __global__ void __launch_bounds__(kThreads) media_positions_kernel(const MediaParams p) {
+  __shared__ int32_t starts[kStaged + 1];
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= p.n) return;
+  const bool token = t < p.n;
+  const int64_t at = token ? p.positions[t] : 0;
   int seq = (int)t;
   if (p.cu) {
+    const int32_t* cu = p.cu;
+    if (p.num_seqs <= kStaged) {
+      for (int i = threadIdx.x; i <= p.num_seqs; i += blockDim.x) starts[i] = p.cu[i];
+      __syncthreads();
+      cu = starts;
+    }
     int lo = 0, hi = p.num_seqs;  // the last sequence that starts at or before t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (p.cu[mid] <= t) lo = mid; else hi = mid - 1;
+      if (cu[mid] <= t) lo = mid; else hi = mid - 1;
     }
-    if (lo >= p.num_seqs || t < p.cu[lo]) return;
+    if (lo >= p.num_seqs || t < cu[lo]) return;
     seq = lo;
   }
-  const int64_t at = p.positions[t];
+  if (!token) return;
   const int row = p.seq_rows ? p.seq_rows[seq] : seq;
+  if (row >= p.rows) report(p.status, PKV_ERR_OUT_OF_RANGE);
+  const bool any = row >= 0 && row < p.rows && p.max_spans > 0;
+  const int32_t* m = p.media + (any ? (int64_t)row * p.max_spans * 5 : 0);
+  int32_t next[4][5];
+  auto fetch = [&](int j0) {  // spans j0 .. j0 + 3, within the row
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) next[j][k] = j0 + j < p.max_spans ? m[(j0 + j) * 5 + k] : 0;
+  };
   int spans = 0;
-  if (row >= p.rows) {
-    report(p.status, PKV_ERR_OUT_OF_RANGE);
-  } else if (row >= 0) {
+  if (any) {
     spans = p.counts[row];
+    fetch(0);
     if (spans < 0 || spans > p.max_spans) {
       report(p.status, PKV_ERR_OUT_OF_RANGE);
       spans = 0;
     }
+  } else if (row >= 0 && row < p.rows && p.counts[row] != 0) {
+    report(p.status, PKV_ERR_OUT_OF_RANGE);
   }
-  const int32_t* m = p.media + (int64_t)max(row, 0) * p.max_spans * 5;
   int64_t lag = 0, end = 0;  // how far positions are behind indexes; the last span's end
   int64_t x0 = at, x1 = at, x2 = at;
-  bool inside = false;
-  for (int j = 0; j < spans; ++j, m += 5) {
-    const int64_t start = m[0], frames = m[1], height = m[2], width = m[3], step = m[4];
-    if (start < end || frames < 1 || height < 1 || width < 1 || step < 0) {
-      report(p.status, PKV_ERR_OUT_OF_RANGE);
-      break;
-    }
-    if (start > at) break;
-    const int64_t plane = height * width, r = at - start;
-    // In 64 bits only planes and spans past 32: a division of 64 bits is some hundred instructions.
-    const bool small = plane <= 0x7fffffff;
-    const int64_t size = small ? frames * plane : r / plane < frames ? r + 1 : frames * plane;  // past r is enough
-    if (r < size) {
-      int64_t f, y, x;
-      if (small && size <= 0xffffffffll) {
-        const uint32_t in = (uint32_t)r % (uint32_t)plane;
-        f = (uint32_t)r / (uint32_t)plane, y = in / (uint32_t)width, x = in % (uint32_t)width;
-      } else {
-        const int64_t in = r % plane;
-        f = r / plane, y = in / width, x = in % width;
+  bool inside = false, more = true;
+  for (int j0 = 0; j0 < spans && more; j0 += 4) {
+    int32_t now[4][5];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) now[j][k] = next[j][k];
+    if (j0 + 4 < spans) fetch(j0 + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!more || j0 + j >= spans) continue;
+      const int64_t start = now[j][0], frames = now[j][1], height = now[j][2], width = now[j][3], step = now[j][4];
+      if (start < end || frames < 1 || height < 1 || width < 1 || step < 0) {
+        report(p.status, PKV_ERR_OUT_OF_RANGE);
+        more = false;
+        continue;
       }
-      x0 = start - lag + f * step, x1 = start - lag + y, x2 = start - lag + x;
-      inside = true;
-      break;
+      if (start > at) {
+        more = false;
+        continue;
+      }
+      const int64_t plane = height * width, r = at - start;
+      // In 64 bits only planes and spans past 32: a division of 64 bits is some hundred instructions.
+      const bool small = plane <= 0x7fffffff;
+      const int64_t size = small ? frames * plane : r / plane < frames ? r + 1 : frames * plane;  // past r is enough
+      if (r < size) {
+        int64_t f, y, x;
+        if (small && size <= 0xffffffffll) {
+          const uint32_t in = (uint32_t)r % (uint32_t)plane;
+          f = (uint32_t)r / (uint32_t)plane, y = in / (uint32_t)width, x = in % (uint32_t)width;
+        } else {
+          const int64_t in = r % plane;
+          f = r / plane, y = in / width, x = in % width;
+        }
+        x0 = start - lag + f * step, x1 = start - lag + y, x2 = start - lag + x;
+        inside = true, more = false;
+        continue;
+      }
+      end = start + size;
+      lag += size - max(max((frames - 1) * step + 1, height), width);
     }
-    end = start + size;
-    lag += size - max(max((frames - 1) * step + 1, height), width);
   }
   if (!inside) x0 = x1 = x2 = at - lag;
   p.out[t] = x0;
