@@ -294,8 +294,8 @@ constexpr int kStaged = 1024;  // sequences whose starts fit the CTA's shared me
 // A thread per token: its sequence by bisection, then its sequence's spans one after another up to the
 // token (a warp's tokens mostly read the same ones). 32 bytes a token; bound by the chain of loads, so
 // the sequences' starts come in one round, a thread's first four spans with their count, and each
-// further four before the last are worked on: 64 sequences of
-// one token 3.9 -> 3.4 us captured, 32 K packed tokens of up to 12 spans 5.1 -> 4.9.
+// further four before the last are worked on (one after another by dependent loads: 64
+// sequences of one token 3.9 us captured, now 3.4; 32 K packed tokens of up to 12 spans 5.1, now 4.9).
 __global__ void __launch_bounds__(kThreads) media_positions_kernel(const MediaParams p) {
   __shared__ int32_t starts[kStaged + 1];
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -454,6 +454,7 @@ extern "C" int pkv_media_positions(const int64_t* positions, int64_t n_tokens, c
                                    const int32_t* media_counts, int32_t rows, int32_t max_spans, int64_t* out,
                                    int64_t out_stride, int32_t* status_dev, pkv_stream_t stream) {
   if (n_tokens < 0 || n_tokens > 0x7fffffff || num_seqs < 0 || rows < 0 || max_spans < 0) return PKV_ERR_INVALID_ARGUMENT;
+  if (max_spans > 0x7fffffff / 5 - 4) return PKV_ERR_UNSUPPORTED;  // a row's numbers are counted in 32 bits
   if (!cu_seqlens && n_tokens != num_seqs) return PKV_ERR_INVALID_ARGUMENT;
   if (n_tokens == 0) return PKV_OK;
   if (!positions || !out || out_stride < n_tokens) return PKV_ERR_INVALID_ARGUMENT;
