@@ -443,33 +443,43 @@ __device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times, u
   __syncthreads();
 }
 
+// 32 bytes in one load: by two of 16 a warp would ask L2 for every 32-byte sector twice.
+__device__ __forceinline__ void load8(float (&v)[8], const float* from) {
+  asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(from)
+               : "memory");
+}
+
 // out = the sum over each token's experts, in their order, of its products; by the whole grid. Eight
 // products' loads go ahead together.
 template <typename T>
 __device__ __forceinline__ void combine(const ExpertParams& p, const float* weight) {
   const int per_row = p.hidden / 8;
-  const int64_t units = (int64_t)p.tokens * per_row;
-  for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (int64_t)gridDim.x * blockDim.x) {
-    const int t = (int)(u / per_row), c = (int)(u - (int64_t)t * per_row) * 8;
+  const uint32_t at = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
+  const int step_t = step / per_row, step_c = step % per_row;
+  for (int t = at / per_row, u = at % per_row; t < p.tokens; t += step_t, u += step_c) {
+    if (u >= per_row) {
+      u -= per_row;
+      if (++t >= p.tokens) break;
+    }
+    const int c = u * 8;
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
     for (int k0 = 0; k0 < p.top_k; k0 += 8) {
-      float4 v[8][2];
-      float w[8];
+      float v[8][8], w[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int a = t * p.top_k + min(k0 + k, p.top_k - 1);
-        const float4* y = reinterpret_cast<const float4*>(p.y + (int64_t)a * p.hidden + c);
-        v[k][0] = __ldcg(y), v[k][1] = __ldcg(y + 1);
+        load8(v[k], p.y + (int64_t)a * p.hidden + c);
         w[k] = weight[a];
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (k0 + k < p.top_k) {
-          sum[0] += w[k] * v[k][0].x, sum[1] += w[k] * v[k][0].y, sum[2] += w[k] * v[k][0].z, sum[3] += w[k] * v[k][0].w;
-          sum[4] += w[k] * v[k][1].x, sum[5] += w[k] * v[k][1].y, sum[6] += w[k] * v[k][1].z, sum[7] += w[k] * v[k][1].w;
-        }
+        if (k0 + k < p.top_k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] += w[k] * v[k][e];
     }
     uint4 o;
     o.x = Dt<T>::pack(sum[0], sum[1]), o.y = Dt<T>::pack(sum[2], sum[3]);
