@@ -96,6 +96,19 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryP
   auto first = [&](int u, int e) { return u < rot_units ? INTER ? 16 * u + 2 * e : 8 * u + e : 2 * p.half + 16 * (u - rot_units) + e; };
   auto second = [&](int u, int e) { return first(u, e) + (u < rot_units ? INTER ? 1 : p.half : 8); };
   const int units = rot_units + (rest + 15) / 16;
+  const int lanes = 1 << p.lanes_log2, sub = threadIdx.x & (lanes - 1);
+  const int groups = blockDim.x >> p.lanes_log2;
+  const bool has_a = sub < units;
+  const int ca = first(sub, 0);
+  const int cb = INTER && sub < rot_units ? ca + 8 : second(sub, 0);
+  const bool has_b = has_a && cb < p.d;
+  // A group's next head is loaded ahead, the first before the angles.
+  uint4 next_a = make_uint4(0, 0, 0, 0), next_b = next_a;
+  auto load = [&](int head) {
+    if (has_a && head < heads) next_a = *reinterpret_cast<const uint4*>(row + head * p.d + ca);
+    if (has_b && head < heads) next_b = *reinterpret_cast<const uint4*>(row + head * p.d + cb);
+  };
+  load(threadIdx.x >> p.lanes_log2);
   for (int i = threadIdx.x; i < 8 * units; i += blockDim.x) {
     const int u = i >> 3, e = i & 7;
     const float2 cs = u < rot_units ? pair_angle(p, t, i) : make_float2(1.f, 0.f);
@@ -118,18 +131,11 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryP
   const int64_t in_block = slot >= 0 ? ((p.layer_base + slot / p.bs) * p.hkv * p.bs + slot % p.bs) * p.d : 0;
   const int64_t head_step = (int64_t)p.bs * p.d;
 
-  const int lanes = 1 << p.lanes_log2, sub = threadIdx.x & (lanes - 1);
-  const int groups = blockDim.x >> p.lanes_log2;
-  const bool has_a = sub < units;
-  const int ca = first(sub, 0);
-  const int cb = INTER && sub < rot_units ? ca + 8 : second(sub, 0);
-  const bool has_b = has_a && cb < p.d;
   for (int h0 = 0; h0 < heads; h0 += groups) {  // the same count for every lane: the shuffles need them all
     const int head = h0 + (threadIdx.x >> p.lanes_log2);
     const bool on_a = has_a && head < heads, on_b = has_b && head < heads;
-    uint4 va = make_uint4(0, 0, 0, 0), vb = va;
-    if (on_a) va = *reinterpret_cast<const uint4*>(row + head * p.d + ca);
-    if (on_b) vb = *reinterpret_cast<const uint4*>(row + head * p.d + cb);
+    const uint4 va = next_a, vb = next_b;
+    load(head + groups);
     const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
     float2 a[4], b[4];  // pairs 2 j and 2 j + 1
     const bool side = INTER && sub < rot_units;  // pair e is word e of the two vectors
