@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int r = second ? it.row * p.rows2 + q * 32 + lane : it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
       const bool in = r < (second ? p.hidden : p.inter);
       T* to_act = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
-      float* to_y = p.y + r;
+      float* to_y = p.y + r - (lane & 3);  // the first of four rows: hidden is a multiple of 8
       // After a wait that ran out the warp goes on to its barriers, without data: the others wait there.
       ok = ok && wait_for(&s.acc_full[b], (c >> 1) & 1, deadline);
       tc_fence_after_sync();
@@ -737,9 +737,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (second) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int at = __shfl_sync(0xffffffffu, list[j], k);
-            if (c0 + k < n && in) to_y[(int64_t)at * p.hidden] = __uint_as_float(v[j & 1][k]);
+          for (int k = 0; k < 16; k += 4) {  // four rows of four columns turned about: 16 bytes of one column a lane
+            uint32_t* x = &v[j & 1][k];
+#pragma unroll
+            for (int h = 0; h < 4; h += 2) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x[h] : x[h + 1], 1);
+              x[h] = lane & 1 ? other : x[h], x[h + 1] = lane & 1 ? x[h + 1] : other;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 2 ? x[h] : x[h + 2], 2);
+              x[h] = lane & 2 ? other : x[h], x[h + 2] = lane & 2 ? x[h + 2] : other;
+            }
+            const int at = __shfl_sync(0xffffffffu, list[j], k + (lane & 3));
+            if (c0 + k + (lane & 3) < n && in)
+              *reinterpret_cast<uint4*>(to_y + (int64_t)at * p.hidden) = make_uint4(x[0], x[1], x[2], x[3]);
           }
         } else {
 #pragma unroll

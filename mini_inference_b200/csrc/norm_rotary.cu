@@ -80,9 +80,10 @@ __device__ __forceinline__ float2 pair_angle(const NormRotaryParams& p, int64_t 
 //   a' = (a A - b B) rs,  b' = (b C + a D) rs,  A = wa cos, B = wb sin, C = wb cos, D = wa sin
 // (A = wa, C = wb, B = D = 0 past the rotated part), so that a head costs three products an element
 // and no weights: the kernel is bound by instructions as much as by bytes. 8192 tokens of 28 / 4 heads
-// of 128 (bf16, three axes, appended) take 31 us = 4.9 TB/s, 0.74 of the copy bandwidth; with weights, cos
-// and sin applied one after another they took 45. Two elements at a time by paired fp32
-// instructions. Four tokens per CTA with their loads ahead of the angles were slower (61-120 us).
+// of 128 (bf16, three axes, appended) take 30 us = 5.0 TB/s, 0.77 of the copy bandwidth; with weights,
+// cos and sin applied one after another they took 45, with each head's load in its own turn 33. Two
+// elements at a time by paired fp32 instructions. Four tokens per CTA with their loads ahead of the
+// angles were slower (61-120 us).
 template <typename T, bool INTER, bool NORM>
 __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryParams p) {
   __shared__ float4 table[NORM ? 2 : 1][8][32];  // q and k: {A A B B}, {C C D D} of two pairs, by unit
@@ -274,7 +275,7 @@ int launch(NormRotaryParams p, int64_t n, bool vec16, bool inter, cudaStream_t s
   const int work = ((p.hq + p.hkv) << p.lanes_log2) + (p.v_out || p.slots ? p.hkv << p.v_log2 : 0);
   // Few tokens: a unit per thread, for latency. More than the SMs hold at once: several units per thread,
   // so that more tokens are under way. 28 / 4 heads of 128, one, three and five units per thread:
-  // 8192 tokens 57, 35 and 31 us; 1013 tokens of 32 / 8 heads 13, 9.1 and 10.8 us.
+  // 8192 tokens 45, 33 and 30 us; 1013 tokens of 32 / 8 heads 8.0, 6.0 and 6.5 us.
   const int per = n > 16 * num_sms() ? 5 : n > 4 * num_sms() ? 3 : 1;
   const int threads = std::min(kThreads, std::max(64, (work + per * 32 - 1) / (per * 32) * 32));
   auto kernel = norm ? inter ? norm_rotary_kernel<T, true, true> : norm_rotary_kernel<T, false, true>
