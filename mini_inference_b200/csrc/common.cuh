@@ -253,8 +253,9 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
   return yes != 0;
 }
-// A value that every lane of a converged warp has, for the compiler to keep it in a uniform register.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// A value that every lane of a converged warp has, for the compiler to keep it in a uniform register
+// (where a reduction's result is; a shuffle's is not).
+__device__ __forceinline__ int uniform(int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); }
 
 // A counter in shared memory that one thread of the CTA raises and others poll.
 __device__ inline int ld_acquire_cta(const int* ptr) {

@@ -345,6 +345,13 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_
   return true;
 }
 
+// The same by a converged warp, in a loop that is one way for all of it.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint64_t deadline) {
+  for (int i = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++i)
+    if ((i & 63) == 0 && __any_sync(0xffffffffu, global_ns() > deadline)) return false;
+  return true;
+}
+
 struct Item {
   bool second;            // down; else gate and up
   int tile, e, n0, n;     // token tile, its expert, its first and number of tokens
@@ -502,12 +509,13 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     expert_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_gu,
                   const __grid_constant__ CUtensorMap map_act, const __grid_constant__ CUtensorMap map_down,
+                  const __grid_constant__ CUtensorMap map_x128, const __grid_constant__ CUtensorMap map_act128,
                   const __grid_constant__ ExpertParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared s;
   uint8_t* ring_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring_b = ring_a + p.stages * kSlotA;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int G = gridDim.x;
 
   if (tid == 0) {
@@ -553,29 +561,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool leader = elect_one();
     int issued = 0, slot = 0;
     uint32_t round = 0;  // of the ring
-    for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G) {
-      const int e = uniform(it.e), rows = it.second ? p.rows2 : p.rows1, wide = 128 / rows;
+    for (int i = blockIdx.x; ok && __all_sync(0xffffffffu, find_item(p, s, i, it)); i += G) {
+      const bool second = uniform(it.second);
+      const int e = uniform(it.e), rows = second ? p.rows2 : p.rows1, wide = 128 / rows;
       const int k1 = uniform(it.chunks), pad = uniform((it.n + 15) & ~15);
-      const int row = uniform(it.row) * (it.second ? p.rows2 : p.rows1 / 2), box = it.second ? p.rows2 : 32;
-      const bool direct = !it.second && p.direct;
+      const int row = uniform(it.row) * (second ? p.rows2 : p.rows1 / 2), box = second ? p.rows2 : 32;
+      const bool direct = !second && p.direct;
       const int first = direct ? 0 : uniform(s.offset[it.e] + it.n0), columns = direct ? p.tile_n : pad;
-      const int rows_b = it.second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
-      if (!weights && it.second) {  // the tile's activations
+      const int rows_b = second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
+      if (!weights && second) {  // the tile's activations
         if (lane == 0)
           for (int n = 1; ld_acquire_gpu(&p.done[it.tile]) < p.per1; ++n)
             if ((n & 63) == 0 && global_ns() > deadline) {
               ok = false;
               break;
             }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_proxy_async_global();
       }
-      const CUtensorMap* map_w = it.second ? &map_down : &map_gu;
-      const CUtensorMap* map_b = it.second ? &map_act : &map_x;
-      const int stack = it.second ? e : 2 * e;
+      const CUtensorMap* map_w = second ? &map_down : &map_gu;
+      const CUtensorMap* map_b = second ? &map_act : &map_x;
+      const CUtensorMap* map_b128 = second ? &map_act128 : &map_x128;
+      const int stack = second ? e : 2 * e;
       for (int ks = 0; ks < k1; ks += wide) {
-        if (round > 0 && !__all_sync(0xffffffffu, wait_for(&s.freed[slot], (round - 1) & 1, deadline))) {
+        if (round > 0 && !wait_warp(&s.freed[slot], (round - 1) & 1, deadline)) {
           ok = false;
           break;
         }
@@ -585,10 +595,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* dst = ring_a + slot * kSlotA;
           if (leader) mbar_arrive_expect_tx(bar, chunks * rows * 128);
           for (int c = 0; c < chunks; ++c, dst += rows * 128) {
-            if (it.second || !p.in16) {
+            if (second || !p.in16) {
               for (int b = 0; b < rows; b += box)
                 if (leader)
-                  tma_load_4d(dst + b * 128, map_w, (ks + c) * kKB, row + (it.second ? b : b / 2), stack, 0, bar, once);
+                  tma_load_4d(dst + b * 128, map_w, (ks + c) * kKB, row + (second ? b : b / 2), stack, 0, bar, once);
             } else {
               if (leader) tma_load_4d(dst, map_w, (ks + c) * kKB, 0, stack, row / 16, bar, once);
             }
@@ -597,8 +607,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* dst = ring_b + slot * p.slot_b;
           if (leader) mbar_arrive_expect_tx(bar, chunks * loaded * 128);
           for (int c = 0; c < chunks; ++c, dst += loaded * 128)
-            for (int b = 0; b < columns; b += rows_b)
-              if (leader) tma_load_2d(dst + b * 128, map_b, (ks + c) * kKB, first + b, bar, reused);
+            for (int b = 0; b < columns;) {
+              // A copy takes this warp some 50 cycles whatever its rows: 128 at once where they are there to read.
+              const bool many = rows_b == 32 && columns - b > 96;
+              if (leader) tma_load_2d(dst + b * 128, many ? map_b128 : map_b, (ks + c) * kKB, first + b, bar, reused);
+              b += many ? 128 : rows_b;
+            }
         }
         ++issued;
         if (++slot == p.stages) slot = 0, ++round;
@@ -617,22 +631,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t a0 = umma_desc_sw128(smem_u32(ring_a), 16, 1024), b0 = umma_desc_sw128(smem_u32(ring_b), 16, 1024);
     int c = 0, slot = 0;
     uint32_t round = 0;
-    for (int i = blockIdx.x; ok && find_item(p, s, i, it); i += G, ++c) {
+    for (int i = blockIdx.x; ok && __all_sync(0xffffffffu, find_item(p, s, i, it)); i += G, ++c) {
+      const bool second = uniform(it.second);
       const int b = c & 1;
-      if (c >= 2 && !__all_sync(0xffffffffu, wait_for(&s.acc_empty[b], ((c >> 1) - 1) & 1, deadline))) {
+      if (c >= 2 && !wait_warp(&s.acc_empty[b], ((c >> 1) - 1) & 1, deadline)) {
         ok = false;
         break;
       }
       tc_fence_after_sync();
-      const int rows = it.second ? p.rows2 : p.rows1, wide = 128 / rows;
+      const int rows = second ? p.rows2 : p.rows1, wide = 128 / rows;
       const int k1 = uniform(it.chunks), pad = uniform((it.n + 15) & ~15);
-      const int columns = !it.second && p.direct ? p.tile_n : pad;
-      const int rows_b = it.second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
+      const int columns = !second && p.direct ? p.tile_n : pad;
+      const int rows_b = second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
       const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, columns);
       const uint32_t d = tmem + (uint32_t)(b * p.tile_n);
       bool more = false;
       for (int ks = 0; ks < k1; ks += wide) {
-        if (!__all_sync(0xffffffffu, wait_for(&s.full[slot], round & 1, deadline))) {
+        if (!wait_warp(&s.full[slot], round & 1, deadline)) {
           ok = false;
           break;
         }
@@ -641,12 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // accumulator are not read. Descriptors count in 16 bytes.
         uint64_t ad = a0 + slot * (kSlotA >> 4), bd = b0 + (uint32_t)(slot * (p.slot_b >> 4));
         for (int n = min(wide, k1 - ks); n; --n, ad += rows * 8, bd += loaded * 8) {
-          if (leader) {
-            umma_f16_ss(d, ad, bd, idesc, more);
-            umma_f16_ss(d, ad + 2, bd + 2, idesc, true);
-            umma_f16_ss(d, ad + 4, bd + 4, idesc, true);
-            umma_f16_ss(d, ad + 6, bd + 6, idesc, true);
-          }
+          umma_f16_ss_x4(leader, d, ad, bd, idesc, more);
           more = true;
         }
         if (leader) umma_commit(&s.freed[slot]);
@@ -1159,7 +1169,7 @@ void launch_router(const ExpertParams& p, int groups, cudaStream_t st) {
 }
 
 template <typename T>
-int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaStream_t st) {
+int launch(const CUtensorMap (&maps)[6], const ExpertParams& p, bool few, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_sms());
   cfg.blockDim = dim3(kThreads);
@@ -1204,7 +1214,7 @@ int launch(const CUtensorMap (&maps)[4], const ExpertParams& p, bool few, cudaSt
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(expert_kernel<T>), 1024 + kRing);
   if (e != cudaSuccess) return cuda_status(e);
   cfg.dynamicSmemBytes = smem;
-  return cuda_status(cudaLaunchKernelEx(&cfg, expert_kernel<T>, maps[0], maps[1], maps[2], maps[3], p));
+  return cuda_status(cudaLaunchKernelEx(&cfg, expert_kernel<T>, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p));
 }
 
 }  // namespace
@@ -1261,7 +1271,7 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.stages = l.stages, p.slot_b = l.slot_b, p.direct = l.direct, p.rows_x = l.rows_x, p.rows_act = l.rows_act;
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
-  CUtensorMap maps[4];
+  CUtensorMap maps[6];
   int rc = PKV_OK;
   if (!l.few && l.direct) rc = make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB, l.rows_x);
   else if (!l.few)
@@ -1276,6 +1286,11 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
     rc = make_matrix_tensor_map(&maps[2], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB,
                                 l.rows_act);
   if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, l.rows2, 1);
+  if (!l.few) maps[4] = maps[0], maps[5] = maps[2];
+  if (rc == PKV_OK && !l.few && !l.direct && l.rows_act == 32)
+    rc = make_matrix_tensor_map(&maps[4], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, 128);
+  if (rc == PKV_OK && !l.few && l.rows_act == 32)
+    rc = make_matrix_tensor_map(&maps[5], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB, 128);
   if (rc != PKV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == PKV_F16 ? launch<__half>(maps, p, l.few, st) : launch<__nv_bfloat16>(maps, p, l.few, st);

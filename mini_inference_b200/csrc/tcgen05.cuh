@@ -51,6 +51,24 @@ __device__ inline void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_
       : "memory");
 }
 
+// Four of them, 64 elements of K in swizzled rows of 128 bytes, by the lane of a converged warp that
+// `issue` names: predicated, so that the warp does not branch.
+__device__ __forceinline__ void umma_f16_ss_x4(bool issue, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred i, p, t;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 i, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@i tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@i tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@i tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@i tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(issue ? 1u : 0u)
+      : "memory");
+}
+
 // D[tmem] (+)= A[tmem] * B[smem]^T: A is K-major in TMEM (lane = row, two 16-bit K
 // elements per 32-bit column, the lower K index in the low half), so one K step of 16
 // spans 8 columns from a_tmem.
