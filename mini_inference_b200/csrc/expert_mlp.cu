@@ -45,6 +45,7 @@ constexpr int kThreads = 384;      // weight copies, token copies, MMA, finished
 constexpr int kRouterTokens = 16;  // tokens of a router CTA
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
 constexpr int kRing = 200 * 1024;  // bytes of the stages
+constexpr int64_t kDropBytes = 16 << 20;  // from this size of y on the lines are worth an instruction each (combine())
 
 // What persists between calls, zero outside them; the rest of the workspace is written before it is read.
 struct Header {
@@ -78,6 +79,7 @@ struct ExpertParams {
   int stages, slot_b;
   bool in16;        // intermediate is a multiple of 16
   bool direct;      // gate and up's token rows: all of x, or the expert's of xs
+  bool drop_y;      // y is dropped from L2 once read
   int rows_x, rows_act;  // token rows of a copy of either product
   uint32_t tmem_cols;
 };
@@ -450,6 +452,9 @@ __device__ __forceinline__ void grid_barrier(const ExpertParams& p, int times, u
   __syncthreads();
 }
 
+// 128 bytes that nothing reads any more: not written back to memory, where they still lie in L2.
+__device__ __forceinline__ void drop_line(const void* line) { asm volatile("discard.global.L2 [%0], 128;" ::"l"(line) : "memory"); }
+
 // 32 bytes in one load: by two of 16 a warp would ask L2 for every 32-byte sector twice.
 __device__ __forceinline__ void load8(float (&v)[8], const float* from) {
   asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -459,7 +464,9 @@ __device__ __forceinline__ void load8(float (&v)[8], const float* from) {
 }
 
 // out = the sum over each token's experts, in their order, of its products; by the whole grid. Eight
-// products' loads go ahead together.
+// products' loads go ahead together. A large y would be written to memory from L2 while it is read, and after:
+// its lines are dropped instead (134 MB at 2048 tokens: 274 us with them written, 267 without; the same for xs
+// behind its last reader took 5 us more).
 template <typename T>
 __device__ __forceinline__ void combine(const ExpertParams& p, const float* weight) {
   const int per_row = p.hidden / 8;
@@ -492,6 +499,11 @@ __device__ __forceinline__ void combine(const ExpertParams& p, const float* weig
     o.x = Dt<T>::pack(sum[0], sum[1]), o.y = Dt<T>::pack(sum[2], sum[3]);
     o.z = Dt<T>::pack(sum[4], sum[5]), o.w = Dt<T>::pack(sum[6], sum[7]);
     *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_stride + c) = o;
+    if (p.drop_y) {  // a line of a product is four lanes'
+      __syncwarp(0xfu << (threadIdx.x & 28));
+      if ((u & 3) == 0)
+        for (int k = 0; k < p.top_k; ++k) drop_line(p.y + (int64_t)(t * p.top_k + k) * p.hidden + c);
+    }
   }
 }
 
@@ -1269,6 +1281,7 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.per1 = (2 * intermediate + l.rows1 - 1) / l.rows1, p.per2 = (hidden + l.rows2 - 1) / l.rows2;
   p.tile_n = l.tile_n;
   p.stages = l.stages, p.slot_b = l.slot_b, p.direct = l.direct, p.rows_x = l.rows_x, p.rows_act = l.rows_act;
+  p.drop_y = hidden % 32 == 0 && n_tokens * top_k * hidden * 4 >= kDropBytes;
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
   CUtensorMap maps[6];

@@ -99,6 +99,14 @@ def test_weights_of_the_chosen_or_of_all(renormalize):
     check(x, router * 4, gate_up, down, 3, renormalize)
 
 
+@pytest.mark.parametrize("tokens,hidden,top_k", [(1031, 576, 8), (1031, 1040, 8), (911, 544, 9), (700, 1024, 16)])
+def test_large_products_one_call_after_another(tokens, hidden, top_k):
+    """16 MB of products and more, whose lines are dropped where they are whole (hidden a multiple of 32)."""
+    ws = ops.expert_mlp_workspace(tokens, 24, top_k, hidden, 64, "cuda")
+    for seed in range(3):
+        check(*make(torch.bfloat16, tokens - 40 * seed, hidden, 64, 24, seed=seed), top_k, workspace=ws)
+
+
 def test_all_tokens_to_one_expert():
     """An expert with every token (several tiles of them) and experts with none."""
     x, router, gate_up, down = make(torch.bfloat16, 700, 256, 128, 8)
