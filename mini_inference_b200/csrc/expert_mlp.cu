@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
     const int t = p.perm[(int64_t)lo * p.tokens + r - offset[lo]] / p.top_k;
     const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + t * p.x_stride);
     uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.xs) + (int64_t)r * p.hidden);
-#pragma unroll 4
-    for (int c = lane; c < vecs; c += 32) to[c] = from[c];
+#pragma unroll 8
+    for (int c = lane; c < vecs; c += 32) to[c] = __ldg(from + c);
   }
 }
 
@@ -1213,7 +1213,7 @@ int launch(const CUtensorMap (&maps)[6], const ExpertParams& p, bool few, cudaSt
   if (rc != PKV_OK) return rc;
   if (!p.direct) {
     cudaLaunchConfig_t gather = {};
-    gather.gridDim = dim3(4 * num_sms());
+    gather.gridDim = dim3(8 * num_sms());
     gather.blockDim = dim3(256);
     gather.stream = st;
     gather.attrs = at + 1;
