@@ -17,13 +17,14 @@
 //    product to the second: the weights of down stream in while the activations are still being
 //    made, and only the tokens' side waits for them (a counter per token tile). Then the
 //    weighted sum over each token's experts, in their order.
-// On one B200: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 140 us =
-// 5.8 TB/s, 0.88 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 130 us = 5.5 TB/s;
-// 2048 tokens of 2048 through 8 of 64 experts of 768 310-340 us = 0.50 PFLOP/s, bound by what L2
-// gives the SMs (a stage's 48 KB in some 1000 cycles, the products take 512) and by the 134 MB of
-// float32 products written and read back; 333 tokens of 896 through 4 of 60 experts of 616 66 us and one
-// token of 2048 through 8 of 64 of 768 27 us, bound by the chain: launches and cold instructions 5 us,
-// logits and choice 4-8, first data 4, the wait between the products 3, the last sums 3.
+// On one B200, captured: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 135 us
+// = 6.0 TB/s, 0.91 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 126 us = 5.7 TB/s;
+// 2048 tokens of 2048 through 8 of 64 experts of 768 261 us = 0.59 PFLOP/s, bound by the ring's latency (four
+// stages of 40 KB on average, one in some 900 cycles: weights take 2600 cycles to come, the roles 500 to 700 a
+// stage; L2 and DRAM are at 41 and 53 %) and by the 134 MB of float32 products written and read back (30 us
+// of sums); 333 tokens of 896 through 4 of 60 experts of 616 57 us and one token of 2048 through 8 of 64 of
+// 768 25 us, bound by the chain: launches and cold instructions 5 us, logits and choice 4-8, first data 4,
+// the wait between the products 3, the last sums 2.
 //
 // No counterpart in the reference, whose MLP is dense (engine/model.py:254-264).
 #include <algorithm>
