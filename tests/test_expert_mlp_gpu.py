@@ -107,6 +107,12 @@ def test_large_products_one_call_after_another(tokens, hidden, top_k):
         check(*make(torch.bfloat16, tokens - 40 * seed, hidden, 64, 24, seed=seed), top_k, workspace=ws)
 
 
+@pytest.mark.parametrize("tokens", [96, 97, 113, 128, 129, 193, 224, 225, 241, 256, 257, 385, 512, 513])
+def test_tiles_at_the_edges_of_their_copies(tokens):
+    """One expert, so that the tiles' sizes are known: rows come 128 or 32 at a time."""
+    check(*make(torch.float16, tokens, 136, 72, 1, seed=tokens), 1)
+
+
 def test_all_tokens_to_one_expert():
     """An expert with every token (several tiles of them) and experts with none."""
     x, router, gate_up, down = make(torch.bfloat16, 700, 256, 128, 8)

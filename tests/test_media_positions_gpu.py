@@ -83,6 +83,38 @@ def test_packed(batch, spans):
     assert (out[:, total:] == -5).all()
 
 
+@pytest.mark.parametrize("batch", [1023, 1024, 1025, 2100])
+def test_many_sequences(batch):
+    """Chunks of 0 to 2 tokens; rows of 0 to 9 spans, which the kernel reads four at a time."""
+    rng = np.random.default_rng(batch)
+    rows, want, pos, counts = [], [], [], []
+    for b in range(batch):
+        r, end = draw(rng, b % 10)
+        n = int(rng.integers(0, 3))
+        first = int(rng.integers(0, end + 3))
+        rows.append(r)
+        want.append(sequence(first + n, r)[first:])
+        pos.append(np.arange(first, first + n))
+        counts.append(n)
+    media, counts_dev = table(rows, cap=9 + batch % 2)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = ops.media_positions(torch.from_numpy(np.concatenate(pos)).cuda(), media, counts_dev, None, cu, status=status)
+    ops.raise_device_errors(status)
+    assert np.array_equal(got.T.cpu().numpy(), np.concatenate(want))
+
+
+@pytest.mark.parametrize("wrong,at,reported", [(4, 100, True), (7, 100, True), (4, 6, False), (8, 100, True)])
+def test_a_later_span_is_wrong(wrong, at, reported):
+    """Reported by the tokens behind it: one in the second span does not read so far."""
+    spans = [(4 * i, 1, 1, 3, 1) for i in range(9)]
+    spans[wrong] = (4 * wrong, 1, 0, 3, 1)
+    media, counts = table([spans])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.media_positions(torch.tensor([at], device="cuda"), media, counts, status=status)
+    assert bool(status.item()) == reported
+
+
 def test_one_token_each():
     """A decode batch: no cu_seqlens; padding rows (-1) have no media; rows given or not."""
     media, counts = table([[(2, 1, 4, 5, 1)], [], [(0, 2, 3, 3, 4), (18, 1, 1, 1, 1)]])
