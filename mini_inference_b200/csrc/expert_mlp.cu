@@ -178,9 +178,11 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
         uint32_t border = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const bool here = lane + 32 * i < p.experts;
-          if (here && v[i] > last + tol) taken |= 1u << i, ++sure;
-          if (here && fabsf(v[i] - last) <= tol) border |= 1u << i;
+          // One difference for both, so that each expert from the last one in upwards is in one of the sets and no
+          // other: a rounded last + tol beside it would leave out an expert that is just there.
+          const bool here = lane + 32 * i < p.experts, near = fabsf(v[i] - last) <= tol;
+          if (here && !near && order_key(v[i]) > order_key(last)) taken |= 1u << i, ++sure;
+          if (here && near) border |= 1u << i;
         }
         sure = __reduce_add_sync(all, sure);
         for (int i = 0; i < NV; ++i)
@@ -203,6 +205,7 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
             const int d = __shfl_xor_sync(all, c, o);
             if (d != 0x7fffffff && (c == 0x7fffffff || s > top || (s == top && d < c))) top = s, c = d;
           }
+          if (c == 0x7fffffff) break;  // none left, which the sets rule out
           if (lane == (c & 31)) taken |= 1u << (c >> 5);
         }
         __syncwarp();
