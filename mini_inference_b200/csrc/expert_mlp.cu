@@ -63,6 +63,7 @@ struct ExpertParams {
   const void* down;
   Header* head;
   float* logits;    // [tokens][experts]
+  float* sizes;     // [tokens][experts at most]: no logit's terms |x_i w_i| sum to more than the largest of a token's
   int32_t* perm;    // [experts][tokens]: an expert's choices, token * top_k + k each
   float* weight;    // [tokens][top_k]
   int32_t* done;    // [token tiles]: row tiles of gate and up that are finished
@@ -137,13 +138,16 @@ __device__ double exact_logit(const ExpertParams& p, int t, int e) {
   return s;
 }
 
-// The top_k experts of a token and their weights, by a warp. Lane l holds experts l, l + 32, ... The
-// float32 logits are off by about 2^-23 of the largest; where the last expert in and the first one
-// out are within 2^-17 of it, those within that of the border are chosen by their float64 logits, so
-// that the choice does not hang on the order of a sum. `exact`: float64 scratch of the warp. Lane k < top_k
-// gets the k-th expert and its weight.
+// The top_k experts of a token and their weights, by a warp. Lane l holds experts l, l + 32, ... A float32
+// logit is off by some part of the sum of its terms' sizes, which large terms that cancel make far more than
+// the logit. `border` is twice that part: where the last expert in and the first one out are no further apart
+// than it allows, those within that of the border are chosen by their float64 logits, so that the choice does
+// not hang on the order of a sum. `sizes`: the token's n sums of sizes; those of rows with an infinity or NaN,
+// whose logits are none either, do not count. `exact`: float64 scratch of the warp. Lane k < top_k gets the k-th
+// expert and its weight.
 template <typename T, int NV>
-__device__ void choose(const ExpertParams& p, int t, double* exact, int& expert, float& weight) {
+__device__ void choose(const ExpertParams& p, int t, float border, const float* sizes, int n_sizes, double* exact, int& expert,
+                       float& weight) {
   const int lane = threadIdx.x & 31;
   const uint32_t all = 0xffffffffu;
   float v[NV];
@@ -152,9 +156,10 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
   for (int i = 0; i < NV; ++i) {
     const int e = lane + 32 * i;
     v[i] = e < p.experts ? __ldcg(&p.logits[(int64_t)t * p.experts + e]) : 0.f;
-    big = max(big, __float_as_uint(fabsf(v[i])));
+    const float size = e < n_sizes ? __ldcg(&sizes[e]) : 0.f;
+    if (size < INFINITY) big = max(big, __float_as_uint(size));
   }
-  const float tol = __uint_as_float(__reduce_max_sync(all, big)) * 0x1p-17f;
+  const float tol = __uint_as_float(__reduce_max_sync(all, big)) * border;
   uint32_t taken = 0;
   int mine_e = 0;
   float mine_v = 0.f, last = 0.f;
@@ -175,18 +180,18 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
       if (tol > 0.f && tol < INFINITY && last - val <= tol) {
         int sure = 0;
         taken = 0;
-        uint32_t border = 0;
+        uint32_t unsure = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           // One difference for both, so that each expert from the last one in upwards is in one of the sets and no
           // other: a rounded last + tol beside it would leave out an expert that is just there.
           const bool here = lane + 32 * i < p.experts, near = fabsf(v[i] - last) <= tol;
           if (here && !near && order_key(v[i]) > order_key(last)) taken |= 1u << i, ++sure;
-          if (here && near) border |= 1u << i;
+          if (here && near) unsure |= 1u << i;
         }
         sure = __reduce_add_sync(all, sure);
         for (int i = 0; i < NV; ++i)
-          for (uint32_t b = __ballot_sync(all, border >> i & 1); b; b &= b - 1) {
+          for (uint32_t b = __ballot_sync(all, unsure >> i & 1); b; b &= b - 1) {
             const int c = 32 * i + __ffs(b) - 1;
             const double s = exact_logit<T>(p, t, c);
             if (lane == 0) exact[c] = s;
@@ -196,7 +201,7 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
           double top = -INFINITY;
           int c = 0x7fffffff;
           for (int i = 0; i < NV; ++i)
-            if ((border & ~taken) >> i & 1) {
+            if ((unsure & ~taken) >> i & 1) {
               const double s = exact[lane + 32 * i];
               if (c == 0x7fffffff || s > top) top = s, c = lane + 32 * i;
             }
@@ -246,6 +251,11 @@ __device__ void choose(const ExpertParams& p, int t, double* exact, int& expert,
 // tokens, the K order free as below), its warps a part of hidden each; grid y shares out the experts.
 // The last CTA of a group of tokens chooses, a warp for a token at a time. 2048 tokens of 2048 in 64
 // experts took 38 us by fp32 products.
+//
+// The same products of |x| and |w| give the sums of the terms' sizes. What a logit may be off: mma.sync lines a
+// step's 16 products and the sum so far up to the largest of them, cuts each at 2^-25 of its power of two and the
+// result at 2^-23 (seen with products of 2^-20 .. 2^-31 beside 1), 5 2^-23 of the warp's sum of sizes at most; the
+// sum over the warps adds 2^-24 for each.
 template <typename T, int MT, int NV>
 __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const ExpertParams p) {
   constexpr int kWarps = MT == 1 ? 16 : 8, kChoosers = NV > 4 ? 8 : kWarps;
@@ -254,7 +264,9 @@ __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const Exper
     float part[kWarps][16 * MT][kRouterTokens];
     double exact[kChoosers][32 * NV];
   } s;
+  __shared__ float s_size[kWarps][kRouterTokens];
   __shared__ int s_last;
+  float size_t0 = 0.f;  // of thread t < kRouterTokens' token: the largest sum so far
   const int group = blockIdx.x, t0 = group * kRouterTokens;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   grid_dep_launch_dependents();  // the next kernel sets itself up, and waits
@@ -271,14 +283,16 @@ __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const Exper
   };
   for (int e0 = blockIdx.y * 16 * MT; e0 < p.experts; e0 += 16 * MT * gridDim.y) {
     const T* row[MT][2];
-    float acc[MT][2][4];
+    float acc[MT][2][4], sizes[MT][2][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         row[m][h] = static_cast<const T*>(p.router) + (int64_t)min(e0 + 16 * m + 8 * h + g, p.experts - 1) * p.hidden;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][j][i] = sizes[m][j][i] = 0.f;
     }
     for (int c = warp * 64; c < p.hidden; c += kWarps * 64 * kSteps) {
       uint4 a[kSteps][MT][2][2], b[kSteps][2][2];
@@ -296,11 +310,17 @@ __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const Exper
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint4 &lo = a[n][m][0][h], &hi = a[n][m][1][h];
+            constexpr uint32_t kAbs = 0x7fff7fffu;
             const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+            const uint32_t s0[4] = {lo.x & kAbs, hi.x & kAbs, lo.y & kAbs, hi.y & kAbs};
+            const uint32_t s1[4] = {lo.z & kAbs, hi.z & kAbs, lo.w & kAbs, hi.w & kAbs};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              mma16816<T>(acc[m][j], a0, b[n][j][h].x, b[n][j][h].y);
-              mma16816<T>(acc[m][j], a1, b[n][j][h].z, b[n][j][h].w);
+              const uint4& x = b[n][j][h];
+              mma16816<T>(acc[m][j], a0, x.x, x.y);
+              mma16816<T>(acc[m][j], a1, x.z, x.w);
+              mma16816<T>(sizes[m][j], s0, x.x & kAbs, x.y & kAbs);
+              mma16816<T>(sizes[m][j], s1, x.z & kAbs, x.w & kAbs);
             }
           }
     }
@@ -310,6 +330,19 @@ __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const Exper
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s.part[warp][16 * m + g + 8 * (i >> 1)][8 * j + 2 * q + (i & 1)] = acc[m][j][i];
+    // The largest of the warp's sums for each token: their sum over the warps is no less than any expert's.
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float most = 0.f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = k; i < 4; i += 2) most = sizes[m][j][i] < INFINITY ? fmaxf(most, sizes[m][j][i]) : most;
+        for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (g == 0) s_size[warp][8 * j + 2 * q + k] = most;
+      }
     __syncthreads();
     for (int i = tid; i < 16 * MT * kRouterTokens; i += 32 * kWarps) {
       const int e = i % (16 * MT), t = i / (16 * MT);
@@ -317,6 +350,13 @@ __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const Exper
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) sum += s.part[k][e][t];
       if (e0 + e < p.experts && t0 + t < p.tokens) p.logits[(int64_t)(t0 + t) * p.experts + e0 + e] = sum;
+    }
+    if (tid < kRouterTokens) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) sum += s_size[k][tid];
+      size_t0 = fmaxf(size_t0, sum);
+      if (t0 + tid < p.tokens) p.sizes[(int64_t)(t0 + tid) * p.experts + blockIdx.y] = size_t0;
     }
     __syncthreads();
   }
@@ -329,10 +369,12 @@ __global__ void __launch_bounds__(MT == 1 ? 512 : 256) router_kernel(const Exper
     __syncthreads();
     if (!s_last) return;
   }
+  // Twice what a logit may be off, a hundredth for the sums of sizes, which are rounded too.
+  const float border = 0x1.03p-22f * (5.f * 4 * ((p.hidden + 64 * kWarps - 1) / (64 * kWarps)) + 0.5f * kWarps);
   for (int t = t0 + warp; warp < kChoosers && t < min(t0 + kRouterTokens, p.tokens); t += kChoosers) {
     int e;
     float w;
-    choose<T, NV>(p, t, s.exact[warp], e, w);
+    choose<T, NV>(p, t, border, p.sizes + (int64_t)t * p.experts, gridDim.y, s.exact[warp], e, w);
     if (lane < p.top_k) {
       const int a = t * p.top_k + lane;
       p.weight[a] = w;
@@ -836,6 +878,7 @@ constexpr int kFewSmem = kFewThreads / 32 * kDepth * kChunk;
 
 struct FewShared {
   float part[8][kFewTokens];       // a logit's parts, by warp
+  float size[8][kFewTokens];       // and those of its terms' sizes
   float weight[kFewChoices];       // of each choice, token * top_k + k
   alignas(16) int expert[kFewChoices];
   uint32_t lead[kFewChoices / 32]; // choices that are their expert's first
@@ -862,9 +905,9 @@ template <typename T>
 __device__ __forceinline__ void few_logits(const ExpertParams& p, FewShared& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vecs = p.hidden / 8;
   for (int e = blockIdx.x; e < p.experts; e += gridDim.x) {
-    float acc[kFewTokens];
+    float acc[kFewTokens], size[kFewTokens];
 #pragma unroll
-    for (int t = 0; t < kFewTokens; ++t) acc[t] = 0.f;
+    for (int t = 0; t < kFewTokens; ++t) acc[t] = size[t] = 0.f;
     const uint4* w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.router) + (int64_t)e * p.hidden);
     for (int c = threadIdx.x; c < vecs; c += kFewThreads) {
       float a[8], b[8];
@@ -874,20 +917,24 @@ __device__ __forceinline__ void few_logits(const ExpertParams& p, FewShared& s) 
         if (t < p.tokens) {
           unpack8<T>(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + t * p.x_stride)[c], b);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[t] += a[i] * b[i];
+          for (int i = 0; i < 8; ++i) acc[t] += a[i] * b[i], size[t] += fabsf(a[i]) * fabsf(b[i]);
         }
     }
 #pragma unroll
     for (int t = 0; t < kFewTokens; ++t) {
       if (t < p.tokens)
-        for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
-      if (lane == 0) s.part[warp][t] = acc[t];
+        for (int o = 16; o; o >>= 1) {
+          acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
+          size[t] += __shfl_xor_sync(0xffffffffu, size[t], o);
+        }
+      if (lane == 0) s.part[warp][t] = acc[t], s.size[warp][t] = size[t];
     }
     __syncthreads();
     if (threadIdx.x < p.tokens) {
-      float sum = 0.f;
-      for (int k = 0; k < kFewThreads / 32; ++k) sum += s.part[k][threadIdx.x];
+      float sum = 0.f, size_sum = 0.f;
+      for (int k = 0; k < kFewThreads / 32; ++k) sum += s.part[k][threadIdx.x], size_sum += s.size[k][threadIdx.x];
       p.logits[(int64_t)threadIdx.x * p.experts + e] = sum;
+      p.sizes[(int64_t)threadIdx.x * p.experts + e] = size_sum;
     }
     __syncthreads();
   }
@@ -904,7 +951,10 @@ __device__ __forceinline__ int few_groups(const ExpertParams& p, FewShared& s, d
   if (warp < p.tokens) {
     int e;
     float w;
-    choose<T, NV>(p, warp, exact + warp * kMaxExperts, e, w);
+    // A thread's terms, five steps of shuffles and eight warps: 2^-24 of the sum of sizes for each addition. Twice
+    // that, and a hundredth for the sums of sizes.
+    const float border = 0x1.03p-23f * (8.f * ((p.hidden / 8 + kFewThreads - 1) / kFewThreads) + 13.f);
+    choose<T, NV>(p, warp, border, p.sizes + (int64_t)warp * p.experts, p.experts, exact + warp * kMaxExperts, e, w);
     if (lane < p.top_k) s.expert[warp * p.top_k + lane] = e, s.weight[warp * p.top_k + lane] = w;
   }
   __syncthreads();
@@ -1080,7 +1130,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
 // ---------------------------------------------------------------- host
 
 struct Layout {
-  int64_t logits, perm, weight, done, xs, act, y, bytes;
+  int64_t logits, sizes, perm, weight, done, xs, act, y, bytes;
   int max_tiles, tile_n, rows1, rows2, stages, slot_b, rows_x, rows_act;
   bool few, direct;
 };
@@ -1152,6 +1202,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
     return here;
   };
   l.logits = take(tokens * experts * 4);
+  l.sizes = take(tokens * experts * 4);
   l.perm = take(tokens * experts * 4);
   l.weight = take(rows * 4);
   l.done = take((std::min<int64_t>(experts, rows) + rows / 32) * 4);  // of the smallest tiles
@@ -1272,6 +1323,7 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.x = x, p.router = router, p.gate_up = gate_up, p.down = down, p.out = out, p.status = status_dev;
   p.head = reinterpret_cast<Header*>(ws);
   p.logits = reinterpret_cast<float*>(ws + l.logits);
+  p.sizes = reinterpret_cast<float*>(ws + l.sizes);
   p.perm = reinterpret_cast<int32_t*>(ws + l.perm);
   p.weight = reinterpret_cast<float*>(ws + l.weight);
   p.done = reinterpret_cast<int32_t*>(ws + l.done);

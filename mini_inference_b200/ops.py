@@ -677,8 +677,8 @@ def expert_mlp(x: torch.Tensor, router: torch.Tensor, gate_up: torch.Tensor, dow
     (silu(gate) * up)`` with ``gate | up = gate_up[e] . x`` (``gate_up`` ``[E, 2 * intermediate,
     hidden]``, ``down`` ``[E, hidden, intermediate]``) and ``w`` the softmax of the chosen logits
     (``renormalize=False``: of all of them). float32 throughout but for one rounding of ``silu(gate) *
-    up`` and one of the result; logits next to the border between chosen and not are compared in
-    float64. ``out`` (contiguous) may not overlap the inputs.
+    up`` and one of the result; logits that float32 sums of their terms do not tell from the border
+    between chosen and not are compared in float64. ``out`` (contiguous) may not overlap the inputs.
     """
     result = _layer.expert_mlp(x, router, gate_up, down, top_k, renormalize, workspace, out, status)
     if type(result) is int:

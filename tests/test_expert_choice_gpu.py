@@ -63,3 +63,32 @@ def test_logits_at_every_step_from_the_border(dtype, batch, twins):
     assert (x.double() @ router.double().T)[:, 0].unique().tolist() == sorted(tops)
     check_choice(x, router, top_k, batch)
     check_choice(x.flip(0), router, top_k, batch)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,hidden", [(5, 2048), (40, 2048), (150, 2048), (7, 1000), (130, 1000)])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_near_ties_behind_large_terms_that_cancel(dtype, batch, hidden, infinite):
+    """Pairs of opposite channels of some thousand, which float32 sums do not come back from to a logit's last bits.
+
+    Experts' rows differ by the last bits of a few elements, so that logits of size 1 are some 2^-13 apart; partial
+    sums past 2048 are rounded to 2^-12 or 2^-13. One more expert whose logit is minus infinity changes nothing.
+    """
+    g = torch.Generator(device="cuda").manual_seed(11)
+    experts, top_k, tokens = 32, 4, 300
+    u = torch.finfo(dtype).eps
+    base = (torch.randn(hidden, generator=g, device="cuda") * hidden ** -0.5).to(dtype)
+    few = 64 if dtype == torch.float16 else 8
+    moved = (torch.rand(experts, hidden, generator=g, device="cuda") < few / hidden) & (base.abs() > 2.0 ** -12)
+    sign = torch.randint(0, 2, (experts, hidden), generator=g, device="cuda") * 2 - 1
+    router = (base.float() * (1 + moved * sign * u)).to(dtype)
+    x = torch.randn(tokens, hidden, generator=g, device="cuda").to(dtype)
+    pairs = 10 + torch.randperm(hidden - 10, generator=g, device="cuda")[:8].view(2, 4)
+    large = (4096 * (1 + torch.rand(tokens, 4, generator=g, device="cuda"))).to(dtype)
+    x[:, pairs[0]], x[:, pairs[1]] = large, -large
+    common = torch.rand(experts, 4, generator=g, device="cuda").add(0.5).to(dtype)
+    router[:, pairs[0]] = router[:, pairs[1]] = common
+    x[:, 0], router[:, 0] = 1, 0
+    if infinite:
+        router[5, 1], x[:, 1] = -torch.inf, 1
+    check_choice(x[:tokens // batch * batch], router, top_k, batch)
