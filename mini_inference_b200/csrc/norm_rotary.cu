@@ -13,6 +13,7 @@
 // No counterpart in the reference, whose layers neither normalise heads nor have more than one
 // axis (engine/model.py:190-251).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -78,13 +79,14 @@ __device__ __forceinline__ float2 pair_angle(const NormRotaryParams& p, int64_t 
 // written once. Norm weight, cos, sin and factor are multiplied once per token and pair, into four
 // numbers for q and four for k:
 //   a' = (a A - b B) rs,  b' = (b C + a D) rs,  A = wa cos, B = wb sin, C = wb cos, D = wa sin
-// (A = wa, C = wb, B = D = 0 past the rotated part), so that a head costs three products an element
+// (A = wa, C = wb, no b in a' and no a in b' past the rotated part), so that a head costs three products an element
 // and no weights: the kernel is bound by instructions as much as by bytes. 8192 tokens of 28 / 4 heads
 // of 128 (bf16, three axes, appended) take 30 us = 5.0 TB/s, 0.77 of the copy bandwidth; with weights,
 // cos and sin applied one after another they took 45, with each head's load in its own turn 33. Two
 // elements at a time by paired fp32 instructions. Four tokens per CTA with their loads ahead of the
 // angles were slower (61-120 us).
-template <typename T, bool INTER, bool NORM>
+// REST: there is a part that is not rotated (its selects cost a whole-head rotation 5 %: 31.6 us).
+template <typename T, bool INTER, bool NORM, bool REST>
 __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryParams p) {
   __shared__ float4 table[NORM ? 2 : 1][8][32];  // q and k: {A A B B}, {C C D D} of two pairs, by unit
   using V = Vec<T, 8>;
@@ -163,9 +165,14 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryP
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float4 ab = table[which][2 * j][sub], cd = table[which][2 * j + 1][sub];
-      float2 x = ffma2(a[j], make_float2(ab.x, ab.y), fmul2(make_float2(-b[j].x, -b[j].y), make_float2(ab.z, ab.w)));
-      float2 y = INTER ? ffma2(a[j], make_float2(cd.z, cd.w), fmul2(b[j], make_float2(cd.x, cd.y)))
-                       : ffma2(b[j], make_float2(cd.x, cd.y), fmul2(a[j], make_float2(cd.z, cd.w)));
+      // Past the rotated part there is no pair: an infinity times nothing would be the other's NaN (-0 to add, which
+      // keeps a -0). Asked of `rest` too, which REST implies: 54 registers, 78 without, where six CTAs fit an SM in
+      // place of seven (1013 rows of half-rotated heads 6.1 and 7.4 us).
+      float2 cross_a = a[j], cross_b = b[j];
+      if (REST && rest && sub >= rot_units) cross_a = make_float2(-0.f, -0.f), cross_b = make_float2(0.f, 0.f);
+      float2 x = ffma2(a[j], make_float2(ab.x, ab.y), fmul2(make_float2(-cross_b.x, -cross_b.y), make_float2(ab.z, ab.w)));
+      float2 y = INTER ? ffma2(cross_a, make_float2(cd.z, cd.w), fmul2(b[j], make_float2(cd.x, cd.y)))
+                       : ffma2(b[j], make_float2(cd.x, cd.y), fmul2(cross_a, make_float2(cd.z, cd.w)));
       if (NORM) x = fmul2(x, rs2), y = fmul2(y, rs2);
       if (INTER && side) {
         (j < 2 ? oa : ob)[(2 * j) & 3] = Dt<T>::pack(x.x, y.x);
@@ -278,8 +285,12 @@ int launch(NormRotaryParams p, int64_t n, bool vec16, bool inter, cudaStream_t s
   // 8192 tokens 45, 33 and 30 us; 1013 tokens of 32 / 8 heads 8.0, 6.0 and 6.5 us.
   const int per = n > 16 * num_sms() ? 5 : n > 4 * num_sms() ? 3 : 1;
   const int threads = std::min(kThreads, std::max(64, (work + per * 32 - 1) / (per * 32) * 32));
-  auto kernel = norm ? inter ? norm_rotary_kernel<T, true, true> : norm_rotary_kernel<T, false, true>
-                     : inter ? norm_rotary_kernel<T, true, false> : norm_rotary_kernel<T, false, false>;
+  auto pick = [&](auto rest) {
+    constexpr bool R = decltype(rest)::value;
+    return norm ? inter ? norm_rotary_kernel<T, true, true, R> : norm_rotary_kernel<T, false, true, R>
+                : inter ? norm_rotary_kernel<T, true, false, R> : norm_rotary_kernel<T, false, false, R>;
+  };
+  auto kernel = 2 * p.half < p.d ? pick(std::true_type{}) : pick(std::false_type{});
   kernel<<<(unsigned)n, threads, 0, st>>>(p);
   return launch_status();
 }

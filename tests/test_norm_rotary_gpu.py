@@ -175,3 +175,36 @@ def test_reports_and_refusals():
         with pytest.raises(PkvError):
             ops.norm_rotary_append(**{**ok, **kw_})
     assert ops.norm_rotary_append(**{**ok, "qkv": qkv[:0], "positions": pos[:, :0].contiguous()})[0].shape == (0, 14, 64)
+
+
+@pytest.mark.parametrize("dtype,d,rotary", [(F16, 64, 32), (BF16, 128, 32), (F16, 80, 16), (BF16, 72, 16), (F16, 36, 18)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_infinity_and_nan_past_the_rotated_part(dtype, d, rotary, interleaved, norm, bad):
+    """One bad element in the part that is not rotated, at each of its places: without norms every other element is as it was."""
+    n = d - rotary
+    qkv, pos, (qw, kw), k, v = setup(dtype, 4, 2, d, n, 3, seed=d)
+    heads = qkv.view(n, -1, d)
+    at = torch.arange(n, device="cuda")
+    heads[at, 1, rotary + at] = bad  # q head 1
+    heads[at, 4, rotary + at] = bad  # k head 0
+    heads[at, 5, rotary + at] = -0.0
+    freq, _ = ops.rotary_frequencies(rotary, 1e4)
+    third = rotary // 6
+    pair = ops.pair_axes([rotary // 2 - 2 * third, third, third])
+    if not norm:
+        qw = kw = None
+    q, ko, _ = ops.norm_rotary_append(ops.make_pool(k, v), 0, qkv, pos, freq, 4, axes=pair, q_weight=qw, k_weight=kw,
+                                      interleaved=interleaved, k_out=True)
+    for got, x, w in ((q, heads[:, :4], qw), (ko, heads[:, 4:6], kw)):
+        want, bound = reference(x, pos, freq, pair, w, 1e-6, interleaved, 1.0)
+        assert torch.equal(got.isnan(), want.isnan())
+        if not norm:
+            assert torch.equal(got[..., rotary:].nan_to_num(7, 8, 9).view(torch.int16),
+                               x[..., rotary:].nan_to_num(7, 8, 9).view(torch.int16))
+        fine = want.isfinite()
+        off = (got.double() - want).abs()[fine]
+        u = torch.finfo(dtype).eps / 2
+        assert (off <= (u * (want.abs() + bound) + bound + 2.0 ** -25)[fine]).all()
+        assert (got.isinf() == want.isinf()).all()
