@@ -292,11 +292,18 @@ class PagedKVCache:
     Memory layout is the reference's: ``k, v: [num_layers, num_blocks + 1,
     num_kv_heads, block_size, head_dim]``, block ``num_blocks`` being the scratch
     block that CUDA-graph padding rows write to.
+
+    ``max_media`` (no counterpart in the reference): the most images and videos of a sequence, see
+    :meth:`set_media`. Not together with ``enable_prefix_caching``, which shares blocks by token ids.
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, block_size: int,
                  max_seqs: int, max_len: int, dtype: torch.dtype, device: torch.device | str,
                  enable_prefix_caching: bool = False, enable_copy_on_write: bool = False, max_media: int = 0) -> None:
+        if max_media < 0:
+            raise ValueError("max_media must not be negative")
+        if max_media and enable_prefix_caching:
+            raise ValueError("prefixes are cached by token ids, which do not tell one image from another: no media with them")
         shape = (num_layers, num_blocks + 1, num_kv_heads, block_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
