@@ -344,8 +344,9 @@ class LLMEngine:
         sp = sampling_params or SamplingParams()
         if not sp.greedy:
             raise NotImplementedError("only greedy requests are served (the LM head is fused with argmax)")
+        prompt = list(prompt)
         self._check_media(media, len(prompt))
-        seq = Sequence(seq_id=self._next_id, prompt_token_ids=list(prompt), sampling=sp,
+        seq = Sequence(seq_id=self._next_id, prompt_token_ids=prompt, sampling=sp,
                        arrival_time=time.perf_counter() if arrival_time is None else arrival_time, media=tuple(media))
         self.scheduler.add(seq)  # raises if the prompt can never fit
         self.sequences[seq.seq_id] = seq

@@ -2,10 +2,13 @@
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
 from mini_inference_b200 import PagedKVCache
+from mini_inference_b200.engine import LLMEngine
 
 
 def cache(**kw):
@@ -19,3 +22,18 @@ def test_no_media_with_prefixes_that_go_by_token_ids():
     with pytest.raises(ValueError):
         cache(max_media=-1)
     assert cache(max_media=1).max_media == 1 and cache(enable_prefix_caching=True).enable_prefix_caching
+
+
+def engine(max_media=2):
+    """An engine that queues requests and runs none."""
+    e = object.__new__(LLMEngine)
+    e.config = SimpleNamespace(max_media=max_media)
+    e.model = SimpleNamespace(cfg=SimpleNamespace(rope_sections=(8, 12, 12), hidden_size=64))
+    e.scheduler, e.sequences, e._next_id = SimpleNamespace(add=lambda seq: None), {}, 0
+    return e
+
+
+def test_a_prompt_may_be_any_iterable_of_ids():
+    e = engine()
+    for prompt in ([3, 1, 2], (3, 1, 2), iter([3, 1, 2]), (t for t in [3, 1, 2]), torch.tensor([3, 1, 2]).numpy()):
+        assert list(e.sequences[e.add_request(prompt)].prompt_token_ids) == [3, 1, 2]
