@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import operator
 import time
 from collections.abc import Callable, Sequence as SequenceOf
 from dataclasses import dataclass, field
@@ -362,11 +363,18 @@ class LLMEngine:
             raise ValueError(f"{len(media)} images and videos, max_media is {self.config.max_media}")
         end = 0
         for m in media:
-            if m.start < end or min(m.frames, m.height, m.width) < 1 or m.step < 0:
-                raise ValueError("media are in order and apart, their sizes positive")
+            try:
+                for v in m.span:
+                    operator.index(v)
+            except TypeError:
+                raise ValueError("a medium's start, sizes and step are whole numbers") from None
+            if m.start < end or min(m.frames, m.height, m.width) < 1 or not 0 <= m.step <= 2**31 - 1:
+                raise ValueError("media are in order and apart, their sizes positive, their step at most 2^31 - 1")
             end = m.start + m.size
-            if m.rows is not None and tuple(m.rows.shape) != (m.size, self.model.cfg.hidden_size):
-                raise ValueError(f"rows must be [{m.size}, {self.model.cfg.hidden_size}]")
+            if m.rows is None:
+                continue
+            if not isinstance(m.rows, torch.Tensor) or tuple(m.rows.shape) != (m.size, self.model.cfg.hidden_size):
+                raise ValueError(f"rows must be a tensor [{m.size}, {self.model.cfg.hidden_size}]")
         if end >= prompt_len:
             raise ValueError("a prompt ends in text")
 

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from mini_inference_b200 import PagedKVCache
-from mini_inference_b200.engine import LLMEngine
+from mini_inference_b200.engine import LLMEngine, Media
 
 
 def cache(**kw):
@@ -37,3 +37,14 @@ def test_a_prompt_may_be_any_iterable_of_ids():
     e = engine()
     for prompt in ([3, 1, 2], (3, 1, 2), iter([3, 1, 2]), (t for t in [3, 1, 2]), torch.tensor([3, 1, 2]).numpy()):
         assert list(e.sequences[e.add_request(prompt)].prompt_token_ids) == [3, 1, 2]
+
+
+@pytest.mark.parametrize("bad", [Media(2, 1, 2, 2, 2**31), Media(2, 1, 2, 2, 1.5), Media(2.0, 1, 2, 2), Media(2, 1, 2.0, 2),
+                                 Media(2, 1, 2, 2, rows=[[0.0] * 64] * 4)])
+def test_media_that_no_step_can_place_are_refused_with_the_request(bad):
+    """Else the request is queued and every step raises."""
+    e = engine()
+    with pytest.raises(ValueError):
+        e.add_request(range(10), media=[bad])
+    assert not e.sequences
+    e.add_request(range(10), media=[Media(2, 1, 2, 2, 2**31 - 1, torch.zeros(4, 64))])
