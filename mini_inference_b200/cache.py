@@ -29,6 +29,7 @@ supports the allocator only, and its contexts raise.
 from __future__ import annotations
 
 import ctypes
+import operator
 from collections.abc import Iterator, Mapping, MutableMapping, Sequence
 
 import numpy as np
@@ -419,7 +420,7 @@ class PagedKVCache:
         again or the slot is allocated again; slots that the native scheduler hands out are set by
         the engine at each prefill.
         """
-        rows, end = tuple(tuple(int(v) for v in s) for s in spans), 0
+        rows, end = tuple(tuple(operator.index(v) for v in s) for s in spans), 0
         for row in rows:
             if len(row) != 5:
                 raise ValueError("a span is (start, frames, height, width, step)")

@@ -48,3 +48,12 @@ def test_media_that_no_step_can_place_are_refused_with_the_request(bad):
         e.add_request(range(10), media=[bad])
     assert not e.sequences
     e.add_request(range(10), media=[Media(2, 1, 2, 2, 2**31 - 1, torch.zeros(4, 64))])
+
+
+def test_spans_are_whole_numbers():
+    c = cache(max_media=1)
+    slot = c.allocate(20)
+    with pytest.raises(TypeError):
+        c.set_media(slot, [(2.7, 1, 2, 2, 1)])
+    c.set_media(slot, [(torch.tensor(2), 1, 2, 2, 1)])
+    assert c._media[slot] == ((2, 1, 2, 2, 1),)
