@@ -220,8 +220,10 @@ class Qwen2Model:
             raise ValueError("rope_sections are pairs of one to three axes")
         # One workspace for the experts of all layers, of the largest step so far (zeroed once, reused):
         # steps of one model must not overlap on the GPU, as with the cache's workspaces. Smaller ones
-        # stay: captured steps hold their addresses.
+        # that captured steps hold the addresses of stay.
         self._expert_workspaces: list[torch.Tensor] = []
+        self._expert_rows = -1  # tokens that the last one holds
+        self._expert_captured = False  # whether a captured step holds it
         self.norm = weights["norm.weight"]
         # The reference's RoPE tables (float32, cast to the model dtype per lookup), built once.
         # Other layouts and scaled frequencies go through ops.rotary_append, which makes the
@@ -265,15 +267,26 @@ class Qwen2Model:
         return F.linear(out.transpose(1, 2).reshape(b, t, cfg.q_size), wo)
 
     def expert_workspace(self, rows: int) -> torch.Tensor:
-        """The experts' workspace, of at least ``rows`` tokens: a larger one is made outside graph captures only."""
-        cfg, ws = self.cfg, self._expert_workspaces[-1] if self._expert_workspaces else None
-        args = (cfg.num_experts, cfg.experts_per_token, cfg.hidden_size, cfg.expert_intermediate_size or cfg.intermediate_size)
-        if ws is None or ws.numel() < ops.expert_mlp_workspace_bytes(rows, *args):
-            if torch.cuda.is_current_stream_capturing():
+        """The experts' workspace, of at least ``rows`` tokens: a larger one is made outside graph captures only.
+
+        An outgrown one is let go unless a capture took it from here; a graph captured around one that
+        was taken before needs the caller to hold on to it.
+        """
+        capturing = torch.cuda.is_current_stream_capturing()
+        if rows > self._expert_rows:
+            if capturing:
                 raise RuntimeError(f"run a step of {rows} tokens before capturing one: the experts' workspace has to grow")
-            ws = ops.expert_mlp_workspace(max(64, 1 << (rows - 1).bit_length()), *args, self.device)
-            self._expert_workspaces.append(ws)
-        return ws
+            if self._expert_workspaces and not self._expert_captured:
+                # Its memory is another's only once the steps up to here are done, whichever stream they ran on.
+                self._expert_workspaces.pop().record_stream(torch.cuda.current_stream(self.device))
+            self._expert_rows, self._expert_captured = -1, False
+            cfg, most = self.cfg, max(64, 1 << (rows - 1).bit_length())
+            self._expert_workspaces.append(ops.expert_mlp_workspace(
+                most, cfg.num_experts, cfg.experts_per_token, cfg.hidden_size,
+                cfg.expert_intermediate_size or cfg.intermediate_size, self.device))
+            self._expert_rows = most
+        self._expert_captured |= capturing
+        return self._expert_workspaces[-1]
 
     def reset_workspaces(self) -> None:
         """Ready the workspaces again after a step that reported a timed-out wait."""
