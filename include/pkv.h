@@ -476,8 +476,9 @@ PKV_API int pkv_media_positions(const int64_t* positions, int64_t n_tokens, cons
  * top_k largest of them (the first among equals), and
  *   out = sum_k w_k * down[e_k] . (silu(gate[e_k] . x) * (up[e_k] . x)),
  * with w the softmax of the chosen logits (renormalize != 0) or their part of the softmax over all.
- * Products, weights and sums are float32; the activations between the two products are rounded to
- * dtype once, and so is out. Logits are float32 sums; those no further from the border between chosen
+ * Products, weights and sums are float32; the activations between the two products are held as two
+ * numbers of dtype, the rounded one and what that left (one past dtype's range is an infinity), and out is
+ * rounded once. Logits are float32 sums; those no further from the border between chosen
  * and not than such sums may be off (a part of the sum of their terms' sizes) are computed in float64,
  * and the choice among them is by these.
  *   x       : [n_tokens, hidden], token t at x + t * x_stride (16-byte aligned, a multiple of 8)

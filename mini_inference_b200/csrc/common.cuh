@@ -375,10 +375,11 @@ int make_rows_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, i
 // head per copy, in the layout [d/64][8][64].
 int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int d, int heads, int64_t rows,
                               int64_t head_stride, int64_t row_stride);
-// Contiguous [stacks, rows, inner] of 16-bit elements with a box of {64, box_rows, box_stacks, 1} (a
-// fourth dimension of one entry), 128-byte swizzle. Rows past a stack's end read as zeros.
+// [stacks, rows, inner] of 16-bit elements (row_stride elements from row to row, 0: contiguous) with a box of
+// {64, box_rows, box_stacks, 1} (a fourth dimension of one entry), 128-byte swizzle. Rows past a stack's end read as
+// zeros.
 int make_stack_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
-                          uint32_t box_rows, uint32_t box_stacks);
+                          uint32_t box_rows, uint32_t box_stacks, uint64_t row_stride = 0);
 // The same with rows, a multiple of `group`, in groups: dimensions {inner, group, stacks, rows / group} and a
 // box of {64, group, box_stacks, box_groups}: a group's rows of each stack, group by group.
 int make_split_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,

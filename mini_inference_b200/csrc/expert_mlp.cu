@@ -45,7 +45,7 @@ constexpr int64_t kMaxItems = 1 << 30;
 constexpr int kThreads = 384;      // weight copies, token copies, MMA, finished activations, 8 epilogue warps
 constexpr int kRouterTokens = 16;  // tokens of a router CTA
 constexpr int kMaxTickets = 1024;  // router groups whose experts are spread over several CTAs
-constexpr int kRing = 200 * 1024;  // bytes of the stages
+constexpr int kRing = 220 * 1024;  // bytes of the stages
 constexpr int64_t kDropBytes = 16 << 20;  // from this size of y on the lines are worth an instruction each (combine())
 
 // What persists between calls, zero outside them; the rest of the workspace is written before it is read.
@@ -68,7 +68,7 @@ struct ExpertParams {
   float* weight;    // [tokens][top_k]
   int32_t* done;    // [token tiles]: row tiles of gate and up that are finished
   void* xs;         // [tokens * top_k][hidden], past kDirectTokens: x by expert
-  void* act;        // [tokens * top_k][inter], an expert's rows one behind the other
+  void* act;        // [2][tokens * top_k][inter], an expert's rows one behind the other: the values rounded, and the rest
   float* y;         // [tokens * top_k][hidden]
   void* out;
   int32_t* status;
@@ -79,12 +79,29 @@ struct ExpertParams {
   int per1, per2;   // items of a tile
   int tile_n;       // tokens of a tile, at most
   int stages, slot_b;
+  int acc_cols;     // columns of an accumulator
   bool in16;        // intermediate is a multiple of 16
   bool direct;      // gate and up's token rows: all of x, or the expert's of xs
   bool drop_y;      // y is dropped from L2 once read
   int rows_x, rows_act;  // token rows of a copy of either product
   uint32_t tmem_cols;
 };
+
+// The activations between the two products are held in two halves, the value rounded to T and what the
+// rounding left, rounded to T: 16 bits of bfloat16, 22 of float16. Rounded once, the result was 1.4 times as far
+// from the exact one as its own rounding puts it, and no longer what up to kFewTokens tokens get. Down's products are
+// taken for both, of the same weights: for few tokens the weights' stream hides them. Both halves of an item's
+// token rows share a stage where it holds them; else the values have the stage of the weights and the rests the next
+// one. Up to kJointRows rows the two halves, a copy's values and then its rests, are the columns of one product, which
+// takes no longer, and the epilogue adds them (300 tokens through 8 of 128 experts, up to 32 rows an expert: 235 us,
+// 251 by two products); more are summed in the accumulator.
+constexpr int kJointRows = 32;
+template <typename T>
+__device__ __forceinline__ void two_halves(float v, T& high, T& rest) {
+  high = Dt<T>::from_f(v);
+  const float low = v - Dt<T>::to_f(high);
+  rest = Dt<T>::from_f(fabsf(low) < INFINITY ? low : 0.f);  // an infinity's rest would be NaN
+}
 
 // Where gate and up's tokens come from: up to kDirectTokens are all loaded for every expert, which takes
 // its columns of the accumulator; more are laid out by expert first (gathering four rows a copy cost
@@ -459,6 +476,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
   }
 }
 
+// A stage holds both halves of `rows` token rows of down.
+__device__ __forceinline__ bool holds_both(const ExpertParams& p, int rows, int chunks) { return 2 * rows * 128 * chunks <= p.slot_b; }
+
 // Item i, by a converged warp; false past the last. Not inlined: the roles share its instructions, which
 // a launch has to fetch anew (they took 6000 cycles before the first copy when each role had its own).
 __device__ __noinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
@@ -568,6 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     expert_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_gu,
                   const __grid_constant__ CUtensorMap map_act, const __grid_constant__ CUtensorMap map_down,
                   const __grid_constant__ CUtensorMap map_x128, const __grid_constant__ CUtensorMap map_act128,
+                  const __grid_constant__ CUtensorMap map_halves,
                   const __grid_constant__ ExpertParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared s;
@@ -638,43 +659,50 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         fence_proxy_async_global();
       }
+      const bool split = second && !holds_both(p, loaded, wide), joint = second && !split && pad <= kJointRows;
       const CUtensorMap* map_w = second ? &map_down : &map_gu;
-      const CUtensorMap* map_b = second ? &map_act : &map_x;
+      const CUtensorMap* map_b = joint ? &map_halves : second ? &map_act : &map_x;
       const CUtensorMap* map_b128 = second ? &map_act128 : &map_x128;
       const int stack = second ? e : 2 * e;
-      for (int ks = 0; ks < k1; ks += wide) {
-        if (round > 0 && !wait_warp(&s.freed[slot], (round - 1) & 1, deadline)) {
-          ok = false;
-          break;
-        }
-        uint64_t* bar = &s.full[slot];
-        const int chunks = min(wide, k1 - ks);
-        if (weights) {
-          uint8_t* dst = ring_a + slot * kSlotA;
-          if (leader) mbar_arrive_expect_tx(bar, chunks * rows * 128);
-          for (int c = 0; c < chunks; ++c, dst += rows * 128) {
-            if (second || !p.in16) {
-              for (int b = 0; b < rows; b += box)
-                if (leader)
-                  tma_load_4d(dst + b * 128, map_w, (ks + c) * kKB, row + (second ? b : b / 2), stack, 0, bar, once);
-            } else {
-              if (leader) tma_load_4d(dst, map_w, (ks + c) * kKB, 0, stack, row / 16, bar, once);
-            }
+      // Stages of a step, and the halves of one that are copied one after another; a joint copy brings both.
+      const int parts = split ? 2 : 1, halves = second && !split && !joint ? 2 : 1, twice = joint ? 2 : 1;
+      for (int ks = 0; ok && ks < k1; ks += wide)
+        for (int part = 0; part < parts; ++part) {
+          if (round > 0 && !wait_warp(&s.freed[slot], (round - 1) & 1, deadline)) {
+            ok = false;
+            break;
           }
-        } else {
-          uint8_t* dst = ring_b + slot * p.slot_b;
-          if (leader) mbar_arrive_expect_tx(bar, chunks * loaded * 128);
-          for (int c = 0; c < chunks; ++c, dst += loaded * 128)
-            for (int b = 0; b < columns;) {
-              // A copy takes this warp some 50 cycles whatever its rows: 128 at once where they are there to read.
-              const bool many = rows_b == 32 && columns - b > 96;
-              if (leader) tma_load_2d(dst + b * 128, many ? map_b128 : map_b, (ks + c) * kKB, first + b, bar, reused);
-              b += many ? 128 : rows_b;
+          uint64_t* bar = &s.full[slot];
+          const int chunks = min(wide, k1 - ks);
+          if (weights) {
+            uint8_t* dst = ring_a + slot * kSlotA;
+            const int fresh = part ? 0 : chunks;  // none for the rests: those of the stage before
+            if (leader) mbar_arrive_expect_tx(bar, fresh * rows * 128);
+            for (int c = 0; c < fresh; ++c, dst += rows * 128) {
+              if (second || !p.in16) {
+                for (int b = 0; b < rows; b += box)
+                  if (leader)
+                    tma_load_4d(dst + b * 128, map_w, (ks + c) * kKB, row + (second ? b : b / 2), stack, 0, bar, once);
+              } else {
+                if (leader) tma_load_4d(dst, map_w, (ks + c) * kKB, 0, stack, row / 16, bar, once);
+              }
             }
+          } else {
+            uint8_t* dst = ring_b + slot * p.slot_b;
+            if (leader) mbar_arrive_expect_tx(bar, chunks * halves * twice * loaded * 128);
+            for (int c = 0; c < chunks; ++c)
+              for (int h = part; h < part + halves; ++h)
+                for (int b = 0; b < columns;) {
+                  // A copy takes this warp some 50 cycles whatever its rows: 128 at once where they are there to read.
+                  const bool many = rows_b == 32 && columns - b > 96;
+                  const int copied = many ? 128 : rows_b;
+                  if (leader) tma_load_4d(dst, many ? map_b128 : map_b, (ks + c) * kKB, first + b, h, 0, bar, reused);
+                  b += copied, dst += copied * twice * 128;
+                }
+          }
+          ++issued;
+          if (++slot == p.stages) slot = 0, ++round;
         }
-        ++issued;
-        if (++slot == p.stages) slot = 0, ++round;
-      }
     }
     if (!ok && lane == 0) {  // this warp's copies have landed before its CTA may leave
       report(p.status, PKV_ERR_TIMEOUT);
@@ -701,24 +729,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int k1 = uniform(it.chunks), pad = uniform((it.n + 15) & ~15);
       const int columns = !second && p.direct ? p.tile_n : pad;
       const int rows_b = second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
-      const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, columns);
-      const uint32_t d = tmem + (uint32_t)(b * p.tile_n);
+      const bool split = second && !holds_both(p, loaded, wide), joint = second && !split && pad <= kJointRows;
+      const int parts = split ? 2 : 1, halves = second && !split && !joint ? 2 : 1, twice = joint ? 2 : 1;
+      const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, joint ? 2 * loaded : columns);
+      const uint32_t d = tmem + (uint32_t)(b * p.acc_cols);
       bool more = false;
-      for (int ks = 0; ks < k1; ks += wide) {
-        if (!wait_warp(&s.full[slot], round & 1, deadline)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
+      for (int ks = 0; ok && ks < k1; ks += wide) {
         // An item of fewer than 128 weight rows reads on into what is behind them: those lanes of the
         // accumulator are not read. Descriptors count in 16 bytes.
-        uint64_t ad = a0 + slot * (kSlotA >> 4), bd = b0 + (uint32_t)(slot * (p.slot_b >> 4));
-        for (int n = min(wide, k1 - ks); n; --n, ad += rows * 8, bd += loaded * 8) {
-          umma_f16_ss_x4(leader, d, ad, bd, idesc, more);
-          more = true;
+        const uint64_t ad = a0 + slot * (kSlotA >> 4);
+        const int with_weights = slot, chunks = min(wide, k1 - ks);
+        for (int part = 0; part < parts; ++part) {
+          if (!wait_warp(&s.full[slot], round & 1, deadline)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          uint64_t bd = b0 + (uint32_t)(slot * (p.slot_b >> 4));
+          for (int n = 0; n < chunks; ++n)
+            for (int h = 0; h < halves; ++h, bd += loaded * twice * 8) {
+              umma_f16_ss_x4(leader, d, ad + n * rows * 8, bd, idesc, more);
+              more = true;
+            }
+          // The weights' stage is free once the rests in the next one are multiplied.
+          if (leader && part == parts - 1) umma_commit(&s.freed[with_weights]);
+          if (leader && part) umma_commit(&s.freed[slot]);
+          if (++slot == p.stages) slot = 0, ++round;
         }
-        if (leader) umma_commit(&s.freed[slot]);
-        if (++slot == p.stages) slot = 0, ++round;
       }
       if (ok && leader) umma_commit(&s.acc_full[b]);
     }
@@ -774,12 +811,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Gate and up: lanes 0 .. 15 hold gate rows, 16 .. 31 the same up rows; of two columns a lane finishes one.
       const int r = second ? it.row * p.rows2 + q * 32 + lane : it.row * (p.rows1 / 2) + q * 16 + (lane & 15);
       const bool in = r < (second ? p.hidden : p.inter);
-      T* to_act = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r;
+      T *to_act = act + (int64_t)(s.offset[it.e] + it.n0) * p.inter + r, *to_rest = to_act + (int64_t)p.tokens * p.top_k * p.inter;
       float* to_y = p.y + r - (lane & 3);  // the first of four rows: hidden is a multiple of 8
       // After a wait that ran out the warp goes on to its barriers, without data: the others wait there.
       ok = ok && wait_for(&s.acc_full[b], (c >> 1) & 1, deadline);
       tc_fence_after_sync();
-      const uint32_t d = tl + (uint32_t)(b * p.tile_n);
+      const uint32_t d = tl + (uint32_t)(b * p.acc_cols);
+      const int pad = (it.n + 15) & ~15, loaded = (pad + p.rows_act - 1) / p.rows_act * p.rows_act;
+      const bool joint = second && pad <= kJointRows && holds_both(p, loaded, 128 / p.rows2);  // then a warp has one block at most
       uint32_t v[2][16];
       auto fetch = [&](int j) {
         if (direct) {  // the columns of the tokens themselves
@@ -789,7 +828,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld16(d + 16 * (2 * j + half), v[j & 1]);
         }
       };
-      if (16 * half < n) fetch(0);
+      if (joint && 16 * half < n) {  // the columns of a copy's values, then of its rests
+        const int at = 16 * half / p.rows_act * 2 * p.rows_act + 16 * half % p.rows_act;
+        tmem_ld16(d + at, v[0]);
+        tmem_ld16(d + at + p.rows_act, v[1]);
+      } else if (16 * half < n) {
+        fetch(0);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int c0 = 16 * (2 * j + half);
@@ -797,6 +842,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int k = 0; k < 16; ++k) asm volatile("" : "+r"(v[j & 1][k]));  // read from here on
+        if (j == 0 && joint) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            asm volatile("" : "+r"(v[1][k]));
+            v[0][k] = __float_as_uint(__uint_as_float(v[0][k]) + __uint_as_float(v[1][k]));
+          }
+        }
         if (j < 7 && c0 + 32 < n) fetch(j + 1);
         if (j == 7 || c0 + 32 >= n) {
           tc_fence_before_sync();
@@ -829,7 +881,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float g = low ? __uint_as_float(x) : other;
             const float u = low ? other : __uint_as_float(y);
             const int col = c0 + k + (low ? 0 : 1);
-            if (in && col < n) to_act[(int64_t)col * p.inter] = Dt<T>::from_f(__fdividef(g, 1.f + __expf(-g)) * u);
+            if (in && col < n) {
+              const int64_t at = (int64_t)col * p.inter;
+              two_halves(__fdividef(g, 1.f + __expf(-g)) * u, to_act[at], to_rest[at]);
+            }
           }
         }
       }
@@ -1089,8 +1144,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
     for (int i = 0; i < 4; ++i) acc[i] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
   };
 
-  // The activations in two halves, the value rounded and what the rounding left: the second costs
-  // products that the weights' stream hides.
   T* act = static_cast<T*>(p.act);
   const int64_t left = (int64_t)p.tokens * p.top_k * p.inter;
   for (int u = me; u < units1; u += warps) {
@@ -1103,10 +1156,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) expert_few_kernel(const Expert
         const float gate = acc[k], up = acc[2 + k];
         const float v = __fdividef(gate, 1.f + __expf(-gate)) * up;
         T* to = act + (int64_t)s.group_a[group][2 * q + k] * p.inter + row * 8 + g;
-        const T high = Dt<T>::from_f(v);
-        const float low = v - Dt<T>::to_f(high);
-        to[0] = high;
-        to[left] = Dt<T>::from_f(fabsf(low) < INFINITY ? low : 0.f);  // an infinity's rest would be NaN
+        two_halves(v, to[0], to[left]);
       }
   }
   grid_barrier(p, 2);  // the first of down's rows are on their way meanwhile
@@ -1148,12 +1198,13 @@ Tiling make_tiling(int64_t tokens, int64_t experts, int top_k, int hidden, int i
   const double rows = (double)tokens * top_k, active = std::min<double>(experts, rows), share = rows / experts;
   // An expert's tokens are its share, more or less: half of those that nearly fill a tile take another.
   const double tiles = direct ? active : active * std::max(1.0, share / tile_n + (share > 0.7 * tile_n ? 0.5 : 0.0));
-  auto pick = [&](int64_t n, int k, int columns, int& best) {
+  auto pick = [&](int64_t n, int k, int columns, int halves, int& best) {
     double least = 1e300;
     for (int r : {128, 64, 32}) {
       const int wide = 128 / r;
       if (tile_n * wide > 272) break;  // at least four stages
-      const double stage = std::max({(kSlotA + 128.0 * columns * wide) / 52, 4.0 * wide * std::max(45.0, columns / 2.0), 500.0});
+      const double stage = std::max({(kSlotA + 128.0 * columns * wide * halves) / 52,
+                                     4.0 * wide * halves * std::max(45.0, columns / 2.0), 500.0});
       const double item = 2500 + ((k + kKB - 1) / kKB + wide - 1) / wide * stage;
       const double time = std::ceil(tiles * (double)((n + r - 1) / r) / sms) * item;
       if (time < 0.95 * least) least = time, best = r;
@@ -1162,7 +1213,7 @@ Tiling make_tiling(int64_t tokens, int64_t experts, int top_k, int hidden, int i
   };
   Tiling t = {};
   const int columns = (int)std::min<double>(tile_n, std::max(16.0, share * 1.2));  // of most tiles
-  t.cycles = pick(2 * (int64_t)inter, hidden, direct ? tile_n : columns, t.rows1) + pick(hidden, inter, columns, t.rows2);
+  t.cycles = pick(2 * (int64_t)inter, hidden, direct ? tile_n : columns, 1, t.rows1) + pick(hidden, inter, columns, 2, t.rows2);
   return t;
 }
 
@@ -1185,15 +1236,19 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
     for (int n : {32, 64, 96, 128, 192, 256}) {  // small ones leave the ring more stages
       if (n >= share && n < most && most <= 256) continue;  // some would spill over into a tile of their own
       const Tiling t = make_tiling(tokens, experts, top_k, hidden, inter, n, false, sms);
-      if (t.cycles < 0.98 * best.cycles) best = t, l.tile_n = n;
+      if (t.cycles < 0.99 * best.cycles) best = t, l.tile_n = n;
     }
   }
   l.rows1 = best.rows1, l.rows2 = best.rows2;
   l.max_tiles = (int)(std::min<int64_t>(experts, rows) + (l.direct ? 0 : rows / l.tile_n));
   l.rows_act = l.tile_n <= 64 ? 16 : 32;
   l.rows_x = l.direct ? l.tile_n : l.rows_act;
-  // A stage's token rows, of as many chunks as its weights have.
-  l.slot_b = (int)up(l.tile_n, l.rows_act) * 128 * (128 / std::min(l.rows1, l.rows2));
+  // A stage's token rows, of as many chunks as its weights have; for down both halves of them where that leaves
+  // four stages (eight up to kDirectTokens tokens, where the stream of weights is what counts), else of those tiles
+  // alone that are half full (holds_both()). 700 tokens of 3584 through 2 of 16 experts of 2368 take 207 us so, 228
+  // with eight; 128 tokens of 2048 through 8 of 64 of 768 127 us, 141 with four.
+  const int chunk = (int)up(l.tile_n, l.rows_act) * 128, one = chunk * (128 / l.rows1), two = chunk * (128 / l.rows2);
+  l.slot_b = std::max(one, kRing / (kSlotA + 2 * two) >= (l.direct ? 8 : 4) ? 2 * two : two);
   l.stages = std::min(kMaxStages, kRing / (kSlotA + l.slot_b));
   int64_t at = up(sizeof(Header), 256);
   auto take = [&](int64_t bytes) {
@@ -1207,7 +1262,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.weight = take(rows * 4);
   l.done = take((std::min<int64_t>(experts, rows) + rows / 32) * 4);  // of the smallest tiles
   l.xs = take(l.direct ? 0 : rows * hidden * 2);
-  l.act = take(rows * inter * (l.few ? 4 : 2));  // few: two halves
+  l.act = take(rows * inter * 4);
   l.y = take(rows * hidden * 4);
   l.bytes = at;
   return l;
@@ -1236,7 +1291,7 @@ void launch_router(const ExpertParams& p, int groups, cudaStream_t st) {
 }
 
 template <typename T>
-int launch(const CUtensorMap (&maps)[6], const ExpertParams& p, bool few, cudaStream_t st) {
+int launch(const CUtensorMap (&maps)[7], const ExpertParams& p, bool few, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_sms());
   cfg.blockDim = dim3(kThreads);
@@ -1281,7 +1336,7 @@ int launch(const CUtensorMap (&maps)[6], const ExpertParams& p, bool few, cudaSt
   const cudaError_t e = attribute.set(reinterpret_cast<const void*>(expert_kernel<T>), 1024 + kRing);
   if (e != cudaSuccess) return cuda_status(e);
   cfg.dynamicSmemBytes = smem;
-  return cuda_status(cudaLaunchKernelEx(&cfg, expert_kernel<T>, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p));
+  return cuda_status(cudaLaunchKernelEx(&cfg, expert_kernel<T>, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], p));
 }
 
 }  // namespace
@@ -1338,28 +1393,33 @@ extern "C" int pkv_expert_mlp(int32_t dtype, const void* x, int64_t x_stride, in
   p.tile_n = l.tile_n;
   p.stages = l.stages, p.slot_b = l.slot_b, p.direct = l.direct, p.rows_x = l.rows_x, p.rows_act = l.rows_act;
   p.drop_y = hidden % 32 == 0 && n_tokens * top_k * hidden * 4 >= kDropBytes;
+  p.acc_cols = std::max(l.tile_n, 2 * std::min(l.tile_n, kJointRows));
   p.tmem_cols = 32;
-  while (p.tmem_cols < 2u * l.tile_n) p.tmem_cols *= 2;
-  CUtensorMap maps[6];
+  while (p.tmem_cols < 2u * p.acc_cols) p.tmem_cols *= 2;
+  CUtensorMap maps[7];
   int rc = PKV_OK;
-  if (!l.few && l.direct) rc = make_matrix_tensor_map(&maps[0], x, dtype, hidden, n_tokens, (uint64_t)x_stride * 2, kKB, l.rows_x);
-  else if (!l.few)
-    rc = make_matrix_tensor_map(&maps[0], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, l.rows_x);
+  // Token rows: one stack of x, and the values and rests of the activations.
+  const uint64_t rows = (uint64_t)n_tokens * top_k;
+  auto x_map = [&](CUtensorMap& map, uint32_t box) {
+    return l.direct ? make_stack_tensor_map(&map, x, dtype, hidden, n_tokens, 1, box, 1, x_stride)
+                    : make_stack_tensor_map(&map, p.xs, dtype, hidden, rows, 1, box, 1);
+  };
+  auto act_map = [&](CUtensorMap& map, uint32_t box, uint32_t halves) {
+    return make_stack_tensor_map(&map, p.act, dtype, intermediate, rows, 2, box, halves);
+  };
+  if (!l.few) rc = x_map(maps[0], l.rows_x);
   // Operand A of the first product alternates 16 gate rows and their 16 up rows: in one copy where an
   // expert's rows are whole groups of 16, else a copy for each 32.
   p.in16 = intermediate % 16 == 0;
   if (rc == PKV_OK && !l.few)
     rc = p.in16 ? make_split_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2, l.rows1 / 32)
                 : make_stack_tensor_map(&maps[1], gate_up, dtype, hidden, intermediate, 2 * (uint64_t)num_experts, 16, 2);
-  if (rc == PKV_OK && !l.few)
-    rc = make_matrix_tensor_map(&maps[2], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB,
-                                l.rows_act);
+  if (rc == PKV_OK && !l.few) rc = act_map(maps[2], l.rows_act, 1);
   if (rc == PKV_OK && !l.few) rc = make_stack_tensor_map(&maps[3], down, dtype, intermediate, hidden, num_experts, l.rows2, 1);
   if (!l.few) maps[4] = maps[0], maps[5] = maps[2];
-  if (rc == PKV_OK && !l.few && !l.direct && l.rows_act == 32)
-    rc = make_matrix_tensor_map(&maps[4], p.xs, dtype, hidden, (uint64_t)n_tokens * top_k, (uint64_t)hidden * 2, kKB, 128);
-  if (rc == PKV_OK && !l.few && l.rows_act == 32)
-    rc = make_matrix_tensor_map(&maps[5], p.act, dtype, intermediate, (uint64_t)n_tokens * top_k, (uint64_t)intermediate * 2, kKB, 128);
+  if (rc == PKV_OK && !l.few && !l.direct && l.rows_act == 32) rc = x_map(maps[4], 128);
+  if (rc == PKV_OK && !l.few && l.rows_act == 32) rc = act_map(maps[5], 128, 1);
+  if (rc == PKV_OK && !l.few) rc = act_map(maps[6], l.rows_act, 2);
   if (rc != PKV_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == PKV_F16 ? launch<__half>(maps, p, l.few, st) : launch<__nv_bfloat16>(maps, p, l.few, st);

@@ -141,8 +141,8 @@ int make_row_group_tensor_map(CUtensorMap* map, const void* base, int dtype, int
 }
 
 int make_stack_tensor_map(CUtensorMap* map, const void* base, int dtype, uint64_t inner, uint64_t rows, uint64_t stacks,
-                          uint32_t box_rows, uint32_t box_stacks) {
-  const uint64_t row = inner * 2, stack = rows * row;
+                          uint32_t box_rows, uint32_t box_stacks, uint64_t row_stride) {
+  const uint64_t row = (row_stride ? row_stride : inner) * 2, stack = rows * row;
   return encode_rows(map, base, dtype, {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)stacks, 1},
                      {(cuuint64_t)row, (cuuint64_t)stack, (cuuint64_t)(stacks * stack)}, {64, box_rows, box_stacks, 1});
 }

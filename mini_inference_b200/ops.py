@@ -676,8 +676,9 @@ def expert_mlp(x: torch.Tensor, router: torch.Tensor, gate_up: torch.Tensor, dow
     ``[E, hidden]``; the first among equals), and the result is the sum over them of ``w * down[e] .
     (silu(gate) * up)`` with ``gate | up = gate_up[e] . x`` (``gate_up`` ``[E, 2 * intermediate,
     hidden]``, ``down`` ``[E, hidden, intermediate]``) and ``w`` the softmax of the chosen logits
-    (``renormalize=False``: of all of them). float32 throughout but for one rounding of ``silu(gate) *
-    up`` and one of the result; logits that float32 sums of their terms do not tell from the border
+    (``renormalize=False``: of all of them). float32 throughout but for one rounding of the result and
+    ``silu(gate) * up``, which is held as two numbers of x's type, the rounded one and what that left
+    (infinite past the type's range); logits that float32 sums of their terms do not tell from the border
     between chosen and not are compared in float64. ``out`` (contiguous) may not overlap the inputs.
     """
     result = _layer.expert_mlp(x, router, gate_up, down, top_k, renormalize, workspace, out, status)
