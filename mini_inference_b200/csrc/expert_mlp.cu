@@ -17,14 +17,14 @@
 //    product to the second: the weights of down stream in while the activations are still being
 //    made, and only the tokens' side waits for them (a counter per token tile). Then the
 //    weighted sum over each token's experts, in their order.
-// On one B200, captured: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 135 us
-// = 6.0 TB/s, 0.91 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 126 us = 5.7 TB/s;
-// 2048 tokens of 2048 through 8 of 64 experts of 768 261 us = 0.59 PFLOP/s, bound by the ring's latency (four
-// stages of 40 KB on average, one in some 900 cycles: weights take 2600 cycles to come, the roles 500 to 700 a
-// stage; L2 and DRAM are at 41 and 53 %) and by the 134 MB of float32 products written and read back (30 us
-// of sums); 333 tokens of 896 through 4 of 60 experts of 616 57 us and one token of 2048 through 8 of 64 of
-// 768 25 us, bound by the chain: launches and cold instructions 5 us, logits and choice 4-8, first data 4,
-// the wait between the products 3, the last sums 2.
+// On one B200, captured: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 140 us
+// = 5.8 TB/s, 0.88 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 120 us = 6.0 TB/s;
+// 2048 tokens of 2048 through 8 of 64 experts of 768 320 us = 0.48 PFLOP/s (0.64 with down's products taken for both
+// halves), bound by what comes into the SMs: a stage of 48 KB for some 500 cycles of products comes at 45 to 52 bytes
+// a cycle and SM (L2 at 36 % of its peak, DRAM at 46, tensor cores at 37), and by the 134 MB of float32 products written
+// and read back (30 us of sums); 333 tokens of 896 through 4 of 60 experts of 616 64 us and one token of 2048
+// through 8 of 64 of 768 25 us, bound by the chain: launches and cold instructions 5 us, logits and choice 4-13,
+// first data 4, the wait between the products 3, the last sums 2.
 //
 // No counterpart in the reference, whose MLP is dense (engine/model.py:254-264).
 #include <algorithm>
@@ -422,7 +422,11 @@ struct Item {
   int tile, e, n0, n;     // token tile, its expert, its first and number of tokens
   int row;                // row tile
   int chunks;             // of 64 elements of K
+  int halves;             // what becomes of the two halves of its token rows
 };
+// Gate and up's rows have none; down's are copied and multiplied one behind the other, jointly (a copy brings both,
+// one product has both as columns), or the rests in a stage of their own.
+enum { kNone, kBoth, kJoint, kSplit };
 
 struct Shared {
   uint64_t full[kMaxStages];   // a stage's weight rows and token rows landed
@@ -476,9 +480,6 @@ __global__ void __launch_bounds__(256) gather_kernel(const ExpertParams p) {
   }
 }
 
-// A stage holds both halves of `rows` token rows of down.
-__device__ __forceinline__ bool holds_both(const ExpertParams& p, int rows, int chunks) { return 2 * rows * 128 * chunks <= p.slot_b; }
-
 // Item i, by a converged warp; false past the last. Not inlined: the roles share its instructions, which
 // a launch has to fetch anew (they took 6000 cycles before the first copy when each role had its own).
 __device__ __noinline__ bool find_item(const ExpertParams& p, const Shared& s, int i, Item& it) {
@@ -498,6 +499,10 @@ __device__ __noinline__ bool find_item(const ExpertParams& p, const Shared& s, i
   // An expert's tiles are alike: one full and one of a few tokens would take SMs unequal times.
   const int count = s.offset[it.e + 1] - s.offset[it.e], tiles = s.tile[it.e + 1] - s.tile[it.e];
   const int size = ((count + tiles - 1) / tiles + 15) & ~15;  // at most tile_n, a multiple of 16: no tile is empty
+  // Of all of an expert's tiles alike, by their size and not by their rows: which rows the last, smaller tile has is a
+  // matter of timing, and the order of their sums must not be.
+  const bool hold = 2 * ((size + p.rows_act - 1) / p.rows_act * p.rows_act) * 128 * (128 / p.rows2) <= p.slot_b;  // in one stage
+  it.halves = !it.second ? kNone : !hold ? kSplit : size <= kJointRows ? kJoint : kBoth;
   it.n0 = (it.tile - s.tile[it.e]) * size;
   it.n = min(size, count - it.n0);
   return true;
@@ -659,13 +664,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         fence_proxy_async_global();
       }
-      const bool split = second && !holds_both(p, loaded, wide), joint = second && !split && pad <= kJointRows;
+      const int how = uniform(it.halves);
+      const bool joint = how == kJoint;
       const CUtensorMap* map_w = second ? &map_down : &map_gu;
       const CUtensorMap* map_b = joint ? &map_halves : second ? &map_act : &map_x;
       const CUtensorMap* map_b128 = second ? &map_act128 : &map_x128;
       const int stack = second ? e : 2 * e;
       // Stages of a step, and the halves of one that are copied one after another; a joint copy brings both.
-      const int parts = split ? 2 : 1, halves = second && !split && !joint ? 2 : 1, twice = joint ? 2 : 1;
+      const int parts = how == kSplit ? 2 : 1, halves = how == kBoth ? 2 : 1, twice = joint ? 2 : 1;
       for (int ks = 0; ok && ks < k1; ks += wide)
         for (int part = 0; part < parts; ++part) {
           if (round > 0 && !wait_warp(&s.freed[slot], (round - 1) & 1, deadline)) {
@@ -729,8 +735,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int k1 = uniform(it.chunks), pad = uniform((it.n + 15) & ~15);
       const int columns = !second && p.direct ? p.tile_n : pad;
       const int rows_b = second ? p.rows_act : p.rows_x, loaded = (columns + rows_b - 1) / rows_b * rows_b;
-      const bool split = second && !holds_both(p, loaded, wide), joint = second && !split && pad <= kJointRows;
-      const int parts = split ? 2 : 1, halves = second && !split && !joint ? 2 : 1, twice = joint ? 2 : 1;
+      const int how = uniform(it.halves);
+      const bool joint = how == kJoint;
+      const int parts = how == kSplit ? 2 : 1, halves = how == kBoth ? 2 : 1, twice = joint ? 2 : 1;
       const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, joint ? 2 * loaded : columns);
       const uint32_t d = tmem + (uint32_t)(b * p.acc_cols);
       bool more = false;
@@ -817,8 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && wait_for(&s.acc_full[b], (c >> 1) & 1, deadline);
       tc_fence_after_sync();
       const uint32_t d = tl + (uint32_t)(b * p.acc_cols);
-      const int pad = (it.n + 15) & ~15, loaded = (pad + p.rows_act - 1) / p.rows_act * p.rows_act;
-      const bool joint = second && pad <= kJointRows && holds_both(p, loaded, 128 / p.rows2);  // then a warp has one block at most
+      const bool joint = it.halves == kJoint;  // then a warp has one block of columns at most
       uint32_t v[2][16];
       auto fetch = [&](int j) {
         if (direct) {  // the columns of the tokens themselves
@@ -1189,7 +1195,8 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // About how long the tiles of `tile_n` tokens take, in cycles, and the weight rows of an item that take least.
 // A stage of 16 KB of weights and its token rows comes at some 52 bytes a cycle from L2 and costs 45 cycles a
-// product at least, an item some 2500 besides; items are dealt out in rounds over the SMs.
+// product at least, an item some 2500 besides; items are dealt out in rounds over the SMs. Down's tokens are two
+// halves.
 struct Tiling {
   double cycles;
   int rows1, rows2;
@@ -1236,7 +1243,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
     for (int n : {32, 64, 96, 128, 192, 256}) {  // small ones leave the ring more stages
       if (n >= share && n < most && most <= 256) continue;  // some would spill over into a tile of their own
       const Tiling t = make_tiling(tokens, experts, top_k, hidden, inter, n, false, sms);
-      if (t.cycles < 0.99 * best.cycles) best = t, l.tile_n = n;
+      if (t.cycles < 0.99 * best.cycles) best = t, l.tile_n = n;  // 2048 tokens of 8 in 64 experts: 256, 320 us, not 192, 345
     }
   }
   l.rows1 = best.rows1, l.rows2 = best.rows2;
@@ -1245,7 +1252,7 @@ Layout make_layout(int64_t tokens, int experts, int top_k, int hidden, int inter
   l.rows_x = l.direct ? l.tile_n : l.rows_act;
   // A stage's token rows, of as many chunks as its weights have; for down both halves of them where that leaves
   // four stages (eight up to kDirectTokens tokens, where the stream of weights is what counts), else of those tiles
-  // alone that are half full (holds_both()). 700 tokens of 3584 through 2 of 16 experts of 2368 take 207 us so, 228
+  // alone that are half full (find_item()). 700 tokens of 3584 through 2 of 16 experts of 2368 take 207 us so, 228
   // with eight; 128 tokens of 2048 through 8 of 64 of 768 127 us, 141 with four.
   const int chunk = (int)up(l.tile_n, l.rows_act) * 128, one = chunk * (128 / l.rows1), two = chunk * (128 / l.rows2);
   l.slot_b = std::max(one, kRing / (kSlotA + 2 * two) >= (l.direct ? 8 : 4) ? 2 * two : two);

@@ -282,3 +282,18 @@ def test_nothing_but_the_result_is_rounded(dtype, tokens, hidden, inter, experts
     want, _ = reference(x, router, gate_up, down, top_k)
     off, rounding = (got - want).norm(), (want.to(dtype).double() - want).norm()
     assert off <= 1.1 * rounding, (off / rounding).item()
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", [(333, 896, 616, 60, 4), (1500, 256, 1024, 24, 4), (400, 512, 512, 8, 2), (2048, 512, 768, 64, 8)])
+def test_the_same_bits_every_time_whatever_the_experts_loads(tokens, hidden, inter, experts, top_k):
+    """Experts of every load, some with several tiles of which the last is smaller: rows go to them in no fixed order."""
+    x, router, gate_up, down = make(torch.bfloat16, tokens, hidden, inter, experts, seed=3)
+    x[:, 0] = 1
+    router[:, 0] = torch.linspace(-1.5, 1.5, experts, device="cuda")
+    first = check(x, router, gate_up, down, top_k)
+    for t in (tokens - 7, tokens):  # other calls of the same size, other loads
+        want = check(x[:t], router, gate_up, down, top_k)
+        for _ in range(12):
+            ws = ops.expert_mlp_workspace(t, experts, top_k, hidden, inter, "cuda")
+            assert torch.equal(ops.expert_mlp(x[:t], router, gate_up, down, top_k, ws), want)
+    assert torch.equal(first, want)
