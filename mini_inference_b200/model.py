@@ -223,7 +223,7 @@ class Qwen2Model:
         # that captured steps hold the addresses of stay.
         self._expert_workspaces: list[torch.Tensor] = []
         self._expert_rows = -1  # tokens that the last one holds
-        self._expert_captured = False  # whether a captured step holds it
+        self._expert_captured = 0  # how many of the first ones stay: up to the last that a captured step holds
         self.norm = weights["norm.weight"]
         # The reference's RoPE tables (float32, cast to the model dtype per lookup), built once.
         # Other layouts and scaled frequencies go through ops.rotary_append, which makes the
@@ -276,16 +276,17 @@ class Qwen2Model:
         if rows > self._expert_rows:
             if capturing:
                 raise RuntimeError(f"run a step of {rows} tokens before capturing one: the experts' workspace has to grow")
-            if self._expert_workspaces and not self._expert_captured:
+            self._expert_rows = -1
+            while len(self._expert_workspaces) > self._expert_captured:
                 # Its memory is another's only once the steps up to here are done, whichever stream they ran on.
                 self._expert_workspaces.pop().record_stream(torch.cuda.current_stream(self.device))
-            self._expert_rows, self._expert_captured = -1, False
             cfg, most = self.cfg, max(64, 1 << (rows - 1).bit_length())
             self._expert_workspaces.append(ops.expert_mlp_workspace(
                 most, cfg.num_experts, cfg.experts_per_token, cfg.hidden_size,
                 cfg.expert_intermediate_size or cfg.intermediate_size, self.device))
             self._expert_rows = most
-        self._expert_captured |= capturing
+        if capturing:
+            self._expert_captured = len(self._expert_workspaces)
         return self._expert_workspaces[-1]
 
     def reset_workspaces(self) -> None:

@@ -63,3 +63,25 @@ def test_a_step_of_no_tokens():
     model = make_model()
     x = torch.empty(0, 192, device="cuda", dtype=torch.float16)
     assert model._experts(0, x, None).shape == (0, 192)
+
+
+@torch.inference_mode()
+def test_a_size_that_is_refused_leaves_what_captures_hold():
+    """More tokens than any call takes: refused each time, and the captured step's workspace is still there."""
+    model = make_model()
+    x = torch.randn(40, 192, device="cuda", dtype=torch.float16)
+    want = model._experts(0, x, None)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = model._experts(0, x, None)
+    first = model._expert_workspaces[0]
+    for grown in (False, True):
+        if grown:
+            model.expert_workspace(1000)
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                model.expert_workspace(2**24 + 1)
+            assert model._expert_workspaces and model._expert_workspaces[0] is first
+    graph.replay()
+    assert torch.equal(out, want)
+    assert torch.equal(model._experts(0, x, None), want)
