@@ -17,12 +17,12 @@
 //    product to the second: the weights of down stream in while the activations are still being
 //    made, and only the tokens' side waits for them (a counter per token tile). Then the
 //    weighted sum over each token's experts, in their order.
-// On one B200, captured: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 140 us
-// = 5.8 TB/s, 0.88 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 120 us = 6.0 TB/s;
-// 2048 tokens of 2048 through 8 of 64 experts of 768 320 us = 0.48 PFLOP/s (0.64 with down's products taken for both
+// On one B200, captured: 64 tokens of 2048 through 8 of 64 experts of 1024 (bf16, 806 MB of weights) 141 us
+// = 5.7 TB/s, 0.87 of the copy bandwidth; 16 tokens of 3584 through 2 of 16 experts of 2368 120 us = 6.0 TB/s;
+// 2048 tokens of 2048 through 8 of 64 experts of 768 326 us = 0.48 PFLOP/s (0.63 with down's products taken for both
 // halves), bound by what comes into the SMs: a stage of 48 KB for some 500 cycles of products comes at 45 to 52 bytes
 // a cycle and SM (L2 at 36 % of its peak, DRAM at 46, tensor cores at 37), and by the 134 MB of float32 products written
-// and read back (30 us of sums); 333 tokens of 896 through 4 of 60 experts of 616 64 us and one token of 2048
+// and read back (30 us of sums); 333 tokens of 896 through 4 of 60 experts of 616 67 us and one token of 2048
 // through 8 of 64 of 768 25 us, bound by the chain: launches and cold instructions 5 us, logits and choice 4-13,
 // first data 4, the wait between the products 3, the last sums 2.
 //

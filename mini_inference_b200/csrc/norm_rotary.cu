@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const NormRotaryP
 }
 
 // Rows, heads or halves that do not start on 16 bytes: a warp per head, an element at a time. The
-// head is read twice (its squares, then its elements), the second time from L1.
+// head is read twice (its squares, then its elements), the second time from L1. 8192 tokens of 28 / 4 heads of
+// 72 (bf16, three axes, appended) take 98 us = 0.86 TB/s, one token 6.9: bound by its instructions, two bytes a lane.
 template <typename T, bool INTER, bool NORM>
 __global__ void __launch_bounds__(kThreads) norm_rotary_any_kernel(const NormRotaryParams p) {
   __shared__ float2 cs[kMaxHalf];
